@@ -41,7 +41,8 @@ HIP_FLAGS = [
 ]
 SOURCES = [
     "pk_abi.cpp", "pk_conv_abi.cpp", "pk_attention_abi.cpp", "pk_layernorm_abi.cpp",
-    "pk_encoder_abi.cpp", "pk_subsampling_abi.cpp", "pk_tdt_abi.cpp", "pk_codes.hip", "pk_conv.hip",
+    "pk_encoder_abi.cpp", "pk_subsampling_abi.cpp", "pk_tdt_abi.cpp", "pk_block_norm_abi.cpp", "pk_q4_abi.cpp",
+    "pk_score_abi.cpp", "pk_codes.hip", "pk_conv.hip", "pk_block_norm.hip", "pk_q4.hip", "pk_score.hip",
     "pk_subsampling.hip", "pk_tdt.hip", "pk_tdt_resident.hip",
     "pk_attention.hip", "pk_layernorm.hip",
     "pk_gemm_f16.hip", "pk_gemm_f16k.hip",

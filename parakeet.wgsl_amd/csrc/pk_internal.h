@@ -342,6 +342,78 @@ uint32_t layernorm_grid(uint32_t rows);
 hipError_t launch_layernorm(bool f16, const LayerNormArgs& args, hipStream_t stream, hipEvent_t start = nullptr,
                             hipEvent_t stop = nullptr);
 
+// The norms around a block (pk_block_norm.hip): output = residual +
+// residual_scale * gate * norm(input), next_output = norm(output). Strides in
+// elements; null gamma, beta, gate, residual and next_output: none.
+struct BlockNormArgs {
+  const void* input;
+  const float* gamma;
+  const float* beta;
+  const void* gate;
+  const void* residual;
+  void* output;
+  const float* next_gamma;
+  const float* next_beta;
+  void* next_output;
+  uint64_t input_stride, gate_stride, residual_stride, output_stride, next_stride;
+  uint32_t rows;      // active rows
+  uint32_t channels;
+  uint32_t gate_rows;  // rows that share a gate row, 0: all
+  float residual_scale;
+  float epsilon;
+  bool rms, f16;
+};
+hipError_t launch_block_norm(const BlockNormArgs& args, hipStream_t stream, hipEvent_t start = nullptr,
+                             hipEvent_t stop = nullptr);
+
+// Token scores (pk_score.hip): log probability of a given token, entropy and
+// the best alternatives of each row of logits; null outputs: none.
+struct ScoreArgs {
+  const void* logits;  // [rows, columns], rows `stride` elements apart
+  const uint32_t* tokens;
+  float* log_probs;
+  float* entropies;
+  uint32_t* top_tokens;  // [rows, alternatives]
+  float* top_log_probs;
+  uint64_t stride;
+  uint32_t rows;  // active rows
+  uint32_t columns;
+  uint32_t alternatives;
+  float inverse_temperature;
+  bool f16;
+};
+hipError_t launch_score(const ScoreArgs& args, hipStream_t stream, hipEvent_t start = nullptr,
+                        hipEvent_t stop = nullptr);
+
+// The product with 4-bit weights and group scales (pk_q4.hip, which has the
+// layout of codes, scales and offsets). Strides in elements.
+struct Q4Args {
+  const void* a;       // [rows, inner]
+  const uint4* codes;  // blocks of 16 columns x 128 k
+  const void* scales;  // [blocks][16][per_block]
+  const void* offsets; // likewise, or null
+  void* out;           // [rows, columns]
+  const float* bias;
+  const void* residual;
+  uint64_t a_stride, out_stride, residual_stride;
+  float residual_scale;
+  int activation;
+  uint32_t rows;  // active rows
+  uint32_t inner;
+  uint32_t columns;
+  uint32_t per_block;  // scales of a column in a block: 1, 2 or 4
+  bool f16;
+};
+// Bytes of a laid-out weight, and where its tables start.
+struct Q4Layout {
+  uint64_t scales, offsets, bytes;
+};
+Q4Layout q4_layout(const Q4Args& args, bool offsets);
+// Writes args.codes, scales and offsets from the packed codes and the tables.
+hipError_t launch_q4_layout(const Q4Args& args, const uint32_t* packed, const void* scales, const void* offsets,
+                            uint32_t group, hipStream_t stream);
+hipError_t launch_q4(const Q4Args& args, hipStream_t stream, hipEvent_t start = nullptr, hipEvent_t stop = nullptr);
+
 // Subsampling front end convolutions (pk_subsampling.hip).
 enum SubsamplingKind { kSubsamplingFused = 0, kSubsamplingDepthwise = 1, kSubsamplingMask = 2 };
 struct SubsamplingArgs {

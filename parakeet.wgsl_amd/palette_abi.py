@@ -1,5 +1,6 @@
 """ctypes binding of libpk_palette.so (include/pk_palette.h, pk_conv.h, pk_attention.h,
-pk_layernorm.h, pk_subsampling.h, pk_encoder.h, pk_tdt.h).
+pk_layernorm.h, pk_subsampling.h, pk_encoder.h, pk_tdt.h, pk_block_norm.h, pk_q4.h,
+pk_score.h).
 
 A thin Python view of the C ABI, used by the tests and the benchmark. It
 raises PaletteError (or PaletteRangeError, mirroring the reference's
@@ -40,6 +41,10 @@ ENCODER_DISPATCHES = ("norm_feed_forward1", "feed-forward1-linear1", "feed-forwa
                       "self-attention-output-residual", "norm_conv", "convolution-pointwise1",
                       "convolution-glu-depthwise-bn-silu", "convolution-pointwise2-residual", "norm_feed_forward2",
                       "feed-forward2-linear1", "feed-forward2-linear2-residual", "norm_out")
+NORM_KIND = {"layer": 0, "rms": 1}
+BLOCK_NORM_MAX_CHANNELS = 16384
+SCORE_NO_TOKEN = 0xFFFFFFFF
+SCORE_MAX_ALTERNATIVES = 32
 EXPAND_LAYOUT = {"row-major": 0, "tile-major": 1}
 
 
@@ -264,6 +269,103 @@ class LayerNormDesc(ctypes.Structure):
         ("next_beta_bytes", ctypes.c_uint64),
         ("next_output", ctypes.c_void_p),
         ("next_output_bytes", ctypes.c_uint64),
+    ]
+
+
+class BlockNormDesc(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("label", ctypes.c_char_p),
+        ("precision", ctypes.c_int32),
+        ("kind", ctypes.c_int32),
+        ("rows", ctypes.c_uint32),
+        ("channels", ctypes.c_uint32),
+        ("input", ctypes.c_void_p),
+        ("input_bytes", ctypes.c_uint64),
+        ("input_stride", ctypes.c_uint32),
+        ("gamma", ctypes.c_void_p),
+        ("gamma_bytes", ctypes.c_uint64),
+        ("beta", ctypes.c_void_p),
+        ("beta_bytes", ctypes.c_uint64),
+        ("gate", ctypes.c_void_p),
+        ("gate_bytes", ctypes.c_uint64),
+        ("gate_stride", ctypes.c_uint32),
+        ("gate_rows", ctypes.c_uint32),
+        ("residual", ctypes.c_void_p),
+        ("residual_bytes", ctypes.c_uint64),
+        ("residual_stride", ctypes.c_uint32),
+        ("has_residual_scale", ctypes.c_int32),
+        ("residual_scale", ctypes.c_float),
+        ("output", ctypes.c_void_p),
+        ("output_bytes", ctypes.c_uint64),
+        ("output_stride", ctypes.c_uint32),
+        ("next_gamma", ctypes.c_void_p),
+        ("next_gamma_bytes", ctypes.c_uint64),
+        ("next_beta", ctypes.c_void_p),
+        ("next_beta_bytes", ctypes.c_uint64),
+        ("next_output", ctypes.c_void_p),
+        ("next_output_bytes", ctypes.c_uint64),
+        ("next_output_stride", ctypes.c_uint32),
+        ("has_epsilon", ctypes.c_int32),
+        ("epsilon", ctypes.c_float),
+    ]
+
+
+class Q4Desc(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("label", ctypes.c_char_p),
+        ("precision", ctypes.c_int32),
+        ("rows", ctypes.c_uint32),
+        ("inner", ctypes.c_uint32),
+        ("columns", ctypes.c_uint32),
+        ("group_size", ctypes.c_uint32),
+        ("a", ctypes.c_void_p),
+        ("a_bytes", ctypes.c_uint64),
+        ("a_stride", ctypes.c_uint32),
+        ("packed", ctypes.c_void_p),
+        ("packed_bytes", ctypes.c_uint64),
+        ("scales", ctypes.c_void_p),
+        ("scales_bytes", ctypes.c_uint64),
+        ("offsets", ctypes.c_void_p),
+        ("offsets_bytes", ctypes.c_uint64),
+        ("output", ctypes.c_void_p),
+        ("output_bytes", ctypes.c_uint64),
+        ("output_stride", ctypes.c_uint32),
+        ("bias", ctypes.c_void_p),
+        ("bias_bytes", ctypes.c_uint64),
+        ("residual", ctypes.c_void_p),
+        ("residual_bytes", ctypes.c_uint64),
+        ("residual_stride", ctypes.c_uint32),
+        ("has_residual_scale", ctypes.c_int32),
+        ("residual_scale", ctypes.c_float),
+        ("activation", ctypes.c_int32),
+    ]
+
+
+class ScoreDesc(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("label", ctypes.c_char_p),
+        ("precision", ctypes.c_int32),
+        ("rows", ctypes.c_uint32),
+        ("columns", ctypes.c_uint32),
+        ("row_stride", ctypes.c_uint32),
+        ("logits", ctypes.c_void_p),
+        ("logits_bytes", ctypes.c_uint64),
+        ("has_temperature", ctypes.c_int32),
+        ("temperature", ctypes.c_float),
+        ("tokens", ctypes.c_void_p),
+        ("tokens_bytes", ctypes.c_uint64),
+        ("log_probs", ctypes.c_void_p),
+        ("log_probs_bytes", ctypes.c_uint64),
+        ("entropies", ctypes.c_void_p),
+        ("entropies_bytes", ctypes.c_uint64),
+        ("alternatives", ctypes.c_uint32),
+        ("top_tokens", ctypes.c_void_p),
+        ("top_tokens_bytes", ctypes.c_uint64),
+        ("top_log_probs", ctypes.c_void_p),
+        ("top_log_probs_bytes", ctypes.c_uint64),
     ]
 
 
@@ -527,6 +629,25 @@ SIGNATURES = {
     "pk_layernorm_enqueue_timed": (ctypes.c_int, [_VP, ctypes.c_uint32, _VP, _VP, _VP]),
     "pk_layernorm_destroy": (ctypes.c_int, [_VP]),
     "pk_layernorm_release": (ctypes.c_int, [_VP]),
+    "pk_block_norm_validate": (ctypes.c_int, [ctypes.POINTER(BlockNormDesc)]),
+    "pk_block_norm_create": (ctypes.c_int, [_VP, ctypes.POINTER(BlockNormDesc), _PPV]),
+    "pk_block_norm_enqueue": (ctypes.c_int, [_VP, ctypes.c_uint32, _VP]),
+    "pk_block_norm_enqueue_timed": (ctypes.c_int, [_VP, ctypes.c_uint32, _VP, _VP, _VP]),
+    "pk_block_norm_destroy": (ctypes.c_int, [_VP]),
+    "pk_block_norm_release": (ctypes.c_int, [_VP]),
+    "pk_q4_validate": (ctypes.c_int, [ctypes.POINTER(Q4Desc)]),
+    "pk_q4_create": (ctypes.c_int, [_VP, ctypes.POINTER(Q4Desc), _VP, _PPV]),
+    "pk_q4_enqueue": (ctypes.c_int, [_VP, ctypes.c_uint32, _VP]),
+    "pk_q4_enqueue_timed": (ctypes.c_int, [_VP, ctypes.c_uint32, _VP, _VP, _VP]),
+    "pk_q4_weight_bytes": (ctypes.c_int, [_VP, ctypes.POINTER(ctypes.c_uint64)]),
+    "pk_q4_destroy": (ctypes.c_int, [_VP]),
+    "pk_q4_release": (ctypes.c_int, [_VP]),
+    "pk_score_validate": (ctypes.c_int, [ctypes.POINTER(ScoreDesc)]),
+    "pk_score_create": (ctypes.c_int, [_VP, ctypes.POINTER(ScoreDesc), _PPV]),
+    "pk_score_enqueue": (ctypes.c_int, [_VP, ctypes.c_uint32, _VP]),
+    "pk_score_enqueue_timed": (ctypes.c_int, [_VP, ctypes.c_uint32, _VP, _VP, _VP]),
+    "pk_score_destroy": (ctypes.c_int, [_VP]),
+    "pk_score_release": (ctypes.c_int, [_VP]),
     "pk_subsampling_output_dimension": (ctypes.c_uint32, [ctypes.c_uint32]),
     "pk_subsampling_valid_length": (ctypes.c_uint32, [ctypes.c_uint32, ctypes.c_uint32]),
     "pk_subsampling_fused_validate": (ctypes.c_int, [ctypes.POINTER(SubsamplingFusedDesc)]),
@@ -1012,6 +1133,129 @@ class LayerNormOp:
         if self.handle:
             check(load().pk_layernorm_release(self.handle))
             self.handle = None
+
+
+class _RowsOp:
+    """An op over the rows of its bindings: create from a descriptor, enqueue
+    on the first rows, destroy and release."""
+
+    _prefix = ""
+
+    def __init__(self, ctx: Context, desc, *create_args):
+        lib = load()
+        self.desc, self.ctx = desc, ctx
+        self._enqueue, self._enqueue_timed, self._destroy, self._release = (
+            getattr(lib, f"pk_{self._prefix}_{call}") for call in ("enqueue", "enqueue_timed", "destroy", "release"))
+        handle = ctypes.c_void_p()
+        check(getattr(lib, f"pk_{self._prefix}_create")(ctx.handle, ctypes.byref(desc), *create_args,
+                                                        ctypes.byref(handle)))
+        self.handle = handle.value
+
+    def enqueue(self, active_rows: int = 0, stream=None, start: "Event" = None, end: "Event" = None) -> None:
+        """Launch on the first `active_rows` rows (0: all); `start` and `end`
+        events, when given, are stamped by the launches themselves."""
+        if start is None and end is None:
+            check(self._enqueue(self.handle, active_rows, stream))
+        else:
+            check(self._enqueue_timed(self.handle, active_rows, stream, start.handle if start else None,
+                                      end.handle if end else None))
+
+    def destroy(self) -> None:
+        check(self._destroy(self.handle))
+
+    def release(self) -> None:
+        if self.handle:
+            check(self._release(self.handle))
+            self.handle = None
+
+
+def block_norm_desc(*, input, output, rows: int, channels: int, kind: str = "layer", gamma=None, beta=None, gate=None,
+                    gate_rows: int = 1, residual=None, residual_scale: float | None = None, next_gamma=None,
+                    next_beta=None, next_output=None, epsilon: float | None = None, input_stride: int = 0,
+                    gate_stride: int = 0, residual_stride: int = 0, output_stride: int = 0,
+                    next_output_stride: int = 0, precision: str | None = None,
+                    label: str = "block-norm") -> BlockNormDesc:
+    """A pk_block_norm_desc: output = residual + residual_scale * gate *
+    norm(input), next_output = norm(output). Row r takes gate row
+    r // gate_rows, or gate row 0 with gate_rows 0; strides in elements, 0 for
+    packed rows."""
+    if precision is None:
+        precision = "f16" if input.dtype == np.float16 else "f32"
+    return BlockNormDesc(ctypes.sizeof(BlockNormDesc), label.encode(), PRECISION[precision], NORM_KIND[kind], rows,
+                         channels, *_slice(input), input_stride, *_slice(gamma), *_slice(beta), *_slice(gate),
+                         gate_stride, gate_rows, *_slice(residual), residual_stride, int(residual_scale is not None),
+                         float(1.0 if residual_scale is None else residual_scale), *_slice(output), output_stride,
+                         *_slice(next_gamma), *_slice(next_beta), *_slice(next_output), next_output_stride,
+                         int(epsilon is not None), float(epsilon or 0.0))
+
+
+class BlockNormOp(_RowsOp):
+    """The norms around a block with its gate and residual (pk_block_norm_*)."""
+
+    _prefix = "block_norm"
+
+    def __init__(self, ctx: Context, **descriptor):
+        super().__init__(ctx, block_norm_desc(**descriptor))
+
+
+def pack_q4(codes: np.ndarray) -> np.ndarray:
+    """Codes 0..15 of [inner, columns] in the packed format of pk_q4.h: uint32
+    words of eight codes in row-major order, the first in the lowest bits."""
+    flat = np.asarray(codes, dtype=np.uint32).reshape(-1)
+    flat = np.concatenate([flat, np.zeros(-len(flat) % 8, np.uint32)]).reshape(-1, 8)
+    return np.bitwise_or.reduce(flat << (4 * np.arange(8, dtype=np.uint32)), axis=1).astype(np.uint32)
+
+
+def q4_desc(*, a, packed, scales, output, rows: int, inner: int, columns: int, group_size: int, offsets=None,
+            bias=None, residual=None, residual_scale: float | None = None, activation: str = "none",
+            a_stride: int = 0, output_stride: int = 0, residual_stride: int = 0, precision: str | None = None,
+            label: str = "q4-gemm") -> Q4Desc:
+    """A pk_q4_desc: output = residual + residual_scale * activation(a @ w +
+    bias) with w = scales * (code - 8) + offsets in groups of group_size
+    inputs (0: one group); strides in elements, 0 for packed rows."""
+    if precision is None:
+        precision = "f16" if a.dtype == np.float16 else "f32"
+    return Q4Desc(ctypes.sizeof(Q4Desc), label.encode(), PRECISION[precision], rows, inner, columns, group_size,
+                  *_slice(a), a_stride, *_slice(packed), *_slice(scales), *_slice(offsets), *_slice(output),
+                  output_stride, *_slice(bias), *_slice(residual), residual_stride,
+                  int(residual_scale is not None), float(residual_scale or 0.0), ACTIVATION[activation])
+
+
+class Q4GemmOp(_RowsOp):
+    """A product with a 4-bit group-scaled weight (pk_q4_*); the weight is laid
+    out in the op, so packed, scales and offsets may be freed afterwards."""
+
+    _prefix = "q4"
+
+    def __init__(self, ctx: Context, *, stream=None, **descriptor):
+        super().__init__(ctx, q4_desc(**descriptor), stream)
+
+    def weight_bytes(self) -> int:
+        value = ctypes.c_uint64()
+        check(load().pk_q4_weight_bytes(self.handle, ctypes.byref(value)))
+        return int(value.value)
+
+
+def score_desc(*, logits, rows: int, columns: int, row_stride: int = 0, temperature: float | None = None, tokens=None,
+               log_probs=None, entropies=None, alternatives: int = 0, top_tokens=None, top_log_probs=None,
+               precision: str | None = None, label: str = "token-scores") -> ScoreDesc:
+    """A pk_score_desc: log_probs of `tokens`, entropies, and the best
+    `alternatives` of each row of logits / temperature."""
+    if precision is None:
+        precision = "f16" if logits.dtype == np.float16 else "f32"
+    return ScoreDesc(ctypes.sizeof(ScoreDesc), label.encode(), PRECISION[precision], rows, columns, row_stride,
+                     *_slice(logits), int(temperature is not None), float(temperature or 0.0), *_slice(tokens),
+                     *_slice(log_probs), *_slice(entropies), alternatives, *_slice(top_tokens),
+                     *_slice(top_log_probs))
+
+
+class TokenScoreOp(_RowsOp):
+    """Scores of given tokens from rows of logits (pk_score_*)."""
+
+    _prefix = "score"
+
+    def __init__(self, ctx: Context, **descriptor):
+        super().__init__(ctx, score_desc(**descriptor))
 
 
 def subsampling_fused_desc(*, input, conv0_weights, conv0_bias, depthwise_weights, depthwise_bias, output,
