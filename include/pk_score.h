@@ -26,6 +26,7 @@ extern "C" {
 #define PK_SCORE_NO_TOKEN 0xffffffffu
 #define PK_SCORE_MAX_ALTERNATIVES 32u
 #define PK_SCORE_MAX_ROWS 4194303u
+#define PK_SCORE_MAX_COLUMNS 1073741824u
 
 typedef struct pk_score_op pk_score_op;
 
@@ -34,7 +35,7 @@ typedef struct pk_score_desc {
   const char *label;
   int32_t precision;             /* pk_precision of the logits */
   uint32_t rows;                 /* 1 to PK_SCORE_MAX_ROWS */
-  uint32_t columns;              /* V, up to 2^31; the logits may start at any element */
+  uint32_t columns;              /* V, 1 to PK_SCORE_MAX_COLUMNS; the logits may start at any element */
   uint32_t row_stride;           /* elements from row to row (0: columns) */
   const void *logits;
   uint64_t logits_bytes;         /* capacity from the pointer to the end of the last row */

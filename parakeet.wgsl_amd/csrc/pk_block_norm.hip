@@ -4,58 +4,89 @@
 //
 // Bound by memory: each matrix is read or written once (2 to 5 elements of
 // traffic for some 20 operations). A row lies in the registers of GROUP
-// threads (a wavefront up to 2048 channels, then 256 or 1024 threads), HELD
-// vectors a thread, as f32 from the first load to the last store, so the
-// second norm costs no memory trip. Variances are of the differences from
-// the mean, a second sum over registers, since E[x^2] - E[x]^2 loses every
-// digit of a row whose mean is far from zero.
+// threads, at most 16 channels a thread (one wavefront up to 1024 channels,
+// 1024 threads for 16384), as f32 from the first load to the last store, so
+// the second norm costs no memory trip, and every load of the row and of both
+// norms' parameters is issued before the first sum waits for any. Variances
+// are of the differences from the mean, a second sum over registers, since
+// E[x^2] - E[x]^2 loses every digit of a row whose mean is far from zero.
+// Vectors of 16 bytes load and store at any address of an element (gfx9's
+// global memory takes unaligned ones); channels beyond the last whole vector
+// are one extra element of the first threads.
 #include "pk_internal.h"
 #include "pk_wave.h"
 
 namespace pk {
 namespace {
 
-constexpr int kThreads = 256;  // of a workgroup, unless one row takes more
+constexpr int kThreads = 256;  // of a workgroup whose rows take a wavefront each
 
-template <typename T, int VEC>
-struct VectorOf {
-  typedef T type __attribute__((ext_vector_type(VEC)));
-};
-template <typename T>
-struct VectorOf<T, 1> {
-  typedef T type;
-};
-
-template <typename T, int VEC, int GROUP, int HELD>
-__global__ __launch_bounds__(GROUP > kThreads ? GROUP : kThreads) void block_norm_kernel(BlockNormArgs args) {
-  typedef typename VectorOf<T, VEC>::type V;
-  constexpr int kRows = GROUP < kThreads ? kThreads / GROUP : 1;  // rows of a workgroup
+template <typename T, int GROUP, int HELD, bool TAIL>
+__global__ __launch_bounds__(GROUP == 64 ? kThreads : GROUP) void block_norm_kernel(BlockNormArgs args) {
+  constexpr int VEC = 16 / sizeof(T);
   constexpr int kWaves = GROUP / 64;
+  typedef T V __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
+  typedef float F4 __attribute__((ext_vector_type(4), aligned(4)));
   __shared__ float partial[4][kWaves];  // a slot for each of the sums: no sum waits for the readers of another
-  const uint32_t row = blockIdx.x * kRows + threadIdx.x / GROUP;
+  const uint32_t row = GROUP == 64
+                           ? blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6))
+                           : blockIdx.x;
   const uint32_t at = threadIdx.x % GROUP;
-  if (row >= args.rows) return;  // whole wavefronts, and whole workgroups where they meet
-  const uint32_t vectors = args.channels / VEC;
+  if (row >= args.rows) return;  // whole wavefronts
+  const uint32_t vectors = args.channels / VEC, tail = TAIL ? args.channels % VEC : 0u;
   const float inverse = 1.0f / (float)args.channels;
 
-  auto load = [&](const void* p, uint64_t from, V (&dst)[HELD]) {
-    const V* v = reinterpret_cast<const V*>(static_cast<const T*>(p) + from);
+  // What a thread holds of a row: HELD vectors, and an element of the tail.
+  // Loads are unconditional, of the row's last vector where a thread has no
+  // i-th one; sums and stores leave those out.
+  struct Raw {
+    V v[HELD];
+    T edge;
+  };
+  struct Row {
+    float v[HELD][VEC];
+    float edge;
+  };
+  const auto has = [&](int i) { return at + i * GROUP < vectors; };
+  const auto place = [&](int i) { return min(at + i * GROUP, vectors - 1u); };
+  const bool has_edge = at < tail;
+  const uint32_t edge = args.channels - 1u - (has_edge ? at : 0u);
+  const auto load = [&](const void* p, uint64_t from) {
+    const T* source = static_cast<const T*>(p) + from;
+    Raw raw;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+      if (TAIL && !vectors) raw.v[i] = (V)(T)0.0f;
+      else raw.v[i] = reinterpret_cast<const V*>(source)[place(i)];
+    }
+    raw.edge = TAIL ? source[edge] : (T)0.0f;
+    return raw;
+  };
+  const auto load_vector = [&](const float* p) {
+    Row x;
 #pragma unroll
     for (int i = 0; i < HELD; ++i)
-      if (at + i * GROUP < vectors) dst[i] = v[at + i * GROUP];
-  };
-  auto element = [](const V& v, int c) -> float {
-    if constexpr (VEC == 1) return (float)v;
-    else return (float)v[c];
+#pragma unroll
+      for (int f = 0; f < VEC / 4; ++f) {
+        F4 q;
+        if (TAIL && !vectors) q = (F4)0.0f;
+        else q = reinterpret_cast<const F4*>(p)[place(i) * (VEC / 4) + f];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x.v[i][4 * f + c] = q[c];
+      }
+    x.edge = TAIL ? p[edge] : 0.0f;
+    return x;
   };
   // The sum of f(x) over the row, the same in every thread of the group.
-  auto total = [&](int slot, auto f, const float (&x)[HELD][VEC]) {
-    float s = 0.0f;
+  const auto total = [&](int slot, auto f, const Row& x) {
+    float s = TAIL && has_edge ? f(x.edge) : 0.0f;
 #pragma unroll
-    for (int i = 0; i < HELD; ++i)
-      if (at + i * GROUP < vectors)
+    for (int i = 0; i < HELD; ++i) {
+      float part = 0.0f;
 #pragma unroll
-        for (int c = 0; c < VEC; ++c) s += f(x[i][c]);
+      for (int c = 0; c < VEC; ++c) part += f(x.v[i][c]);
+      s += has(i) ? part : 0.0f;
+    }
     s = wave::sum(s);
     if constexpr (kWaves > 1) {
       if ((threadIdx.x & 63) == 0) partial[slot][threadIdx.x >> 6] = s;
@@ -66,93 +97,100 @@ __global__ __launch_bounds__(GROUP > kThreads ? GROUP : kThreads) void block_nor
     }
     return s;
   };
-  auto normalize = [&](int slot, const float* gamma, const float* beta, float (&x)[HELD][VEC]) {
+  const auto normalize = [&](int slot, const Row& gamma, const Row& beta, Row& x) {
     float mean = 0.0f;
     if (!args.rms) mean = total(slot, [](float v) { return v; }, x) * inverse;
     const float power = total(slot + 1, [mean](float v) { return (v - mean) * (v - mean); }, x) * inverse;
     const float scale = 1.0f / __builtin_sqrtf(power + args.epsilon);
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-      const uint32_t v = at + i * GROUP;
-      if (v >= vectors) continue;
-#pragma unroll
-      for (int c = 0; c < VEC; ++c) {
-        const float b = beta ? beta[v * VEC + c] : 0.0f;
-        x[i][c] = __builtin_fmaf((x[i][c] - mean) * scale, gamma[v * VEC + c], b);
-      }
-    }
-  };
-  auto store = [&](void* p, uint64_t from, const float (&x)[HELD][VEC]) {
-    V* out = reinterpret_cast<V*>(static_cast<T*>(p) + from);
-#pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-      if (at + i * GROUP >= vectors) continue;
-      V v;
+    for (int i = 0; i < HELD; ++i)
 #pragma unroll
       for (int c = 0; c < VEC; ++c)
-        if constexpr (VEC == 1) v = (T)x[i][c];
-        else v[c] = (T)x[i][c];
-      out[at + i * GROUP] = v;
+        x.v[i][c] = __builtin_fmaf((x.v[i][c] - mean) * scale, gamma.v[i][c], beta.v[i][c]);
+    x.edge = __builtin_fmaf((x.edge - mean) * scale, gamma.edge, beta.edge);
+  };
+  const auto store = [&](void* p, uint64_t from, const Row& x) {
+    T* target = static_cast<T*>(p) + from;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+      if (!has(i)) continue;
+      V v;
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) v[c] = (T)x.v[i][c];
+      reinterpret_cast<V*>(target)[at + i * GROUP] = v;
     }
+    if (TAIL && has_edge) target[edge] = (T)x.edge;
   };
 
-  V in[HELD], gate[HELD], residual[HELD];
-  load(args.input, row * args.input_stride, in);
-  if (args.gate) load(args.gate, (args.gate_rows ? row / args.gate_rows : 0u) * args.gate_stride, gate);
-  if (args.residual) load(args.residual, row * args.residual_stride, residual);
-  float x[HELD][VEC];
+  const Raw in = load(args.input, row * args.input_stride);
+  Raw residual, gate;
+  if (args.residual) residual = load(args.residual, row * args.residual_stride);
+  if (args.gate) gate = load(args.gate, (args.gate_rows ? row / args.gate_rows : 0u) * args.gate_stride);
+  Row gamma, beta = {}, next_gamma, next_beta = {};
+  if (args.gamma) gamma = load_vector(args.gamma);
+  if (args.beta) beta = load_vector(args.beta);
+  if (args.next_output) next_gamma = load_vector(args.next_gamma);
+  if (args.next_beta) next_beta = load_vector(args.next_beta);
+  Row x;
 #pragma unroll
   for (int i = 0; i < HELD; ++i)
 #pragma unroll
-    for (int c = 0; c < VEC; ++c) x[i][c] = element(in[i], c);
-  if (args.gamma) normalize(0, args.gamma, args.beta, x);
+    for (int c = 0; c < VEC; ++c) x.v[i][c] = (float)in.v[i][c];
+  x.edge = (float)in.edge;
+  if (args.gamma) normalize(0, gamma, beta, x);
+  if (args.gate) {
 #pragma unroll
-  for (int i = 0; i < HELD; ++i)
+    for (int i = 0; i < HELD; ++i)
 #pragma unroll
-    for (int c = 0; c < VEC; ++c) {
-      if (args.gate) x[i][c] *= element(gate[i], c);
-      x[i][c] = __builtin_fmaf(args.residual_scale, x[i][c], args.residual ? element(residual[i], c) : 0.0f);
-    }
+      for (int c = 0; c < VEC; ++c) x.v[i][c] *= (float)gate.v[i][c];
+    x.edge *= (float)gate.edge;
+  }
+  const float scale = args.residual_scale;
+  if (args.residual) {
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) x.v[i][c] = __builtin_fmaf(scale, x.v[i][c], (float)residual.v[i][c]);
+    x.edge = __builtin_fmaf(scale, x.edge, (float)residual.edge);
+  } else {
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) x.v[i][c] *= scale;
+    x.edge *= scale;
+  }
   store(args.output, row * args.output_stride, x);
   if (args.next_output) {
-    normalize(2, args.next_gamma, args.next_beta, x);
+    normalize(2, next_gamma, next_beta, x);
     store(args.next_output, row * args.next_stride, x);
   }
 }
 
 typedef void (*Kernel)(BlockNormArgs);
 
-// Threads of a row's group by channels, and the vectors each holds.
-template <typename T, int VEC>
+// The kernel for rows of `channels`, and the threads of a row.
+template <typename T, bool TAIL>
 Kernel pick(uint32_t channels, uint32_t* group) {
-  *group = channels <= 2048u ? 64u : channels <= 8192u ? 256u : 1024u;
-  if (channels <= 512u) return block_norm_kernel<T, VEC, 64, 8 / VEC>;
-  if (channels <= 1024u) return block_norm_kernel<T, VEC, 64, 16 / VEC>;
-  if (channels <= 2048u) return block_norm_kernel<T, VEC, 64, 32 / VEC>;
-  if (channels <= 4096u) return block_norm_kernel<T, VEC, 256, 16 / VEC>;
-  if (channels <= 8192u) return block_norm_kernel<T, VEC, 256, 32 / VEC>;
-  return block_norm_kernel<T, VEC, 1024, 16 / VEC>;
+  constexpr int VEC = 16 / sizeof(T);
+  *group = channels <= 1024u ? 64u : channels <= 2048u ? 128u : channels <= 4096u ? 256u : channels <= 8192u ? 512u : 1024u;
+  if (channels <= 512u) return block_norm_kernel<T, 64, 8 / VEC, TAIL>;
+  if (channels <= 1024u) return block_norm_kernel<T, 64, 16 / VEC, TAIL>;
+  if (channels <= 2048u) return block_norm_kernel<T, 128, 16 / VEC, TAIL>;
+  if (channels <= 4096u) return block_norm_kernel<T, 256, 16 / VEC, TAIL>;
+  if (channels <= 8192u) return block_norm_kernel<T, 512, 16 / VEC, TAIL>;
+  return block_norm_kernel<T, 1024, 16 / VEC, TAIL>;
+}
+template <typename T>
+Kernel pick(uint32_t channels, uint32_t* group) {
+  return channels % (16 / sizeof(T)) ? pick<T, true>(channels, group) : pick<T, false>(channels, group);
 }
 
 }  // namespace
 
 hipError_t launch_block_norm(const BlockNormArgs& args, hipStream_t stream, hipEvent_t start, hipEvent_t stop) {
-  const uint32_t elem = args.f16 ? 2u : 4u;
-  // 16-byte vectors where every row of every matrix starts on 16 bytes.
-  uint64_t bits = (uint64_t)args.channels * elem;
-  const auto rows_at = [&](const void* p, uint64_t stride) {
-    if (p) bits |= reinterpret_cast<uintptr_t>(p) | stride * elem;
-  };
-  rows_at(args.input, args.input_stride);
-  rows_at(args.gate, args.gate_stride);
-  rows_at(args.residual, args.residual_stride);
-  rows_at(args.output, args.output_stride);
-  rows_at(args.next_output, args.next_stride);
-  const bool wide = bits % 16u == 0u;
   uint32_t group = 0;
-  const Kernel kernel = args.f16 ? (wide ? pick<_Float16, 8>(args.channels, &group) : pick<_Float16, 1>(args.channels, &group))
-                                 : (wide ? pick<float, 4>(args.channels, &group) : pick<float, 1>(args.channels, &group));
-  const uint32_t threads = group > (uint32_t)kThreads ? group : (uint32_t)kThreads, each = threads / group;
+  const Kernel kernel = args.f16 ? pick<_Float16>(args.channels, &group) : pick<float>(args.channels, &group);
+  const uint32_t threads = group == 64u ? (uint32_t)kThreads : group, each = threads / group;
   const dim3 grid((args.rows + each - 1u) / each), block(threads);
   if (start || stop)
     hipExtLaunchKernelGGL(kernel, grid, block, 0, stream, start, stop, 0, args);

@@ -366,6 +366,13 @@ struct BlockNormArgs {
 hipError_t launch_block_norm(const BlockNormArgs& args, hipStream_t stream, hipEvent_t start = nullptr,
                              hipEvent_t stop = nullptr);
 
+// What a part of a row of logits x knows: m = max x, r = sum of 2^((x - m) s)
+// over all but one that is m, t = sum of that times (x - m) s, s = log2(e) /
+// temperature. m minus infinity: r is 0, or NaN if one is.
+struct ScorePart {
+  float m, r, t, unused;
+};
+
 // Token scores (pk_score.hip): log probability of a given token, entropy and
 // the best alternatives of each row of logits; null outputs: none.
 struct ScoreArgs {
@@ -381,7 +388,20 @@ struct ScoreArgs {
   uint32_t alternatives;
   float inverse_temperature;
   bool f16;
+  // Rows split over groups: a record and `alternatives` keys for each part.
+  uint32_t span;  // elements of a part, set by the launch
+  ScorePart* parts;
+  uint64_t* part_keys;
+  uint64_t records;  // that the workspace holds
 };
+// Groups of threads that a launch of few rows aims for: one for each of the
+// 256 compute units.
+constexpr uint32_t kScoreFill = 256;
+// Records of workspace for up to args.rows rows (0: none), their bytes, and
+// the binding of a workspace.
+uint64_t score_workspace(const ScoreArgs& args);
+uint64_t score_workspace_bytes(const ScoreArgs& args, uint64_t records);
+void score_bind_workspace(ScoreArgs* args, void* workspace, uint64_t records);
 hipError_t launch_score(const ScoreArgs& args, hipStream_t stream, hipEvent_t start = nullptr,
                         hipEvent_t stop = nullptr);
 

@@ -16,6 +16,7 @@ struct pk_score_op {
   std::string label;
   uint32_t rows = 0;
   pk::ScoreArgs args{};
+  void* workspace = nullptr;
   bool destroyed = false;
 };
 
@@ -30,7 +31,7 @@ int validate_score(const pk_score_desc* d) {
   const char* label = score_label(d->label);
   if (d->precision != PK_PRECISION_F16 && d->precision != PK_PRECISION_F32)
     return fail(PK_INVALID_ARGUMENT, "%s has an unsupported precision %d", label, d->precision);
-  if (d->rows == 0 || d->rows > PK_SCORE_MAX_ROWS || d->columns == 0 || d->columns > 0x80000000u)
+  if (d->rows == 0 || d->rows > PK_SCORE_MAX_ROWS || d->columns == 0 || d->columns > PK_SCORE_MAX_COLUMNS)
     return fail(PK_RANGE_ERROR, "Invalid token score shape for %s", label);
   if (d->row_stride && d->row_stride < d->columns)
     return fail(PK_RANGE_ERROR, "%s row stride must be at least the columns", label);
@@ -92,11 +93,7 @@ int pk_score_create(pk_context* ctx, const pk_score_desc* d, pk_score_op** out) 
   *out = nullptr;
   if (int s = validate_score(d)) return s;
   std::string label = score_label(d->label);
-  auto* op = new pk_score_op();
-  op->ctx = ctx;
-  op->label.swap(label);
-  op->rows = d->rows;
-  pk::ScoreArgs& a = op->args;
+  pk::ScoreArgs a{};
   a.logits = d->logits;
   a.stride = d->row_stride ? d->row_stride : d->columns;
   a.tokens = d->tokens;
@@ -109,6 +106,29 @@ int pk_score_create(pk_context* ctx, const pk_score_desc* d, pk_score_op** out) 
   a.alternatives = d->alternatives;
   a.inverse_temperature = d->has_temperature ? 1.0f / d->temperature : 1.0f;
   a.f16 = d->precision == PK_PRECISION_F16;
+  void* workspace = nullptr;
+  if (const uint64_t records = pk::score_workspace(a)) {
+    const uint64_t bytes = pk::score_workspace_bytes(a, records);
+    DeviceScope device(ctx->device);
+    PK_HIP(device.status(), "hipSetDevice");
+    const hipError_t e = hipMalloc(&workspace, bytes);
+    if (e != hipSuccess) {
+      (void)hipGetLastError();
+      return fail(PK_ALLOCATION_FAILURE, "%s: cannot allocate %llu bytes of workspace: %s", label.c_str(),
+                  (unsigned long long)bytes, hipGetErrorString(e));
+    }
+    pk::score_bind_workspace(&a, workspace, records);
+  }
+  auto* op = new (std::nothrow) pk_score_op();
+  if (!op) {
+    free_on(ctx->device, workspace);
+    return fail(PK_ALLOCATION_FAILURE, "%s: out of host memory", label.c_str());
+  }
+  op->ctx = ctx;
+  op->label.swap(label);
+  op->rows = d->rows;
+  op->args = a;
+  op->workspace = workspace;
   *out = op;
   return ok();
 } catch (const std::bad_alloc&) {
@@ -135,11 +155,16 @@ int pk_score_enqueue_timed(pk_score_op* op, uint32_t active_rows, void* stream, 
 }
 
 int pk_score_destroy(pk_score_op* op) {
-  if (op) op->destroyed = true;
+  if (!op || op->destroyed) return ok();
+  op->destroyed = true;
+  free_on(op->ctx->device, op->workspace);
+  op->workspace = nullptr;
   return ok();
 }
 
 int pk_score_release(pk_score_op* op) {
+  if (!op) return ok();
+  pk_score_destroy(op);
   delete op;
   return ok();
 }
