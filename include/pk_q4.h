@@ -25,6 +25,7 @@ extern "C" {
 #endif
 
 #define PK_Q4_MAX_ROWS 1048560u
+#define PK_Q4_MAX_STRIDE 16777216u
 
 typedef struct pk_q4_op pk_q4_op;
 
@@ -33,13 +34,13 @@ typedef struct pk_q4_desc {
   const char *label;
   int32_t precision;             /* pk_precision of a, scales, offsets, residual and output */
   uint32_t rows;                 /* M capacity, 1 to PK_Q4_MAX_ROWS */
-  uint32_t inner;                /* K */
+  uint32_t inner;                /* K, 1 to PK_Q4_MAX_STRIDE */
   uint32_t columns;              /* N; ceil(K / 128) * ceil(N / 16) below 2^24 */
   uint32_t group_size;           /* G: a power of two from 32 on, or 0 (one group: G = K);
                                     the last group may be short */
   const void *a;                 /* [rows, inner], rows a_stride elements apart (0: inner) */
   uint64_t a_bytes;
-  uint32_t a_stride;
+  uint32_t a_stride;             /* at most PK_Q4_MAX_STRIDE */
   const uint32_t *packed;        /* codes of [inner, columns], K-major, 8 per word, LSB first */
   uint64_t packed_bytes;         /* exactly 4 * ceil(inner * columns / 8) */
   const void *scales;            /* [ceil(inner / G), columns] */

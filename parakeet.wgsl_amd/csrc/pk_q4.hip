@@ -19,8 +19,6 @@ typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
-constexpr int kWaves = 4;  // wavefronts that share the K blocks of a tile
-
 // Bit of code j (0..7) in its word.
 __host__ __device__ constexpr uint32_t nibble_at(uint32_t j) { return 4u * (j >> 1) + 16u * (j & 1u); }
 
@@ -58,106 +56,679 @@ __global__ void layout_scales(const T* source, T* target, uint32_t inner, uint32
   target[id] = n < columns && k < inner ? source[(uint64_t)(k / group) * columns + n] : (T)0.0f;
 }
 
-// Codes of a word as f16 of code - 8: a[2t], a[2t + 1] from nibble t.
-__device__ __forceinline__ half8 decode(uint32_t word) {
-  const half2 low = {(_Float16)-1032.0f, (_Float16)-1032.0f}, high = {(_Float16)-72.0f, (_Float16)-72.0f};
-  const half2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
-  half8 f;
-#pragma unroll
-  for (int t = 0; t < 4; t += 2) {
-    const uint32_t w = word >> (4 * t);
-    const half2 p = __builtin_bit_cast(half2, (w & 0x000f000fu) | 0x64006400u) + low;
-    const half2 q = __builtin_elementwise_fma(__builtin_bit_cast(half2, (w & 0x00f000f0u) | 0x64006400u), sixteenth, high);
-    f[2 * t] = p[0];
-    f[2 * t + 1] = p[1];
-    f[2 * t + 2] = q[0];
-    f[2 * t + 3] = q[1];
+// The constants of decode in registers: as literals each pair would take two
+// instructions (and, or) where one has three operands.
+struct Decoder {
+  uint32_t low = 0x000f000fu, high = 0x00f000f0u, base = 0x64006400u;
+  __device__ __forceinline__ Decoder() {
+    asm("" : "+s"(low));
+    asm("" : "+s"(high));
+    asm("" : "+v"(base));
   }
-  return f;
-}
+  // Codes of a word as f16 of code - 8: f[2t], f[2t + 1] from nibble t.
+  __device__ __forceinline__ half8 operator()(uint32_t word) const {
+    const half2 minus_1032 = (half2)(_Float16)-1032.0f, minus_72 = (half2)(_Float16)-72.0f;
+    half8 f;
+#pragma unroll
+    for (int t = 0; t < 4; t += 2) {
+      const uint32_t w = word >> (4 * t);
+      const half2 p = __builtin_bit_cast(half2, (w & low) | base) + minus_1032;
+      const half2 q = __builtin_elementwise_fma(__builtin_bit_cast(half2, (w & high) | base),
+                                                (half2)(_Float16)0.0625f, minus_72);
+      f[2 * t] = p[0];
+      f[2 * t + 1] = p[1];
+      f[2 * t + 2] = q[0];
+      f[2 * t + 3] = q[1];
+    }
+    return f;
+  }
+};
 
-// Eight elements of a row of `a` from k on, zero from K on.
+// 16 bytes of a row of `a`.
 template <typename T>
-__device__ __forceinline__ void load_row(const T* row, uint32_t k, uint32_t inner, bool wide, T (&dst)[8]) {
-  if (wide && k + 8u <= inner) {
-    typedef T V __attribute__((ext_vector_type(16 / sizeof(T))));
-    constexpr int N = 16 / sizeof(T);
+struct Chunk {
+  static constexpr int N = 16 / sizeof(T);
+  typedef T V __attribute__((ext_vector_type(N)));
+  V v;
+  typedef T U __attribute__((ext_vector_type(N), aligned(sizeof(T))));  // at any address of an element
+  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const U*>(p); }
+  // p[0] is element k of a row; what lies from K on is zero.
+  __device__ __forceinline__ void load(const T* p, uint32_t k, uint32_t inner) {
+    if (k + N <= inner) {
+      load(p);
+    } else {
 #pragma unroll
-    for (int p = 0; p < 8 / N; ++p) {
-      const V v = *reinterpret_cast<const V*>(row + k + N * p);
-#pragma unroll
-      for (int c = 0; c < N; ++c) dst[N * p + c] = v[c];
+      for (int j = 0; j < N; ++j) v[j] = k + j < inner ? p[j] : (T)0.0f;
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) dst[j] = k + j < inner ? row[k + j] : (T)0.0f;
   }
+};
+
+// Eight elements of a row in k order: a lane's operand of 32 k.
+template <typename T>
+struct Fragment {
+  Chunk<T> c[8 / Chunk<T>::N];
+};
+
+// acc += a . b over 32 k.
+__device__ __forceinline__ void multiply(const Fragment<_Float16>& a, const half8& b, floatx4& acc) {
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.c[0].v, b, acc, 0, 0, 0);
+}
+__device__ __forceinline__ void multiply(const Fragment<float>& a, const half8& b, floatx4& acc) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.c[j / 4].v[j % 4], (float)b[j], acc, 0, 0, 0);
 }
 
-// One workgroup: 16 rows x 16 columns, its wavefronts every kWaves-th block.
-template <typename T, int PER>
-__global__ __launch_bounds__(64 * kWaves) void q4_kernel(Q4Args args, bool wide) {
-  __shared__ float partial[kWaves][16][17];
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  const uint32_t column = lane & 15u, quad = lane >> 4;
-  const uint32_t nb = blockIdx.x, m0 = blockIdx.y * 16u;
-  const uint32_t kblocks = (args.inner + 127u) / 128u;
-  const T* row = static_cast<const T*>(args.a) + (uint64_t)min(m0 + column, args.rows - 1u) * args.a_stride;
-  floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (uint32_t kb = wave; kb < kblocks; kb += kWaves) {
-    const uint64_t block = (uint64_t)nb * kblocks + kb;
-    const uint4 words = args.codes[block * 64u + lane];
-    const uint32_t w[4] = {words.x, words.y, words.z, words.w};
-    floatx4 part = {0.0f, 0.0f, 0.0f, 0.0f}, sums = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      T a[8];
-      load_row(row, kb * 128u + 32u * i + 8u * quad, args.inner, wide, a);
-      const half8 b = decode(w[i]);
-      if constexpr (sizeof(T) == 2) {
-        half8 av, one;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          av[j] = a[j];
-          one[j] = (_Float16)1.0f;
-        }
-        part = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, b, part, 0, 0, 0);
-        if (args.offsets) sums = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, one, sums, 0, 0, 0);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          part = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], (float)b[j], part, 0, 0, 0);
-          if (args.offsets) sums = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], 1.0f, sums, 0, 0, 0);
-        }
-      }
-      if ((i + 1) % (4 / PER) == 0) {  // the end of a group, or of the block
-        const uint64_t at = (block * 16u + column) * PER + i / (4 / PER);
-        const float scale = (float)static_cast<const T*>(args.scales)[at];
-        const float offset = args.offsets ? (float)static_cast<const T*>(args.offsets)[at] : 0.0f;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          acc[r] = __builtin_fmaf(part[r], scale, acc[r]);
-          if (args.offsets) acc[r] = __builtin_fmaf(sums[r], offset, acc[r]);
-          part[r] = sums[r] = 0.0f;
-        }
-      }
-    }
-  }
-#pragma unroll
-  for (int r = 0; r < 4; ++r) partial[wave][4 * quad + r][column] = acc[r];
-  __syncthreads();
-  const uint32_t m = m0 + threadIdx.x / 16u, n = nb * 16u + threadIdx.x % 16u;
-  if (m >= args.rows || n >= args.columns) return;
-  float v = 0.0f;
-#pragma unroll
-  for (int p = 0; p < kWaves; ++p) v += partial[p][threadIdx.x / 16u][threadIdx.x % 16u];
+// The activation of one output.
+__device__ __forceinline__ float activate(int activation, float v) {
+  if (activation == kActSilu) return v * __builtin_amdgcn_rcpf(1.0f + __expf(-v));
+  if (activation == kActRelu) return v > 0.0f ? v : (v != v ? v : 0.0f);
+  return v;
+}
+
+// bias, activation and residual of one output, stored.
+template <typename T>
+__device__ __forceinline__ void finish(const Q4Args& args, uint32_t m, uint32_t n, float v) {
   if (args.bias) v += args.bias[n];
-  if (args.activation == kActSilu) v = v / (1.0f + __expf(-v));
-  else if (args.activation == kActRelu) v = v > 0.0f ? v : (v != v ? v : 0.0f);
+  v = activate(args.activation, v);
   if (args.residual)
     v = __builtin_fmaf(args.residual_scale, v,
                        (float)static_cast<const T*>(args.residual)[(uint64_t)m * args.residual_stride + n]);
   static_cast<T*>(args.out)[(uint64_t)m * args.out_stride + n] = (T)v;
+}
+
+// The same for 8 columns from n on, those behind the edge left out.
+__device__ __forceinline__ void finish_row(const Q4Args& args, uint32_t m, uint32_t n, float (&v)[8]) {
+  typedef float F __attribute__((ext_vector_type(4), aligned(4)));
+  if (n + 8u > args.columns) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (n + j < args.columns) finish<_Float16>(args, m, n + j, v[j]);
+    return;
+  }
+  if (args.bias) {
+    const F lo = *reinterpret_cast<const F*>(args.bias + n), hi = *reinterpret_cast<const F*>(args.bias + n + 4u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += j < 4 ? lo[j] : hi[j - 4];
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = activate(args.activation, v[j]);
+  Chunk<_Float16> x;
+  if (args.residual) {
+    x.load(static_cast<const _Float16*>(args.residual) + (uint64_t)m * args.residual_stride + n);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __builtin_fmaf(args.residual_scale, v[j], (float)x.v[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x.v[j] = (_Float16)v[j];
+  *reinterpret_cast<Chunk<_Float16>::U*>(static_cast<_Float16*>(args.out) + (uint64_t)m * args.out_stride + n) = x.v;
+}
+
+// LDS bytes of the rows of `a` in a panel kernel.
+constexpr uint32_t kPanelBytes = 80u * 1024u;
+// Elements from row to row of the panel: whole blocks of K and 16 bytes, so
+// that the rows of a fragment lie in different banks.
+template <typename T>
+__host__ __device__ constexpr uint32_t panel_stride(uint32_t inner) {
+  return (inner + 127u) / 128u * 128u + 16u / sizeof(T);
+}
+
+// Copies all rows of `a` into LDS, zeros behind K, four chunks a thread at a
+// time.
+template <typename T>
+__device__ __forceinline__ void copy_panel(const Q4Args& args, void* lds) {
+  constexpr uint32_t kChunks = 128u / Chunk<T>::N;
+  const uint32_t chunks = (args.inner + 127u) / 128u * kChunks;
+  // Thread and step as rows and chunks; one row needs no division.
+  uint32_t r = 0u, c = threadIdx.x, step_rows = 0u, step = blockDim.x;
+  if (args.rows > 1u) {
+    r = threadIdx.x / chunks;
+    c = threadIdx.x % chunks;
+    step_rows = blockDim.x / chunks;
+    step = blockDim.x % chunks;
+  }
+  while (r < args.rows) {
+    Chunk<T> x[4];
+    uint32_t to[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const bool has = r < args.rows && c < chunks;
+      to[t] = has ? r * panel_stride<T>(args.inner) + c * Chunk<T>::N : ~0u;
+      if (has)
+        x[t].load(static_cast<const T*>(args.a) + r * args.a_stride + c * Chunk<T>::N, c * Chunk<T>::N, args.inner);
+      r += step_rows;
+      c += step;
+      if (c >= chunks) {
+        c -= min(c, chunks);
+        ++r;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      if (to[t] != ~0u) *reinterpret_cast<Chunk<T>*>(static_cast<T*>(lds) + to[t]) = x[t];
+  }
+}
+
+// Wavefronts of a workgroup: as many as have registers for what they hold.
+template <typename T, int MT, int NT, bool PANEL>
+__host__ __device__ constexpr int most_waves() {
+  return MT * NT >= 4 || (sizeof(T) == 4 && !PANEL) ? 8 : 16;
+}
+
+// Few rows. One workgroup: up to 16 MT rows x 16 NT columns; its wavefronts
+// take every W-th block of K and their sums meet in LDS, so no memory is
+// shared between workgroups. Codes and scales are loaded two blocks ahead.
+// Fragments are read from LDS, since loaded as they are the lanes of one
+// instruction touch 16 rows four times over: PANEL copies the rows whole
+// before the first block, otherwise each wavefront copies its own block of
+// 128 k, loaded a block ahead, through an area of its own.
+template <typename T, int PER, int MT, int NT, bool OFFSETS, bool PANEL>
+__global__ __launch_bounds__((64 * most_waves<T, MT, NT, PANEL>())) void q4_rows_kernel(Q4Args args) {
+  constexpr int kMost = most_waves<T, MT, NT, PANEL>();
+  constexpr int kStep = 4 / PER;           // matrix instructions of a group
+  constexpr int kChunks = 128 / Chunk<T>::N;        // of a row and block
+  constexpr int kStage = 16 * MT * kChunks;         // of a wavefront's area
+  constexpr int kCopies = kStage / 64;              // chunks a lane copies
+  constexpr uint32_t kRowsBytes = PANEL ? kPanelBytes : kMost * kStage * 16u;
+  constexpr uint32_t kSumsBytes = kMost * 16 * MT * (16 * NT + 1) * 4u;
+  __shared__ uint4 lds[(kRowsBytes > kSumsBytes ? kRowsBytes : kSumsBytes) / 16u];
+  const uint32_t lane = threadIdx.x & 63u, waves = blockDim.x >> 6;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));  // addresses stay scalar
+  const uint32_t column = lane & 15u, quad = lane >> 4;
+  const uint32_t m0 = blockIdx.y * (16u * MT);
+  const uint32_t kblocks = (args.inner + 127u) / 128u, nblocks = (args.columns + 15u) / 16u;
+  typedef T S __attribute__((ext_vector_type(PER == 1 ? 2 : PER)));  // a column's scales of a block
+
+  uint64_t base[NT];  // first block of each column block (the last one again behind the edge)
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) base[nt] = (uint64_t)min(blockIdx.x * NT + nt, nblocks - 1u) * kblocks;
+  struct Weight {
+    uint4 codes[NT];
+    S scales[NT], offsets[NT];
+  };
+  const auto load_weight = [&](uint32_t kb, Weight& w) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const uint64_t block = base[nt] + kb;
+      w.codes[nt] = (args.codes + block * 64u)[lane];
+      const T* scales = static_cast<const T*>(args.scales) + block * (16u * PER);
+      const T* offsets = static_cast<const T*>(args.offsets) + block * (16u * PER);
+      if constexpr (PER == 1) {
+        w.scales[nt][0] = scales[column];
+        if (OFFSETS) w.offsets[nt][0] = offsets[column];
+      } else {
+        w.scales[nt] = reinterpret_cast<const S*>(scales)[column];
+        if (OFFSETS) w.offsets[nt] = reinterpret_cast<const S*>(offsets)[column];
+      }
+    }
+  };
+
+  // A wavefront's block of rows: chunk c of row r lies at c ^ (r & 15), which
+  // spreads the 16 rows of a fragment over the banks.
+  Chunk<T>* stage = reinterpret_cast<Chunk<T>*>(lds) + (PANEL ? 0 : wave * kStage);
+  Chunk<T> copy[PANEL ? 1 : kCopies];
+  const T* tile = static_cast<const T*>(args.a) + (uint64_t)m0 * args.a_stride;
+  uint32_t from[PANEL ? 1 : kCopies];  // of a chunk in the tile's rows, in elements from the block's first
+  if constexpr (!PANEL)
+#pragma unroll
+    for (int t = 0; t < kCopies; ++t) {
+      const uint32_t id = t * 64u + lane, r = id / kChunks, c = (id % kChunks) ^ (r & 15u);
+      from[t] = (min(m0 + r, args.rows - 1u) - m0) * (uint32_t)args.a_stride + c * Chunk<T>::N;
+    }
+  const auto load_rows = [&](uint32_t kb) {
+    const T* block = tile + kb * 128u;
+    if (kb * 128u + 128u <= args.inner) {
+#pragma unroll
+      for (int t = 0; t < kCopies; ++t) copy[t].load(block + from[t]);
+    } else {
+#pragma unroll
+      for (int t = 0; t < kCopies; ++t) {
+        const uint32_t id = t * 64u + lane, c = (id % kChunks) ^ ((id / kChunks) & 15u);
+        copy[t].load(block + from[t], kb * 128u + c * Chunk<T>::N, args.inner);
+      }
+    }
+  };
+  // Fragment of the 16 rows mt, step i of block kb.
+  const auto fragment = [&](uint32_t kb, int i, int mt) {
+    Fragment<T> f;
+    constexpr int kParts = 8 / Chunk<T>::N;
+#pragma unroll
+    for (int p = 0; p < kParts; ++p) {
+      if constexpr (PANEL) {
+        const uint32_t r = min(column, args.rows - 1u);
+        f.c[p] = *reinterpret_cast<const Chunk<T>*>(reinterpret_cast<const T*>(lds) + r * panel_stride<T>(args.inner) +
+                                                    kb * 128u + 32u * i + 8u * quad + p * Chunk<T>::N);
+      } else {
+        const uint32_t r = 16u * mt + column, c = (4u * i + quad) * kParts + p;
+        f.c[p] = stage[r * kChunks + (c ^ (r & 15u))];
+      }
+    }
+    return f;
+  };
+
+  // Workgroups of an XCD (every eighth) start at different blocks of K, so
+  // that they do not all ask its L2 for the same lines: 3% to 8% at 16 to 64
+  // rows of 4096 and 8192.
+  const uint32_t shift = PANEL ? 0u : (blockIdx.x >> 3) % kblocks;
+  const auto turned = [&](uint32_t kb) { return kb + shift < kblocks ? kb + shift : kb + shift - kblocks; };
+  Weight ahead[2];
+  if constexpr (PANEL) {
+    copy_panel<T>(args, lds);  // m0 is 0: a panel has at most 16 rows
+  } else {
+    if (wave < kblocks) load_rows(turned(wave));
+  }
+  if (wave < kblocks) load_weight(turned(wave), ahead[0]);
+  if (wave + waves < kblocks) load_weight(turned(wave + waves), ahead[1]);
+  if constexpr (PANEL) __syncthreads();
+
+  floatx4 acc[MT][NT], part[MT][NT], sums[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = (floatx4)0.0f;
+  const half8 one = (half8)(_Float16)1.0f;
+  const Decoder decode;
+
+  for (uint32_t kb = wave; kb < kblocks; kb += waves) {
+    const Weight w = ahead[0];
+    ahead[0] = ahead[1];
+    if (kb + 2u * waves < kblocks) load_weight(turned(kb + 2u * waves), ahead[1]);
+    if constexpr (!PANEL) {
+#pragma unroll
+      for (int t = 0; t < kCopies; ++t) stage[t * 64u + lane] = copy[t];
+      if (kb + waves < kblocks) load_rows(turned(kb + waves));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      Fragment<T> a[MT];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) a[mt] = fragment(kb, i, mt);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const half8 b = decode(reinterpret_cast<const uint32_t(&)[4]>(w.codes[nt])[i]);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          if (i % kStep == 0) part[mt][nt] = (floatx4)0.0f;  // the first of a group adds to the constant
+          multiply(a[mt], b, part[mt][nt]);
+        }
+      }
+      if constexpr (OFFSETS)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          if (i % kStep == 0) sums[mt] = (floatx4)0.0f;
+          multiply(a[mt], one, sums[mt]);
+        }
+      if ((i + 1) % kStep == 0) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              acc[mt][nt][r] = __builtin_fmaf(part[mt][nt][r], (float)w.scales[nt][i / kStep], acc[mt][nt][r]);
+              if (OFFSETS)
+                acc[mt][nt][r] = __builtin_fmaf(sums[mt][r], (float)w.offsets[nt][i / kStep], acc[mt][nt][r]);
+            }
+        }
+      }
+    }
+  }
+  float* partial = reinterpret_cast<float*>(lds);  // [waves][16 MT][16 NT + 1]
+  constexpr int kWidth = 16 * NT + 1;
+  __syncthreads();  // every wavefront has read its rows
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        partial[(wave * 16u * MT + 16 * mt + 4 * quad + r) * kWidth + 16 * nt + column] = acc[mt][nt][r];
+  __syncthreads();
+  const uint32_t outputs = min(args.rows - m0, 16u * MT) * (16u * NT);
+  for (uint32_t id = threadIdx.x; id < outputs; id += blockDim.x) {
+    const uint32_t m = id / (16u * NT), n = id % (16u * NT);
+    if (blockIdx.x * (16u * NT) + n >= args.columns) continue;
+    float v = 0.0f;
+#pragma unroll 4
+    for (uint32_t w = 0; w < waves; ++w) v += partial[(w * 16u * MT + m) * kWidth + n];
+    finish<T>(args, m0 + m, blockIdx.x * (16u * NT) + n, v);
+  }
+}
+
+// One to four f32 rows on the VALU: a matrix instruction of f32 operands takes
+// 32 cycles for 4 k whatever the rows, an fma that reads its weight as f16
+// (v_fma_mix_f32) 4 for each row. The rows lie in LDS whole, a lane
+// multiplies the codes of its column and quarter of 32 k, and the quarters
+// and wavefronts meet at the end.
+template <int PER, int ROWS, bool OFFSETS>
+__global__ __launch_bounds__(1024) void q4_vector_kernel(Q4Args args) {
+  constexpr int kStep = 4 / PER;
+  __shared__ uint4 lds[kPanelBytes / 16u];
+  const uint32_t lane = threadIdx.x & 63u, waves = blockDim.x >> 6;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t column = lane & 15u, quad = lane >> 4;
+  const uint32_t kblocks = (args.inner + 127u) / 128u;
+  const uint64_t base = (uint64_t)blockIdx.x * kblocks;
+  const uint32_t stride = panel_stride<float>(args.inner);
+  typedef float S __attribute__((ext_vector_type(PER == 1 ? 2 : PER)));
+  struct Weight {
+    uint4 codes;
+    S scales, offsets;
+  };
+  const auto load_weight = [&](uint32_t kb, Weight& w) {
+    w.codes = (args.codes + (base + kb) * 64u)[lane];
+    const float* scales = static_cast<const float*>(args.scales) + (base + kb) * (16u * PER);
+    const float* offsets = static_cast<const float*>(args.offsets) + (base + kb) * (16u * PER);
+    if constexpr (PER == 1) {
+      w.scales[0] = scales[column];
+      if (OFFSETS) w.offsets[0] = offsets[column];
+    } else {
+      w.scales = reinterpret_cast<const S*>(scales)[column];
+      if (OFFSETS) w.offsets = reinterpret_cast<const S*>(offsets)[column];
+    }
+  };
+  copy_panel<float>(args, lds);
+  Weight ahead[2];
+  if (wave < kblocks) load_weight(wave, ahead[0]);
+  if (wave + waves < kblocks) load_weight(wave + waves, ahead[1]);
+  __syncthreads();
+
+  const Decoder decode;
+  const float* rows = reinterpret_cast<const float*>(lds) + 8u * quad;
+  float acc[ROWS] = {}, part[ROWS], sums[ROWS];
+  for (uint32_t kb = wave; kb < kblocks; kb += waves) {
+    const Weight w = ahead[0];
+    ahead[0] = ahead[1];
+    if (kb + 2u * waves < kblocks) load_weight(kb + 2u * waves, ahead[1]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const half8 b = decode(reinterpret_cast<const uint32_t(&)[4]>(w.codes)[i]);
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        const Chunk<float>* from = reinterpret_cast<const Chunk<float>*>(
+            rows + min((uint32_t)r, args.rows - 1u) * stride + kb * 128u + 32u * i);
+        const Chunk<float> a[2] = {from[0], from[1]};
+        if (i % kStep == 0) part[r] = sums[r] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          part[r] = __builtin_fmaf(a[j / 4].v[j % 4], (float)b[j], part[r]);
+          if (OFFSETS) sums[r] += a[j / 4].v[j % 4];
+        }
+        if ((i + 1) % kStep == 0) {
+          acc[r] = __builtin_fmaf(part[r], w.scales[i / kStep], acc[r]);
+          if (OFFSETS) acc[r] = __builtin_fmaf(sums[r], w.offsets[i / kStep], acc[r]);
+        }
+      }
+    }
+  }
+  float* partial = reinterpret_cast<float*>(lds);  // [waves][ROWS][16]
+  __syncthreads();                                 // every wavefront has read its rows
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    acc[r] += __shfl_xor(acc[r], 16, 64);
+    acc[r] += __shfl_xor(acc[r], 32, 64);
+    if (quad == 0) partial[(wave * ROWS + r) * 16u + column] = acc[r];
+  }
+  __syncthreads();
+  for (uint32_t id = threadIdx.x; id < args.rows * 16u; id += blockDim.x) {
+    const uint32_t m = id / 16u, n = blockIdx.x * 16u + id % 16u;
+    if (n >= args.columns) continue;
+    float v = 0.0f;
+#pragma unroll 4
+    for (uint32_t w = 0; w < waves; ++w) v += partial[(w * ROWS + m) * 16u + id % 16u];
+    finish<float>(args, m, n, v);
+  }
+}
+
+// Many rows, f16. One workgroup: 64 rows x 128 columns, a wavefront 32 of the
+// columns. The rows go through LDS, a block of 128 k at a time in two
+// buffers; codes go from memory to registers, where each wavefront makes its
+// own operands of them: 9 VALU operations per 4 matrix instructions, beside
+// the 16 that a group's scales take for each 16 columns.
+constexpr int kTileRows = 64, kTileColumns = 128;
+template <int PER, bool OFFSETS>
+__global__ __launch_bounds__(256, OFFSETS ? 2 : 3) void q4_tile_kernel(Q4Args args) {
+  typedef _Float16 T;
+  constexpr int kStep = 4 / PER;
+  constexpr int kChunks = 16, kCopies = kTileRows * kChunks / 256;
+  constexpr int kWidth = 32 + 4;  // f32 columns of a wavefront's part on its way out
+  typedef T S __attribute__((ext_vector_type(PER == 1 ? 2 : PER)));
+  __shared__ uint4 lds[2][kTileRows * kChunks];
+  static_assert(sizeof(lds) >= 4 * 32 * kWidth * sizeof(float), "the outputs pass through the rows' buffers");
+  const uint32_t lane = threadIdx.x & 63u, column = lane & 15u, quad = lane >> 4;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t kblocks = (args.inner + 127u) / 128u, nblocks = (args.columns + 15u) / 16u;
+  // Workgroups of one XCD (every eighth) take neighbouring tiles of one
+  // column of tiles: its weights stay in their L2.
+  const uint32_t row_tiles = (args.rows + kTileRows - 1u) / kTileRows;
+  const uint32_t id = xcd_local_order(blockIdx.x, gridDim.x);
+  const uint32_t m0 = id % row_tiles * kTileRows, n0 = id / row_tiles * kTileColumns;
+  const uint32_t wn = wave * 32u;
+
+  uint64_t base[2];
+#pragma unroll
+  for (int nt = 0; nt < 2; ++nt) base[nt] = (uint64_t)min((n0 + wn) / 16u + nt, nblocks - 1u) * kblocks;
+  struct Weight {
+    uint4 codes[2];
+    S scales[2], offsets[2];
+  };
+  const auto load_weight = [&](uint32_t kb, Weight& w) {
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+      const uint64_t block = base[nt] + kb;
+      w.codes[nt] = (args.codes + block * 64u)[lane];
+      const T* scales = static_cast<const T*>(args.scales) + block * (16u * PER);
+      const T* offsets = static_cast<const T*>(args.offsets) + block * (16u * PER);
+      if constexpr (PER == 1) {
+        w.scales[nt][0] = scales[column];
+        if (OFFSETS) w.offsets[nt][0] = offsets[column];
+      } else {
+        w.scales[nt] = reinterpret_cast<const S*>(scales)[column];
+        if (OFFSETS) w.offsets[nt] = reinterpret_cast<const S*>(offsets)[column];
+      }
+    }
+  };
+  const T* tile = static_cast<const T*>(args.a) + (uint64_t)m0 * args.a_stride;
+  uint32_t from[kCopies];
+#pragma unroll
+  for (int t = 0; t < kCopies; ++t) {
+    const uint32_t at = t * 256u + threadIdx.x, r = at / kChunks, c = (at % kChunks) ^ (r & 15u);
+    from[t] = (min(m0 + r, args.rows - 1u) - m0) * (uint32_t)args.a_stride + c * 8u;
+  }
+  Chunk<T> copy[kCopies];
+  const auto load_rows = [&](uint32_t kb) {
+    const T* block = tile + kb * 128u;
+#pragma unroll
+    for (int t = 0; t < kCopies; ++t) copy[t].load(block + from[t]);
+  };
+  const auto load_last_rows = [&](uint32_t kb) {  // K ends within this block
+    const T* block = tile + kb * 128u;
+#pragma unroll
+    for (int t = 0; t < kCopies; ++t) {
+      const uint32_t at = t * 256u + threadIdx.x, c = (at % kChunks) ^ ((at / kChunks) & 15u);
+      copy[t].load(block + from[t], kb * 128u + c * 8u, args.inner);
+    }
+  };
+  const auto store_rows = [&](int buffer) {
+#pragma unroll
+    for (int t = 0; t < kCopies; ++t) reinterpret_cast<Chunk<T>*>(lds[buffer])[t * 256u + threadIdx.x] = copy[t];
+  };
+
+  const half8 one = (half8)(_Float16)1.0f;
+  const Decoder decode;
+  floatx4 acc[4][2];
+#pragma unroll
+  for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) acc[mt][nt] = (floatx4)0.0f;
+
+  const auto multiply_block = [&](uint32_t kb, const Weight& w) {
+    const Chunk<T>* rows = reinterpret_cast<const Chunk<T>*>(lds[kb & 1u]);
+    floatx4 part[4][2], sums[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      Fragment<T> a[4];
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        const uint32_t r = 16u * mt + column;
+        a[mt].c[0] = rows[r * kChunks + ((4u * i + quad) ^ column)];
+      }
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        const half8 b = decode(reinterpret_cast<const uint32_t(&)[4]>(w.codes[nt])[i]);
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+          if (i % kStep == 0) part[mt][nt] = (floatx4)0.0f;
+          multiply(a[mt], b, part[mt][nt]);
+        }
+      }
+      if constexpr (OFFSETS)
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+          if (i % kStep == 0) sums[mt] = (floatx4)0.0f;
+          multiply(a[mt], one, sums[mt]);
+        }
+      if ((i + 1) % kStep == 0) {
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              acc[mt][nt][r] = __builtin_fmaf(part[mt][nt][r], (float)w.scales[nt][i / kStep], acc[mt][nt][r]);
+              if (OFFSETS)
+                acc[mt][nt][r] = __builtin_fmaf(sums[mt][r], (float)w.offsets[nt][i / kStep], acc[mt][nt][r]);
+            }
+      }
+      __builtin_amdgcn_sched_barrier(0);  // one step's operands at a time in registers
+    }
+  };
+  // Whole blocks, the next one's loads under way while one is multiplied,
+  // then the block that K ends in.
+  const uint32_t whole = args.inner / 128u;
+  Weight w, next;
+  load_weight(0, w);
+  if (whole) load_rows(0);
+  else load_last_rows(0);
+  store_rows(0);
+  __syncthreads();
+  for (uint32_t kb = 0; kb + 1u < whole; ++kb) {
+    load_rows(kb + 1u);
+    load_weight(kb + 1u, next);
+    multiply_block(kb, w);
+    store_rows((kb + 1u) & 1u);
+    w = next;
+    __syncthreads();
+  }
+  if (whole && kblocks > whole) {
+    load_last_rows(whole);
+    load_weight(whole, next);
+    multiply_block(whole - 1u, w);
+    store_rows(whole & 1u);
+    w = next;
+    __syncthreads();
+  }
+  multiply_block(kblocks - 1u, w);
+  __syncthreads();
+
+  // Out through LDS, 32 rows at a time, so that a lane stores 8 columns.
+  float* part_out = reinterpret_cast<float*>(lds) + wave * (32 * kWidth);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          part_out[(16 * mt + 4 * quad + r) * kWidth + 16 * nt + column] = acc[2 * half + mt][nt][r];
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {
+      const uint32_t r = 16u * pass + (lane >> 2), c = 8u * (lane & 3u);
+      const uint32_t m = m0 + 32u * half + r, n = n0 + wn + c;
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = part_out[r * kWidth + c + j];
+      if (m < args.rows) finish_row(args, m, n, v);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+typedef void (*Kernel)(Q4Args);
+// The instantiation of a kernel template for a weight.
+#define PK_Q4_PICK(args, KERNEL)                                                                            \
+  ((args).offsets ? ((args).per_block == 1u ? KERNEL(1, true) : (args).per_block == 2u ? KERNEL(2, true)    \
+                                                                                        : KERNEL(4, true))  \
+                  : ((args).per_block == 1u ? KERNEL(1, false) : (args).per_block == 2u ? KERNEL(2, false)  \
+                                                                                         : KERNEL(4, false)))
+template <typename T, int MT, int NT, bool PANEL>
+Kernel pick_rows(const Q4Args& args) {
+#define PK_Q4_ROWS(PER, OFFSETS) q4_rows_kernel<T, PER, MT, NT, OFFSETS, PANEL>
+  return PK_Q4_PICK(args, PK_Q4_ROWS);
+#undef PK_Q4_ROWS
+}
+template <int ROWS>
+Kernel pick_vector(const Q4Args& args) {
+#define PK_Q4_VECTOR(PER, OFFSETS) q4_vector_kernel<PER, ROWS, OFFSETS>
+  return PK_Q4_PICK(args, PK_Q4_VECTOR);
+#undef PK_Q4_VECTOR
+}
+Kernel pick_tile(const Q4Args& args) {
+#define PK_Q4_TILE(PER, OFFSETS) q4_tile_kernel<PER, OFFSETS>
+  return PK_Q4_PICK(args, PK_Q4_TILE);
+#undef PK_Q4_TILE
+}
+
+// A launch: kernel, grid and threads.
+struct Q4Plan {
+  Kernel kernel;
+  dim3 grid;
+  uint32_t threads;
+};
+Q4Plan plan(const Q4Args& args) {
+  const auto tiles = [](uint32_t n, uint32_t size) { return (n + size - 1u) / size; };
+  const uint32_t kblocks = tiles(args.inner, 128u), nblocks = tiles(args.columns, 16u);
+  const auto threads = [&](uint32_t most) { return 64u * (kblocks < most ? kblocks : most); };
+  // Wavefronts of the kernels with the rows in LDS: two blocks of K each,
+  // from 4 (1 x 640 x 1032 3.2 us, 3.6 with one block each) to `most`.
+  const auto panel_threads = [&](uint32_t most) {
+    const uint32_t two = kblocks / 2u < 4u ? 4u : kblocks / 2u;
+    return threads(two < most ? two : most);
+  };
+  const uint64_t row_bytes =
+      args.f16 ? panel_stride<_Float16>(args.inner) * 2ull : panel_stride<float>(args.inner) * 4ull;
+  const bool panel = args.rows <= 16u && args.rows * row_bytes <= kPanelBytes;
+  if (!args.f16) {
+    // 1 x 4096 x 4096: 4.2 us on the VALU, 8.1 on the matrix units; 4 rows 7.8 and 9.5.
+    if (panel && args.rows <= 4u)
+      return {args.rows == 1u ? pick_vector<1>(args) : args.rows == 2u ? pick_vector<2>(args) : pick_vector<4>(args),
+              dim3(nblocks), panel_threads(16u)};
+    if (panel) return {pick_rows<float, 1, 1, true>(args), dim3(nblocks), panel_threads(16u)};
+    return {pick_rows<float, 1, 1, false>(args), dim3(nblocks, tiles(args.rows, 16u)), threads(8u)};
+  }
+  // The tiles need the compute units full: 192 tiles (1504 x 4096 x 1024) take
+  // 28.0 us and rows 34.0, 128 tiles (256 x 1024 x 4096 and x 4096) 9.7 and
+  // 27.5, and rows 10.6 and 24.
+  const uint64_t tiled = (uint64_t)tiles(args.rows, kTileRows) * tiles(args.columns, kTileColumns);
+  if (args.rows > 64u && tiled >= 160u) return {pick_tile(args), dim3((uint32_t)tiled), 256u};
+  // 8 wavefronts (1 x 8192 x 8192 8.3 us, 16 8.8; 8 x 2048 x 8192 4.5 and 5.2).
+  if (panel) return {pick_rows<_Float16, 1, 1, true>(args), dim3(nblocks), panel_threads(8u)};
+  // Two column blocks a wavefront, which share the rows' reads, where a
+  // workgroup for each compute unit is left: 32 x 4096 x 8192 9.2 us (one:
+  // 12.6), but 32 x 4096 x 4096, where half would be left, 8.0 (one: 7.0).
+  const uint32_t mt = args.rows <= 16u ? 1u : args.rows <= 32u ? 2u : 4u, row_tiles = tiles(args.rows, 16u * mt);
+  const bool two = (uint64_t)tiles(nblocks, 2u) * row_tiles >= 256u;
+  const dim3 grid(two ? tiles(nblocks, 2u) : nblocks, row_tiles);
+  if (mt == 1u)
+    return {two ? pick_rows<_Float16, 1, 2, false>(args) : pick_rows<_Float16, 1, 1, false>(args), grid, threads(16u)};
+  if (mt == 2u)
+    return {two ? pick_rows<_Float16, 2, 2, false>(args) : pick_rows<_Float16, 2, 1, false>(args), grid,
+            threads(two ? 8u : 16u)};
+  return {two ? pick_rows<_Float16, 4, 2, false>(args) : pick_rows<_Float16, 4, 1, false>(args), grid, threads(8u)};
 }
 
 }  // namespace
@@ -200,18 +771,11 @@ hipError_t launch_q4_layout(const Q4Args& args, const uint32_t* packed, const vo
 }
 
 hipError_t launch_q4(const Q4Args& args, hipStream_t stream, hipEvent_t start, hipEvent_t stop) {
-  typedef void (*Kernel)(Q4Args, bool);
-  static const Kernel kernels[2][3] = {
-      {q4_kernel<float, 1>, q4_kernel<float, 2>, q4_kernel<float, 4>},
-      {q4_kernel<_Float16, 1>, q4_kernel<_Float16, 2>, q4_kernel<_Float16, 4>}};
-  const Kernel kernel = kernels[args.f16][args.per_block >> 1];
-  const uint64_t elem = args.f16 ? 2u : 4u;
-  const bool wide = (reinterpret_cast<uintptr_t>(args.a) | args.a_stride * elem) % 16u == 0;
-  const dim3 grid((args.columns + 15u) / 16u, (args.rows + 15u) / 16u);
+  const Q4Plan p = plan(args);
   if (start || stop)
-    hipExtLaunchKernelGGL(kernel, grid, dim3(64 * kWaves), 0, stream, start, stop, 0, args, wide);
+    hipExtLaunchKernelGGL(p.kernel, p.grid, dim3(p.threads), 0, stream, start, stop, 0, args);
   else
-    hipLaunchKernelGGL(kernel, grid, dim3(64 * kWaves), 0, stream, args, wide);
+    hipLaunchKernelGGL(p.kernel, p.grid, dim3(p.threads), 0, stream, args);
   return hipGetLastError();
 }
 

@@ -37,6 +37,9 @@ int validate_q4(const pk_q4_desc* d) {
   const uint64_t blocks = (((uint64_t)d->inner + 127u) / 128u) * (((uint64_t)d->columns + 15u) / 16u);
   if (d->rows == 0 || d->inner == 0 || d->columns == 0 || d->rows > PK_Q4_MAX_ROWS || blocks >= 1u << 24)
     return fail(PK_RANGE_ERROR, "Invalid q4 shape [%u, %u, %u] for %s", d->rows, d->inner, d->columns, label);
+  // Offsets into a tile of rows are 32 bits.
+  if (d->inner > PK_Q4_MAX_STRIDE || d->a_stride > PK_Q4_MAX_STRIDE)
+    return fail(PK_RANGE_ERROR, "%s inner and a stride must be at most %u", label, PK_Q4_MAX_STRIDE);
   if (d->group_size && (d->group_size < 32u || (d->group_size & (d->group_size - 1u)) != 0))
     return fail(PK_RANGE_ERROR, "%s group size must be a power of two from 32 on, or 0", label);
   if (d->activation < PK_ACTIVATION_NONE || d->activation > PK_ACTIVATION_RELU)

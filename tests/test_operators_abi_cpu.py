@@ -137,6 +137,7 @@ def test_q4_accepts(abi):
     (dict(rows=0), "PaletteRangeError", "Invalid q4 shape [0, 64, 40] for head"),
     (dict(rows=1048561), "PaletteRangeError", "Invalid q4 shape"),
     (dict(inner=1 << 20, columns=1 << 20), "PaletteRangeError", "Invalid q4 shape"),
+    (dict(a_stride=16777217), "PaletteRangeError", "head inner and a stride must be at most 16777216"),
     (dict(group_size=16), "PaletteRangeError", "head group size must be a power of two from 32 on, or 0"),
     (dict(group_size=96), "PaletteRangeError", "head group size must be a power of two from 32 on, or 0"),
     (dict(residual_scale=float("nan")), "PaletteError", "head residual scale must be finite"),
