@@ -3,8 +3,9 @@
  * (include/pk_palette.h), the fused Conformer convolution tail
  * (include/pk_conv.h), the relative-position attention
  * (include/pk_attention.h), the row LayerNorm (include/pk_layernorm.h), the
- * subsampling convolutions (include/pk_subsampling.h) and the encoder graph
- * (include/pk_encoder.h). It is the thin native layer under the JavaScript
+ * subsampling convolutions (include/pk_subsampling.h), the encoder graph
+ * (include/pk_encoder.h), the norms around a block (include/pk_block_norm.h),
+ * the 4-bit product (include/pk_q4.h) and token scores (include/pk_score.h). It is the thin native layer under the JavaScript
  * host in ../host: every function forwards to one pk_* call, converts device
  * pointers to BigInt, and turns a failing pk_status into a thrown Error
  * (RangeError for PK_RANGE_ERROR, as the reference throws RangeError for
@@ -24,10 +25,13 @@
 #include <string.h>
 
 #include "pk_attention.h"
+#include "pk_block_norm.h"
 #include "pk_conv.h"
 #include "pk_encoder.h"
 #include "pk_layernorm.h"
 #include "pk_palette.h"
+#include "pk_q4.h"
+#include "pk_score.h"
 #include "pk_subsampling.h"
 #include "pk_tdt.h"
 
@@ -851,6 +855,184 @@ static napi_value js_attention_plan(napi_env env, napi_callback_info info) {
   return obj;
 }
 
+/* ---- block norm, 4-bit product, token scores ------------------------------ */
+
+/* The optional binding `name` with its capacity `nameBytes`. */
+static void prop_binding(napi_env env, napi_value o, const char *name, void *pointer, uint64_t *bytes) {
+  char key[32];
+  uint64_t address = 0;
+  *bytes = 0;
+  if (prop_u64(env, o, name, &address)) {
+    snprintf(key, sizeof key, "%sBytes", name);
+    prop_u64(env, o, key, bytes);
+  }
+  void *p = (void *)(uintptr_t)address;
+  memcpy(pointer, &p, sizeof p);
+}
+
+/* The optional number `name`; *has tells whether it is there. */
+static void prop_float(napi_env env, napi_value o, const char *name, int32_t *has, float *out) {
+  napi_value v;
+  double value = 0;
+  if (!prop(env, o, name, &v) || napi_get_value_double(env, v, &value) != napi_ok) return;
+  *has = 1;
+  *out = (float)value;
+}
+
+/* {label, precision, kind, rows, channels, input, gamma?, beta?, gate?,
+   gateRows?, residual?, residualScale?, output, nextGamma?, nextBeta?,
+   nextOutput?, epsilon?}, each binding with its Bytes and each matrix with
+   an optional Stride */
+static int parse_block_norm_desc(napi_env env, napi_value o, pk_block_norm_desc *d, char **label) {
+  memset(d, 0, sizeof *d);
+  d->struct_size = sizeof *d;
+  *label = NULL;
+  parse_precision(env, o, &d->precision);
+  uint32_t kind = 0;
+  if (!prop_u32(env, o, "rows", &d->rows) || !prop_u32(env, o, "channels", &d->channels) ||
+      !prop_u32(env, o, "kind", &kind)) {
+    bad_argument(env, "block norm descriptor is missing a required field");
+    return 0;
+  }
+  d->kind = (int32_t)kind;
+  prop_binding(env, o, "input", &d->input, &d->input_bytes);
+  prop_u32(env, o, "inputStride", &d->input_stride);
+  prop_binding(env, o, "gamma", &d->gamma, &d->gamma_bytes);
+  prop_binding(env, o, "beta", &d->beta, &d->beta_bytes);
+  prop_binding(env, o, "gate", &d->gate, &d->gate_bytes);
+  prop_u32(env, o, "gateStride", &d->gate_stride);
+  d->gate_rows = 1;
+  prop_u32(env, o, "gateRows", &d->gate_rows);
+  prop_binding(env, o, "residual", &d->residual, &d->residual_bytes);
+  prop_u32(env, o, "residualStride", &d->residual_stride);
+  prop_float(env, o, "residualScale", &d->has_residual_scale, &d->residual_scale);
+  prop_binding(env, o, "output", &d->output, &d->output_bytes);
+  prop_u32(env, o, "outputStride", &d->output_stride);
+  prop_binding(env, o, "nextGamma", &d->next_gamma, &d->next_gamma_bytes);
+  prop_binding(env, o, "nextBeta", &d->next_beta, &d->next_beta_bytes);
+  prop_binding(env, o, "nextOutput", &d->next_output, &d->next_output_bytes);
+  prop_u32(env, o, "nextOutputStride", &d->next_output_stride);
+  prop_float(env, o, "epsilon", &d->has_epsilon, &d->epsilon);
+  *label = prop_string(env, o, "label");
+  d->label = *label;
+  return 1;
+}
+
+/* {label, precision, rows, inner, columns, groupSize, a, packed, scales,
+   offsets?, output, bias?, residual?, residualScale?, activation}, each
+   binding with its Bytes, a, output and residual with an optional Stride */
+static int parse_q4_desc(napi_env env, napi_value o, pk_q4_desc *d, char **label) {
+  memset(d, 0, sizeof *d);
+  d->struct_size = sizeof *d;
+  *label = NULL;
+  parse_precision(env, o, &d->precision);
+  uint32_t activation = 0;
+  if (!prop_u32(env, o, "rows", &d->rows) || !prop_u32(env, o, "inner", &d->inner) ||
+      !prop_u32(env, o, "columns", &d->columns) || !prop_u32(env, o, "groupSize", &d->group_size) ||
+      !prop_u32(env, o, "activation", &activation)) {
+    bad_argument(env, "q4 descriptor is missing a required field");
+    return 0;
+  }
+  d->activation = (int32_t)activation;
+  prop_binding(env, o, "a", &d->a, &d->a_bytes);
+  prop_u32(env, o, "aStride", &d->a_stride);
+  prop_binding(env, o, "packed", &d->packed, &d->packed_bytes);
+  prop_binding(env, o, "scales", &d->scales, &d->scales_bytes);
+  prop_binding(env, o, "offsets", &d->offsets, &d->offsets_bytes);
+  prop_binding(env, o, "output", &d->output, &d->output_bytes);
+  prop_u32(env, o, "outputStride", &d->output_stride);
+  prop_binding(env, o, "bias", &d->bias, &d->bias_bytes);
+  prop_binding(env, o, "residual", &d->residual, &d->residual_bytes);
+  prop_u32(env, o, "residualStride", &d->residual_stride);
+  prop_float(env, o, "residualScale", &d->has_residual_scale, &d->residual_scale);
+  *label = prop_string(env, o, "label");
+  d->label = *label;
+  return 1;
+}
+
+/* {label, precision, rows, columns, rowStride?, logits, temperature?,
+   tokens?, logProbs?, entropies?, alternatives?, topTokens?, topLogProbs?},
+   each binding with its Bytes */
+static int parse_score_desc(napi_env env, napi_value o, pk_score_desc *d, char **label) {
+  memset(d, 0, sizeof *d);
+  d->struct_size = sizeof *d;
+  *label = NULL;
+  parse_precision(env, o, &d->precision);
+  if (!prop_u32(env, o, "rows", &d->rows) || !prop_u32(env, o, "columns", &d->columns)) {
+    bad_argument(env, "token score descriptor is missing a required field");
+    return 0;
+  }
+  prop_u32(env, o, "rowStride", &d->row_stride);
+  prop_binding(env, o, "logits", &d->logits, &d->logits_bytes);
+  prop_float(env, o, "temperature", &d->has_temperature, &d->temperature);
+  prop_binding(env, o, "tokens", &d->tokens, &d->tokens_bytes);
+  prop_binding(env, o, "logProbs", &d->log_probs, &d->log_probs_bytes);
+  prop_binding(env, o, "entropies", &d->entropies, &d->entropies_bytes);
+  prop_u32(env, o, "alternatives", &d->alternatives);
+  prop_binding(env, o, "topTokens", &d->top_tokens, &d->top_tokens_bytes);
+  prop_binding(env, o, "topLogProbs", &d->top_log_probs, &d->top_log_probs_bytes);
+  *label = prop_string(env, o, "label");
+  d->label = *label;
+  return 1;
+}
+
+/* finalize, validate(desc), enqueue(op, activeRows, stream?, startEvent?,
+   endEvent?) and destroy(op) of the ops above */
+#define ROWS_OP(name)                                                                              \
+  static void name##_finalize(napi_env env, void *data, void *hint) {                              \
+    (void)env;                                                                                     \
+    (void)hint;                                                                                    \
+    pk_##name##_release((pk_##name##_op *)data);                                                   \
+  }                                                                                                \
+  static napi_value js_##name##_validate(napi_env env, napi_callback_info info) {                  \
+    napi_value argv[1];                                                                            \
+    if (!get_args(env, info, 1, argv)) return NULL;                                                \
+    pk_##name##_desc d;                                                                            \
+    char *label;                                                                                   \
+    if (!parse_##name##_desc(env, argv[0], &d, &label)) return NULL;                               \
+    const int status = pk_##name##_validate(&d);                                                   \
+    free(label);                                                                                   \
+    if (status != PK_OK) return throw_status(env, status);                                         \
+    return undefined(env);                                                                         \
+  }                                                                                                \
+  static napi_value js_##name##_enqueue(napi_env env, napi_callback_info info) {                   \
+    napi_value argv[5];                                                                            \
+    uint32_t rows = 0;                                                                             \
+    if (!get_args(env, info, 5, argv)) return NULL;                                                \
+    if (!is_nullish(env, argv[1]) && !get_u32(env, argv[1], &rows))                                \
+      return bad_argument(env, "active rows must be a non-negative integer");                      \
+    PK_CALL(env, pk_##name##_enqueue_timed((pk_##name##_op *)get_external(env, argv[0]), rows,     \
+                                           get_external(env, argv[2]), get_external(env, argv[3]), \
+                                           get_external(env, argv[4])));                           \
+    return undefined(env);                                                                         \
+  }                                                                                                \
+  static napi_value js_##name##_destroy(napi_env env, napi_callback_info info) {                   \
+    napi_value argv[1];                                                                            \
+    if (!get_args(env, info, 1, argv)) return NULL;                                                \
+    PK_CALL(env, pk_##name##_destroy((pk_##name##_op *)get_external(env, argv[0])));               \
+    return undefined(env);                                                                         \
+  }                                                                                                \
+  static napi_value js_##name##_create(napi_env env, napi_callback_info info) {                    \
+    napi_value argv[2], ext;                                                                       \
+    if (!get_args(env, info, 2, argv)) return NULL;                                                \
+    pk_##name##_desc d;                                                                            \
+    char *label;                                                                                   \
+    if (!parse_##name##_desc(env, argv[1], &d, &label)) return NULL;                               \
+    pk_##name##_op *op = NULL;                                                                     \
+    pk_context *ctx = (pk_context *)get_external(env, argv[0]);                                    \
+    const int status = CREATE_##name(ctx, &d, &op);                                                \
+    free(label);                                                                                   \
+    if (status != PK_OK) return throw_status(env, status);                                         \
+    NAPI_CALL(env, napi_create_external(env, op, name##_finalize, NULL, &ext));                    \
+    return ext;                                                                                    \
+  }
+#define CREATE_block_norm(ctx, d, op) pk_block_norm_create(ctx, d, op)
+#define CREATE_q4(ctx, d, op) pk_q4_create(ctx, d, NULL, op)
+#define CREATE_score(ctx, d, op) pk_score_create(ctx, d, op)
+ROWS_OP(block_norm)
+ROWS_OP(q4)
+ROWS_OP(score)
+
 /* ---- row LayerNorm ------------------------------------------------------- */
 
 static void layernorm_finalize(napi_env env, void *data, void *hint) {
@@ -1601,6 +1783,18 @@ static napi_value init(napi_env env, napi_value exports) {
       {"layernormCreate", js_layernorm_create},
       {"layernormEnqueue", js_layernorm_enqueue},
       {"layernormDestroy", js_layernorm_destroy},
+      {"blockNormValidate", js_block_norm_validate},
+      {"blockNormCreate", js_block_norm_create},
+      {"blockNormEnqueue", js_block_norm_enqueue},
+      {"blockNormDestroy", js_block_norm_destroy},
+      {"q4Validate", js_q4_validate},
+      {"q4Create", js_q4_create},
+      {"q4Enqueue", js_q4_enqueue},
+      {"q4Destroy", js_q4_destroy},
+      {"scoreValidate", js_score_validate},
+      {"scoreCreate", js_score_create},
+      {"scoreEnqueue", js_score_enqueue},
+      {"scoreDestroy", js_score_destroy},
       {"subsamplingOutputDimension", js_subsampling_output_dimension},
       {"subsamplingValidLength", js_subsampling_valid_length},
       {"subsamplingValidate", js_subsampling_validate},

@@ -396,6 +396,125 @@ export declare class LayerNormKernel {
 
 export declare function channelTensorRecords(channels: number): { sourceRecord: TensorRecord; runtimeRecord: TensorRecord };
 
+/* ---- Block norm, 4-bit product, token scores (no counterpart in the reference) ---- */
+
+/** A dispatch over rows; shape.rows selects the active ones. */
+export declare class RowsDispatch {
+  readonly label: string;
+  readonly output: ArenaSlice;
+  encode(encoder: HipCommandEncoder, timestampWrites?: TimestampWrites, shape?: EncoderDispatchShape): void;
+  destroy(): void;
+}
+
+/** output = residual + residualScale * gate * norm(input), next.output = norm(output); strides in elements. */
+export interface BlockNormDescriptor {
+  readonly label: string;
+  readonly rows: number;
+  /** 1 to 16384. */
+  readonly channels: number;
+  /** Of both norms; default "layer". */
+  readonly kind?: "layer" | "rms";
+  readonly input: ArenaSlice;
+  readonly inputStride?: number;
+  /** float32 "channel" [channels]; without it the input is not normalised. */
+  readonly gamma?: GpuTensor;
+  readonly beta?: GpuTensor;
+  readonly gate?: ArenaSlice;
+  readonly gateStride?: number;
+  /** Row r takes gate row floor(r / gateRows), or gate row 0 with 0; default 1. */
+  readonly gateRows?: number;
+  readonly residual?: ArenaSlice;
+  readonly residualStride?: number;
+  /** Default 1. */
+  readonly residualScale?: number;
+  /** May be the input's or the residual's slice. */
+  readonly output: ArenaSlice;
+  readonly outputStride?: number;
+  readonly next?: { readonly gamma: GpuTensor; readonly beta?: GpuTensor; readonly output: ArenaSlice;
+                    readonly outputStride?: number };
+  /** Default 1e-5. */
+  readonly epsilon?: number;
+}
+
+export declare class BlockNormKernel {
+  static create(device: HipGpuDevice, arena: GpuActivationArena,
+                executionProfile?: { precision: "fp16" | "fp32" }): Promise<BlockNormKernel>;
+  validateDescriptor(descriptor: BlockNormDescriptor): void;
+  createDispatch(descriptor: BlockNormDescriptor): RowsDispatch;
+  destroy(): void;
+}
+
+/** output = residual + residualScale * activation(a . w + bias), w = scales * (code - 8) + offsets by groups. */
+export interface Q4GemmDescriptor {
+  readonly label: string;
+  readonly rows: number;
+  readonly inner: number;
+  readonly columns: number;
+  /** A power of two from 32 on, or 0: one group. */
+  readonly groupSize: number;
+  readonly a: ArenaSlice;
+  readonly aStride?: number;
+  /** Tensors of q4TensorRecords; laid out at createDispatch, not read afterwards. */
+  readonly packed: GpuTensor;
+  readonly scales: GpuTensor;
+  readonly offsets?: GpuTensor;
+  /** float32 [columns]. */
+  readonly bias?: GpuTensor;
+  /** May be the residual's slice. */
+  readonly output: ArenaSlice;
+  readonly outputStride?: number;
+  readonly residual?: ArenaSlice;
+  readonly residualStride?: number;
+  readonly residualScale?: number;
+  readonly activation?: "none" | "silu" | "relu";
+}
+
+export declare class Q4GemmKernel {
+  static create(device: HipGpuDevice, arena: GpuActivationArena,
+                executionProfile?: { precision: "fp16" | "fp32" }): Promise<Q4GemmKernel>;
+  validateDescriptor(descriptor: Q4GemmDescriptor): void;
+  createDispatch(descriptor: Q4GemmDescriptor): RowsDispatch;
+  destroy(): void;
+}
+
+export declare function q4TensorRecords(weight: { inner: number; columns: number; groupSize: number;
+                                                  dtype?: "float16" | "float32" }): {
+  packed: { sourceRecord: TensorRecord; runtimeRecord: TensorRecord };
+  scales: { sourceRecord: TensorRecord; runtimeRecord: TensorRecord };
+  offsets: { sourceRecord: TensorRecord; runtimeRecord: TensorRecord };
+};
+
+/** Log probabilities of tokens, entropies and best alternatives of rows of logits / temperature. */
+export interface TokenScoreDescriptor {
+  readonly label: string;
+  readonly rows: number;
+  readonly columns: number;
+  /** Elements from row to row; default columns. */
+  readonly rowStride?: number;
+  readonly logits: ArenaSlice;
+  /** Default 1. */
+  readonly temperature?: number;
+  /** u32 [rows] with logProbs f32 [rows]; SCORE_NO_TOKEN: log probability 0. */
+  readonly tokens?: ArenaSlice;
+  readonly logProbs?: ArenaSlice;
+  /** f32 [rows]. */
+  readonly entropies?: ArenaSlice;
+  /** 0 to 32, with topTokens u32 and topLogProbs f32 [rows, alternatives]. */
+  readonly alternatives?: number;
+  readonly topTokens?: ArenaSlice;
+  readonly topLogProbs?: ArenaSlice;
+}
+
+export declare class TokenScoreKernel {
+  static create(device: HipGpuDevice, arena: GpuActivationArena,
+                executionProfile?: { precision: "fp16" | "fp32" }): Promise<TokenScoreKernel>;
+  validateDescriptor(descriptor: TokenScoreDescriptor): void;
+  createDispatch(descriptor: TokenScoreDescriptor): RowsDispatch;
+  destroy(): void;
+}
+
+export declare const SCORE_NO_TOKEN: number;
+
 /* ---- Subsampling front end (src/webgpu/kernels/subsampling.ts) ---- */
 
 /** subsampling.ts:119-122 */

@@ -30,6 +30,11 @@
  *                                      the numeric contract in pk_attention_validate)
  *   RelativeAttentionDispatch.encode / destroy   :51-97
  *   LayerNormKernel / LayerNormDispatch  src/webgpu/kernels/layernorm.ts:29-281
+ *   BlockNormKernel, Q4GemmKernel, TokenScoreKernel, RowsDispatch
+ *                                      no counterpart: the norms around a
+ *                                      block with gate and residual, products
+ *                                      with 4-bit weights, token scores
+ *                                      (include/pk_block_norm.h, pk_q4.h, pk_score.h)
  *   FusedSubsamplingConv0Depthwise2Kernel, DepthwiseSubsamplingKernel,
  *   SubsamplingTimeMaskKernel, SubsamplingDispatch,
  *   subsamplingOutputDimension / subsamplingValidLength
@@ -1157,6 +1162,184 @@ function channelTensorRecords(channels) {
   return { sourceRecord: record, runtimeRecord: record };
 }
 
+/* ------------------------- block norm, 4-bit product, token scores ---- */
+
+/** A dispatch over the rows of its bindings; `native` is the addon's prefix. */
+class RowsDispatch {
+  constructor(label, output, op, rows, nativeName) {
+    this.label = label;
+    this.output = output;
+    this.op = op;
+    this.rows = rows;
+    this.nativeName = nativeName;
+    this.destroyed = false;
+  }
+
+  /** shape.rows selects the active rows. */
+  encode(encoder, timestampWrites, shape) {
+    if (this.destroyed) throw new Error(`${this.label} was destroyed`);
+    const rows = shape === undefined || shape.rows === undefined ? this.rows : shape.rows;
+    if (!isSafe(rows) || rows <= 0 || rows > this.rows)
+      throw new RangeError(`${this.label} active rows must be in [1, ${this.rows}]`);
+    const op = this.op, enqueue = native()[`${this.nativeName}Enqueue`];
+    encoder.record(() => {
+      const [begin, end] = timestampEvents(timestampWrites);
+      enqueue(op, rows, null, begin, end);
+    });
+  }
+
+  destroy() {
+    if (this.destroyed) return;
+    this.destroyed = true;
+    native()[`${this.nativeName}Destroy`](this.op);
+  }
+}
+
+/** A kernel whose dispatches are RowsDispatch; subclasses give `prefix` (the
+ * addon's), `what` (for messages), `nativeDescriptor` and `result`. */
+class RowsKernel {
+  constructor(device, arena, executionProfile) {
+    this.device = device;
+    this.arena = arena;
+    this.precision = precisionOf(executionProfile);
+    this.destroyed = false;
+  }
+
+  /** Fields `name` and `nameBytes` of an arena slice or a tensor, none if undefined. */
+  bindingOf(name, value) {
+    if (value === undefined || value === null) return {};
+    const binding = value.binding === undefined ? this.arena.binding(value) : value.binding;
+    return { [name]: addressOf(binding), [`${name}Bytes`]: binding.size };
+  }
+
+  sizesOf(descriptor, names) {
+    const sizes = {};
+    for (const name of names) {
+      const value = descriptor[name];
+      if (value === undefined) continue;
+      if (!isSafe(value) || value < 0 || value > 0xffffffff)
+        throw new RangeError(`${descriptor.label} ${name} must be a non-negative 32-bit integer`);
+      sizes[name] = value;
+    }
+    return sizes;
+  }
+
+  validateDescriptor(descriptor) {
+    native()[`${this.prefix}Validate`](this.nativeDescriptor(descriptor));
+  }
+
+  createDispatch(descriptor) {
+    if (this.destroyed) throw new Error(`Parakeet ${this.what} kernel was destroyed`);
+    const op = native()[`${this.prefix}Create`](this.device.context, this.nativeDescriptor(descriptor));
+    return new RowsDispatch(descriptor.label, this.result(descriptor), op, descriptor.rows, this.prefix);
+  }
+
+  destroy() {
+    this.destroyed = true;
+  }
+}
+
+class BlockNormKernel extends RowsKernel {
+  static create(device, arena, executionProfile) {
+    return Promise.resolve(new BlockNormKernel(device, arena, executionProfile));
+  }
+
+  get prefix() { return "blockNorm"; }
+  get what() { return "block norm"; }
+  result(descriptor) { return descriptor.output; }
+
+  nativeDescriptor(descriptor) {
+    const { label, channels } = descriptor, next = descriptor.next || {};
+    const kind = { layer: 0, rms: 1 }[descriptor.kind === undefined ? "layer" : descriptor.kind];
+    if (kind === undefined) throw new Error(`${label} has an unsupported norm kind ${descriptor.kind}`);
+    for (const [tensor, name] of [[descriptor.gamma, "gamma"], [descriptor.beta, "beta"], [next.gamma, "next gamma"],
+                                  [next.beta, "next beta"]])
+      if (tensor !== undefined) requireChannelTensor(tensor, channels, channels * 4, `${label} ${name}`);
+    const d = Object.assign(
+      { label, precision: this.precision, kind },
+      this.sizesOf(descriptor, ["rows", "channels", "inputStride", "gateStride", "gateRows", "residualStride",
+                                "outputStride"]),
+      this.bindingOf("input", descriptor.input), this.bindingOf("gamma", descriptor.gamma),
+      this.bindingOf("beta", descriptor.beta), this.bindingOf("gate", descriptor.gate),
+      this.bindingOf("residual", descriptor.residual), this.bindingOf("output", descriptor.output),
+      this.bindingOf("nextGamma", next.gamma), this.bindingOf("nextBeta", next.beta),
+      this.bindingOf("nextOutput", next.output));
+    if (next.outputStride !== undefined) d.nextOutputStride = next.outputStride;
+    if (descriptor.residualScale !== undefined) d.residualScale = descriptor.residualScale;
+    if (descriptor.epsilon !== undefined) d.epsilon = descriptor.epsilon;
+    return d;
+  }
+}
+
+class Q4GemmKernel extends RowsKernel {
+  static create(device, arena, executionProfile) {
+    return Promise.resolve(new Q4GemmKernel(device, arena, executionProfile));
+  }
+
+  get prefix() { return "q4"; }
+  get what() { return "4-bit GEMM"; }
+  result(descriptor) { return descriptor.output; }
+
+  nativeDescriptor(descriptor) {
+    const { label } = descriptor;
+    const activation = { none: 0, silu: 1, relu: 2 }[descriptor.activation === undefined ? "none" : descriptor.activation];
+    if (activation === undefined) throw new Error(`${label} has an unsupported activation ${descriptor.activation}`);
+    const d = Object.assign(
+      { label, precision: this.precision, activation },
+      this.sizesOf(descriptor, ["rows", "inner", "columns", "groupSize", "aStride", "outputStride", "residualStride"]),
+      this.bindingOf("a", descriptor.a), this.bindingOf("packed", descriptor.packed),
+      this.bindingOf("scales", descriptor.scales), this.bindingOf("offsets", descriptor.offsets),
+      this.bindingOf("output", descriptor.output), this.bindingOf("bias", descriptor.bias),
+      this.bindingOf("residual", descriptor.residual));
+    if (descriptor.residualScale !== undefined) d.residualScale = descriptor.residualScale;
+    return d;
+  }
+}
+
+class TokenScoreKernel extends RowsKernel {
+  static create(device, arena, executionProfile) {
+    return Promise.resolve(new TokenScoreKernel(device, arena, executionProfile));
+  }
+
+  get prefix() { return "score"; }
+  get what() { return "token score"; }
+  result(descriptor) { return descriptor.logProbs || descriptor.entropies || descriptor.topTokens; }
+
+  nativeDescriptor(descriptor) {
+    const d = Object.assign(
+      { label: descriptor.label, precision: this.precision },
+      this.sizesOf(descriptor, ["rows", "columns", "rowStride", "alternatives"]),
+      this.bindingOf("logits", descriptor.logits), this.bindingOf("tokens", descriptor.tokens),
+      this.bindingOf("logProbs", descriptor.logProbs), this.bindingOf("entropies", descriptor.entropies),
+      this.bindingOf("topTokens", descriptor.topTokens), this.bindingOf("topLogProbs", descriptor.topLogProbs));
+    if (descriptor.temperature !== undefined) d.temperature = descriptor.temperature;
+    return d;
+  }
+}
+
+/** A token of a padded position, and of a place behind the last alternative. */
+const SCORE_NO_TOKEN = 0xffffffff;
+
+/** Records of a 4-bit weight: packed codes and the tables of scales and
+ * offsets ([groups, columns] of the profile's element). */
+function q4TensorRecords({ inner, columns, groupSize, dtype }) {
+  const type = dtype === undefined ? "float16" : dtype;
+  const groups = groupSize ? Math.ceil(inner / groupSize) : 1;
+  const words = Math.ceil((inner * columns) / 8);
+  const records = (record) => ({ sourceRecord: record, runtimeRecord: record });
+  const table = records({
+    dtype: type, logicalShape: [groups, columns], storageShape: [groups, columns],
+    byteLength: groups * columns * (type === "float16" ? 2 : 4), layout: "group-by-output",
+  });
+  return {
+    packed: records({
+      dtype: "uint32", logicalShape: [inner, columns], storageShape: [words], byteLength: words * 4,
+      layout: "k-major-4-bit-lsb",
+    }),
+    scales: table, offsets: table,
+  };
+}
+
 /** The begin / end events of a timestampWrites descriptor (or nulls). */
 function timestampEvents(timestampWrites) {
   const qs = timestampWrites ? timestampWrites.querySet : null;
@@ -1960,6 +2143,12 @@ module.exports = {
   LayerNormKernel,
   LayerNormDispatch,
   channelTensorRecords,
+  BlockNormKernel,
+  Q4GemmKernel,
+  TokenScoreKernel,
+  RowsDispatch,
+  q4TensorRecords,
+  SCORE_NO_TOKEN,
   subsamplingOutputDimension,
   subsamplingValidLength,
   subsamplingTensorRecords,
