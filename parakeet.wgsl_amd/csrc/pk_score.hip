@@ -122,15 +122,23 @@ struct Shared {
   uint32_t count;
 };
 
+// log(1 + r), r >= 0: the logarithm of u = 1 + r rounded, times r / (u - 1),
+// which takes out what the rounding of u did (W. Kahan's form). Logarithm and
+// reciprocal are the hardware's, within 1 ulp.
+__device__ __forceinline__ float log_one_plus(float r) {
+  const float u = 1.0f + r;
+  return u == 1.0f ? r : __builtin_amdgcn_logf(u) * kLn2 * (r * __builtin_amdgcn_rcpf(u - 1.0f));
+}
+
 // The row's results from its whole sums.
 struct RowScores {
   float m, scale, spread;
   bool empty;
   __device__ RowScores(const ScoreArgs& args, const ScorePart& p)
-      : m(p.m), scale(args.inverse_temperature), spread(log1pf(p.r)), empty(p.m == -kInf && p.r == 0.0f) {}
+      : m(p.m), scale(args.inverse_temperature), spread(log_one_plus(p.r)), empty(p.m == -kInf && p.r == 0.0f) {}
   // The entropy and the log probability of `token`, whose logit is given.
   __device__ void store_row(const ScoreArgs& args, uint32_t row, const ScorePart& p, uint32_t token, float logit) const {
-    if (args.entropies) args.entropies[row] = empty ? 0.0f : spread - p.t * kLn2 / (1.0f + p.r);
+    if (args.entropies) args.entropies[row] = empty ? 0.0f : spread - p.t * kLn2 * __builtin_amdgcn_rcpf(1.0f + p.r);
     if (args.tokens)
       args.log_probs[row] = token < args.columns ? log_prob(logit) : token == 0xffffffffu ? 0.0f : __builtin_nanf("");
   }
@@ -252,21 +260,37 @@ __global__ __launch_bounds__(GROUP < 256 ? 256 : GROUP, GROUP > 256 ? 8 : 1) voi
   const float zero = m == -kInf ? 0.0f : exponent(m);
   float r = 0.0f, t = 0.0f;
   uint32_t equal = 0;  // of the wavefront, counted on the scalar unit
-  const auto add = [&](float v) {
+  const auto add = [&](float v, bool watch) {
     const float d = exponent(v);
-    const bool is_top = d == zero;
-    const float e = is_top ? 0.0f : __builtin_amdgcn_exp2f(d);
-    equal += (uint32_t)__popcll(__ballot(is_top));
+    float e = __builtin_amdgcn_exp2f(d);
+    if (watch) {
+      const bool is_top = d == zero;
+      e = is_top ? 0.0f : e;
+      equal += (uint32_t)__popcll(__ballot(is_top));
+    }
     r += e;
     t = __builtin_fmaf(e, fmaxf(d, -200.0f), t);  // 0 times minus infinity is 0 here
   };
+  const auto add_all = [&](bool watch) {
 #pragma unroll
-  for (int i = 0; i < HELD; ++i) {
+    for (int i = 0; i < HELD; ++i) {
 #pragma unroll
-    for (int c = 0; c < VEC; ++c) add((float)held[i][c]);
-    __builtin_amdgcn_sched_barrier(0);  // one vector's values at a time in registers
+      for (int c = 0; c < VEC; ++c) add((float)held[i][c], watch);
+      __builtin_amdgcn_sched_barrier(0);  // one vector's values at a time in registers
+    }
+    add(single, watch);
+  };
+  if constexpr (kWaves == 1 || HELD == 8) {  // the second pass would take registers that 8 vectors need
+    add_all(true);
+  } else {
+    // Only a wavefront that holds a maximum looks for it, in a second pass.
+    add_all(false);
+    forget(held);
+    if (__any(mine == m)) {
+      r = t = 0.0f;
+      add_all(true);
+    }
   }
-  add(single);
   r = wave::sum(r);
   t = wave::sum(t);
   float maxima = (float)equal;
@@ -454,6 +478,11 @@ constexpr Variant kVariants[] = {
     {256, 2, score_kernel<T, 256, 2>},   {256, 4, score_kernel<T, 256, 4>}, {256, 8, score_kernel<T, 256, 8>},
     {1024, 4, score_kernel<T, 1024, 4>}, {1024, 8, score_kernel<T, 1024, 8>},
 };
+// In place of a {64, 4} and a {256, 8} where every group has a compute unit
+// to itself: 32 rows of 2048 f16 logits 4.2 us instead of 5.2, of 16384 6.0
+// instead of 7.1; from 512 rows on they are slower.
+template <typename T>
+constexpr Variant kFewRows[] = {{256, 1, score_kernel<T, 256, 1>}, {1024, 2, score_kernel<T, 1024, 2>}};
 
 // The parts of a row, and the kernel that holds one.
 struct ScorePlan {
@@ -465,9 +494,12 @@ ScorePlan plan(const ScoreArgs& args) {
   const Variant* table = args.f16 ? kVariants<_Float16> : kVariants<float>;
   const uint32_t most = 1024u * 8u * vec;  // the longest part of one group
   uint32_t parts = (args.columns + most - 1u) / most;
-  // Too few groups for the compute units: parts of at least 4096 logits
-  // instead, as many as make kScoreFill groups.
-  if ((uint64_t)args.rows * parts < kScoreFill) {
+  // Few long rows: parts of at least 4096 logits instead, as many as make
+  // kScoreFill groups. The second launch takes some 4 us, which a group gains
+  // back on 65536 logits and 2048 for each row: 32 rows of 65536 10.5 us (whole
+  // 11.1) and 64 12.4 (11.6), 8 of 131072 9.5 (14.8) and 64 14.1 (16.4), but 1
+  // row of 32000 9.1 (7.4).
+  if ((uint64_t)args.rows * parts < kScoreFill && args.columns >= 65536u && args.columns / args.rows >= 2048u) {
     const uint32_t wanted = (kScoreFill + args.rows - 1u) / args.rows, smallest = (args.columns + 4095u) / 4096u;
     const uint32_t more = wanted < smallest ? wanted : smallest;
     if (more > parts) parts = more;
@@ -478,6 +510,11 @@ ScorePlan plan(const ScoreArgs& args) {
   p.variant = table;
   const uint32_t vectors = (p.span < args.columns ? p.span : args.columns) / vec;
   while (p.variant->group * p.variant->held < vectors) ++p.variant;
+  if ((uint64_t)args.rows * p.parts <= kScoreFill) {
+    const Variant* few = args.f16 ? kFewRows<_Float16> : kFewRows<float>;
+    if (p.variant == table + 2) p.variant = few;
+    if (p.variant == table + 5) p.variant = few + 1;
+  }
   return p;
 }
 

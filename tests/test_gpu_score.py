@@ -129,7 +129,8 @@ def check(got, logits, tokens, k, temperature=1.0, rows=None):
 @pytest.mark.parametrize("dtype", [np.float16, np.float32])
 @pytest.mark.parametrize("rows,columns", [(1, 1), (2, 2), (3, 5), (5, 63), (4, 64), (3, 65), (7, 511), (6, 1025),
                                           (300, 1025), (2, 4096), (3, 5001), (2, 16384), (2, 32000), (5, 50257),
-                                          (1, 131072), (9, 70001), (2, 262144)])
+                                          (1, 131072), (9, 70001), (2, 262144), (520, 2000),
+                                          (300, 16001), (90, 66000)])
 def test_matches_float64(abi, ctx, scope, dtype, rows, columns):
     rng = np.random.default_rng(rows * 11 + columns)
     logits, tokens = make(rng, dtype, rows, columns)
