@@ -220,7 +220,9 @@ __global__ __launch_bounds__(GROUP < 256 ? 256 : GROUP, GROUP > 256 ? 8 : 1) voi
   if (kWaves > 1 && at == 0) s.count = 0;
 
   // Maxima: of each vector, the thread, its subset (GROUP / 64 lanes) and the group.
-  float top[HELD], mine = single;
+  // The operands of a maximum are quiet first: of a signalling NaN and a
+  // number it is a NaN, and the next one loses the number.
+  float top[HELD], mine = __builtin_canonicalizef(single);
 #pragma unroll
   for (int i = 0; i < HELD; ++i) {
     const V w = held[i];
@@ -231,7 +233,8 @@ __global__ __launch_bounds__(GROUP < 256 ? 256 : GROUP, GROUP > 256 ? 8 : 1) voi
                                                   __builtin_shufflevector(pairs, pairs, 2, 3));
       top[i] = fmaxf((float)pair[0], (float)pair[1]);
     } else {
-      top[i] = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
+      top[i] = fmaxf(fmaxf(__builtin_canonicalizef(w[0]), __builtin_canonicalizef(w[1])),
+                     fmaxf(__builtin_canonicalizef(w[2]), __builtin_canonicalizef(w[3])));
     }
     mine = fmaxf(mine, top[i]);
   }

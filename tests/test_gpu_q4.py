@@ -189,6 +189,18 @@ def test_infinities_and_nan_stay_in_their_rows(abi, ctx, scope, dtype):
     assert np.isnan(got[1]).all() and not np.isfinite(got[20]).any()
 
 
+@pytest.mark.parametrize("dtype,size", [(np.float16, 2.0 ** -18), (np.float32, 2.0 ** -132)])
+@pytest.mark.parametrize("rows", [1, 3, 20, 700])
+def test_subnormal_activations(abi, ctx, scope, dtype, size, rows):
+    """Activations below the type's smallest normal number keep their value:
+    scales bring the outputs back among the normal ones."""
+    case = make(np.random.default_rng(rows), dtype, rows, 300, 2064, 64, True)
+    case["a"] = (case["a"].astype(np.float64) * size).astype(dtype)
+    up = dtype(2.0 ** 10) if dtype == np.float16 else dtype(2.0 ** 60)
+    case["scales"], case["offsets"] = case["scales"] * up, case["offsets"] * up
+    check(run(abi, ctx, scope, case), case)
+
+
 @pytest.mark.parametrize("rows", [1, 16, 100])
 def test_output_on_the_residual_and_freed_weight(abi, ctx, scope, rows):
     """The output may be the residual; the op keeps its own copy of the weight."""

@@ -205,6 +205,41 @@ def test_infinities_and_nan(abi, ctx, scope, dtype, columns):
     check(run(abi, ctx, scope, logits, tokens, 4), logits, tokens, 4)
 
 
+@pytest.mark.parametrize("dtype,bits,signalling", [(np.float16, np.uint16, 0x7D00), (np.float32, np.uint32, 0x7FA00000)])
+@pytest.mark.parametrize("columns", [300, 9000])
+def test_signalling_nan(abi, ctx, scope, dtype, bits, signalling, columns):
+    """A NaN that arithmetic would turn quiet hides none of its neighbours."""
+    logits, tokens = make(np.random.default_rng(columns), dtype, 4, columns)
+    for row in range(3):
+        at = int(np.argmax(logits[row])) ^ (row + 1)  # beside the largest, in its vector
+        logits.view(bits)[row, min(at, columns - 1)] = signalling
+    got = run(abi, ctx, scope, logits, tokens, 4)
+    check(got, logits, tokens, 4)
+
+
+@pytest.mark.parametrize("dtype,bits,signalling", [(np.float16, np.uint16, 0x7D00), (np.float32, np.uint32, 0x7FA00000)])
+@pytest.mark.parametrize("columns", [31, 300, 1900, 9000])
+def test_signalling_nan_outside_the_vectors(abi, ctx, scope, dtype, bits, signalling, columns):
+    """The element before the first 16-byte boundary, and the one of a lane
+    behind the last, beside the largest logit in the same lane's vector."""
+    lead = 16 // np.dtype(dtype).itemsize - 1
+    logits, tokens = make(np.random.default_rng(columns), dtype, 2, columns, peak=False)
+    stride = columns + -columns % (lead + 1)
+    logits.view(bits)[:, 0] = signalling
+    logits[0, 1], logits[1, 2] = 60, 60
+    check(run(abi, ctx, scope, logits, tokens, 4, lead=lead, stride=stride), logits, tokens, 4)
+    logits[:, 0] = 1
+    logits.view(bits)[:, -1] = signalling
+    check(run(abi, ctx, scope, logits, tokens, 4, stride=stride), logits, tokens, 4)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("temperature", [2.0 ** -20, 2.0 ** 20])
+def test_temperature_limits(abi, ctx, scope, dtype, temperature):
+    logits, tokens = make(np.random.default_rng(4), dtype, 3, 2000)
+    check(run(abi, ctx, scope, logits, tokens, 3, temperature=temperature), logits, tokens, 3, temperature)
+
+
 def test_tokens_outside(abi, ctx, scope):
     logits, tokens = make(np.random.default_rng(5), np.float16, 6, 1025)
     tokens[1], tokens[2], tokens[3], tokens[4] = NONE, 1025, 1031, NONE - 1
