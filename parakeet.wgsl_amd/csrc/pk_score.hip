@@ -137,7 +137,8 @@ struct RowScores {
   __device__ RowScores(const ScoreArgs& args, const ScorePart& p)
       : m(p.m), scale(args.inverse_temperature), spread(log_one_plus(p.r)), empty(p.m == -kInf && p.r == 0.0f) {}
   // The entropy and the log probability of `token`, whose logit is given.
-  __device__ void store_row(const ScoreArgs& args, uint32_t row, const ScorePart& p, uint32_t token, float logit) const {
+  __device__ void store_row(const ScoreArgs& args, uint32_t row, const ScorePart& p, uint32_t token,
+                            float logit) const {
     if (args.entropies) args.entropies[row] = empty ? 0.0f : spread - p.t * kLn2 * __builtin_amdgcn_rcpf(1.0f + p.r);
     if (args.tokens)
       args.log_probs[row] = token < args.columns ? log_prob(logit) : token == 0xffffffffu ? 0.0f : __builtin_nanf("");
@@ -348,7 +349,9 @@ __global__ __launch_bounds__(GROUP < 256 ? 256 : GROUP, GROUP > 256 ? 8 : 1) voi
     part.r = r;
     part.t = 0.0f;
   } else {
-    const float correction = kHalf ? __builtin_amdgcn_exp2f(-zero) : 1.0f;
+    // zero is at most half a step of c, a step of an f16 logit 2^13 times that:
+    // where zero is far from 0 every other term is 0, and 2^-zero infinite.
+    const float correction = kHalf ? __builtin_amdgcn_exp2f(fmaxf(-100.0f, fminf(100.0f, -zero))) : 1.0f;
     part.t = correction * __builtin_fmaf(-zero, r, t);
     part.r = __builtin_fmaf(correction, r, maxima - 1.0f);
   }
@@ -397,7 +400,8 @@ __global__ __launch_bounds__(kJoining) void score_join_kernel(ScoreArgs args, ui
   float target = 0.0f;
   if (at == 0 && token < args.columns) {
     const uint64_t from = row * args.stride + token;
-    target = args.f16 ? (float)static_cast<const _Float16*>(args.logits)[from] : static_cast<const float*>(args.logits)[from];
+    target = args.f16 ? (float)static_cast<const _Float16*>(args.logits)[from]
+                      : static_cast<const float*>(args.logits)[from];
   }
   // No key below a part's K-th is one of the row's K best: that part has K.
   float m = mine.m;
@@ -563,7 +567,8 @@ hipError_t launch_score(const ScoreArgs& given, hipStream_t stream, hipEvent_t s
   if (const hipError_t e = hipGetLastError()) return e;
   if (!split) return hipSuccess;
   if (stop)
-    hipExtLaunchKernelGGL(score_join_kernel, dim3(args.rows), dim3(kJoining), 0, stream, nullptr, stop, 0, args, p.parts);
+    hipExtLaunchKernelGGL(score_join_kernel, dim3(args.rows), dim3(kJoining), 0, stream, nullptr, stop, 0, args,
+                          p.parts);
   else
     hipLaunchKernelGGL(score_join_kernel, dim3(args.rows), dim3(kJoining), 0, stream, args, p.parts);
   return hipGetLastError();

@@ -240,6 +240,18 @@ def test_temperature_limits(abi, ctx, scope, dtype, temperature):
     check(run(abi, ctx, scope, logits, tokens, 3, temperature=temperature), logits, tokens, 3, temperature)
 
 
+@pytest.mark.parametrize("temperature", [2.0 ** -20, 2.0 ** -16])
+def test_large_f16_logits_at_low_temperatures(abi, ctx, scope, temperature):
+    """Where the product of the largest logit and 1 / T passes 2^31, its
+    rounding alone is worth an exponent that f32 does not hold."""
+    logits, tokens = make(np.random.default_rng(6), np.float16, 64, 300)
+    logits[:32] = -np.abs(logits[:32]) - 2000
+    logits[np.arange(64), tokens] = np.linspace(-1500, -200, 64)
+    logits[32:, 7] = np.linspace(2000, 65504, 32)
+    logits[40:, 9] = logits[40:, 7]
+    check(run(abi, ctx, scope, logits, tokens, 4, temperature=temperature), logits, tokens, 4, temperature)
+
+
 def test_tokens_outside(abi, ctx, scope):
     logits, tokens = make(np.random.default_rng(5), np.float16, 6, 1025)
     tokens[1], tokens[2], tokens[3], tokens[4] = NONE, 1025, 1031, NONE - 1
