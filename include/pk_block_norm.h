@@ -41,9 +41,7 @@ typedef struct pk_block_norm_op pk_block_norm_op;
 /* Matrices are rows of `channels` elements of the profile's type, each row
    `*_stride` elements after the one before (0: channels), at any address
    that fits their elements; `*_bytes` is the capacity from the pointer on
-   and must reach the end of the last row. Rows whose start is 16-byte
-   aligned throughout (pointer, stride and channels) load and store 16 bytes
-   at a time. */
+   and must reach the end of the last row. */
 typedef struct pk_block_norm_desc {
   uint32_t struct_size;          /* sizeof(pk_block_norm_desc) */
   const char *label;

@@ -35,7 +35,7 @@ typedef struct pk_q4_desc {
   int32_t precision;             /* pk_precision of a, scales, offsets, residual and output */
   uint32_t rows;                 /* M capacity, 1 to PK_Q4_MAX_ROWS */
   uint32_t inner;                /* K, 1 to PK_Q4_MAX_STRIDE */
-  uint32_t columns;              /* N; ceil(K / 128) * ceil(N / 16) below 2^24 */
+  uint32_t columns;              /* N; ceil(K / 128) * ceil(N / 16) below 2^24, M * N at most 2^35 */
   uint32_t group_size;           /* G: a power of two from 32 on, or 0 (one group: G = K);
                                     the last group may be short */
   const void *a;                 /* [rows, inner], rows a_stride elements apart (0: inner) */
@@ -61,8 +61,7 @@ typedef struct pk_q4_desc {
 } pk_q4_desc;
 
 /* a, output and residual may start at any address that fits their elements
-   and have any stride; where `a` is 16-byte aligned in pointer and stride
-   its rows load 16 bytes at a time. The output may be the residual (the same
+   and have any stride. The output may be the residual (the same
    pointer and stride); any other overlap with a or the residual is refused,
    where columns of one buffer (the same stride) do not overlap if their
    columns do not. */

@@ -183,7 +183,8 @@ typedef void (*Kernel)(BlockNormArgs);
 template <typename T, bool TAIL>
 Kernel pick(uint32_t channels, uint32_t* group) {
   constexpr int VEC = 16 / sizeof(T);
-  *group = channels <= 1024u ? 64u : channels <= 2048u ? 128u : channels <= 4096u ? 256u : channels <= 8192u ? 512u : 1024u;
+  *group = channels <= 1024u ? 64u : channels <= 2048u ? 128u : channels <= 4096u ? 256u : channels <= 8192u ? 512u
+                                                                                                             : 1024u;
   if (channels <= 512u) return block_norm_kernel<T, 64, 8 / VEC, TAIL>;
   if (channels <= 1024u) return block_norm_kernel<T, 64, 16 / VEC, TAIL>;
   if (channels <= 2048u) return block_norm_kernel<T, 128, 16 / VEC, TAIL>;

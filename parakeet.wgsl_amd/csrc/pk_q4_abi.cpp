@@ -32,10 +32,12 @@ int validate_q4(const pk_q4_desc* d) {
   const char* label = q4_label(d->label);
   if (d->precision != PK_PRECISION_F16 && d->precision != PK_PRECISION_F32)
     return fail(PK_INVALID_ARGUMENT, "%s has an unsupported precision %d", label, d->precision);
-  // A launch has at most 2^16 - 1 tiles of 16 rows, and the layout one thread
-  // a word, less than 2^32.
+  // A launch has at most 2^16 - 1 tiles of 16 rows, and less than 2^32
+  // threads: the layout one a word, the product 256 a tile of 64 x 128
+  // outputs, of which 2^35 outputs take less than 2^24 (65 rows take two).
   const uint64_t blocks = (((uint64_t)d->inner + 127u) / 128u) * (((uint64_t)d->columns + 15u) / 16u);
-  if (d->rows == 0 || d->inner == 0 || d->columns == 0 || d->rows > PK_Q4_MAX_ROWS || blocks >= 1u << 24)
+  if (d->rows == 0 || d->inner == 0 || d->columns == 0 || d->rows > PK_Q4_MAX_ROWS || blocks >= 1u << 24 ||
+      (uint64_t)d->rows * d->columns > 1ull << 35)
     return fail(PK_RANGE_ERROR, "Invalid q4 shape [%u, %u, %u] for %s", d->rows, d->inner, d->columns, label);
   // Offsets into a tile of rows are 32 bits.
   if (d->inner > PK_Q4_MAX_STRIDE || d->a_stride > PK_Q4_MAX_STRIDE)
@@ -73,7 +75,8 @@ int validate_q4(const pk_q4_desc* d) {
   }
   const uint64_t packed = ((uint64_t)d->inner * d->columns + 7u) / 8u * 4u;
   if (d->packed_bytes != packed || !aligned(d->packed, 4))
-    return fail(PK_INVALID_ARGUMENT, "%s packed must be %llu bytes of whole words", label, (unsigned long long)packed);
+    return fail(PK_INVALID_ARGUMENT, "%s packed must be %llu bytes of whole words", label,
+                (unsigned long long)packed);
   const uint32_t group = d->group_size ? d->group_size : d->inner;
   const uint64_t table = (uint64_t)((d->inner + group - 1u) / group) * d->columns * elem;
   if (d->scales_bytes != table || !aligned(d->scales, elem) ||

@@ -189,6 +189,15 @@ def score_args(rows=8, columns=1025, stride=1032, elem=2, k=4, **over):
     return dict(kw, **over)
 
 
+def test_q4_launch_limit(abi):
+    """Row and column counts whose tiles no launch holds."""
+    columns = (1 << 28) - 16
+    kw = dict(a=Fake(1 << 50, 1 << 40), packed=Fake(1 << 51, columns * 4), scales=Fake(1 << 52, columns * 2),
+              output=Fake(1 << 53, 1 << 50), inner=8, columns=columns, group_size=0, precision="f16", label="wide")
+    abi.check(abi.load().pk_q4_validate(ctypes.byref(abi.q4_desc(rows=128, **kw))))
+    refused(abi, "q4", abi.q4_desc(rows=129, **kw), abi.PaletteRangeError, "Invalid q4 shape [129, 8, ")
+
+
 def test_score_accepts(abi):
     def ok(**over):
         desc = abi.score_desc(**score_args(**over))
