@@ -423,6 +423,10 @@ struct Q4Args {
   uint32_t columns;
   uint32_t per_block;  // scales of a column in a block: 1, 2 or 4
   bool f16;
+  // Tiles split along K: the sums of each part.
+  uint32_t span;  // blocks of K of a part, set by the launch
+  float* parts;
+  uint64_t part_bytes;  // that the workspace holds
 };
 // Bytes of a laid-out weight, and where its tables start.
 struct Q4Layout {
@@ -432,6 +436,8 @@ Q4Layout q4_layout(const Q4Args& args, bool offsets);
 // Writes args.codes, scales and offsets from the packed codes and the tables.
 hipError_t launch_q4_layout(const Q4Args& args, const uint32_t* packed, const void* scales, const void* offsets,
                             uint32_t group, hipStream_t stream);
+// Bytes of workspace for up to args.rows rows.
+uint64_t q4_workspace(const Q4Args& args);
 hipError_t launch_q4(const Q4Args& args, hipStream_t stream, hipEvent_t start = nullptr, hipEvent_t stop = nullptr);
 
 // Subsampling front end convolutions (pk_subsampling.hip).

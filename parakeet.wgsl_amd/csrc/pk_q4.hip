@@ -484,8 +484,11 @@ __global__ __launch_bounds__(1024) void q4_vector_kernel(Q4Args args) {
 // columns. The rows go through LDS, a block of 128 k at a time in two
 // buffers; codes go from memory to registers, where each wavefront makes its
 // own operands of them: 9 VALU operations per 4 matrix instructions, beside
-// the 16 that a group's scales take for each 16 columns.
+// the 16 that a group's scales take for each 16 columns. Of few tiles
+// blockIdx.y is a part of K, whose sums go to a workspace as they lie in the
+// lanes, and a second launch adds the parts in their order.
 constexpr int kTileRows = 64, kTileColumns = 128;
+constexpr uint32_t kTileVectors = kTileRows * kTileColumns / 4;  // of a lane's four rows
 template <int PER, bool OFFSETS>
 __global__ __launch_bounds__(256, OFFSETS ? 2 : 3) void q4_tile_kernel(Q4Args args) {
   typedef _Float16 T;
@@ -603,16 +606,17 @@ __global__ __launch_bounds__(256, OFFSETS ? 2 : 3) void q4_tile_kernel(Q4Args ar
       __builtin_amdgcn_sched_barrier(0);  // one step's operands at a time in registers
     }
   };
-  // Whole blocks, the next one's loads under way while one is multiplied,
-  // then the block that K ends in.
-  const uint32_t whole = args.inner / 128u;
+  // This part's whole blocks, the next one's loads under way while one is
+  // multiplied, then the block that K ends in.
+  const uint32_t first = blockIdx.y * args.span, last = min(first + args.span, kblocks);
+  const uint32_t whole = min(args.inner / 128u, last);
   Weight w, next;
-  load_weight(0, w);
-  if (whole) load_rows(0);
-  else load_last_rows(0);
-  store_rows(0);
+  load_weight(first, w);
+  if (whole > first) load_rows(first);
+  else load_last_rows(first);
+  store_rows(first & 1u);
   __syncthreads();
-  for (uint32_t kb = 0; kb + 1u < whole; ++kb) {
+  for (uint32_t kb = first; kb + 1u < whole; ++kb) {
     load_rows(kb + 1u);
     load_weight(kb + 1u, next);
     multiply_block(kb, w);
@@ -620,7 +624,7 @@ __global__ __launch_bounds__(256, OFFSETS ? 2 : 3) void q4_tile_kernel(Q4Args ar
     w = next;
     __syncthreads();
   }
-  if (whole && kblocks > whole) {
+  if (whole > first && last > whole) {
     load_last_rows(whole);
     load_weight(whole, next);
     multiply_block(whole - 1u, w);
@@ -628,7 +632,15 @@ __global__ __launch_bounds__(256, OFFSETS ? 2 : 3) void q4_tile_kernel(Q4Args ar
     w = next;
     __syncthreads();
   }
-  multiply_block(kblocks - 1u, w);
+  multiply_block(last - 1u, w);
+  if (gridDim.y > 1u) {
+    floatx4* sums = reinterpret_cast<floatx4*>(args.parts) + ((uint64_t)blockIdx.y * gridDim.x + id) * kTileVectors;
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) sums[(wave * 8u + 2 * mt + nt) * 64u + lane] = acc[mt][nt];
+    return;
+  }
   __syncthreads();
 
   // Out through LDS, 32 rows at a time, so that a lane stores 8 columns.
@@ -656,6 +668,23 @@ __global__ __launch_bounds__(256, OFFSETS ? 2 : 3) void q4_tile_kernel(Q4Args ar
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     __builtin_amdgcn_wave_barrier();
   }
+}
+
+// Adds the parts of tiles split along K, four rows of a column a thread.
+__global__ __launch_bounds__(256) void q4_join_kernel(Q4Args args, uint32_t tiles, uint32_t parts) {
+  const uint32_t at = blockIdx.x * 256u + threadIdx.x, tile = at / kTileVectors, v = at % kTileVectors;
+  const uint32_t row_tiles = (args.rows + kTileRows - 1u) / kTileRows;
+  const uint32_t lane = v & 63u, nt = (v >> 6) & 1u, mt = (v >> 7) & 3u, wave = v >> 9;
+  const uint32_t m = tile % row_tiles * kTileRows + 16u * mt + 4u * (lane >> 4);
+  const uint32_t n = tile / row_tiles * kTileColumns + 32u * wave + 16u * nt + (lane & 15u);
+  if (m >= args.rows || n >= args.columns) return;
+  const floatx4* sums = reinterpret_cast<const floatx4*>(args.parts) + at;
+  floatx4 sum = (floatx4)0.0f;
+#pragma unroll 8
+  for (uint32_t p = 0; p < parts; ++p) sum += sums[(uint64_t)p * tiles * kTileVectors];
+#pragma unroll
+  for (uint32_t r = 0; r < 4u; ++r)
+    if (m + r < args.rows) finish<_Float16>(args, m + r, n, sum[r]);
 }
 
 typedef void (*Kernel)(Q4Args);
@@ -686,8 +715,10 @@ Kernel pick_tile(const Q4Args& args) {
 // A launch: kernel, grid and threads.
 struct Q4Plan {
   Kernel kernel;
-  dim3 grid;
+  dim3 grid;  // y of a tile kernel: parts of K, `span` blocks each
   uint32_t threads;
+  uint32_t span;  // 0: no tile kernel
+  uint64_t part_bytes() const { return span && grid.y > 1u ? (uint64_t)grid.x * grid.y * kTileVectors * 16u : 0u; }
 };
 Q4Plan plan(const Q4Args& args) {
   const auto tiles = [](uint32_t n, uint32_t size) { return (n + size - 1u) / size; };
@@ -706,17 +737,28 @@ Q4Plan plan(const Q4Args& args) {
     // 1 x 4096 x 4096: 4.2 us on the VALU, 8.1 on the matrix units; 4 rows 7.8 and 9.5.
     if (panel && args.rows <= 4u)
       return {args.rows == 1u ? pick_vector<1>(args) : args.rows == 2u ? pick_vector<2>(args) : pick_vector<4>(args),
-              dim3(nblocks), panel_threads(16u)};
-    if (panel) return {pick_rows<float, 1, 1, true>(args), dim3(nblocks), panel_threads(16u)};
-    return {pick_rows<float, 1, 1, false>(args), dim3(nblocks, tiles(args.rows, 16u)), threads(8u)};
+              dim3(nblocks), panel_threads(16u), 0u};
+    if (panel) return {pick_rows<float, 1, 1, true>(args), dim3(nblocks), panel_threads(16u), 0u};
+    return {pick_rows<float, 1, 1, false>(args), dim3(nblocks, tiles(args.rows, 16u)), threads(8u), 0u};
   }
-  // The tiles need the compute units full: 192 tiles (1504 x 4096 x 1024) take
-  // 28.0 us and rows 34.0, 128 tiles (256 x 1024 x 4096 and x 4096) 9.7 and
-  // 27.5, and rows 10.6 and 24.
+  // Too few tiles to fill the compute units: with much work each, as many
+  // parts along K as make two for each. The second launch takes some 4 us, won
+  // back from 4000 blocks of K and tile on: 80 tiles (64 x 8192 x 10240) 23.2
+  // us, rows below 35.4; 96 (192 x 8192 x 4096) 24.1 and 34.7; 160 (320 x 4096 x
+  // 4096) 22.1, tiles whole 27.8; 64 (64 x 8192 x 8192) 20.0 and rows 21.4; but
+  // with 2048 blocks (128 x 4096 x 4096) 14.4 and 12.5, with 16 blocks along K
+  // (256 x 2048 x 8192) 19.7, tiles whole 16.7, and 24 x 8192 x 8192 18.7 and rows 13.2.
   const uint64_t tiled = (uint64_t)tiles(args.rows, kTileRows) * tiles(args.columns, kTileColumns);
-  if (args.rows > 64u && tiled >= 160u) return {pick_tile(args), dim3((uint32_t)tiled), 256u};
+  if (args.rows > 32u && tiled <= 256u && kblocks >= 32u && tiled * kblocks >= 4000u) {
+    const uint32_t span = tiles(kblocks, 512u / (uint32_t)tiled);
+    return {pick_tile(args), dim3((uint32_t)tiled, tiles(kblocks, span)), 256u, span};
+  }
+  // Whole tiles need the compute units full: 192 (1504 x 2048 x 1024) take
+  // 17.1 us and rows 18.6, 128 (256 x 1024 x 4096 and 512 x 2048 x 2048) 10.1 and
+  // 16.2, and rows 11.0 and 16.0, 64 (256 x 2048 x 2048) 16.0 and 8.7.
+  if (args.rows > 64u && tiled >= 160u) return {pick_tile(args), dim3((uint32_t)tiled), 256u, kblocks};
   // 8 wavefronts (1 x 8192 x 8192 8.3 us, 16 8.8; 8 x 2048 x 8192 4.5 and 5.2).
-  if (panel) return {pick_rows<_Float16, 1, 1, true>(args), dim3(nblocks), panel_threads(8u)};
+  if (panel) return {pick_rows<_Float16, 1, 1, true>(args), dim3(nblocks), panel_threads(8u), 0u};
   // Two column blocks a wavefront, which share the rows' reads, where a
   // workgroup for each compute unit is left: 32 x 4096 x 8192 9.2 us (one:
   // 12.6), but 32 x 4096 x 4096, where half would be left, 8.0 (one: 7.0).
@@ -724,11 +766,12 @@ Q4Plan plan(const Q4Args& args) {
   const bool two = (uint64_t)tiles(nblocks, 2u) * row_tiles >= 256u;
   const dim3 grid(two ? tiles(nblocks, 2u) : nblocks, row_tiles);
   if (mt == 1u)
-    return {two ? pick_rows<_Float16, 1, 2, false>(args) : pick_rows<_Float16, 1, 1, false>(args), grid, threads(16u)};
+    return {two ? pick_rows<_Float16, 1, 2, false>(args) : pick_rows<_Float16, 1, 1, false>(args), grid, threads(16u),
+            0u};
   if (mt == 2u)
     return {two ? pick_rows<_Float16, 2, 2, false>(args) : pick_rows<_Float16, 2, 1, false>(args), grid,
-            threads(two ? 8u : 16u)};
-  return {two ? pick_rows<_Float16, 4, 2, false>(args) : pick_rows<_Float16, 4, 1, false>(args), grid, threads(8u)};
+            threads(two ? 8u : 16u), 0u};
+  return {two ? pick_rows<_Float16, 4, 2, false>(args) : pick_rows<_Float16, 4, 1, false>(args), grid, threads(8u), 0u};
 }
 
 }  // namespace
@@ -770,12 +813,36 @@ hipError_t launch_q4_layout(const Q4Args& args, const uint32_t* packed, const vo
   return hipSuccess;
 }
 
-hipError_t launch_q4(const Q4Args& args, hipStream_t stream, hipEvent_t start, hipEvent_t stop) {
+uint64_t q4_workspace(const Q4Args& args) {
+  Q4Args some = args;
+  uint64_t bytes = 0;
+  const auto count = [&](uint32_t rows) {
+    some.rows = rows;
+    const uint64_t wanted = plan(some).part_bytes();
+    if (wanted > bytes) bytes = wanted;
+  };
+  for (uint32_t rows = kTileRows; rows < args.rows && rows <= 512u * kTileRows; rows += kTileRows) count(rows);
+  count(args.rows);
+  return bytes;
+}
+
+hipError_t launch_q4(const Q4Args& given, hipStream_t stream, hipEvent_t start, hipEvent_t stop) {
+  Q4Args args = given;
   const Q4Plan p = plan(args);
-  if (start || stop)
-    hipExtLaunchKernelGGL(p.kernel, p.grid, dim3(p.threads), 0, stream, start, stop, 0, args);
+  args.span = p.span;
+  const uint64_t bytes = p.part_bytes();
+  if (bytes > args.part_bytes) return hipErrorInvalidValue;
+  if (start || (stop && !bytes))
+    hipExtLaunchKernelGGL(p.kernel, p.grid, dim3(p.threads), 0, stream, start, bytes ? nullptr : stop, 0, args);
   else
     hipLaunchKernelGGL(p.kernel, p.grid, dim3(p.threads), 0, stream, args);
+  if (const hipError_t e = hipGetLastError()) return e;
+  if (!bytes) return hipSuccess;
+  const dim3 grid(p.grid.x * (kTileVectors / 256u));
+  if (stop)
+    hipExtLaunchKernelGGL(q4_join_kernel, grid, dim3(256), 0, stream, nullptr, stop, 0, args, p.grid.x, p.grid.y);
+  else
+    hipLaunchKernelGGL(q4_join_kernel, grid, dim3(256), 0, stream, args, p.grid.x, p.grid.y);
   return hipGetLastError();
 }
 

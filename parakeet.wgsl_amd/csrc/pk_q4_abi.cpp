@@ -19,6 +19,7 @@ struct pk_q4_op {
   pk::Q4Args args{};
   void* weight = nullptr;
   uint64_t weight_bytes = 0;
+  void* workspace = nullptr;
   bool destroyed = false;
 };
 
@@ -141,12 +142,24 @@ int pk_q4_create(pk_context* ctx, const pk_q4_desc* d, void* stream, pk_q4_op** 
   a.codes = reinterpret_cast<const uint4*>(base);
   a.scales = base + at.scales;
   a.offsets = d->offsets ? base + at.offsets : nullptr;
+  void* workspace = nullptr;
+  if ((a.part_bytes = pk::q4_workspace(a))) {
+    const hipError_t room = hipMalloc(&workspace, a.part_bytes);
+    if (room != hipSuccess) {
+      (void)hipGetLastError();
+      (void)hipFree(weight);
+      return fail(PK_ALLOCATION_FAILURE, "%s: cannot allocate %llu bytes of workspace: %s", label.c_str(),
+                  (unsigned long long)a.part_bytes, hipGetErrorString(room));
+    }
+    a.parts = static_cast<float*>(workspace);
+  }
   hipError_t e = pk::launch_q4_layout(a, d->packed, d->scales, d->offsets, d->group_size ? d->group_size : d->inner, st);
   const hipError_t done = hipStreamSynchronize(st);
   if (e == hipSuccess) e = done;
   pk_q4_op* op = e == hipSuccess ? new (std::nothrow) pk_q4_op() : nullptr;
   if (!op) {
     (void)hipFree(weight);
+    (void)hipFree(workspace);
     if (e == hipSuccess) return fail(PK_ALLOCATION_FAILURE, "%s: out of host memory", label.c_str());
     return fail(PK_DEVICE_ERROR, "%s weight layout failed: %s", label.c_str(), hipGetErrorString(e));
   }
@@ -156,6 +169,7 @@ int pk_q4_create(pk_context* ctx, const pk_q4_desc* d, void* stream, pk_q4_op** 
   op->args = a;
   op->weight = weight;
   op->weight_bytes = at.bytes;
+  op->workspace = workspace;
   *out = op;
   return ok();
 } catch (const std::bad_alloc&) {
@@ -191,7 +205,8 @@ int pk_q4_destroy(pk_q4_op* op) {
   if (!op || op->destroyed) return ok();
   op->destroyed = true;
   free_on(op->ctx->device, op->weight);
-  op->weight = nullptr;
+  free_on(op->ctx->device, op->workspace);
+  op->weight = op->workspace = nullptr;
   op->weight_bytes = 0;
   return ok();
 }

@@ -249,3 +249,60 @@ def test_graph_and_refused_capture(abi, ctx, scope):
         ctx.synchronize()
     graph.release()
     op.release()
+
+
+@pytest.mark.parametrize("rows,inner,columns,group,offsets", [
+    (500, 17300, 512, 128, False),  # the last part is one block, K ends in it
+    (500, 17408, 512, 0, True), (130, 4100, 5500, 64, True), (40, 8200, 8190, 32, True), (64, 8192, 8192, 128, False)])
+def test_split_along_k(abi, ctx, scope, rows, inner, columns, group, offsets):
+    """Few tiles of many rows with a long K: parts of K meet in a workspace."""
+    rng = np.random.default_rng(rows + inner)
+    case = make(rng, np.float16, rows, inner, columns, group, offsets, bias=True, activation="silu", residual=True,
+                residual_scale=0.5)
+    check(run(abi, ctx, scope, case, strides=dict(a=inner + 3, output=columns + 5, residual=columns + 1),
+              leads=dict(output=1)), case)
+
+
+def test_split_row_counts_launches_and_graph(abi, ctx, scope):
+    """One op at row counts with and without parts, launched again and again,
+    timed, and replayed from a graph between eager launches."""
+    rows, inner, columns = 700, 4200, 4000
+    case = make(np.random.default_rng(5), np.float16, rows, inner, columns, 128, True)
+    want, tol = reference(case)
+    kw = operands(abi, scope, case)
+    op = abi.Q4GemmOp(ctx, **kw)
+    graph = None
+    try:
+        def read(n):
+            ctx.synchronize()
+            got = kw["output"].download()
+            far = np.abs(got[:n].astype(np.float64) - want[:n]) - tol[:n]
+            assert (far <= 0).all(), (n, far.max())
+            assert (got[n:] == 321).all(), n
+            return got
+        kw["output"].upload(np.full((rows, columns), 321, np.float16))
+        first = {}
+        for n in (1, 32, 33, 300, 448, 512, 513, 700):
+            op.enqueue(n)
+            first[n] = read(n)[:n]
+        for n in (300, 700, 300):
+            kw["output"].upload(np.full((rows, columns), 321, np.float16))
+            op.enqueue(n)
+            np.testing.assert_array_equal(read(n)[:n], first[n])
+        start, end = abi.Event(ctx), abi.Event(ctx)
+        op.enqueue(300, start=start, end=end)
+        ctx.synchronize()
+        assert 0 < start.elapsed_ms(end) < 1000
+        start.destroy(), end.destroy()
+        graph = abi.Graph.capture(ctx, ctx.stream)
+        with graph:
+            op.enqueue(300, ctx.stream)
+        for n in (300, 64, 700):
+            kw["output"].upload(np.full((rows, columns), 321, np.float16))
+            op.enqueue(n)
+            graph.launch()
+            np.testing.assert_array_equal(read(max(n, 300))[:300], first[300])
+    finally:
+        if graph:
+            graph.release()
+        op.release()
