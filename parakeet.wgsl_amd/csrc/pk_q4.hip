@@ -119,6 +119,24 @@ __device__ __forceinline__ void multiply(const Fragment<float>& a, const half8& 
     acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.c[j / 4].v[j % 4], (float)b[j], acc, 0, 0, 0);
 }
 
+// acc[mt][nt] += a[mt] . b; one f32 instruction waits for the one whose sum it
+// adds to, so those of a k go before the next k.
+template <int MT, int NT>
+__device__ __forceinline__ void multiply(const Fragment<_Float16> (&a)[MT], const half8& b, floatx4 (&acc)[MT][NT],
+                                         int nt) {
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) multiply(a[mt], b, acc[mt][nt]);
+}
+template <int MT, int NT>
+__device__ __forceinline__ void multiply(const Fragment<float> (&a)[MT], const half8& b, floatx4 (&acc)[MT][NT],
+                                         int nt) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+      acc[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[mt].c[j / 4].v[j % 4], (float)b[j], acc[mt][nt], 0, 0, 0);
+}
+
 // The activation of one output.
 __device__ __forceinline__ float activate(int activation, float v) {
   if (activation == kActSilu) return v * __builtin_amdgcn_rcpf(1.0f + __expf(-v));
@@ -138,12 +156,14 @@ __device__ __forceinline__ void finish(const Q4Args& args, uint32_t m, uint32_t 
 }
 
 // The same for 8 columns from n on, those behind the edge left out.
+template <typename T>
 __device__ __forceinline__ void finish_row(const Q4Args& args, uint32_t m, uint32_t n, float (&v)[8]) {
+  constexpr int N = Chunk<T>::N;
   typedef float F __attribute__((ext_vector_type(4), aligned(4)));
   if (n + 8u > args.columns) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (n + j < args.columns) finish<_Float16>(args, m, n + j, v[j]);
+      if (n + j < args.columns) finish<T>(args, m, n + j, v[j]);
     return;
   }
   if (args.bias) {
@@ -153,15 +173,18 @@ __device__ __forceinline__ void finish_row(const Q4Args& args, uint32_t m, uint3
   }
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = activate(args.activation, v[j]);
-  Chunk<_Float16> x;
-  if (args.residual) {
-    x.load(static_cast<const _Float16*>(args.residual) + (uint64_t)m * args.residual_stride + n);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = __builtin_fmaf(args.residual_scale, v[j], (float)x.v[j]);
+  for (int p = 0; p < 8; p += N) {
+    Chunk<T> x;
+    if (args.residual) {
+      x.load(static_cast<const T*>(args.residual) + (uint64_t)m * args.residual_stride + n + p);
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[p + j] = __builtin_fmaf(args.residual_scale, v[p + j], (float)x.v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) x.v[j] = (T)v[p + j];
+    *reinterpret_cast<typename Chunk<T>::U*>(static_cast<T*>(args.out) + (uint64_t)m * args.out_stride + n + p) = x.v;
   }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) x.v[j] = (_Float16)v[j];
-  *reinterpret_cast<Chunk<_Float16>::U*>(static_cast<_Float16*>(args.out) + (uint64_t)m * args.out_stride + n) = x.v;
 }
 
 // LDS bytes of the rows of `a` in a panel kernel.
@@ -480,7 +503,7 @@ __global__ __launch_bounds__(1024) void q4_vector_kernel(Q4Args args) {
   }
 }
 
-// Many rows, f16. One workgroup: 64 rows x 128 columns, a wavefront 32 of the
+// Many rows. One workgroup: 64 rows x 128 columns, a wavefront 32 of the
 // columns. The rows go through LDS, a block of 128 k at a time in two
 // buffers; codes go from memory to registers, where each wavefront makes its
 // own operands of them: 9 VALU operations per 4 matrix instructions, beside
@@ -489,11 +512,10 @@ __global__ __launch_bounds__(1024) void q4_vector_kernel(Q4Args args) {
 // lanes, and a second launch adds the parts in their order.
 constexpr int kTileRows = 64, kTileColumns = 128;
 constexpr uint32_t kTileVectors = kTileRows * kTileColumns / 4;  // of a lane's four rows
-template <int PER, bool OFFSETS>
-__global__ __launch_bounds__(256, OFFSETS ? 2 : 3) void q4_tile_kernel(Q4Args args) {
-  typedef _Float16 T;
+template <typename T, int PER, bool OFFSETS>
+__global__ __launch_bounds__(256, OFFSETS || sizeof(T) == 4 ? 2 : 3) void q4_tile_kernel(Q4Args args) {
   constexpr int kStep = 4 / PER;
-  constexpr int kChunks = 16, kCopies = kTileRows * kChunks / 256;
+  constexpr int kChunks = 128 / Chunk<T>::N, kCopies = kTileRows * kChunks / 256;
   constexpr int kWidth = 32 + 4;  // f32 columns of a wavefront's part on its way out
   typedef T S __attribute__((ext_vector_type(PER == 1 ? 2 : PER)));
   __shared__ uint4 lds[2][kTileRows * kChunks];
@@ -536,7 +558,7 @@ __global__ __launch_bounds__(256, OFFSETS ? 2 : 3) void q4_tile_kernel(Q4Args ar
 #pragma unroll
   for (int t = 0; t < kCopies; ++t) {
     const uint32_t at = t * 256u + threadIdx.x, r = at / kChunks, c = (at % kChunks) ^ (r & 15u);
-    from[t] = (min(m0 + r, args.rows - 1u) - m0) * (uint32_t)args.a_stride + c * 8u;
+    from[t] = (min(m0 + r, args.rows - 1u) - m0) * (uint32_t)args.a_stride + c * Chunk<T>::N;
   }
   Chunk<T> copy[kCopies];
   const auto load_rows = [&](uint32_t kb) {
@@ -549,7 +571,7 @@ __global__ __launch_bounds__(256, OFFSETS ? 2 : 3) void q4_tile_kernel(Q4Args ar
 #pragma unroll
     for (int t = 0; t < kCopies; ++t) {
       const uint32_t at = t * 256u + threadIdx.x, c = (at % kChunks) ^ ((at / kChunks) & 15u);
-      copy[t].load(block + from[t], kb * 128u + c * 8u, args.inner);
+      copy[t].load(block + from[t], kb * 128u + c * Chunk<T>::N, args.inner);
     }
   };
   const auto store_rows = [&](int buffer) {
@@ -574,16 +596,17 @@ __global__ __launch_bounds__(256, OFFSETS ? 2 : 3) void q4_tile_kernel(Q4Args ar
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
         const uint32_t r = 16u * mt + column;
-        a[mt].c[0] = rows[r * kChunks + ((4u * i + quad) ^ column)];
+        constexpr int kParts = 8 / Chunk<T>::N;
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) a[mt].c[p] = rows[r * kChunks + (((4u * i + quad) * kParts + p) ^ column)];
       }
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt) {
         const half8 b = decode(reinterpret_cast<const uint32_t(&)[4]>(w.codes[nt])[i]);
+        if (i % kStep == 0)
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) {
-          if (i % kStep == 0) part[mt][nt] = (floatx4)0.0f;
-          multiply(a[mt], b, part[mt][nt]);
-        }
+          for (int mt = 0; mt < 4; ++mt) part[mt][nt] = (floatx4)0.0f;
+        multiply(a, b, part, nt);
       }
       if constexpr (OFFSETS)
 #pragma unroll
@@ -663,7 +686,7 @@ __global__ __launch_bounds__(256, OFFSETS ? 2 : 3) void q4_tile_kernel(Q4Args ar
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = part_out[r * kWidth + c + j];
-      if (m < args.rows) finish_row(args, m, n, v);
+      if (m < args.rows) finish_row<T>(args, m, n, v);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -671,6 +694,7 @@ __global__ __launch_bounds__(256, OFFSETS ? 2 : 3) void q4_tile_kernel(Q4Args ar
 }
 
 // Adds the parts of tiles split along K, four rows of a column a thread.
+template <typename T>
 __global__ __launch_bounds__(256) void q4_join_kernel(Q4Args args, uint32_t tiles, uint32_t parts) {
   const uint32_t at = blockIdx.x * 256u + threadIdx.x, tile = at / kTileVectors, v = at % kTileVectors;
   const uint32_t row_tiles = (args.rows + kTileRows - 1u) / kTileRows;
@@ -684,7 +708,7 @@ __global__ __launch_bounds__(256) void q4_join_kernel(Q4Args args, uint32_t tile
   for (uint32_t p = 0; p < parts; ++p) sum += sums[(uint64_t)p * tiles * kTileVectors];
 #pragma unroll
   for (uint32_t r = 0; r < 4u; ++r)
-    if (m + r < args.rows) finish<_Float16>(args, m + r, n, sum[r]);
+    if (m + r < args.rows) finish<T>(args, m + r, n, sum[r]);
 }
 
 typedef void (*Kernel)(Q4Args);
@@ -707,9 +731,11 @@ Kernel pick_vector(const Q4Args& args) {
 #undef PK_Q4_VECTOR
 }
 Kernel pick_tile(const Q4Args& args) {
-#define PK_Q4_TILE(PER, OFFSETS) q4_tile_kernel<PER, OFFSETS>
-  return PK_Q4_PICK(args, PK_Q4_TILE);
+#define PK_Q4_TILE(PER, OFFSETS) q4_tile_kernel<_Float16, PER, OFFSETS>
+#define PK_Q4_TILE_F32(PER, OFFSETS) q4_tile_kernel<float, PER, OFFSETS>
+  return args.f16 ? PK_Q4_PICK(args, PK_Q4_TILE) : PK_Q4_PICK(args, PK_Q4_TILE_F32);
 #undef PK_Q4_TILE
+#undef PK_Q4_TILE_F32
 }
 
 // A launch: kernel, grid and threads.
@@ -733,6 +759,28 @@ Q4Plan plan(const Q4Args& args) {
   const uint64_t row_bytes =
       args.f16 ? panel_stride<_Float16>(args.inner) * 2ull : panel_stride<float>(args.inner) * 4ull;
   const bool panel = args.rows <= 16u && args.rows * row_bytes <= kPanelBytes;
+  // Too few tiles to fill the compute units: with much work each, as many
+  // parts along K as make two for each. The second launch takes some 4 us.
+  // f16, won back from 4000 blocks of K and tile on: 80 tiles (64 x 8192 x
+  // 10240) 23.2 us, rows below 35.4; 96 (192 x 8192 x 4096) 24.1 and 34.7; 160 (320
+  // x 4096 x 4096) 22.1, tiles whole 27.8; 64 (64 x 8192 x 8192) 20.0 and rows 21.4;
+  // but with 2048 blocks (128 x 4096 x 4096) 14.4 and 12.5, with 16 blocks along
+  // K (256 x 2048 x 8192) 19.7, whole 16.7, and 24 x 8192 x 8192 18.7 and rows 13.2.
+  // f32, whose blocks take eight times as long, from 1024 on: 128 x 4096 x 4096
+  // 44.2 and rows 55.9, 256 x 1024 x 4096 28.2 and 36.8, 64 x 4096 x 4096 27.8 and
+  // 28.8; but 48 x 4096 x 4096 27.2 and 23.3, 64 x 1024 x 4096 13.5 and 10.4, and
+  // 1504 x 1024 x 1024 (192 tiles, 8 blocks along K) 44.3, whole 41.9.
+  const uint64_t tiled = (uint64_t)tiles(args.rows, kTileRows) * tiles(args.columns, kTileColumns);
+  if (args.rows > (args.f16 ? 32u : 48u) && tiled <= 256u && kblocks >= (tiled < 160u ? 8u : 32u) &&
+      tiled * kblocks >= (args.f16 ? 4000u : 1024u)) {
+    const uint32_t span = tiles(kblocks, 512u / (uint32_t)tiled);
+    return {pick_tile(args), dim3((uint32_t)tiled, tiles(kblocks, span)), 256u, span};
+  }
+  // Whole tiles need the compute units full: f16, 192 (1504 x 2048 x 1024) take
+  // 17.1 us and rows 18.6, 128 (256 x 1024 x 4096 and 512 x 2048 x 2048) 10.1 and
+  // 16.2, and rows 11.0 and 16.0, 64 (256 x 2048 x 2048) 16.0 and 8.7; f32, 216
+  // (1504 x 640 x 1032) 30.0 and rows 48.6.
+  if (args.rows > 64u && tiled >= 160u) return {pick_tile(args), dim3((uint32_t)tiled), 256u, kblocks};
   if (!args.f16) {
     // 1 x 4096 x 4096: 4.2 us on the VALU, 8.1 on the matrix units; 4 rows 7.8 and 9.5.
     if (panel && args.rows <= 4u)
@@ -741,22 +789,6 @@ Q4Plan plan(const Q4Args& args) {
     if (panel) return {pick_rows<float, 1, 1, true>(args), dim3(nblocks), panel_threads(16u), 0u};
     return {pick_rows<float, 1, 1, false>(args), dim3(nblocks, tiles(args.rows, 16u)), threads(8u), 0u};
   }
-  // Too few tiles to fill the compute units: with much work each, as many
-  // parts along K as make two for each. The second launch takes some 4 us, won
-  // back from 4000 blocks of K and tile on: 80 tiles (64 x 8192 x 10240) 23.2
-  // us, rows below 35.4; 96 (192 x 8192 x 4096) 24.1 and 34.7; 160 (320 x 4096 x
-  // 4096) 22.1, tiles whole 27.8; 64 (64 x 8192 x 8192) 20.0 and rows 21.4; but
-  // with 2048 blocks (128 x 4096 x 4096) 14.4 and 12.5, with 16 blocks along K
-  // (256 x 2048 x 8192) 19.7, tiles whole 16.7, and 24 x 8192 x 8192 18.7 and rows 13.2.
-  const uint64_t tiled = (uint64_t)tiles(args.rows, kTileRows) * tiles(args.columns, kTileColumns);
-  if (args.rows > 32u && tiled <= 256u && kblocks >= 32u && tiled * kblocks >= 4000u) {
-    const uint32_t span = tiles(kblocks, 512u / (uint32_t)tiled);
-    return {pick_tile(args), dim3((uint32_t)tiled, tiles(kblocks, span)), 256u, span};
-  }
-  // Whole tiles need the compute units full: 192 (1504 x 2048 x 1024) take
-  // 17.1 us and rows 18.6, 128 (256 x 1024 x 4096 and 512 x 2048 x 2048) 10.1 and
-  // 16.2, and rows 11.0 and 16.0, 64 (256 x 2048 x 2048) 16.0 and 8.7.
-  if (args.rows > 64u && tiled >= 160u) return {pick_tile(args), dim3((uint32_t)tiled), 256u, kblocks};
   // 8 wavefronts (1 x 8192 x 8192 8.3 us, 16 8.8; 8 x 2048 x 8192 4.5 and 5.2).
   if (panel) return {pick_rows<_Float16, 1, 1, true>(args), dim3(nblocks), panel_threads(8u), 0u};
   // Two column blocks a wavefront, which share the rows' reads, where a
@@ -839,10 +871,11 @@ hipError_t launch_q4(const Q4Args& given, hipStream_t stream, hipEvent_t start, 
   if (const hipError_t e = hipGetLastError()) return e;
   if (!bytes) return hipSuccess;
   const dim3 grid(p.grid.x * (kTileVectors / 256u));
+  const auto join = args.f16 ? q4_join_kernel<_Float16> : q4_join_kernel<float>;
   if (stop)
-    hipExtLaunchKernelGGL(q4_join_kernel, grid, dim3(256), 0, stream, nullptr, stop, 0, args, p.grid.x, p.grid.y);
+    hipExtLaunchKernelGGL(join, grid, dim3(256), 0, stream, nullptr, stop, 0, args, p.grid.x, p.grid.y);
   else
-    hipLaunchKernelGGL(q4_join_kernel, grid, dim3(256), 0, stream, args, p.grid.x, p.grid.y);
+    hipLaunchKernelGGL(join, grid, dim3(256), 0, stream, args, p.grid.x, p.grid.y);
   return hipGetLastError();
 }
 

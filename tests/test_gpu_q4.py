@@ -251,6 +251,26 @@ def test_graph_and_refused_capture(abi, ctx, scope):
     op.release()
 
 
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("rows,inner,columns,group", [(640, 300, 2100, 64), (1504, 128, 1032, 0), (1504, 40, 1032, 32),
+                                                      (800, 260, 1700, 128)])
+def test_tiles(abi, ctx, scope, dtype, rows, inner, columns, group):
+    """Many rows and columns: whole tiles, edges in every direction."""
+    case = make(np.random.default_rng(inner), dtype, rows, inner, columns, group, inner == 300, bias=True,
+                activation="relu", residual=True)
+    check(run(abi, ctx, scope, case), case)
+    del case["residual"]
+    check(run(abi, ctx, scope, case, strides=dict(a=inner + 1, output=columns + 3), leads=dict(a=1, output=1)), case)
+
+
+@pytest.mark.parametrize("rows,inner,columns,group,offsets", [
+    (500, 4200, 512, 128, False), (130, 1100, 5500, 64, True), (49, 8192, 2050, 32, True)])
+def test_split_along_k_f32(abi, ctx, scope, rows, inner, columns, group, offsets):
+    case = make(np.random.default_rng(rows), np.float32, rows, inner, columns, group, offsets, bias=True,
+                activation="silu", residual=True, residual_scale=2.0)
+    check(run(abi, ctx, scope, case, strides=dict(a=inner + 1, output=columns + 2)), case)
+
+
 @pytest.mark.parametrize("rows,inner,columns,group,offsets", [
     (500, 17300, 512, 128, False),  # the last part is one block, K ends in it
     (500, 17408, 512, 0, True), (130, 4100, 5500, 64, True), (40, 8200, 8190, 32, True), (64, 8192, 8192, 128, False)])
