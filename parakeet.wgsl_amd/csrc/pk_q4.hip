@@ -10,6 +10,15 @@
 // a pair out as two f16 (1024 + code or 1024 + 16 code, whose ulp is a code),
 // and one packed operation makes them code - 8.
 // Scales follow in the same order, per_block (1, 2 or 4) a column and block.
+//
+// One row is bound by the weight's bytes: 1 x 4096 x 8192 5.7 us (3.5 at the
+// rate of a copy, 4.9 TB/s). From some 32 rows on it is the instructions: a
+// SIMD issues a matrix instruction (8.05 ns) or an fma (1.25 ns) but hardly
+// both at once, one and 8 fma take 17.1 ns, so that decoding and scaling
+// count in full: per 32 k and 16 columns 9 and, once a group, 16 operations
+// for 4 matrix instructions. 64 x 8192 x 8192 with offsets 24.1 us, of which
+// 10.2 are these instructions and the rest waits for rows and codes; 1504 x
+// 1024 x 4096 20.3 us, 0.62 PFLOP/s, and x 4096 x 4096 60 us, 0.84.
 #include "pk_internal.h"
 
 namespace pk {
@@ -136,6 +145,32 @@ __device__ __forceinline__ void multiply(const Fragment<float> (&a)[MT], const h
     for (int mt = 0; mt < MT; ++mt)
       acc[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[mt].c[j / 4].v[j % 4], (float)b[j], acc[mt][nt], 0, 0, 0);
 }
+
+// The sums of 16 rows over the k of a group, in each lane those of its four
+// rows of output: a product with ones. f32: a lane adds what it holds and one
+// instruction a group adds the lanes, where a product would take eight for
+// each 32 k (1504 x 1024 x 4096, groups of 32: 130 us, 161 with those).
+template <typename T>
+struct RowSums;
+template <>
+struct RowSums<_Float16> {
+  floatx4 s;
+  __device__ __forceinline__ void clear() { s = (floatx4)0.0f; }
+  __device__ __forceinline__ void add(const Fragment<_Float16>& a) { multiply(a, (half8)(_Float16)1.0f, s); }
+  __device__ __forceinline__ floatx4 total() const { return s; }
+};
+template <>
+struct RowSums<float> {
+  float s;
+  __device__ __forceinline__ void clear() { s = 0.0f; }
+  __device__ __forceinline__ void add(const Fragment<float>& a) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += a.c[j / 4].v[j % 4];
+  }
+  __device__ __forceinline__ floatx4 total() const {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(s, 1.0f, (floatx4)0.0f, 0, 0, 0);
+  }
+};
 
 // The activation of one output.
 __device__ __forceinline__ float activate(int activation, float v) {
@@ -344,12 +379,12 @@ __global__ __launch_bounds__((64 * most_waves<T, MT, NT, PANEL>())) void q4_rows
   if (wave + waves < kblocks) load_weight(turned(wave + waves), ahead[1]);
   if constexpr (PANEL) __syncthreads();
 
-  floatx4 acc[MT][NT], part[MT][NT], sums[MT];
+  floatx4 acc[MT][NT], part[MT][NT];
+  RowSums<T> sums[MT];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = (floatx4)0.0f;
-  const half8 one = (half8)(_Float16)1.0f;
   const Decoder decode;
 
   for (uint32_t kb = wave; kb < kblocks; kb += waves) {
@@ -378,19 +413,21 @@ __global__ __launch_bounds__((64 * most_waves<T, MT, NT, PANEL>())) void q4_rows
       if constexpr (OFFSETS)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          if (i % kStep == 0) sums[mt] = (floatx4)0.0f;
-          multiply(a[mt], one, sums[mt]);
+          if (i % kStep == 0) sums[mt].clear();
+          sums[mt].add(a[mt]);
         }
       if ((i + 1) % kStep == 0) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
+          floatx4 sum;
+          if constexpr (OFFSETS) sum = sums[mt].total();
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               acc[mt][nt][r] = __builtin_fmaf(part[mt][nt][r], (float)w.scales[nt][i / kStep], acc[mt][nt][r]);
               if (OFFSETS)
-                acc[mt][nt][r] = __builtin_fmaf(sums[mt][r], (float)w.offsets[nt][i / kStep], acc[mt][nt][r]);
+                acc[mt][nt][r] = __builtin_fmaf(sum[r], (float)w.offsets[nt][i / kStep], acc[mt][nt][r]);
             }
         }
       }
@@ -579,7 +616,6 @@ __global__ __launch_bounds__(256, OFFSETS || sizeof(T) == 4 ? 2 : 3) void q4_til
     for (int t = 0; t < kCopies; ++t) reinterpret_cast<Chunk<T>*>(lds[buffer])[t * 256u + threadIdx.x] = copy[t];
   };
 
-  const half8 one = (half8)(_Float16)1.0f;
   const Decoder decode;
   floatx4 acc[4][2];
 #pragma unroll
@@ -589,7 +625,8 @@ __global__ __launch_bounds__(256, OFFSETS || sizeof(T) == 4 ? 2 : 3) void q4_til
 
   const auto multiply_block = [&](uint32_t kb, const Weight& w) {
     const Chunk<T>* rows = reinterpret_cast<const Chunk<T>*>(lds[kb & 1u]);
-    floatx4 part[4][2], sums[4];
+    floatx4 part[4][2];
+    RowSums<T> sums[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       Fragment<T> a[4];
@@ -611,20 +648,23 @@ __global__ __launch_bounds__(256, OFFSETS || sizeof(T) == 4 ? 2 : 3) void q4_til
       if constexpr (OFFSETS)
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) {
-          if (i % kStep == 0) sums[mt] = (floatx4)0.0f;
-          multiply(a[mt], one, sums[mt]);
+          if (i % kStep == 0) sums[mt].clear();
+          sums[mt].add(a[mt]);
         }
       if ((i + 1) % kStep == 0) {
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt)
+        for (int mt = 0; mt < 4; ++mt) {
+          floatx4 sum;
+          if constexpr (OFFSETS) sum = sums[mt].total();
 #pragma unroll
           for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               acc[mt][nt][r] = __builtin_fmaf(part[mt][nt][r], (float)w.scales[nt][i / kStep], acc[mt][nt][r]);
               if (OFFSETS)
-                acc[mt][nt][r] = __builtin_fmaf(sums[mt][r], (float)w.offsets[nt][i / kStep], acc[mt][nt][r]);
+                acc[mt][nt][r] = __builtin_fmaf(sum[r], (float)w.offsets[nt][i / kStep], acc[mt][nt][r]);
             }
+        }
       }
       __builtin_amdgcn_sched_barrier(0);  // one step's operands at a time in registers
     }

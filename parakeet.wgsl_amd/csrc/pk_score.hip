@@ -1,8 +1,11 @@
 // pk_score.hip - token scores for gfx950 (include/pk_score.h has the formulas
 // and what rows of infinities and NaN give).
 //
-// Bound by memory: a logit is loaded once and stays in registers, as 16-byte
-// vectors, through the maximum, the sums relative to it and the search for
+// Bound by memory where rows are many and f32: 2048 of 32000 logits 50.3 us,
+// 5.2 TB/s where a copy reaches 4.9. f16 is bound by the VALU, some 10
+// operations a logit (two converts, fma, exponential, sums): 3008 of 1025 5.4
+// us, 3.0 of them the launch. A logit is loaded once and stays in registers,
+// as 16-byte vectors, through the maximum, the sums relative to it and the search for
 // alternatives. A group of 64, 256 or 1024 threads holds a row, or a part of
 // one: rows longer than a group holds, and long rows when there are few, are
 // split, and a second launch joins the parts' maxima, sums and alternatives.
