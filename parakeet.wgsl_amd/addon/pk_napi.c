@@ -5,7 +5,8 @@
  * (include/pk_attention.h), the row LayerNorm (include/pk_layernorm.h), the
  * subsampling convolutions (include/pk_subsampling.h), the encoder graph
  * (include/pk_encoder.h), the norms around a block (include/pk_block_norm.h),
- * the 4-bit product (include/pk_q4.h) and token scores (include/pk_score.h). It is the thin native layer under the JavaScript
+ * the 4-bit product (include/pk_q4.h) and token scores
+ * (include/pk_score.h). It is the thin native layer under the JavaScript
  * host in ../host: every function forwards to one pk_* call, converts device
  * pointers to BigInt, and turns a failing pk_status into a thrown Error
  * (RangeError for PK_RANGE_ERROR, as the reference throws RangeError for
