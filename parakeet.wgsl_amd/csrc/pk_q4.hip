@@ -101,14 +101,24 @@ struct Chunk {
   V v;
   typedef T U __attribute__((ext_vector_type(N), aligned(sizeof(T))));  // at any address of an element
   __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const U*>(p); }
-  // p[0] is element k of a row; what lies from K on is zero.
+  // p[0] is element k of a row; what lies from K on is zero. Without a branch
+  // for each chunk, which would have it wait for the one before: the row's
+  // last 16 bytes, shifted by what lies behind K (64 x 1000 x 1000 7.4 us, with a
+  // branch for each 9.3).
   __device__ __forceinline__ void load(const T* p, uint32_t k, uint32_t inner) {
-    if (k + N <= inner) {
-      load(p);
-    } else {
+    if (inner < (uint32_t)N) {
 #pragma unroll
       for (int j = 0; j < N; ++j) v[j] = k + j < inner ? p[j] : (T)0.0f;
+      return;
     }
+    const uint32_t behind = k + N > inner ? k + N - inner : 0u;
+    load(p - behind);
+    typedef uint64_t words __attribute__((ext_vector_type(2)));
+    const words w = __builtin_bit_cast(words, v);
+    const uint32_t bits = behind * (8u * sizeof(T)), part = bits & 63u;
+    const uint64_t low = bits < 64u ? w[0] : w[1], high = bits < 64u ? w[1] : 0u;
+    const words shifted = {low >> part | (high << 1) << (63u - part), high >> part};
+    v = __builtin_bit_cast(V, bits < 128u ? shifted : (words)0);
   }
 };
 
@@ -179,14 +189,22 @@ __device__ __forceinline__ float activate(int activation, float v) {
   return v;
 }
 
+// What an output adds: its bias and residual.
+struct Extra {
+  float bias = 0.0f, residual = 0.0f;
+};
+template <typename T>
+__device__ __forceinline__ Extra load_extra(const Q4Args& args, uint32_t m, uint32_t n) {
+  Extra e;
+  if (args.bias) e.bias = args.bias[n];
+  if (args.residual) e.residual = (float)static_cast<const T*>(args.residual)[(uint64_t)m * args.residual_stride + n];
+  return e;
+}
 // bias, activation and residual of one output, stored.
 template <typename T>
-__device__ __forceinline__ void finish(const Q4Args& args, uint32_t m, uint32_t n, float v) {
-  if (args.bias) v += args.bias[n];
-  v = activate(args.activation, v);
-  if (args.residual)
-    v = __builtin_fmaf(args.residual_scale, v,
-                       (float)static_cast<const T*>(args.residual)[(uint64_t)m * args.residual_stride + n]);
+__device__ __forceinline__ void finish(const Q4Args& args, uint32_t m, uint32_t n, float v, const Extra& e) {
+  v = activate(args.activation, args.bias ? v + e.bias : v);
+  if (args.residual) v = __builtin_fmaf(args.residual_scale, v, e.residual);
   static_cast<T*>(args.out)[(uint64_t)m * args.out_stride + n] = (T)v;
 }
 
@@ -198,7 +216,7 @@ __device__ __forceinline__ void finish_row(const Q4Args& args, uint32_t m, uint3
   if (n + 8u > args.columns) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (n + j < args.columns) finish<T>(args, m, n + j, v[j]);
+      if (n + j < args.columns) finish<T>(args, m, n + j, v[j], load_extra<T>(args, m, n + j));
     return;
   }
   if (args.bias) {
@@ -445,13 +463,26 @@ __global__ __launch_bounds__((64 * most_waves<T, MT, NT, PANEL>())) void q4_rows
         partial[(wave * 16u * MT + 16 * mt + 4 * quad + r) * kWidth + 16 * nt + column] = acc[mt][nt][r];
   __syncthreads();
   const uint32_t outputs = min(args.rows - m0, 16u * MT) * (16u * NT);
-  for (uint32_t id = threadIdx.x; id < outputs; id += blockDim.x) {
-    const uint32_t m = id / (16u * NT), n = id % (16u * NT);
-    if (blockIdx.x * (16u * NT) + n >= args.columns) continue;
-    float v = 0.0f;
+  // kBatch outputs a thread at a time, whose residuals are under way together.
+  constexpr uint32_t kBatch = MT == 1 ? 1u : 4u;
+  for (uint32_t from = threadIdx.x; from < outputs; from += kBatch * blockDim.x) {
+    Extra extra[kBatch];
+    bool has[kBatch];
+#pragma unroll
+    for (uint32_t b = 0; b < kBatch; ++b) {
+      const uint32_t id = from + b * blockDim.x, n = blockIdx.x * (16u * NT) + id % (16u * NT);
+      has[b] = id < outputs && n < args.columns;
+      if (has[b]) extra[b] = load_extra<T>(args, m0 + id / (16u * NT), n);
+    }
+#pragma unroll
+    for (uint32_t b = 0; b < kBatch; ++b) {
+      if (!has[b]) continue;
+      const uint32_t id = from + b * blockDim.x, m = id / (16u * NT), n = id % (16u * NT);
+      float v = 0.0f;
 #pragma unroll 4
-    for (uint32_t w = 0; w < waves; ++w) v += partial[(w * 16u * MT + m) * kWidth + n];
-    finish<T>(args, m0 + m, blockIdx.x * (16u * NT) + n, v);
+      for (uint32_t w = 0; w < waves; ++w) v += partial[(w * 16u * MT + m) * kWidth + n];
+      finish<T>(args, m0 + m, blockIdx.x * (16u * NT) + n, v, extra[b]);
+    }
   }
 }
 
@@ -536,7 +567,7 @@ __global__ __launch_bounds__(1024) void q4_vector_kernel(Q4Args args) {
     float v = 0.0f;
 #pragma unroll 4
     for (uint32_t w = 0; w < waves; ++w) v += partial[(w * ROWS + m) * 16u + id % 16u];
-    finish<float>(args, m, n, v);
+    finish<float>(args, m, n, v, load_extra<float>(args, m, n));
   }
 }
 
@@ -746,9 +777,13 @@ __global__ __launch_bounds__(256) void q4_join_kernel(Q4Args args, uint32_t tile
   floatx4 sum = (floatx4)0.0f;
 #pragma unroll 8
   for (uint32_t p = 0; p < parts; ++p) sum += sums[(uint64_t)p * tiles * kTileVectors];
+  Extra extra[4];
 #pragma unroll
   for (uint32_t r = 0; r < 4u; ++r)
-    if (m + r < args.rows) finish<T>(args, m + r, n, sum[r]);
+    if (m + r < args.rows) extra[r] = load_extra<T>(args, m + r, n);
+#pragma unroll
+  for (uint32_t r = 0; r < 4u; ++r)
+    if (m + r < args.rows) finish<T>(args, m + r, n, sum[r], extra[r]);
 }
 
 typedef void (*Kernel)(Q4Args);
@@ -786,10 +821,41 @@ struct Q4Plan {
   uint32_t span;  // 0: no tile kernel
   uint64_t part_bytes() const { return span && grid.y > 1u ? (uint64_t)grid.x * grid.y * kTileVectors * 16u : 0u; }
 };
+
+// f16 kernels of few rows: rows and columns of a workgroup in 16, wavefronts
+// at most, and the us that a compute unit takes for a block of K and for the
+// rest of a workgroup, fitted to 150 products of 32 to 300 rows, K 512 to 8192,
+// N 256 to 8192 (groups of 128, no offsets).
+struct RowsShape {
+  uint32_t mt, nt, waves;
+  float block, rest;
+};
+constexpr RowsShape kRowsShapes[] = {{1, 1, 16, 0.07f, 0.3f},   {1, 2, 16, 0.115f, 0.35f}, {2, 1, 16, 0.12f, 0.6f},
+                                     {2, 2, 8, 0.165f, 0.8f},  {4, 1, 8, 0.215f, 1.6f},  {4, 2, 8, 0.26f, 2.0f}};
+// The kernels of kRowsShapes.
+Kernel pick_rows_f16(const Q4Args& args, uint32_t shape) {
+  switch (shape) {
+    case 0: return pick_rows<_Float16, 1, 1, false>(args);
+    case 1: return pick_rows<_Float16, 1, 2, false>(args);
+    case 2: return pick_rows<_Float16, 2, 1, false>(args);
+    case 3: return pick_rows<_Float16, 2, 2, false>(args);
+    case 4: return pick_rows<_Float16, 4, 1, false>(args);
+    default: return pick_rows<_Float16, 4, 2, false>(args);
+  }
+}
+// us of a launch of f16 tiles, `blocks` of K each, fitted to the same products:
+// a compute unit holds three, of which one leaves it idle half the time.
+float tile_time(uint64_t tiles, uint32_t blocks) {
+  const float each = (float)((tiles + 255u) / 256u);
+  return 1.5f * each + (each > 1.0f ? 0.55f * each : 0.72f) * (float)blocks;
+}
+
 Q4Plan plan(const Q4Args& args) {
   const auto tiles = [](uint32_t n, uint32_t size) { return (n + size - 1u) / size; };
   const uint32_t kblocks = tiles(args.inner, 128u), nblocks = tiles(args.columns, 16u);
-  const auto threads = [&](uint32_t most) { return 64u * (kblocks < most ? kblocks : most); };
+  // Four wavefronts at least, for the outputs if not for K: 64 x 60 x 614 with
+  // a residual 7.2 us, with one for its one block 11.1.
+  const auto threads = [&](uint32_t most) { return 64u * (kblocks < 4u ? 4u : kblocks < most ? kblocks : most); };
   // Wavefronts of the kernels with the rows in LDS: two blocks of K each,
   // from 4 (1 x 640 x 1032 3.2 us, 3.6 with one block each) to `most`.
   const auto panel_threads = [&](uint32_t most) {
@@ -799,29 +865,24 @@ Q4Plan plan(const Q4Args& args) {
   const uint64_t row_bytes =
       args.f16 ? panel_stride<_Float16>(args.inner) * 2ull : panel_stride<float>(args.inner) * 4ull;
   const bool panel = args.rows <= 16u && args.rows * row_bytes <= kPanelBytes;
-  // Too few tiles to fill the compute units: with much work each, as many
-  // parts along K as make two for each. The second launch takes some 4 us.
-  // f16, won back from 4000 blocks of K and tile on: 80 tiles (64 x 8192 x
-  // 10240) 23.2 us, rows below 35.4; 96 (192 x 8192 x 4096) 24.1 and 34.7; 160 (320
-  // x 4096 x 4096) 22.1, tiles whole 27.8; 64 (64 x 8192 x 8192) 20.0 and rows 21.4;
-  // but with 2048 blocks (128 x 4096 x 4096) 14.4 and 12.5, with 16 blocks along
-  // K (256 x 2048 x 8192) 19.7, whole 16.7, and 24 x 8192 x 8192 18.7 and rows 13.2.
-  // f32, whose blocks take eight times as long, from 1024 on: 128 x 4096 x 4096
-  // 44.2 and rows 55.9, 256 x 1024 x 4096 28.2 and 36.8, 64 x 4096 x 4096 27.8 and
-  // 28.8; but 48 x 4096 x 4096 27.2 and 23.3, 64 x 1024 x 4096 13.5 and 10.4, and
-  // 1504 x 1024 x 1024 (192 tiles, 8 blocks along K) 44.3, whole 41.9.
+  // Tiles whole, or too few to fill the compute units in as many parts along K
+  // as make two for each.
   const uint64_t tiled = (uint64_t)tiles(args.rows, kTileRows) * tiles(args.columns, kTileColumns);
-  if (args.rows > (args.f16 ? 32u : 48u) && tiled <= 256u && kblocks >= (tiled < 160u ? 8u : 32u) &&
-      tiled * kblocks >= (args.f16 ? 4000u : 1024u)) {
-    const uint32_t span = tiles(kblocks, 512u / (uint32_t)tiled);
-    return {pick_tile(args), dim3((uint32_t)tiled, tiles(kblocks, span)), 256u, span};
-  }
-  // Whole tiles need the compute units full: f16, 192 (1504 x 2048 x 1024) take
-  // 17.1 us and rows 18.6, 128 (256 x 1024 x 4096 and 512 x 2048 x 2048) 10.1 and
-  // 16.2, and rows 11.0 and 16.0, 64 (256 x 2048 x 2048) 16.0 and 8.7; f32, 216
-  // (1504 x 640 x 1032) 30.0 and rows 48.6.
-  if (args.rows > 64u && tiled >= 160u) return {pick_tile(args), dim3((uint32_t)tiled), 256u, kblocks};
+  const uint32_t most_parts = tiled <= 256u ? 512u / (uint32_t)tiled : 1u;
+  const uint32_t span = tiles(kblocks, most_parts), parts = tiles(kblocks, span);
+  const auto tile_plan = [&](uint32_t blocks) {
+    return Q4Plan{pick_tile(args), dim3((uint32_t)tiled, tiles(kblocks, blocks)), 256u, blocks};
+  };
   if (!args.f16) {
+    // A block of a tile takes eight times as long as in f16: parts, whose
+    // second launch takes some 4 us, win from 1024 blocks of K and tile on: 128
+    // x 4096 x 4096 44.2 us and rows 55.9, 256 x 1024 x 4096 28.2 and 36.8, 64 x
+    // 4096 x 4096 27.8 and 28.8; but 48 x 4096 x 4096 27.2 and 23.3, 64 x 1024 x
+    // 4096 13.5 and 10.4, and 1504 x 1024 x 1024 (192 tiles, 8 blocks along K)
+    // 44.3, whole 41.9. Whole tiles: 216 (1504 x 640 x 1032) 30.0 and rows 48.6.
+    if (args.rows > 48u && parts > 1u && kblocks >= (tiled < 160u ? 8u : 32u) && tiled * kblocks >= 1024u)
+      return tile_plan(span);
+    if (args.rows > 64u && tiled >= 160u) return tile_plan(kblocks);
     // 1 x 4096 x 4096: 4.2 us on the VALU, 8.1 on the matrix units; 4 rows 7.8 and 9.5.
     if (panel && args.rows <= 4u)
       return {args.rows == 1u ? pick_vector<1>(args) : args.rows == 2u ? pick_vector<2>(args) : pick_vector<4>(args),
@@ -831,19 +892,29 @@ Q4Plan plan(const Q4Args& args) {
   }
   // 8 wavefronts (1 x 8192 x 8192 8.3 us, 16 8.8; 8 x 2048 x 8192 4.5 and 5.2).
   if (panel) return {pick_rows<_Float16, 1, 1, true>(args), dim3(nblocks), panel_threads(8u), 0u};
-  // Two column blocks a wavefront, which share the rows' reads, where a
-  // workgroup for each compute unit is left: 32 x 4096 x 8192 9.2 us (one:
-  // 12.6), but 32 x 4096 x 4096, where half would be left, 8.0 (one: 7.0).
-  const uint32_t mt = args.rows <= 16u ? 1u : args.rows <= 32u ? 2u : 4u, row_tiles = tiles(args.rows, 16u * mt);
-  const bool two = (uint64_t)tiles(nblocks, 2u) * row_tiles >= 256u;
-  const dim3 grid(two ? tiles(nblocks, 2u) : nblocks, row_tiles);
-  if (mt == 1u)
-    return {two ? pick_rows<_Float16, 1, 2, false>(args) : pick_rows<_Float16, 1, 1, false>(args), grid, threads(16u),
-            0u};
-  if (mt == 2u)
-    return {two ? pick_rows<_Float16, 2, 2, false>(args) : pick_rows<_Float16, 2, 1, false>(args), grid,
-            threads(two ? 8u : 16u), 0u};
-  return {two ? pick_rows<_Float16, 4, 2, false>(args) : pick_rows<_Float16, 4, 1, false>(args), grid, threads(8u), 0u};
+  // The kernel that the times above make the fastest: 64 x 4096 x 2048 6.4 us
+  // with 16 rows a workgroup, 7.0 with 32, 9.7 with 64, parts of tiles 12.5; 64 x
+  // 4096 x 4096 10.9, 8.6, 10.8 and 13.3; 64 x 4096 x 8192 21.4, 16.1, 12.9 and 15.3;
+  // 300 x 8192 x 1024 22.9, 22.3, 29.3 and 17.0; 300 x 2048 x 8192 54.4, 45.2, 35.5
+  // and tiles whole 22.3. Parts: 5.5 us for the sums' way through memory and
+  // the second launch.
+  uint32_t best = 0;
+  float time = 0.0f;
+  dim3 grid;
+  for (uint32_t i = 0; i < sizeof(kRowsShapes) / sizeof(kRowsShapes[0]); ++i) {
+    const RowsShape& s = kRowsShapes[i];
+    if (s.mt > 1u && args.rows <= 8u * s.mt) break;  // half of its rows at most
+    const uint32_t x = tiles(nblocks, s.nt), y = tiles(args.rows, 16u * s.mt);
+    const float t = (float)(((uint64_t)x * y + 255u) / 256u) * (s.rest + s.block * (float)kblocks);
+    if (i && t >= time) continue;
+    best = i;
+    time = t;
+    grid = dim3(x, y);
+  }
+  const float whole = tile_time(tiled, kblocks), split = 5.5f + tile_time(tiled * parts, span);
+  if (parts > 1u && split < time && split < whole) return tile_plan(span);
+  if (whole < time) return tile_plan(kblocks);
+  return {pick_rows_f16(args, best), grid, threads(kRowsShapes[best].waves), 0u};
 }
 
 }  // namespace
@@ -893,7 +964,8 @@ uint64_t q4_workspace(const Q4Args& args) {
     const uint64_t wanted = plan(some).part_bytes();
     if (wanted > bytes) bytes = wanted;
   };
-  for (uint32_t rows = kTileRows; rows < args.rows && rows <= 512u * kTileRows; rows += kTileRows) count(rows);
+  // A plan depends on the rows in 16; more than 512 tiles are never split.
+  for (uint32_t rows = 16u; rows < args.rows && rows <= 512u * kTileRows; rows += 16u) count(rows);
   count(args.rows);
   return bytes;
 }
