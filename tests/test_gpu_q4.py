@@ -78,7 +78,8 @@ def operands(abi, scope, case, strides=None, leads=None):
         if n in case:
             kw[n] = scope.put(case[n])
     rows, columns = len(case["a"]), case["codes"].shape[1]
-    values = {"a": case["a"], "output": np.full((rows, columns), 321, case["a"].dtype), "residual": case.get("residual")}
+    values = {"a": case["a"], "output": np.full((rows, columns), 321, case["a"].dtype),
+              "residual": case.get("residual")}
     for n, v in values.items():
         if v is None:
             continue
@@ -249,6 +250,17 @@ def test_graph_and_refused_capture(abi, ctx, scope):
         ctx.synchronize()
     graph.release()
     op.release()
+
+
+@pytest.mark.parametrize("rows,inner,columns,group,offsets", [
+    (250, 300, 1100, 32, True), (87, 300, 5003, 64, True), (60, 1500, 8200, 0, False), (50, 2100, 7000, 128, True),
+    (63, 1990, 8190, 32, True), (1000, 2050, 200, 64, False)])
+def test_workgroups_of_16_to_64_rows(abi, ctx, scope, rows, inner, columns, group, offsets):
+    """Shapes between the few rows of a stream and whole tiles, with edges."""
+    case = make(np.random.default_rng(rows), np.float16, rows, inner, columns, group, offsets, bias=True,
+                activation="silu", residual=True, residual_scale=0.5)
+    strides = dict(output=columns + 1, residual=columns + 3)
+    check(run(abi, ctx, scope, case, strides=strides, leads=dict(output=1)), case)
 
 
 @pytest.mark.parametrize("dtype", [np.float16, np.float32])
