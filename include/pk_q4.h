@@ -73,10 +73,9 @@ int pk_q4_create(pk_context *ctx, const pk_q4_desc *desc, void *stream, pk_q4_op
 /* The first `active_rows` rows (0 = all); rows behind them are left as they
    were. A row's outputs may differ in their last bits between row counts
    (another order of the sum over K), never from launch to launch of one
-   count. May be captured into graphs. Tiles split along K (33 rows and more
-   of a long K, when they are few) meet in memory of the op: launches of one
-   op, eager or replayed, must be ordered by the caller, as their outputs ask
-   for anyway. */
+   count. May be captured into graphs. Few tiles of a long K are split along
+   it and meet in memory of the op: launches of one op, eager or replayed,
+   must be ordered by the caller, as their outputs ask for anyway. */
 int pk_q4_enqueue(pk_q4_op *op, uint32_t active_rows, void *stream);
 int pk_q4_enqueue_timed(pk_q4_op *op, uint32_t active_rows, void *stream, void *start_event, void *end_event);
 /* Device bytes of the weight in the op: half a byte per weight (K padded to
