@@ -170,13 +170,16 @@ def _buffer(tensor):
 
 
 _context = None
+_LEGACY_STREAM = 1  # hipStreamLegacy: torch's default stream, whose handle 0 stands for the context's own in a call
 
 
 class State:
     """What a user's program holds between calls: its tensors, and the
-    framework's op over them where that is what runs."""
+    framework's op over them where that is what runs, with the stream that it
+    works on, torch's current one when the state was made."""
 
     op = None
+    stream = None
 
     def __init__(self, case, tensors, outputs):
         self.case, self.tensors, self.outputs = case, tensors, outputs
@@ -242,6 +245,7 @@ def prepare(case, seed):
     state = State(case, t, outputs)
     if own:
         state.op = _op(case, t, outputs)
+        state.stream = torch.cuda.current_stream().cuda_stream or _LEGACY_STREAM
     return state
 
 
@@ -318,8 +322,11 @@ def _run_score(case, t):
 
 
 def run(state):
+    """One pass, in order with what the stream that was torch's current one in
+    `prepare` holds, as the plain form is. `own`: the outputs are the state's,
+    which the next pass on that stream writes again."""
     if own:
-        state.op.enqueue()
+        state.op.enqueue(0, state.stream)
         return state.outputs
     return {"norm": _run_norm, "q4": _run_q4, "score": _run_score}[state.case["kind"]](state.case, state.tensors)
 
