@@ -20,6 +20,7 @@
 // 10.2 are these instructions and the rest waits for rows and codes; 1504 x
 // 1024 x 4096 20.3 us, 0.62 PFLOP/s, and x 4096 x 4096 60 us, 0.84.
 #include "pk_internal.h"
+#include "pk_wave.h"
 
 namespace pk {
 namespace {
@@ -415,6 +416,7 @@ __global__ __launch_bounds__((64 * most_waves<T, MT, NT, PANEL>())) void q4_rows
     if constexpr (!PANEL) {
 #pragma unroll
       for (int t = 0; t < kCopies; ++t) stage[t * 64u + lane] = copy[t];
+      wave::sync();  // a lane reads what others copied
       if (kb + waves < kblocks) load_rows(turned(kb + waves));
     }
 #pragma unroll
@@ -453,6 +455,7 @@ __global__ __launch_bounds__((64 * most_waves<T, MT, NT, PANEL>())) void q4_rows
         }
       }
     }
+    if constexpr (!PANEL) wave::sync();  // every lane has read, and the next block is copied
   }
   float* partial = reinterpret_cast<float*>(lds);  // [waves][16 MT][16 NT + 1]
   constexpr int kWidth = 16 * NT + 1;
@@ -751,8 +754,7 @@ __global__ __launch_bounds__(256, OFFSETS || sizeof(T) == 4 ? 2 : 3) void q4_til
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           part_out[(16 * mt + 4 * quad + r) * kWidth + 16 * nt + column] = acc[2 * half + mt][nt][r];
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    wave::sync();
 #pragma unroll
     for (int pass = 0; pass < 2; ++pass) {
       const uint32_t r = 16u * pass + (lane >> 2), c = 8u * (lane & 3u);
@@ -762,8 +764,7 @@ __global__ __launch_bounds__(256, OFFSETS || sizeof(T) == 4 ? 2 : 3) void q4_til
       for (int j = 0; j < 8; ++j) v[j] = part_out[r * kWidth + c + j];
       if (m < args.rows) finish_row<T>(args, m, n, v);
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    wave::sync();
   }
 }
 

@@ -52,13 +52,8 @@ __device__ __forceinline__ uint64_t wave_max_key(uint64_t key) {
 // Orders LDS traffic between the threads of a group.
 template <int GROUP>
 __device__ __forceinline__ void group_sync() {
-  if constexpr (GROUP > 64) {
-    __syncthreads();
-  } else {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  }
+  if constexpr (GROUP > 64) __syncthreads();
+  else wave::sync();
 }
 
 // A threshold that at least `count` of the 64 lanes' values reach, close to

@@ -3,7 +3,7 @@
 // register (a shift within 16 lanes, then the broadcast of a row's last lane
 // into the next), where a shuffle goes through the LDS crossbar. The result
 // is lane 63's, read into a scalar register, so it is uniform, and the order
-// of the sums is fixed.
+// of the sums is fixed. sync() orders what lanes exchange through LDS.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -39,6 +39,16 @@ __device__ __forceinline__ float max(float x) {
   return __uint_as_float(reduce_bits(__float_as_uint(x), 0xff800000u, [](uint32_t a, uint32_t b) {
     return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
   }));
+}
+
+// LDS that lanes of this wavefront wrote before is what its lanes read behind,
+// and what they read before is not overwritten yet. The LDS takes a
+// wavefront's accesses in their order, so this is an order for the compiler,
+// which sees one lane's addresses, and no instruction.
+__device__ __forceinline__ void sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 }  // namespace wave
