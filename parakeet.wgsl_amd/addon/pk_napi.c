@@ -858,26 +858,47 @@ static napi_value js_attention_plan(napi_env env, napi_callback_info info) {
 
 /* ---- block norm, 4-bit product, token scores ------------------------------ */
 
-/* The optional binding `name` with its capacity `nameBytes`. */
-static void prop_binding(napi_env env, napi_value o, const char *name, void *pointer, uint64_t *bytes) {
+/* Optional fields: nothing where `name` is absent (or undefined or null), and
+   an error where its value is not one of the field's, so that no field is left
+   out because it was given wrongly. */
+static int bad_field(napi_env env, const char *name, const char *what) {
+  char message[96];
+  snprintf(message, sizeof message, "%s must be %s", name, what);
+  bad_argument(env, message);
+  return 0;
+}
+
+static int optional_u32(napi_env env, napi_value o, const char *name, uint32_t *out) {
+  napi_value v;
+  if (!prop(env, o, name, &v) || get_u32(env, v, out)) return 1;
+  return bad_field(env, name, "a non-negative 32-bit integer");
+}
+
+/* *has tells whether it is there. */
+static int optional_float(napi_env env, napi_value o, const char *name, int32_t *has, float *out) {
+  napi_value v;
+  double value = 0;
+  if (!prop(env, o, name, &v)) return 1;
+  if (napi_get_value_double(env, v, &value) != napi_ok) return bad_field(env, name, "a number");
+  *has = 1;
+  *out = (float)value;
+  return 1;
+}
+
+/* The binding `name` with its capacity `nameBytes`, which has to be there with it. */
+static int optional_binding(napi_env env, napi_value o, const char *name, void *pointer, uint64_t *bytes) {
   char key[32];
+  napi_value v;
   uint64_t address = 0;
   *bytes = 0;
-  if (prop_u64(env, o, name, &address)) {
+  if (prop(env, o, name, &v)) {
+    if (!get_u64(env, v, &address)) return bad_field(env, name, "a device pointer");
     snprintf(key, sizeof key, "%sBytes", name);
-    prop_u64(env, o, key, bytes);
+    if (!prop_u64(env, o, key, bytes)) return bad_field(env, key, "a byte count");
   }
   void *p = (void *)(uintptr_t)address;
   memcpy(pointer, &p, sizeof p);
-}
-
-/* The optional number `name`; *has tells whether it is there. */
-static void prop_float(napi_env env, napi_value o, const char *name, int32_t *has, float *out) {
-  napi_value v;
-  double value = 0;
-  if (!prop(env, o, name, &v) || napi_get_value_double(env, v, &value) != napi_ok) return;
-  *has = 1;
-  *out = (float)value;
+  return 1;
 }
 
 /* {label, precision, kind, rows, channels, input, gamma?, beta?, gate?,
@@ -896,24 +917,24 @@ static int parse_block_norm_desc(napi_env env, napi_value o, pk_block_norm_desc 
     return 0;
   }
   d->kind = (int32_t)kind;
-  prop_binding(env, o, "input", &d->input, &d->input_bytes);
-  prop_u32(env, o, "inputStride", &d->input_stride);
-  prop_binding(env, o, "gamma", &d->gamma, &d->gamma_bytes);
-  prop_binding(env, o, "beta", &d->beta, &d->beta_bytes);
-  prop_binding(env, o, "gate", &d->gate, &d->gate_bytes);
-  prop_u32(env, o, "gateStride", &d->gate_stride);
   d->gate_rows = 1;
-  prop_u32(env, o, "gateRows", &d->gate_rows);
-  prop_binding(env, o, "residual", &d->residual, &d->residual_bytes);
-  prop_u32(env, o, "residualStride", &d->residual_stride);
-  prop_float(env, o, "residualScale", &d->has_residual_scale, &d->residual_scale);
-  prop_binding(env, o, "output", &d->output, &d->output_bytes);
-  prop_u32(env, o, "outputStride", &d->output_stride);
-  prop_binding(env, o, "nextGamma", &d->next_gamma, &d->next_gamma_bytes);
-  prop_binding(env, o, "nextBeta", &d->next_beta, &d->next_beta_bytes);
-  prop_binding(env, o, "nextOutput", &d->next_output, &d->next_output_bytes);
-  prop_u32(env, o, "nextOutputStride", &d->next_output_stride);
-  prop_float(env, o, "epsilon", &d->has_epsilon, &d->epsilon);
+  if (!optional_binding(env, o, "input", &d->input, &d->input_bytes) ||
+      !optional_u32(env, o, "inputStride", &d->input_stride) ||
+      !optional_binding(env, o, "gamma", &d->gamma, &d->gamma_bytes) ||
+      !optional_binding(env, o, "beta", &d->beta, &d->beta_bytes) ||
+      !optional_binding(env, o, "gate", &d->gate, &d->gate_bytes) ||
+      !optional_u32(env, o, "gateStride", &d->gate_stride) || !optional_u32(env, o, "gateRows", &d->gate_rows) ||
+      !optional_binding(env, o, "residual", &d->residual, &d->residual_bytes) ||
+      !optional_u32(env, o, "residualStride", &d->residual_stride) ||
+      !optional_float(env, o, "residualScale", &d->has_residual_scale, &d->residual_scale) ||
+      !optional_binding(env, o, "output", &d->output, &d->output_bytes) ||
+      !optional_u32(env, o, "outputStride", &d->output_stride) ||
+      !optional_binding(env, o, "nextGamma", &d->next_gamma, &d->next_gamma_bytes) ||
+      !optional_binding(env, o, "nextBeta", &d->next_beta, &d->next_beta_bytes) ||
+      !optional_binding(env, o, "nextOutput", &d->next_output, &d->next_output_bytes) ||
+      !optional_u32(env, o, "nextOutputStride", &d->next_output_stride) ||
+      !optional_float(env, o, "epsilon", &d->has_epsilon, &d->epsilon))
+    return 0;
   *label = prop_string(env, o, "label");
   d->label = *label;
   return 1;
@@ -935,17 +956,17 @@ static int parse_q4_desc(napi_env env, napi_value o, pk_q4_desc *d, char **label
     return 0;
   }
   d->activation = (int32_t)activation;
-  prop_binding(env, o, "a", &d->a, &d->a_bytes);
-  prop_u32(env, o, "aStride", &d->a_stride);
-  prop_binding(env, o, "packed", &d->packed, &d->packed_bytes);
-  prop_binding(env, o, "scales", &d->scales, &d->scales_bytes);
-  prop_binding(env, o, "offsets", &d->offsets, &d->offsets_bytes);
-  prop_binding(env, o, "output", &d->output, &d->output_bytes);
-  prop_u32(env, o, "outputStride", &d->output_stride);
-  prop_binding(env, o, "bias", &d->bias, &d->bias_bytes);
-  prop_binding(env, o, "residual", &d->residual, &d->residual_bytes);
-  prop_u32(env, o, "residualStride", &d->residual_stride);
-  prop_float(env, o, "residualScale", &d->has_residual_scale, &d->residual_scale);
+  if (!optional_binding(env, o, "a", &d->a, &d->a_bytes) || !optional_u32(env, o, "aStride", &d->a_stride) ||
+      !optional_binding(env, o, "packed", &d->packed, &d->packed_bytes) ||
+      !optional_binding(env, o, "scales", &d->scales, &d->scales_bytes) ||
+      !optional_binding(env, o, "offsets", &d->offsets, &d->offsets_bytes) ||
+      !optional_binding(env, o, "output", &d->output, &d->output_bytes) ||
+      !optional_u32(env, o, "outputStride", &d->output_stride) ||
+      !optional_binding(env, o, "bias", &d->bias, &d->bias_bytes) ||
+      !optional_binding(env, o, "residual", &d->residual, &d->residual_bytes) ||
+      !optional_u32(env, o, "residualStride", &d->residual_stride) ||
+      !optional_float(env, o, "residualScale", &d->has_residual_scale, &d->residual_scale))
+    return 0;
   *label = prop_string(env, o, "label");
   d->label = *label;
   return 1;
@@ -963,15 +984,16 @@ static int parse_score_desc(napi_env env, napi_value o, pk_score_desc *d, char *
     bad_argument(env, "token score descriptor is missing a required field");
     return 0;
   }
-  prop_u32(env, o, "rowStride", &d->row_stride);
-  prop_binding(env, o, "logits", &d->logits, &d->logits_bytes);
-  prop_float(env, o, "temperature", &d->has_temperature, &d->temperature);
-  prop_binding(env, o, "tokens", &d->tokens, &d->tokens_bytes);
-  prop_binding(env, o, "logProbs", &d->log_probs, &d->log_probs_bytes);
-  prop_binding(env, o, "entropies", &d->entropies, &d->entropies_bytes);
-  prop_u32(env, o, "alternatives", &d->alternatives);
-  prop_binding(env, o, "topTokens", &d->top_tokens, &d->top_tokens_bytes);
-  prop_binding(env, o, "topLogProbs", &d->top_log_probs, &d->top_log_probs_bytes);
+  if (!optional_u32(env, o, "rowStride", &d->row_stride) ||
+      !optional_binding(env, o, "logits", &d->logits, &d->logits_bytes) ||
+      !optional_float(env, o, "temperature", &d->has_temperature, &d->temperature) ||
+      !optional_binding(env, o, "tokens", &d->tokens, &d->tokens_bytes) ||
+      !optional_binding(env, o, "logProbs", &d->log_probs, &d->log_probs_bytes) ||
+      !optional_binding(env, o, "entropies", &d->entropies, &d->entropies_bytes) ||
+      !optional_u32(env, o, "alternatives", &d->alternatives) ||
+      !optional_binding(env, o, "topTokens", &d->top_tokens, &d->top_tokens_bytes) ||
+      !optional_binding(env, o, "topLogProbs", &d->top_log_probs, &d->top_log_probs_bytes))
+    return 0;
   *label = prop_string(env, o, "label");
   d->label = *label;
   return 1;

@@ -1224,6 +1224,14 @@ class RowsKernel {
     return sizes;
   }
 
+  /** The field `name`, a number, none if undefined. */
+  numberOf(descriptor, name) {
+    const value = descriptor[name];
+    if (value === undefined) return {};
+    if (typeof value !== "number") throw new Error(`${descriptor.label} ${name} must be a number`);
+    return { [name]: value };
+  }
+
   validateDescriptor(descriptor) {
     native()[`${this.prefix}Validate`](this.nativeDescriptor(descriptor));
   }
@@ -1255,7 +1263,7 @@ class BlockNormKernel extends RowsKernel {
     for (const [tensor, name] of [[descriptor.gamma, "gamma"], [descriptor.beta, "beta"], [next.gamma, "next gamma"],
                                   [next.beta, "next beta"]])
       if (tensor !== undefined) requireChannelTensor(tensor, channels, channels * 4, `${label} ${name}`);
-    const d = Object.assign(
+    return Object.assign(
       { label, precision: this.precision, kind },
       this.sizesOf(descriptor, ["rows", "channels", "inputStride", "gateStride", "gateRows", "residualStride",
                                 "outputStride"]),
@@ -1263,11 +1271,9 @@ class BlockNormKernel extends RowsKernel {
       this.bindingOf("beta", descriptor.beta), this.bindingOf("gate", descriptor.gate),
       this.bindingOf("residual", descriptor.residual), this.bindingOf("output", descriptor.output),
       this.bindingOf("nextGamma", next.gamma), this.bindingOf("nextBeta", next.beta),
-      this.bindingOf("nextOutput", next.output));
-    if (next.outputStride !== undefined) d.nextOutputStride = next.outputStride;
-    if (descriptor.residualScale !== undefined) d.residualScale = descriptor.residualScale;
-    if (descriptor.epsilon !== undefined) d.epsilon = descriptor.epsilon;
-    return d;
+      this.bindingOf("nextOutput", next.output),
+      this.sizesOf({ label, nextOutputStride: next.outputStride }, ["nextOutputStride"]),
+      this.numberOf(descriptor, "residualScale"), this.numberOf(descriptor, "epsilon"));
   }
 }
 
@@ -1284,15 +1290,13 @@ class Q4GemmKernel extends RowsKernel {
     const { label } = descriptor;
     const activation = { none: 0, silu: 1, relu: 2 }[descriptor.activation === undefined ? "none" : descriptor.activation];
     if (activation === undefined) throw new Error(`${label} has an unsupported activation ${descriptor.activation}`);
-    const d = Object.assign(
+    return Object.assign(
       { label, precision: this.precision, activation },
       this.sizesOf(descriptor, ["rows", "inner", "columns", "groupSize", "aStride", "outputStride", "residualStride"]),
       this.bindingOf("a", descriptor.a), this.bindingOf("packed", descriptor.packed),
       this.bindingOf("scales", descriptor.scales), this.bindingOf("offsets", descriptor.offsets),
       this.bindingOf("output", descriptor.output), this.bindingOf("bias", descriptor.bias),
-      this.bindingOf("residual", descriptor.residual));
-    if (descriptor.residualScale !== undefined) d.residualScale = descriptor.residualScale;
-    return d;
+      this.bindingOf("residual", descriptor.residual), this.numberOf(descriptor, "residualScale"));
   }
 }
 
@@ -1306,14 +1310,13 @@ class TokenScoreKernel extends RowsKernel {
   result(descriptor) { return descriptor.logProbs || descriptor.entropies || descriptor.topTokens; }
 
   nativeDescriptor(descriptor) {
-    const d = Object.assign(
+    return Object.assign(
       { label: descriptor.label, precision: this.precision },
       this.sizesOf(descriptor, ["rows", "columns", "rowStride", "alternatives"]),
       this.bindingOf("logits", descriptor.logits), this.bindingOf("tokens", descriptor.tokens),
       this.bindingOf("logProbs", descriptor.logProbs), this.bindingOf("entropies", descriptor.entropies),
-      this.bindingOf("topTokens", descriptor.topTokens), this.bindingOf("topLogProbs", descriptor.topLogProbs));
-    if (descriptor.temperature !== undefined) d.temperature = descriptor.temperature;
-    return d;
+      this.bindingOf("topTokens", descriptor.topTokens), this.bindingOf("topLogProbs", descriptor.topLogProbs),
+      this.numberOf(descriptor, "temperature"));
   }
 }
 
