@@ -20,13 +20,20 @@ struct Region {
 };
 
 // Whether the regions share a byte. Regions of one stride (columns of one
-// buffer) are compared row by row; of two strides that interleave, any
-// common range counts.
+// buffer) and a single row, whatever stride it came with, are compared row by
+// row; of two strides that interleave, any common range counts.
 inline bool overlap(const Region& x, const Region& y) {
   if (!x.data || !y.data || !x.rows || !y.rows) return false;
   const uintptr_t a = reinterpret_cast<uintptr_t>(x.data), b = reinterpret_cast<uintptr_t>(y.data);
   if (a + x.extent() <= b || b + y.extent() <= a) return false;
-  if (x.stride != y.stride || x.rows < 2 || y.rows < 2) return true;
+  if (x.rows < 2 || y.rows < 2) {
+    const Region &one = x.rows < 2 ? x : y, &rows = x.rows < 2 ? y : x;
+    const uintptr_t p = reinterpret_cast<uintptr_t>(one.data), q = reinterpret_cast<uintptr_t>(rows.data);
+    // The first of the rows that ends behind the start of the one.
+    const uint64_t i = p < q + rows.row_bytes ? 0 : (p - q - rows.row_bytes) / rows.stride + 1;
+    return i < rows.rows && q + i * rows.stride < p + one.row_bytes;
+  }
+  if (x.stride != y.stride) return true;
   const uint64_t from_x = (b >= a ? (b - a) : x.stride - (a - b) % x.stride) % x.stride;
   return from_x < x.row_bytes || x.stride - from_x < y.row_bytes;
 }
