@@ -141,7 +141,11 @@ struct RowScores {
     if (args.tokens)
       args.log_probs[row] = token < args.columns ? log_prob(logit) : token == 0xffffffffu ? 0.0f : __builtin_nanf("");
   }
-  __device__ float log_prob(float x) const { return empty ? -kInf : (x - m) * scale - spread; }
+  // Halves of x and m: their difference is a number where that of x and m is
+  // beyond f32, and twice the scale brings a temperature above 1 back.
+  __device__ float log_prob(float x) const {
+    return empty ? -kInf : (0.5f * x - 0.5f * m) * (2.0f * scale) - spread;
+  }
   // Alternative k of the row; key 0: none.
   __device__ void store(const ScoreArgs& args, uint32_t row, uint32_t k, uint64_t key) const {
     const uint64_t at = (uint64_t)row * args.alternatives + k;
