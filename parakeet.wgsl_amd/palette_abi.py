@@ -1201,7 +1201,11 @@ class BlockNormOp(_RowsOp):
 def pack_q4(codes: np.ndarray) -> np.ndarray:
     """Codes 0..15 of [inner, columns] in the packed format of pk_q4.h: uint32
     words of eight codes in row-major order, the first in the lowest bits."""
-    flat = np.asarray(codes, dtype=np.uint32).reshape(-1)
+    codes = np.asarray(codes)
+    whole = codes.dtype.kind in "iub" or bool((codes == np.floor(codes)).all())
+    if not whole or (codes.size and (codes.min() < 0 or codes.max() > 15)):
+        raise ValueError("codes must be whole numbers from 0 to 15")
+    flat = codes.astype(np.uint32).reshape(-1)
     flat = np.concatenate([flat, np.zeros(-len(flat) % 8, np.uint32)]).reshape(-1, 8)
     return np.bitwise_or.reduce(flat << (4 * np.arange(8, dtype=np.uint32)), axis=1).astype(np.uint32)
 
