@@ -13,7 +13,12 @@
  * v / (1 + exp(-v)) without the reference's clamp. Products and sums are f32
  * in both profiles (f16: f16 operands in exact products; f32: f32 operands),
  * scales are applied to each group's sum in f32, and an output is rounded
- * once. An infinity or a NaN in a row of `a` touches that row alone.
+ * once. A group's sums of a (code - 8) and, for its offset, of a have to stay
+ * within f32: they do where the magnitudes of `a` add up to less than 2^125
+ * over a group (f16: always). Where they do not, or an activation is an
+ * infinity or a NaN, outputs of that row are infinities or NaN, NaN also where
+ * the formula has an infinity (with offsets the two sums may be opposite
+ * ones), and no other row is touched.
  */
 #ifndef PK_Q4_H
 #define PK_Q4_H
