@@ -16,8 +16,10 @@
  *   (x - mean) / sqrt(mean((x - mean)^2) + epsilon) * gamma + beta
  * and PK_NORM_RMS x / sqrt(mean(x^2) + epsilon) * gamma + beta, a missing
  * beta counting as zero. Everything between loading and storing is f32: the
- * second norm sees y before its rounding. A row with an infinity or a NaN
- * has NaN where the formula has it and touches no other row.
+ * second norm sees y before its rounding. The squares that a norm adds up have
+ * to stay within f32: they do where its operands, the input or y, lie below
+ * 2^56 in magnitude. A row with an infinity or a NaN has NaN where the formula
+ * has it and touches no other row.
  */
 #ifndef PK_BLOCK_NORM_H
 #define PK_BLOCK_NORM_H
