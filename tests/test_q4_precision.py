@@ -62,3 +62,86 @@ def test_rows_copied_by_their_wavefronts(abi, ctx, scope, dtype, rows, inner, co
             np.testing.assert_array_equal(kw["output"].download(), want.astype(dtype))
     finally:
         op.release()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offsets", [False, True])
+@pytest.mark.parametrize("dtype,rows,inner,columns,group", [
+    # parts of K that meet in a workspace, tiles whole, rows whole in LDS
+    (np.float16, 500, 17300, 512, 128), (np.float16, 130, 4100, 5500, 64), (np.float16, 64, 8192, 8200, 32),
+    (np.float16, 700, 1100, 2100, 0), (np.float16, 16, 2300, 300, 32), (np.float16, 1, 12000, 100, 128),
+    (np.float32, 500, 4200, 512, 128), (np.float32, 130, 1100, 5500, 64), (np.float32, 700, 600, 2100, 32),
+    (np.float32, 5, 1100, 300, 64), (np.float32, 4, 2300, 100, 32), (np.float32, 1, 12000, 100, 0)])
+def test_whole_numbers(abi, ctx, scope, dtype, rows, inner, columns, group, offsets):
+    case, want = whole(np.random.default_rng(rows * 3 + inner), dtype, rows, inner, columns, group, offsets)
+    np.testing.assert_array_equal(q4.run(abi, ctx, scope, case), want.astype(dtype))
+
+
+# The f32 sizes of test_gpu_q4's long axes, row counts, tiles and parts of K.
+F32 = [(rows, inner, columns, 64, False, False) for rows in (1, 20)
+       for inner, columns in ((4096, 64), (64, 4096), (8192, 16), (2560, 2560), (9000, 129))] + \
+      [(rows, 1024, 520, 128, True, False) for rows in (1, 2, 4, 5, 8, 9, 31, 32, 48, 100, 257)] + \
+      [(640, 300, 2100, 64, True, False), (1504, 128, 1032, 0, False, False), (800, 260, 1700, 128, False, False),
+       (500, 4200, 512, 128, False, True), (130, 1100, 5500, 64, True, True), (49, 8192, 2050, 32, True, True)]
+
+
+def f32_case(rows, inner, columns, group, offsets, epilogue):
+    more = dict(activation="silu", residual=True, residual_scale=2.0) if epilogue else {}
+    return q4.make(np.random.default_rng(rows * inner + columns), np.float32, rows, inner, columns, group, offsets,
+                   bias=True, **more)
+
+
+def f32_reference(case, a=None, parts=1, cast=np.float64, weight=np.float64):
+    """(outputs, tolerance) in float64; with other activations, with the weight
+    of another type, or with the sum over K as that many parts of type `cast`."""
+    inner, columns = case["codes"].shape
+    at = np.arange(inner) // (case["group_size"] or inner)
+    scaled = case["scales"].astype(np.float64)[at] * (case["codes"].astype(np.float64) - 8)
+    offset = case["offsets"].astype(np.float64)[at] if "offsets" in case else np.zeros((1, columns))
+    w = (scaled + offset).astype(weight).astype(np.float64)
+    x = (case["a"] if a is None else a).astype(np.float64)
+    ends = np.linspace(0, inner, parts + 1).astype(int)
+    v = sum((x[:, i:j] @ w[i:j]).astype(cast).astype(np.float64) for i, j in zip(ends, ends[1:]))
+    squares = x ** 2
+    size = np.sqrt(squares @ (scaled ** 2) + (squares @ np.broadcast_to(offset ** 2, w.shape)))
+    tol = 12 * 2.0 ** -24 * np.sqrt(inner) * size
+    v = v + case["bias"]
+    tol = tol + 2.0 ** -24 * np.abs(v)
+    if case["activation"] == "silu":
+        y = v / (1 + np.exp(-v))
+        tol, v = 1.1 * tol + (np.abs(v) + 4) * 2.0 ** -23 * np.abs(y), y
+    if "residual" in case:
+        v = case["residual"] + case["residual_scale"] * v
+        tol = abs(case["residual_scale"]) * tol + 2.0 ** -23 * np.abs(v)
+    return v, tol + 2.0 ** -24 * np.abs(v) + 2.0 ** -149
+
+
+@pytest.mark.parametrize("size", F32)
+def test_what_the_f32_tolerance_rejects(size):
+    """It takes an f32 product, and neither f16 operands nor parts of sums in f16."""
+    case = f32_case(*size)
+    want, tol = f32_reference(case)
+    inner = size[1]
+
+    def worst(**other):
+        return (np.abs(f32_reference(case, **other)[0] - want) / tol).max()
+    assert worst(a=case["a"].astype(np.float16)) > 2
+    assert worst(weight=np.float16) > 2
+    assert worst(parts=min(8, inner // 32), cast=np.float16) > 2
+    at = np.arange(inner) // (case["group_size"] or inner)
+    w = case["scales"][at] * (case["codes"].astype(np.float32) - 8)
+    if "offsets" in case:
+        w = w + case["offsets"][at]
+    plain = dict(case, activation="none")
+    plain.pop("residual", None)
+    v, v_tol = f32_reference(plain)
+    assert (np.abs((case["a"] @ w).astype(np.float64) + case["bias"] - v) <= v_tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", F32)
+def test_f32_products_keep_their_digits(abi, ctx, scope, size):
+    case = f32_case(*size)
+    want, tol = f32_reference(case)
+    got = q4.run(abi, ctx, scope, case).astype(np.float64)
+    assert (np.abs(got - want) <= tol).all(), (np.abs(got - want) / tol).max()
