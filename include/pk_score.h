@@ -4,8 +4,9 @@
  * alternatives, in one pass over the logits. Same library, contexts, streams,
  * events and status codes as pk_palette.h. No counterpart in the reference,
  * whose decoder returns the tokens it chose and no measure of how sure it was
- * (tdt-decoder.ts:84-130); pk_tdt.h is that decoder, and the token columns and
- * the duration columns of its 1032-wide head rows are two bindings here.
+ * (tdt-decoder.ts:84-130). The caller brings the logits, of a head product
+ * (pk_q4.h, pk_palette.h) for instance: pk_tdt.h keeps those of its decoder to
+ * itself. Token and duration columns of one head row are two bindings.
  *
  * With z = logits / temperature over the V columns of a row,
  *   log p = z - log(sum exp z),   entropy = -sum p log p   (nats),
@@ -60,7 +61,9 @@ typedef struct pk_score_desc {
    - a logit of minus infinity (a masked token) has probability 0: its log
      probability is minus infinity and it is never an alternative. Places
      beyond the last possible alternative hold PK_SCORE_NO_TOKEN and minus
-     infinity;
+     infinity. The type's lowest number masks too, but counts as an
+     alternative, and rows that it leaves few others take several times as
+     long;
    - a row of minus infinities has entropy 0, no alternatives, and log
      probability minus infinity for every token;
    - a row with a NaN or plus infinity has NaN for its entropy and every log

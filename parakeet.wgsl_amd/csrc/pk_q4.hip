@@ -16,9 +16,9 @@
 // SIMD issues a matrix instruction (8.05 ns) or an fma (1.25 ns) but hardly
 // both at once, one and 8 fma take 17.1 ns, so that decoding and scaling
 // count in full: per 32 k and 16 columns 9 and, once a group, 16 operations
-// for 4 matrix instructions. 64 x 8192 x 8192 with offsets 24.1 us, of which
+// for 4 matrix instructions. 64 x 8192 x 8192 with offsets 24.2 us, of which
 // 10.2 are these instructions and the rest waits for rows and codes; 1504 x
-// 1024 x 4096 20.3 us, 0.62 PFLOP/s, and x 4096 x 4096 60 us, 0.84.
+// 1024 x 4096 20.1 us, 0.63 PFLOP/s, and x 4096 x 4096 60 us, 0.84.
 #include "pk_internal.h"
 #include "pk_wave.h"
 
@@ -586,6 +586,7 @@ __global__ __launch_bounds__(1024) void q4_vector_kernel(Q4Args args) {
 // lanes, and a second launch adds the parts in their order.
 constexpr int kTileRows = 64, kTileColumns = 128;
 constexpr uint32_t kTileVectors = kTileRows * kTileColumns / 4;  // of a lane's four rows
+constexpr uint32_t kMostSplitTiles = 256;  // one for each compute unit: more are not split along K
 template <typename T, int PER, bool OFFSETS>
 __global__ __launch_bounds__(256, OFFSETS || sizeof(T) == 4 ? 2 : 3) void q4_tile_kernel(Q4Args args) {
   constexpr int kStep = 4 / PER;
@@ -828,8 +829,11 @@ struct Q4Plan {
 
 // f16 kernels of few rows: rows and columns of a workgroup in 16, wavefronts
 // at most, and the us that a compute unit takes for a block of K and for the
-// rest of a workgroup, fitted to 150 products of 32 to 300 rows, K 512 to 8192,
-// N 256 to 8192 (groups of 128, no offsets).
+// rest of a workgroup, fitted to products of 32 to 300 rows, K 512 to 8192, N
+// 256 to 8192, groups of 128 without offsets. Smaller groups and offsets make
+// all kernels slower alike: over 63 products of 17 to 1504 rows each, the
+// choice takes 1.012 to 1.019 times the fastest kernel's time in the mean for
+// groups of 32, 64 and 128, with offsets and without, and 1.18 at most.
 struct RowsShape {
   uint32_t mt, nt, waves;
   float block, rest;
@@ -847,7 +851,8 @@ Kernel pick_rows_f16(const Q4Args& args, uint32_t shape) {
   }
 }
 // us of a launch of f16 tiles, `blocks` of K each, fitted to the same products:
-// a compute unit holds three, of which one leaves it idle half the time.
+// a compute unit holds three (with offsets two), of which one leaves it idle
+// half the time.
 float tile_time(uint64_t tiles, uint32_t blocks) {
   const float each = (float)((tiles + 255u) / 256u);
   return 1.5f * each + (each > 1.0f ? 0.55f * each : 0.72f) * (float)blocks;
@@ -871,7 +876,7 @@ Q4Plan plan(const Q4Args& args) {
   // Tiles whole, or too few to fill the compute units in as many parts along K
   // as make two for each, but 16, which a thread of the join adds in turn.
   const uint64_t tiled = (uint64_t)tiles(args.rows, kTileRows) * tiles(args.columns, kTileColumns);
-  const uint32_t most_parts = tiled <= 32u ? 16u : tiled <= 256u ? 512u / (uint32_t)tiled : 1u;
+  const uint32_t most_parts = tiled <= 32u ? 16u : tiled <= kMostSplitTiles ? 2u * kMostSplitTiles / (uint32_t)tiled : 1u;
   const uint32_t span = tiles(kblocks, most_parts), parts = tiles(kblocks, span);
   const auto tile_plan = [&](uint32_t blocks) {
     return Q4Plan{pick_tile(args), dim3((uint32_t)tiled, tiles(kblocks, blocks)), 256u, blocks};
@@ -967,8 +972,8 @@ uint64_t q4_workspace(const Q4Args& args) {
     const uint64_t wanted = plan(some).part_bytes();
     if (wanted > bytes) bytes = wanted;
   };
-  // A plan depends on the rows in 16; more than 512 tiles are never split.
-  for (uint32_t rows = 16u; rows < args.rows && rows <= 512u * kTileRows; rows += 16u) count(rows);
+  // A plan depends on the rows in 16, and takes a tile at least for 64.
+  for (uint32_t rows = 16u; rows < args.rows && rows <= kMostSplitTiles * kTileRows; rows += 16u) count(rows);
   count(args.rows);
   return bytes;
 }
