@@ -91,7 +91,9 @@ static int get_u64(napi_env env, napi_value v, uint64_t *out) {
   }
   if (t == napi_number) {
     double d;
-    if (napi_get_value_double(env, v, &d) != napi_ok || d < 0 || d > 9007199254740991.0 || d != (double)(uint64_t)d)
+    /* NaN fails both comparisons: it has no integer to convert to */
+    if (napi_get_value_double(env, v, &d) != napi_ok || !(d >= 0 && d <= 9007199254740991.0) ||
+        d != (double)(uint64_t)d)
       return 0;
     *out = (uint64_t)d;
     return 1;
