@@ -876,7 +876,8 @@ Q4Plan plan(const Q4Args& args) {
   // Tiles whole, or too few to fill the compute units in as many parts along K
   // as make two for each, but 16, which a thread of the join adds in turn.
   const uint64_t tiled = (uint64_t)tiles(args.rows, kTileRows) * tiles(args.columns, kTileColumns);
-  const uint32_t most_parts = tiled <= 32u ? 16u : tiled <= kMostSplitTiles ? 2u * kMostSplitTiles / (uint32_t)tiled : 1u;
+  const uint32_t most_parts =
+      tiled <= 32u ? 16u : tiled <= kMostSplitTiles ? 2u * kMostSplitTiles / (uint32_t)tiled : 1u;
   const uint32_t span = tiles(kblocks, most_parts), parts = tiles(kblocks, span);
   const auto tile_plan = [&](uint32_t blocks) {
     return Q4Plan{pick_tile(args), dim3((uint32_t)tiled, tiles(kblocks, blocks)), 256u, blocks};
