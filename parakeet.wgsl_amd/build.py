@@ -42,7 +42,9 @@ HIP_FLAGS = [
 SOURCES = [
     "pk_abi.cpp", "pk_conv_abi.cpp", "pk_attention_abi.cpp", "pk_layernorm_abi.cpp",
     "pk_encoder_abi.cpp", "pk_subsampling_abi.cpp", "pk_tdt_abi.cpp", "pk_block_norm_abi.cpp", "pk_q4_abi.cpp",
-    "pk_score_abi.cpp", "pk_codes.hip", "pk_conv.hip", "pk_block_norm.hip", "pk_q4.hip", "pk_score.hip",
+    "pk_score_abi.cpp", "pk_cache_abi.cpp", "pk_verify_abi.cpp",
+    "pk_codes.hip", "pk_conv.hip", "pk_block_norm.hip", "pk_q4.hip", "pk_score.hip",
+    "pk_cache_append.hip", "pk_cache_attention.hip", "pk_verify.hip",
     "pk_subsampling.hip", "pk_tdt.hip", "pk_tdt_resident.hip",
     "pk_attention.hip", "pk_layernorm.hip",
     "pk_gemm_f16.hip", "pk_gemm_f16k.hip",

@@ -440,6 +440,96 @@ hipError_t launch_q4_layout(const Q4Args& args, const uint32_t* packed, const vo
 uint64_t q4_workspace(const Q4Args& args);
 hipError_t launch_q4(const Q4Args& args, hipStream_t stream, hipEvent_t start = nullptr, hipEvent_t stop = nullptr);
 
+// The paged cache of include/pk_cache.h: what append and attention share.
+// Strides in elements.
+struct CacheView {
+  const uint32_t* row_starts;  // [sequences + 1]
+  const uint32_t* lengths;     // [sequences]
+  const uint32_t* page_table;  // [sequences, pages_per_sequence]
+  uint64_t page_stride;
+  uint32_t rows;               // of the bindings
+  uint32_t sequences;          // active ones
+  uint32_t pages_per_sequence;
+  uint32_t pages;
+  uint32_t page_size;
+  uint32_t page_magic;         // t / page_size = t * page_magic >> page_shift
+  uint32_t page_shift;
+  uint32_t kv_heads;
+  uint32_t head_dim;
+
+  // With s = floor(log2 size), magic = floor(2^(31 + s) / size) + 1 is off by
+  // less than 2^(s + 1) / 2^(31 + s) of a page a token: exact below 2^30 tokens.
+  __host__ void set_page_size(uint32_t size) {
+    uint32_t s = 0;
+    while ((size >> s) > 1u) ++s;
+    page_size = size;
+    page_shift = 31u + s;
+    page_magic = (uint32_t)((1ull << page_shift) / size + 1u);
+  }
+  __device__ uint32_t page_of(uint32_t token) const { return (uint32_t)(((uint64_t)token * page_magic) >> page_shift); }
+  // Tokens that the tables have places for.
+  __host__ __device__ uint32_t capacity() const { return pages_per_sequence * page_size; }
+  // Element of a token's row for kv head 0 (others follow page_size * head_dim
+  // elements apart), or no_place.
+  static constexpr uint64_t no_place = ~0ull;
+  __device__ uint64_t place(uint32_t sequence, uint32_t token) const {
+    const uint32_t at = page_of(token);
+    const uint32_t page = page_table[(uint64_t)sequence * pages_per_sequence + at];
+    return page < pages ? page * page_stride + (uint64_t)(token - at * page_size) * head_dim : no_place;
+  }
+};
+
+// Cache append (pk_cache_append.hip).
+struct CacheAppendArgs {
+  CacheView cache;
+  const void *queries, *keys, *values;  // queries null: none
+  void* query_output;
+  void *key_cache, *value_cache;
+  const float* frequencies;
+  const uint32_t* positions;  // or null
+  uint64_t query_stride, query_output_stride, key_stride, value_stride;
+  uint32_t heads;             // of the queries
+  uint32_t rotary_dim;
+  bool neighbours, f16;
+};
+hipError_t launch_cache_append(const CacheAppendArgs& args, hipStream_t stream, hipEvent_t start = nullptr,
+                               hipEvent_t stop = nullptr);
+
+// Cache attention (pk_cache_attention.hip).
+struct CacheAttentionArgs {
+  CacheView cache;
+  const void* queries;
+  void* output;
+  const void *key_cache, *value_cache;
+  uint64_t query_stride, output_stride;
+  uint32_t heads;
+  uint32_t window;  // tokens a row sees, 0: all
+  float scale;
+  float cap;        // of the scores, 0: none
+  bool causal, f16;
+};
+hipError_t launch_cache_attention(const CacheAttentionArgs& args, hipStream_t stream, hipEvent_t start = nullptr,
+                                  hipEvent_t stop = nullptr);
+
+// Verification of drafted tokens (pk_verify.hip).
+struct VerifyArgs {
+  const void *target, *draft;  // rows of logits; draft null: none
+  uint64_t target_stride, draft_stride;
+  const uint32_t* row_starts;
+  const uint32_t* tokens;
+  const float* uniforms;
+  const float* draws;
+  uint32_t* accepted;
+  uint32_t* next_tokens;
+  uint32_t rows;
+  uint32_t sequences;  // active ones
+  uint32_t columns;
+  double scale;        // log2(e) / temperature
+  bool greedy, f16;
+};
+hipError_t launch_verify(const VerifyArgs& args, hipStream_t stream, hipEvent_t start = nullptr,
+                         hipEvent_t stop = nullptr);
+
 // Subsampling front end convolutions (pk_subsampling.hip).
 enum SubsamplingKind { kSubsamplingFused = 0, kSubsamplingDepthwise = 1, kSubsamplingMask = 2 };
 struct SubsamplingArgs {

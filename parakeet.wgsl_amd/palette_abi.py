@@ -1,6 +1,6 @@
 """ctypes binding of libpk_palette.so (include/pk_palette.h, pk_conv.h, pk_attention.h,
 pk_layernorm.h, pk_subsampling.h, pk_encoder.h, pk_tdt.h, pk_block_norm.h, pk_q4.h,
-pk_score.h).
+pk_score.h, pk_cache.h, pk_verify.h).
 
 A thin Python view of the C ABI, used by the tests and the benchmark. It
 raises PaletteError (or PaletteRangeError, mirroring the reference's
@@ -43,6 +43,10 @@ ENCODER_DISPATCHES = ("norm_feed_forward1", "feed-forward1-linear1", "feed-forwa
                       "feed-forward2-linear1", "feed-forward2-linear2-residual", "norm_out")
 NORM_KIND = {"layer": 0, "rms": 1}
 BLOCK_NORM_MAX_CHANNELS = 16384
+ROTARY = {"halves": 0, "neighbours": 1}
+VERIFY_MODE = {"sample": 0, "greedy": 1}
+CACHE_NO_PAGE = 0xFFFFFFFF
+VERIFY_NO_TOKEN = 0xFFFFFFFF
 SCORE_NO_TOKEN = 0xFFFFFFFF
 SCORE_MAX_ALTERNATIVES = 32
 EXPAND_LAYOUT = {"row-major": 0, "tile-major": 1}
@@ -369,6 +373,121 @@ class ScoreDesc(ctypes.Structure):
     ]
 
 
+class CacheAppendDesc(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("label", ctypes.c_char_p),
+        ("precision", ctypes.c_int32),
+        ("rows", ctypes.c_uint32),
+        ("sequences", ctypes.c_uint32),
+        ("heads", ctypes.c_uint32),
+        ("kv_heads", ctypes.c_uint32),
+        ("head_dim", ctypes.c_uint32),
+        ("queries", ctypes.c_void_p),
+        ("queries_bytes", ctypes.c_uint64),
+        ("query_stride", ctypes.c_uint32),
+        ("query_output", ctypes.c_void_p),
+        ("query_output_bytes", ctypes.c_uint64),
+        ("query_output_stride", ctypes.c_uint32),
+        ("keys", ctypes.c_void_p),
+        ("keys_bytes", ctypes.c_uint64),
+        ("key_stride", ctypes.c_uint32),
+        ("values", ctypes.c_void_p),
+        ("values_bytes", ctypes.c_uint64),
+        ("value_stride", ctypes.c_uint32),
+        ("rotary_dim", ctypes.c_uint32),
+        ("rotary", ctypes.c_int32),
+        ("frequencies", ctypes.c_void_p),
+        ("frequencies_bytes", ctypes.c_uint64),
+        ("positions", ctypes.c_void_p),
+        ("positions_bytes", ctypes.c_uint64),
+        ("row_starts", ctypes.c_void_p),
+        ("row_starts_bytes", ctypes.c_uint64),
+        ("lengths", ctypes.c_void_p),
+        ("lengths_bytes", ctypes.c_uint64),
+        ("page_table", ctypes.c_void_p),
+        ("page_table_bytes", ctypes.c_uint64),
+        ("pages_per_sequence", ctypes.c_uint32),
+        ("pages", ctypes.c_uint32),
+        ("page_size", ctypes.c_uint32),
+        ("page_stride", ctypes.c_uint64),
+        ("key_cache", ctypes.c_void_p),
+        ("key_cache_bytes", ctypes.c_uint64),
+        ("value_cache", ctypes.c_void_p),
+        ("value_cache_bytes", ctypes.c_uint64),
+    ]
+
+
+class CacheAttentionDesc(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("label", ctypes.c_char_p),
+        ("precision", ctypes.c_int32),
+        ("rows", ctypes.c_uint32),
+        ("sequences", ctypes.c_uint32),
+        ("heads", ctypes.c_uint32),
+        ("kv_heads", ctypes.c_uint32),
+        ("head_dim", ctypes.c_uint32),
+        ("queries", ctypes.c_void_p),
+        ("queries_bytes", ctypes.c_uint64),
+        ("query_stride", ctypes.c_uint32),
+        ("output", ctypes.c_void_p),
+        ("output_bytes", ctypes.c_uint64),
+        ("output_stride", ctypes.c_uint32),
+        ("causal", ctypes.c_int32),
+        ("window", ctypes.c_uint32),
+        ("has_scale", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("score_cap", ctypes.c_float),
+        ("row_starts", ctypes.c_void_p),
+        ("row_starts_bytes", ctypes.c_uint64),
+        ("lengths", ctypes.c_void_p),
+        ("lengths_bytes", ctypes.c_uint64),
+        ("page_table", ctypes.c_void_p),
+        ("page_table_bytes", ctypes.c_uint64),
+        ("pages_per_sequence", ctypes.c_uint32),
+        ("pages", ctypes.c_uint32),
+        ("page_size", ctypes.c_uint32),
+        ("page_stride", ctypes.c_uint64),
+        ("key_cache", ctypes.c_void_p),
+        ("key_cache_bytes", ctypes.c_uint64),
+        ("value_cache", ctypes.c_void_p),
+        ("value_cache_bytes", ctypes.c_uint64),
+    ]
+
+
+class VerifyDesc(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("label", ctypes.c_char_p),
+        ("precision", ctypes.c_int32),
+        ("mode", ctypes.c_int32),
+        ("rows", ctypes.c_uint32),
+        ("sequences", ctypes.c_uint32),
+        ("columns", ctypes.c_uint32),
+        ("target", ctypes.c_void_p),
+        ("target_bytes", ctypes.c_uint64),
+        ("target_stride", ctypes.c_uint32),
+        ("draft", ctypes.c_void_p),
+        ("draft_bytes", ctypes.c_uint64),
+        ("draft_stride", ctypes.c_uint32),
+        ("has_temperature", ctypes.c_int32),
+        ("temperature", ctypes.c_float),
+        ("row_starts", ctypes.c_void_p),
+        ("row_starts_bytes", ctypes.c_uint64),
+        ("tokens", ctypes.c_void_p),
+        ("tokens_bytes", ctypes.c_uint64),
+        ("uniforms", ctypes.c_void_p),
+        ("uniforms_bytes", ctypes.c_uint64),
+        ("draws", ctypes.c_void_p),
+        ("draws_bytes", ctypes.c_uint64),
+        ("accepted", ctypes.c_void_p),
+        ("accepted_bytes", ctypes.c_uint64),
+        ("next_tokens", ctypes.c_void_p),
+        ("next_tokens_bytes", ctypes.c_uint64),
+    ]
+
+
 class SubsamplingFusedDesc(ctypes.Structure):
     _fields_ = [
         ("struct_size", ctypes.c_uint32),
@@ -648,6 +767,24 @@ SIGNATURES = {
     "pk_score_enqueue_timed": (ctypes.c_int, [_VP, ctypes.c_uint32, _VP, _VP, _VP]),
     "pk_score_destroy": (ctypes.c_int, [_VP]),
     "pk_score_release": (ctypes.c_int, [_VP]),
+    "pk_cache_append_validate": (ctypes.c_int, [ctypes.POINTER(CacheAppendDesc)]),
+    "pk_cache_append_create": (ctypes.c_int, [_VP, ctypes.POINTER(CacheAppendDesc), _PPV]),
+    "pk_cache_append_enqueue": (ctypes.c_int, [_VP, ctypes.c_uint32, _VP]),
+    "pk_cache_append_enqueue_timed": (ctypes.c_int, [_VP, ctypes.c_uint32, _VP, _VP, _VP]),
+    "pk_cache_append_destroy": (ctypes.c_int, [_VP]),
+    "pk_cache_append_release": (ctypes.c_int, [_VP]),
+    "pk_cache_attention_validate": (ctypes.c_int, [ctypes.POINTER(CacheAttentionDesc)]),
+    "pk_cache_attention_create": (ctypes.c_int, [_VP, ctypes.POINTER(CacheAttentionDesc), _PPV]),
+    "pk_cache_attention_enqueue": (ctypes.c_int, [_VP, ctypes.c_uint32, _VP]),
+    "pk_cache_attention_enqueue_timed": (ctypes.c_int, [_VP, ctypes.c_uint32, _VP, _VP, _VP]),
+    "pk_cache_attention_destroy": (ctypes.c_int, [_VP]),
+    "pk_cache_attention_release": (ctypes.c_int, [_VP]),
+    "pk_verify_validate": (ctypes.c_int, [ctypes.POINTER(VerifyDesc)]),
+    "pk_verify_create": (ctypes.c_int, [_VP, ctypes.POINTER(VerifyDesc), _PPV]),
+    "pk_verify_enqueue": (ctypes.c_int, [_VP, ctypes.c_uint32, _VP]),
+    "pk_verify_enqueue_timed": (ctypes.c_int, [_VP, ctypes.c_uint32, _VP, _VP, _VP]),
+    "pk_verify_destroy": (ctypes.c_int, [_VP]),
+    "pk_verify_release": (ctypes.c_int, [_VP]),
     "pk_subsampling_output_dimension": (ctypes.c_uint32, [ctypes.c_uint32]),
     "pk_subsampling_valid_length": (ctypes.c_uint32, [ctypes.c_uint32, ctypes.c_uint32]),
     "pk_subsampling_fused_validate": (ctypes.c_int, [ctypes.POINTER(SubsamplingFusedDesc)]),
@@ -1260,6 +1397,93 @@ class TokenScoreOp(_RowsOp):
 
     def __init__(self, ctx: Context, **descriptor):
         super().__init__(ctx, score_desc(**descriptor))
+
+
+def cache_append_desc(*, keys, values, rows: int, sequences: int, kv_heads: int, head_dim: int, row_starts, lengths,
+                      page_table, pages_per_sequence: int, key_cache, value_cache, pages: int, page_size: int,
+                      heads: int = 0, queries=None, query_output=None, query_stride: int = 0,
+                      query_output_stride: int = 0, key_stride: int = 0, value_stride: int = 0, rotary_dim: int = 0,
+                      rotary: str = "halves", frequencies=None, positions=None, page_stride: int = 0,
+                      precision: str | None = None, label: str = "cache-append") -> CacheAppendDesc:
+    """A pk_cache_append_desc: rotated queries to query_output, rotated keys and
+    values into the pages of their sequences; strides in elements, 0 for
+    packed rows and pages."""
+    if precision is None:
+        precision = "f16" if keys.dtype == np.float16 else "f32"
+    return CacheAppendDesc(ctypes.sizeof(CacheAppendDesc), label.encode(), PRECISION[precision], rows, sequences, heads,
+                           kv_heads, head_dim, *_slice(queries), query_stride, *_slice(query_output),
+                           query_output_stride, *_slice(keys), key_stride, *_slice(values), value_stride, rotary_dim,
+                           ROTARY[rotary], *_slice(frequencies), *_slice(positions), *_slice(row_starts),
+                           *_slice(lengths), *_slice(page_table), pages_per_sequence, pages, page_size, page_stride,
+                           *_slice(key_cache), *_slice(value_cache))
+
+
+class _SequencesOp(_RowsOp):
+    """An op over the rows of sequences: `active_sequences` are its first ones."""
+
+    def enqueue(self, active_sequences: int = 0, stream=None, start: "Event" = None, end: "Event" = None) -> None:
+        super().enqueue(active_sequences, stream, start, end)
+
+
+class CacheAppendOp(_SequencesOp):
+    """New tokens of sequences into a paged cache (pk_cache_append_*)."""
+
+    _prefix = "cache_append"
+
+    def __init__(self, ctx: Context, **descriptor):
+        super().__init__(ctx, cache_append_desc(**descriptor))
+
+
+def cache_attention_desc(*, queries, output, rows: int, sequences: int, heads: int, kv_heads: int, head_dim: int,
+                         row_starts, lengths, page_table, pages_per_sequence: int, key_cache, value_cache, pages: int,
+                         page_size: int, query_stride: int = 0, output_stride: int = 0, causal: bool = True,
+                         window: int = 0, scale: float | None = None, score_cap: float | None = None,
+                         page_stride: int = 0, precision: str | None = None,
+                         label: str = "cache-attention") -> CacheAttentionDesc:
+    """A pk_cache_attention_desc: softmax(scale * q . k, capped) . v over the
+    tokens of a sequence that a row sees; strides in elements, 0 for packed
+    rows and pages."""
+    if precision is None:
+        precision = "f16" if queries.dtype == np.float16 else "f32"
+    return CacheAttentionDesc(ctypes.sizeof(CacheAttentionDesc), label.encode(), PRECISION[precision], rows, sequences,
+                              heads, kv_heads, head_dim, *_slice(queries), query_stride, *_slice(output),
+                              output_stride, int(causal), window, int(scale is not None), float(scale or 0.0),
+                              float(score_cap or 0.0), *_slice(row_starts), *_slice(lengths), *_slice(page_table),
+                              pages_per_sequence, pages, page_size, page_stride, *_slice(key_cache),
+                              *_slice(value_cache))
+
+
+class CacheAttentionOp(_SequencesOp):
+    """Attention of new tokens over a paged cache (pk_cache_attention_*)."""
+
+    _prefix = "cache_attention"
+
+    def __init__(self, ctx: Context, **descriptor):
+        super().__init__(ctx, cache_attention_desc(**descriptor))
+
+
+def verify_desc(*, target, rows: int, sequences: int, columns: int, row_starts, tokens, accepted, next_tokens,
+                mode: str = "sample", target_stride: int = 0, draft=None, draft_stride: int = 0, uniforms=None, draws=None,
+                temperature: float | None = None, precision: str | None = None,
+                label: str = "draft-verification") -> VerifyDesc:
+    """A pk_verify_desc: how many drafted tokens stand against the target's
+    logits, and the token that follows. Mode "greedy" reads no draft logits,
+    uniforms or draws."""
+    if precision is None:
+        precision = "f16" if target.dtype == np.float16 else "f32"
+    return VerifyDesc(ctypes.sizeof(VerifyDesc), label.encode(), PRECISION[precision], VERIFY_MODE[mode], rows,
+                      sequences, columns, *_slice(target), target_stride, *_slice(draft), draft_stride,
+                      int(temperature is not None), float(temperature or 0.0), *_slice(row_starts), *_slice(tokens),
+                      *_slice(uniforms), *_slice(draws), *_slice(accepted), *_slice(next_tokens))
+
+
+class DraftVerifyOp(_SequencesOp):
+    """Drafted tokens against a target model's logits (pk_verify_*)."""
+
+    _prefix = "verify"
+
+    def __init__(self, ctx: Context, **descriptor):
+        super().__init__(ctx, verify_desc(**descriptor))
 
 
 def subsampling_fused_desc(*, input, conv0_weights, conv0_bias, depthwise_weights, depthwise_bias, output,
