@@ -25,6 +25,7 @@ struct pk_cache_attention_op {
   std::string label;
   uint32_t sequences = 0;
   pk::CacheAttentionArgs args{};
+  void* workspace = nullptr;
   bool destroyed = false;
 };
 
@@ -305,12 +306,32 @@ int pk_cache_attention_create(pk_context* ctx, const pk_cache_attention_desc* d,
   a.cap = d->score_cap;
   a.causal = d->causal != 0;
   a.f16 = d->precision == PK_PRECISION_F16;
+  const uint64_t elem = a.f16 ? 2u : 4u;
+  a.wide_rows = aligned(a.queries, 16) && aligned(a.output, 16) && a.query_stride * elem % 16u == 0 &&
+                a.output_stride * elem % 16u == 0;
+  void* workspace = nullptr;
+  if (const uint64_t bytes = pk::cache_attention_workspace(a)) {
+    DeviceScope device(ctx->device);
+    PK_HIP(device.status(), "hipSetDevice");
+    const hipError_t e = hipMalloc(&workspace, bytes);
+    if (e != hipSuccess) {
+      (void)hipGetLastError();
+      return fail(PK_ALLOCATION_FAILURE, "%s: cannot allocate %llu bytes of workspace: %s", label.c_str(),
+                  (unsigned long long)bytes, hipGetErrorString(e));
+    }
+    a.workspace = workspace;
+    a.workspace_bytes = bytes;
+  }
   auto* op = new (std::nothrow) pk_cache_attention_op();
-  if (!op) return fail(PK_ALLOCATION_FAILURE, "%s: out of host memory", label.c_str());
+  if (!op) {
+    free_on(ctx->device, workspace);
+    return fail(PK_ALLOCATION_FAILURE, "%s: out of host memory", label.c_str());
+  }
   op->ctx = ctx;
   op->label.swap(label);
   op->sequences = d->sequences;
   op->args = a;
+  op->workspace = workspace;
   *out = op;
   return ok();
 } catch (const std::bad_alloc&) {
@@ -334,7 +355,10 @@ int pk_cache_attention_enqueue_timed(pk_cache_attention_op* op, uint32_t active_
 }
 
 int pk_cache_attention_destroy(pk_cache_attention_op* op) {
-  if (op) op->destroyed = true;
+  if (!op || op->destroyed) return ok();
+  op->destroyed = true;
+  free_on(op->ctx->device, op->workspace);
+  op->workspace = nullptr;
   return ok();
 }
 

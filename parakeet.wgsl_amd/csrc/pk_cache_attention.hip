@@ -1,6 +1,20 @@
 // pk_cache_attention.hip - attention of new tokens over a paged cache for
 // gfx950 (include/pk_cache.h has the formulas and what the arrays may hold).
+//
+// A unit is one kv head of one sequence and up to R of the rows that read it: the
+// G = heads / kv_heads query heads of the sequence's new tokens, token by
+// token. Lengths are known on the device alone, so the launch brings more
+// workgroups than there are units, and each finds its item from the arrays:
+// the tokens of all units over the workgroups left give the longest part, and
+// units longer than that are split into equal parts, so that one long sequence
+// among short ones fills the device too. Parts meet in memory of the op and a second
+// launch joins them in their order.
+//
+// Scores are computed transposed, S^T = K Q^T: a lane then holds scores of
+// one row, its running maximum and sum stay in that lane, and the exponentials
+// are at once the operand of O^T = V^T P^T.
 #include "pk_internal.h"
+#include "pk_wave.h"
 
 namespace pk {
 namespace {
@@ -8,12 +22,22 @@ namespace {
 constexpr float kInf = __builtin_inff();
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr int kThreads = 256;
-constexpr int kMaxDim = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr uint32_t kMaxDim = 256;
+// The running maximum, in log2 units, is moved when a score passes it by more:
+// exponentials stay below 2^8, and most tiles move nothing.
+constexpr float kMargin = 8.0f;
 
-// Tokens [low, high) that the row at `position` of a sequence of `length` sees.
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+
+// Tokens [low, high).
 struct Seen {
   uint32_t low, high;
 };
+// What a row at `position` of a sequence of `length` tokens sees.
 __device__ __forceinline__ Seen seen_by(const CacheAttentionArgs& args, uint32_t length, int64_t position) {
   const uint32_t held = min(length, args.cache.capacity());
   if (!args.causal) return {0u, held};
@@ -22,6 +46,235 @@ __device__ __forceinline__ Seen seen_by(const CacheAttentionArgs& args, uint32_t
   const uint32_t low = args.window && p >= args.window ? p - args.window + 1u : 0u;
   return {min(low, high), high};
 }
+// What any of `count` rows from `first` on sees.
+__device__ __forceinline__ Seen seen_by(const CacheAttentionArgs& args, uint32_t length, int64_t first,
+                                        uint32_t count) {
+  const Seen last = seen_by(args, length, first + count - 1);
+  const Seen start = seen_by(args, length, first < 0 ? 0 : first);
+  return {min(start.low, last.high), last.high};
+}
+
+// A unit, as the launch that joins finds it.
+struct Unit {
+  uint32_t slot, parts;        // the record of its first item, and how many
+  uint32_t row, rows;          // first row of the sequence, rows of all heads in the unit
+  uint32_t head, first;        // kv head, first of the sequence's rows of all heads
+};
+// What the host chose for a launch: most_units + more workgroups.
+struct Plan {
+  uint32_t most_units;
+  uint32_t more;      // 0: no unit is split
+  uint32_t shortest;  // tokens of a part, at least
+};
+// Memory of the op: the number of units, the units, then a record of each
+// item of a split unit: maxima and sums of its rows, then their outputs before the division.
+// A unit of more than `longest` tokens has less than 2 span / longest parts, and all
+// spans add up to at most `more` times longest: 2 * more records.
+struct Workspace {
+  uint32_t* units_count;
+  Unit* units;
+  float2* sums;    // [records][R]
+  float* outputs;  // [records][R][dim]
+};
+constexpr uint64_t kHeader = 256;
+__host__ __device__ constexpr uint64_t units_bytes(const Plan& p) {
+  return (p.most_units * sizeof(Unit) + 255u) / 256u * 256u;
+}
+uint64_t workspace_bytes(const Plan& p, uint32_t R, uint32_t dim) {
+  return kHeader + units_bytes(p) + 2ull * p.more * R * (sizeof(float2) + 4u * dim);
+}
+__device__ inline Workspace bind(void* memory, const Plan& plan, uint32_t R) {
+  uint8_t* p = static_cast<uint8_t*>(memory);
+  Workspace w;
+  w.units_count = reinterpret_cast<uint32_t*>(p);
+  w.units = reinterpret_cast<Unit*>(p + kHeader);
+  w.sums = reinterpret_cast<float2*>(p + kHeader + units_bytes(plan));
+  w.outputs = reinterpret_cast<float*>(w.sums + 2ull * plan.more * R);
+  return w;
+}
+
+// What a workgroup does: a part of a unit.
+struct Item {
+  uint32_t sequence, head;   // kv head
+  uint32_t row;              // first row of the sequence
+  uint32_t first, rows;      // rows of all heads: the first of the sequence's, how many
+  uint32_t length;
+  int64_t position;          // of the sequence's first row
+  uint32_t new_tokens;
+  uint32_t parts, part;
+  uint32_t unit;             // number of the unit
+  uint32_t slot;             // of the unit's first part, if it has several
+  bool live;
+};
+
+// Finds item `index`; every wavefront for itself, lanes over the sequences.
+template <int R>
+__device__ __forceinline__ Item find_item(const CacheAttentionArgs& args, const Plan& plan, uint32_t index,
+                                          uint32_t* units_count) {
+  const CacheView& cache = args.cache;
+  const uint32_t lane = threadIdx.x & 63u, group = args.heads / cache.kv_heads;
+  struct Of {
+    uint32_t start, count, tiles, span;
+  };
+  const auto of = [&](uint32_t s) {
+    Of x = {0, 0, 0, 0};
+    if (s < cache.sequences) {
+      x.start = min(cache.row_starts[s], cache.rows);
+      const uint32_t end = min(cache.row_starts[s + 1], cache.rows), length = cache.lengths[s];
+      x.count = end > x.start ? end - x.start : 0u;
+      x.tiles = (x.count * group + R - 1u) / R;
+      const Seen seen = seen_by(args, length, (int64_t)length - x.count, x.count);
+      x.span = x.count ? max(1u, seen.high - seen.low) : 0u;
+    }
+    return x;
+  };
+  // All units, and all their tokens.
+  uint32_t units = 0;
+  float tokens = 0.0f;
+  Of mine = of(lane);
+  for (uint32_t s = lane; s < cache.sequences; s += 64u) {
+    if (s != lane) mine = of(s);
+    units += mine.tiles * cache.kv_heads;
+    tokens += (float)(mine.tiles * cache.kv_heads) * (float)mine.span;
+  }
+#pragma unroll
+  for (int off = 32; off; off >>= 1) {
+    units += __shfl_xor(units, off, 64);
+    tokens += __shfl_xor(tokens, off, 64);
+  }
+  *units_count = units;
+  // Parts of at most `longest` tokens: sum(ceil(span / longest)) over the units is at
+  // most tokens / longest + units. The quotient is rounded up by more than its
+  // and the sum's roundings. More units than there can be come from row starts
+  // that decrease: those are not split.
+  uint32_t longest = 0x7fffffffu;
+  if (plan.more && units <= plan.most_units)
+    longest = max(plan.shortest, (uint32_t)min(tokens / (float)plan.more * 1.0001f + 1.0f, 2e9f));
+  Item item;
+  item.live = false;
+  uint32_t items_before = 0, units_before = 0, slots_before = 0;
+  for (uint32_t base = 0; base < cache.sequences; base += 64u) {
+    const uint32_t s = base + lane;
+    if (cache.sequences > 64u) mine = of(s);
+    const uint32_t parts = mine.span ? (mine.span + longest - 1u) / longest : 0u;
+    const uint32_t have = mine.tiles * cache.kv_heads, items = have * parts, slots = parts > 1u ? items : 0u;
+    uint32_t items_to = items, units_to = have, slots_to = slots;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const uint32_t a = __shfl_up(items_to, off, 64), b = __shfl_up(units_to, off, 64), c = __shfl_up(slots_to, off, 64);
+      if ((int)lane >= off) {
+        items_to += a;
+        units_to += b;
+        slots_to += c;
+      }
+    }
+    const uint64_t hit = __ballot(index < items_before + items_to);
+    if (hit) {
+      const int at = __builtin_ctzll(hit);
+      const uint32_t owned = __shfl(items, at, 64), each = __shfl(parts, at, 64), tiles = __shfl(mine.tiles, at, 64);
+      const uint32_t before = items_before + __shfl(items_to, at, 64) - owned;
+      const uint32_t local = index - before, unit = local / each;
+      item.live = true;
+      item.sequence = base + at;
+      item.parts = each;
+      item.part = local - unit * each;
+      item.head = unit / tiles;
+      item.first = (unit - item.head * tiles) * R;
+      item.row = __shfl(mine.start, at, 64);
+      item.new_tokens = __shfl(mine.count, at, 64);
+      item.rows = min((uint32_t)R, item.new_tokens * group - item.first);
+      item.length = cache.lengths[item.sequence];
+      item.position = (int64_t)item.length - item.new_tokens;
+      item.unit = units_before + __shfl(units_to, at, 64) - tiles * cache.kv_heads + unit;
+      item.slot = slots_before + __shfl(slots_to - slots, at, 64) + unit * each;
+      break;
+    }
+    items_before += __shfl(items_to, 63, 64);
+    units_before += __shfl(units_to, 63, 64);
+    slots_before += __shfl(slots_to, 63, 64);
+  }
+  return item;
+}
+
+// tanh: by the exponential, and near 0, where that loses digits, by its series.
+__device__ __forceinline__ float tanh_of(float x) {
+  const float e = __builtin_amdgcn_exp2f(2.0f * kLog2E * x);
+  const float far = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + e);
+  const float x2 = x * x;
+  const float near = __builtin_fmaf(
+      x * x2, __builtin_fmaf(x2, __builtin_fmaf(x2, __builtin_fmaf(x2, 0.021869489f, -0.053968254f), 0.13333333f),
+                             -0.33333333f), x);
+  return fabsf(x) < 0.25f ? near : far;
+}
+
+// From the product of a query and a key to the score in log2 units.
+struct Score {
+  float before, after;
+  bool capped;
+  __device__ explicit Score(const CacheAttentionArgs& args)
+      : before(args.cap > 0.0f ? args.scale / args.cap : args.scale * kLog2E), after(args.cap * kLog2E),
+        capped(args.cap > 0.0f) {}
+  __device__ __forceinline__ float operator()(float dot) const {
+    return capped ? after * tanh_of(dot * before) : dot * before;
+  }
+};
+
+// Where the tokens of one kv head of a sequence lie, in pieces of 16 bytes
+// from the start of a cache: 64 GiB of cache are 2^32 of them.
+template <typename T>
+struct Places {
+  const uint32_t* table;
+  uint32_t row, page, head;  // pieces of a token, from page to page, and to the head
+  uint32_t count, size, magic, shift;
+  __device__ Places(const CacheView& c, uint32_t sequence, uint32_t kv)
+      : table(c.page_table + (uint64_t)sequence * c.pages_per_sequence),
+        row((uint32_t)(c.head_dim * sizeof(T) / 16u)), page((uint32_t)(c.page_stride * sizeof(T) / 16u)),
+        head(kv * c.page_size * (uint32_t)(c.head_dim * sizeof(T) / 16u)), count(c.pages), size(c.page_size),
+        magic(c.page_magic), shift(c.page_shift) {}
+  static constexpr uint32_t none = 0xffffffffu;
+  __device__ __forceinline__ uint32_t at(uint32_t token) const {
+    return (uint32_t)(((uint64_t)token * magic) >> shift);
+  }
+  // The table's entry of a token below `end`.
+  __device__ __forceinline__ uint32_t entry(uint32_t token, uint32_t end) const {
+    return token < end ? table[at(token)] : none;
+  }
+  __device__ __forceinline__ uint32_t place(uint32_t token, uint32_t entry) const {
+    return entry * page + head + (token - at(token) * size) * row;
+  }
+};
+
+// The part [from, to) of the tokens that an item works on.
+__device__ __forceinline__ Seen part_of(const CacheAttentionArgs& args, const Item& item) {
+  const uint32_t group = args.heads / args.cache.kv_heads;
+  const uint32_t token = item.first / group, last = (item.first + item.rows - 1u) / group;
+  const Seen all = seen_by(args, item.length, item.position + token, last - token + 1u);
+  if (item.parts == 1u) return all;
+  const uint32_t each = ((all.high - all.low) / item.parts + 32u) & ~31u;
+  const uint64_t low = all.low + (uint64_t)item.part * each;
+  return {(uint32_t)min(low, (uint64_t)all.high), (uint32_t)min(low + each, (uint64_t)all.high)};
+}
+
+// Writes element d of row r of an item: the output, or what the join needs.
+template <typename T, int R>
+struct Result {
+  const CacheAttentionArgs& args;
+  const Item& item;
+  const Workspace& work;
+  __device__ T* output(uint32_t r) const {
+    const uint32_t group = args.heads / args.cache.kv_heads, i = item.first + r, token = i / group;
+    return static_cast<T*>(args.output) + (item.row + token) * args.output_stride +
+           (uint64_t)(item.head * group + (i - token * group)) * args.cache.head_dim;
+  }
+  __device__ float* partial(uint32_t r) const {
+    return work.outputs + ((uint64_t)(item.slot + item.part) * R + r) * args.cache.head_dim;
+  }
+  __device__ void sums(uint32_t r, float m, float l) const {
+    work.sums[(uint64_t)(item.slot + item.part) * R + r] = make_float2(m, l);
+  }
+};
+// 1 / l, and 0 where no score counted.
+__device__ __forceinline__ float inverse(float m, float l) { return m == -kInf && l == 0.0f ? 0.0f : 1.0f / l; }
 
 __device__ __forceinline__ float block_reduce(float x, bool largest, float* scratch) {
 #pragma unroll
@@ -33,75 +286,560 @@ __device__ __forceinline__ float block_reduce(float x, bool largest, float* scra
   if ((threadIdx.x & 63u) == 0) scratch[threadIdx.x >> 6] = x;
   __syncthreads();
   x = scratch[0];
-  for (int w = 1; w < kThreads / 64; ++w) x = largest ? fmaxf(x, scratch[w]) : x + scratch[w];
+  for (int w = 1; w < kWaves; ++w) x = largest ? fmaxf(x, scratch[w]) : x + scratch[w];
   return x;
 }
 
-// One row of one head: a thread scores a token, then sums an element.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void cache_attention_row_kernel(CacheAttentionArgs args) {
-  __shared__ float query[kMaxDim], weight[kThreads], scratch[kThreads / 64];
-  __shared__ uint64_t places[kThreads];
-  __shared__ uint32_t owner;
+// An item without matrix instructions: a thread scores a token, then sums an element.
+// A product of matrices multiplies every value of a tile by every row's exponential, so that an
+// infinity or a NaN that only a later row sees would reach the earlier ones as
+// 0 * inf: items whose output is not finite come here.
+template <typename T, int R>
+__device__ __forceinline__ void careful_item(const CacheAttentionArgs& args, const Item& item, const Workspace& work,
+                                             float* lds) {
+  float *query = lds, *weight = lds + kMaxDim, *scratch = weight + kThreads;
+  uint32_t* places = reinterpret_cast<uint32_t*>(scratch + kWaves);
   const CacheView& cache = args.cache;
-  const uint32_t at = threadIdx.x, row = blockIdx.x, head = blockIdx.y, dim = cache.head_dim;
-  if (at == 0) owner = ~0u;
-  __syncthreads();
-  for (uint32_t s = at; s < cache.sequences; s += kThreads)
-    if (row >= min(cache.row_starts[s], cache.rows) && row < min(cache.row_starts[s + 1], cache.rows)) owner = s;
-  __syncthreads();
-  const uint32_t s = owner;
-  if (s >= cache.sequences) return;
-  const uint32_t length = cache.lengths[s];
-  const int64_t position = (int64_t)length - (min(cache.row_starts[s + 1], cache.rows) - row);
-  const Seen seen = seen_by(args, length, position);
-  const uint64_t kv = (uint64_t)(head / (args.heads / cache.kv_heads)) * cache.page_size * dim;
-  const T* q = static_cast<const T*>(args.queries) + row * args.query_stride + (uint64_t)head * dim;
-  if (at < dim) query[at] = (float)q[at];
-  float m = -kInf, l = 0.0f, out = 0.0f;
-  for (uint32_t t0 = seen.low; t0 < seen.high; t0 += kThreads) {
+  const uint32_t at = threadIdx.x, dim = cache.head_dim, group = args.heads / cache.kv_heads;
+  const Seen part = part_of(args, item);
+  const Places<T> map(cache, item.sequence, item.head);
+  const Score score(args);
+  const Result<T, R> result{args, item, work};
+  constexpr uint32_t kPiece = 16 / sizeof(T);
+  for (uint32_t r = 0; r < item.rows; ++r) {
+    const uint32_t i = item.first + r, token = i / group;
+    const Seen own = seen_by(args, item.length, item.position + token);
+    const uint32_t low = max(own.low, part.low), high = min(own.high, part.high);
+    const T* q = static_cast<const T*>(args.queries) + (item.row + token) * args.query_stride +
+                 (uint64_t)(item.head * group + (i - token * group)) * dim;
     __syncthreads();
-    const uint32_t t = t0 + at;
-    const uint64_t place = t < seen.high ? cache.place(s, t) : CacheView::no_place;
-    float z = -kInf;
-    if (place != CacheView::no_place) {
-      const T* k = static_cast<const T*>(args.key_cache) + place + kv;
-      float dot = 0.0f;
-      for (uint32_t d = 0; d < dim; ++d) dot = __builtin_fmaf(query[d], (float)k[d], dot);
-      z = dot * args.scale;
-      if (args.cap > 0.0f) z = args.cap * tanhf(z / args.cap);
+    if (at < dim) query[at] = (float)q[at];
+    float m = -kInf, l = 0.0f, out = 0.0f;
+    for (uint32_t t0 = low; t0 < high; t0 += kThreads) {
+      __syncthreads();
+      const uint32_t t = t0 + at, entry = map.entry(t, high);
+      const uint32_t place = entry < map.count ? map.place(t, entry) : Places<T>::none;
+      float z = -kInf;
+      if (place != Places<T>::none) {
+        const T* k = static_cast<const T*>(args.key_cache) + (uint64_t)place * kPiece;
+        float dot = 0.0f;
+        for (uint32_t d = 0; d < dim; ++d) dot = __builtin_fmaf(query[d], (float)k[d], dot);
+        z = score(dot);
+      }
+      places[at] = place;
+      const float top = fmaxf(m, block_reduce(z, true, scratch));
+      const float base = top == -kInf ? 0.0f : top;
+      const float p = __builtin_amdgcn_exp2f(z - base), old = __builtin_amdgcn_exp2f(m - base);
+      m = top;
+      weight[at] = p;
+      l = l * old + block_reduce(p, false, scratch);
+      __syncthreads();
+      if (at < dim) {
+        out *= old;
+        const uint32_t count = min((uint32_t)kThreads, high - t0);
+        for (uint32_t j = 0; j < count; ++j)
+          if (places[j] != Places<T>::none)
+            out = __builtin_fmaf(weight[j], (float)(static_cast<const T*>(args.value_cache) + (uint64_t)places[j] * kPiece)[at],
+                                 out);
+      }
     }
-    places[at] = place;
-    const float top = fmaxf(m, block_reduce(z, true, scratch));
-    const float base = top == -kInf ? 0.0f : top;
-    const float p = __builtin_amdgcn_exp2f((z - base) * kLog2E), old = __builtin_amdgcn_exp2f((m - base) * kLog2E);
-    m = top;
-    weight[at] = p;
-    l = l * old + block_reduce(place != CacheView::no_place ? p : 0.0f, false, scratch);
-    __syncthreads();
-    if (at < dim) {
-      out *= old;
-      const uint32_t count = min((uint32_t)kThreads, seen.high - t0);
-      for (uint32_t i = 0; i < count; ++i)
-        if (places[i] != CacheView::no_place)
-          out = __builtin_fmaf(weight[i], (float)(static_cast<const T*>(args.value_cache) + places[i] + kv)[at], out);
+    if (item.parts == 1u) {
+      if (at < dim) result.output(r)[at] = (T)(out * inverse(m, l));
+    } else {
+      if (at < dim) result.partial(r)[at] = out;
+      if (at == 0) result.sums(r, m, l);
     }
   }
-  if (at < dim)
-    (static_cast<T*>(args.output) + row * args.output_stride + (uint64_t)head * dim)[at] =
-        (T)(m == -kInf && l == 0.0f ? 0.0f : out / l);
+}
+
+// The kernels of few rows: the wavefronts of a workgroup hold the same RB blocks of
+// 16 rows and take the steps of tokens in turn, each with maxima, sums and
+// outputs of its own, which meet in LDS at the end.
+//
+// f16: steps of 32 tokens. Keys come from the cache straight into the operand
+// of v_mfma_f32_16x16x32_f16 (a lane has 16 bytes of one token, the order of
+// the channels being free as long as queries have the same); values go
+// through LDS, whose transposed reads give four tokens of a channel, in the
+// order in which the scores lie. f32: steps of 16 tokens, v_mfma_f32_16x16x4_f32,
+// whose operands take keys and values as they lie.
+//
+// The loads of a step's keys are issued when the step before has used its own, those of
+// its values likewise, and the entries of the page table a step ahead of the keys, before
+// the values: loads return in their order, and nothing waits for more than it needs.
+template <typename T>
+struct Step;
+template <>
+struct Step<_Float16> {
+  static constexpr int kTokens = 32;
+};
+template <>
+struct Step<float> {
+  static constexpr int kTokens = 16;
+};
+
+template <typename T, int DP, int RB>
+struct FewShape {
+  static constexpr int kTokens = Step<T>::kTokens;
+  static constexpr int kValueBytes = sizeof(T) == 2 ? kTokens * DP * 2 : 0;  // of a wavefront
+  static constexpr int kSlice = 64, kSliceRow = kSlice + 4;                  // channels that are joined at a time
+  static constexpr int kJoinBytes = kWaves * RB * 16 * kSliceRow * 4;
+  static constexpr int kCarefulBytes = (int)(kMaxDim + kThreads + kWaves + kThreads) * 4;
+  static constexpr int kSums = 2 * kWaves * RB * 16 * 4;
+  static constexpr int largest(int a, int b) { return a > b ? a : b; }
+  static constexpr int kLds = kSums + 16 + largest(largest(kWaves * kValueBytes, kJoinBytes), kCarefulBytes);
+};
+
+template <typename T, int DP, int RB, bool WHOLE>
+__global__ __launch_bounds__(kThreads) void cache_attention_few_kernel(CacheAttentionArgs args, Plan plan) {
+  typedef FewShape<T, DP, RB> Shape;
+  constexpr int R = 16 * RB, STEP = Shape::kTokens, TB = STEP / 16;  // token blocks of a step
+  constexpr bool kHalf = sizeof(T) == 2;
+  constexpr int PIECE = 16 / sizeof(T);
+  constexpr int KS = DP / (4 * PIECE);         // pieces of a key in a lane
+  constexpr int VR = DP / PIECE;               // pieces of a value row
+  constexpr int VS = STEP * VR / 64;           // pieces of a step's values in a lane
+  constexpr int OB = DP / 16;                  // blocks of 16 channels
+  typedef T V __attribute__((ext_vector_type(PIECE)));
+  __shared__ __attribute__((aligned(16))) uint8_t lds[Shape::kLds];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = lane & 15u, quarter = lane >> 4;
+  const CacheView& cache = args.cache;
+
+  uint32_t units;
+  const Item item = find_item<R>(args, plan, blockIdx.x, &units);
+  const Workspace work = bind(args.workspace, plan, R);
+  if (plan.more && blockIdx.x == 0 && threadIdx.x == 0) *work.units_count = min(units, plan.most_units);
+  if (!item.live) return;
+  if (plan.more && item.part == 0 && item.unit < plan.most_units && threadIdx.x == 0)
+    work.units[item.unit] = {item.slot, item.parts, item.row, item.rows, item.head, item.first};
+  const Seen part = part_of(args, item);
+  const uint32_t group = args.heads / cache.kv_heads, dim = cache.head_dim;
+  const Places<T> map(cache, item.sequence, item.head);
+  const Score score(args);
+  const uint32_t pieces = dim / PIECE;
+
+  // Queries, and what their rows see.
+  V query[RB][KS];
+  uint32_t low[RB], high[RB];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const uint32_t r = 16u * b + col;
+    low[b] = high[b] = 0;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) query[b][k] = V{};
+    if (r < item.rows) {
+      const uint32_t i = item.first + r, token = i / group;
+      const Seen own = seen_by(args, item.length, item.position + token);
+      low[b] = own.low;
+      high[b] = own.high;
+      const T* q = static_cast<const T*>(args.queries) + (item.row + token) * args.query_stride +
+                   (uint64_t)(item.head * group + (i - token * group)) * dim;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const uint32_t c = 4u * k + quarter;
+        if (WHOLE || c < pieces) {
+          if (args.wide_rows) {
+            query[b][k] = *reinterpret_cast<const V*>(q + c * PIECE);
+          } else {
+#pragma unroll
+            for (int e = 0; e < PIECE; ++e) query[b][k][e] = q[c * PIECE + e];
+          }
+        }
+      }
+    }
+  }
+  // Tokens that all rows of the unit see.
+  uint32_t common_low = 0, common_high = 0xffffffffu;
+  {
+    const uint32_t t0 = item.first / group, t1 = (item.first + item.rows - 1u) / group;
+    common_high = seen_by(args, item.length, item.position + t0).high;
+    common_low = seen_by(args, item.length, item.position + t1).low;
+  }
+
+  float m[RB], l[RB];
+  floatx4 out[RB][OB];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    m[b] = -kInf;
+    l[b] = 0.0f;
+#pragma unroll
+    for (int o = 0; o < OB; ++o) out[b][o] = floatx4{};
+  }
+
+  const uint8_t *keys = static_cast<const uint8_t*>(args.key_cache), *values = static_cast<const uint8_t*>(args.value_cache);
+  _Float16* tile = reinterpret_cast<_Float16*>(lds + Shape::kSums + 16 + wave * Shape::kValueBytes);
+  V key[TB][KS], value[VS];
+  const auto shuffled = [&](uint32_t x, uint32_t from) {
+    return (uint32_t)__builtin_amdgcn_ds_bpermute((int)(from * 4u), (int)x);
+  };
+  const auto load_keys = [&](uint32_t places) {
+#pragma unroll
+    for (int t = 0; t < TB; ++t) {
+      const uint64_t from = (uint64_t)shuffled(places, 16u * t + col) * 16u;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const uint32_t c = 4u * k + quarter;
+        if (WHOLE || c < pieces) key[t][k] = *reinterpret_cast<const V*>(keys + from + c * 16u);
+        else key[t][k] = V{};
+      }
+    }
+  };
+  // f16: 16 bytes of a row of the step, in their order; f32: channels 64 s + 4
+  // col + c of the tokens 4 quarter + r.
+  const auto value_token = [&](int i) { return kHalf ? (uint32_t)i * (64u / VR) + lane / VR : 4u * quarter + (i & 3); };
+  const auto value_piece = [&](int i) { return kHalf ? lane % VR : (uint32_t)(i >> 2) * 16u + col; };
+  const auto load_values = [&](uint32_t places, uint32_t live) {
+    if (WHOLE && live == (uint32_t)((1ull << STEP) - 1ull)) {
+#pragma unroll
+      for (int i = 0; i < VS; ++i)
+        value[i] = *reinterpret_cast<const V*>(values + ((uint64_t)shuffled(places, value_token(i)) + value_piece(i)) * 16u);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VS; ++i) {
+        const uint32_t token = value_token(i), c = value_piece(i), place = shuffled(places, token);
+        value[i] = V{};
+        if ((live >> token & 1u) && (WHOLE || c < pieces))
+          value[i] = *reinterpret_cast<const V*>(values + ((uint64_t)place + c) * 16u);
+      }
+    }
+  };
+
+  constexpr uint32_t kStride = kWaves * STEP;
+  const uint32_t mine = lane % STEP;
+  uint32_t t0 = part.low + wave * STEP;
+  uint32_t entry = map.entry(t0 + mine, part.high);
+  const auto places_of = [&](uint32_t from, uint32_t* live) {
+    const bool held = entry < map.count;
+    *live = (uint32_t)__ballot(held) & (uint32_t)((1ull << STEP) - 1ull);
+    return held ? map.place(from + mine, entry) : 0u;
+  };
+  uint32_t live = 0, places = 0;
+  if (t0 < part.high) {
+    places = places_of(t0, &live);
+    load_keys(places);
+    entry = map.entry(t0 + kStride + mine, part.high);
+    load_values(places, live);
+  }
+  for (; t0 < part.high; t0 += kStride) {
+    floatx4 s[RB][TB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+      for (int t = 0; t < TB; ++t) {
+        s[b][t] = floatx4{};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          if constexpr (kHalf) {
+            s[b][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key[t][k], query[b][k], s[b][t], 0, 0, 0);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              s[b][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(key[t][k][e], query[b][k][e], s[b][t], 0, 0, 0);
+          }
+        }
+      }
+    const uint32_t live_now = live;
+    const bool more = t0 + kStride < part.high;
+    if (more) {
+      places = places_of(t0 + kStride, &live);
+      load_keys(places);
+      entry = map.entry(t0 + 2u * kStride + mine, part.high);
+    }
+    // Scores, and the hidden ones among them.
+    const bool whole = live_now == (uint32_t)((1ull << STEP) - 1ull) && t0 >= common_low && t0 + STEP <= common_high;
+    V weights[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      float top = -kInf;
+#pragma unroll
+      for (int t = 0; t < TB; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float z = score(s[b][t][j]);
+          if (!whole) {
+            const uint32_t at = 16u * t + 4u * quarter + j, token = t0 + at;
+            z = (live_now >> at & 1u) && token >= low[b] && token < high[b] ? z : -kInf;
+          }
+          s[b][t][j] = z;
+          top = fmaxf(top, z);
+        }
+      if (__any(top > m[b] + kMargin)) {
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        top = fmaxf(top, m[b]);
+        const float old = m[b] == top ? 1.0f : __builtin_amdgcn_exp2f(m[b] - top);
+        m[b] = top;
+        l[b] *= old;
+#pragma unroll
+        for (int o = 0; o < OB; ++o) out[b][o] *= old;
+      }
+      const float base = m[b] == -kInf ? 0.0f : m[b];
+#pragma unroll
+      for (int t = 0; t < TB; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float p = __builtin_amdgcn_exp2f(s[b][t][j] - base);
+          l[b] += p;
+          if constexpr (kHalf) weights[b][4 * t + j] = (_Float16)p;
+          else weights[b][j] = p;
+        }
+    }
+    if constexpr (kHalf) {
+      // 32 bytes of a row, a granule, are found at the row's granule xor a number of the
+      // row, so that the 8 rows of a read lie on different banks.
+      const auto turned = [](uint32_t row) { return DP >= 128 ? row & 7u : row >> 1 & 3u; };
+      wave::sync();
+#pragma unroll
+      for (int i = 0; i < VS; ++i) {
+        const uint32_t row = value_token(i), c = value_piece(i);
+        *reinterpret_cast<V*>(tile + row * DP + ((c >> 1) ^ turned(row)) * 16u + (c & 1u) * 8u) = value[i];
+      }
+      if (more) load_values(places, live);
+      wave::sync();
+#pragma unroll
+      for (int o = 0; o < OB; ++o) {
+        V v;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const uint32_t row = 16u * t + 4u * quarter + (col >> 2);
+          const _Float16* from = tile + row * DP + ((uint32_t)o ^ turned(row)) * 16u + (col & 3u) * 4u;
+          const half4 four = __builtin_bit_cast(
+              half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)from));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[4 * t + e] = four[e];
+        }
+#pragma unroll
+        for (int b = 0; b < RB; ++b) out[b][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, weights[b], out[b][o], 0, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VS; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int b = 0; b < RB; ++b)
+            out[b][(i >> 2) * 4 + c] =
+                __builtin_amdgcn_mfma_f32_16x16x4f32(value[i][c], weights[b][i & 3], out[b][(i >> 2) * 4 + c], 0, 0, 0);
+      if (more) load_values(places, live);
+    }
+  }
+
+  // The wavefronts' maxima and sums, and whether an output that another row's
+  // tokens could have spoiled is not a number.
+  float* sums = reinterpret_cast<float*>(lds);
+  uint32_t* strange = reinterpret_cast<uint32_t*>(lds + Shape::kSums);
+  if (threadIdx.x == 0) *strange = 0;
+  bool odd = false;
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    l[b] += __shfl_xor(l[b], 16, 64);
+    l[b] += __shfl_xor(l[b], 32, 64);
+    if (quarter == 0) {
+      sums[wave * R + 16 * b + col] = m[b];
+      sums[kWaves * R + wave * R + 16 * b + col] = l[b];
+    }
+#pragma unroll
+    for (int o = 0; o < OB; ++o)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) odd |= !(fabsf(out[b][o][j]) < kInf);
+  }
+  __syncthreads();
+  if (args.causal && item.new_tokens > 1u && __any(odd) && lane == 0) *strange = 1;
+  float scale[RB];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    float top = -kInf;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, sums[w * R + 16 * b + col]);
+    scale[b] = m[b] == top ? 1.0f : __builtin_amdgcn_exp2f(m[b] - top);
+  }
+  __syncthreads();
+  if (*strange) {
+    careful_item<T, R>(args, item, work, reinterpret_cast<float*>(lds + Shape::kSums + 16));
+    return;
+  }
+  float* slices = reinterpret_cast<float*>(lds + Shape::kSums + 16);
+  const Result<T, R> result{args, item, work};
+#pragma unroll
+  for (int at = 0; at < DP; at += Shape::kSlice) {
+    if (at) __syncthreads();
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      float* to = slices + (wave * R + 16 * b + col) * Shape::kSliceRow;
+#pragma unroll
+      for (int o = 0; o < 4; ++o) {
+        const floatx4 x = out[b][at / 16 + o] * scale[b];
+        if constexpr (kHalf) {
+          *reinterpret_cast<floatx4*>(to + 16 * o + 4 * quarter) = x;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) to[16 * quarter + 4 * j + o] = x[j];
+        }
+      }
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < item.rows * (Shape::kSlice / 4); i += kThreads) {
+      const uint32_t r = i / (Shape::kSlice / 4), d = i % (Shape::kSlice / 4) * 4u;
+      if (at + d >= dim) continue;
+      floatx4 x = *reinterpret_cast<const floatx4*>(slices + r * Shape::kSliceRow + d);
+      float top = sums[r];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) {
+        x += *reinterpret_cast<const floatx4*>(slices + (w * R + r) * Shape::kSliceRow + d);
+        top = fmaxf(top, sums[w * R + r]);
+      }
+      float all = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float own = sums[w * R + r];
+        all = __builtin_fmaf(sums[kWaves * R + w * R + r], own == top ? 1.0f : __builtin_amdgcn_exp2f(own - top), all);
+      }
+      if (item.parts > 1u) {
+        *reinterpret_cast<floatx4*>(result.partial(r) + at + d) = x;
+        if (at + d == 0) result.sums(r, top, all);
+        continue;
+      }
+      x *= inverse(top, all);
+      T* to = result.output(r) + at + d;
+      if (args.wide_rows) {
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        T4 four;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) four[e] = (T)x[e];
+        *reinterpret_cast<T4*>(to) = four;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[e] = (T)x[e];
+      }
+    }
+  }
+}
+
+// Joins the parts of a unit: a wavefront takes a row, its lanes 4 channels each.
+template <typename T, int R>
+__global__ __launch_bounds__(kThreads) void cache_attention_join_kernel(CacheAttentionArgs args, Plan plan) {
+  const Workspace work = bind(args.workspace, plan, R);
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  const Unit unit = work.units[blockIdx.x];
+  if (blockIdx.x >= *work.units_count || unit.parts <= 1u) return;
+  const uint32_t group = args.heads / args.cache.kv_heads, dim = args.cache.head_dim;
+  const uint32_t d = 4u * lane < dim ? 4u * lane : 0u;  // all lanes take part in the exchange
+  for (uint32_t r = blockIdx.y * 16u + wave; r < min(unit.rows, blockIdx.y * 16u + 16u); r += kWaves) {
+    const float2* sums = work.sums + (uint64_t)unit.slot * R + r;
+    float top = -kInf;
+    for (uint32_t p = lane; p < unit.parts; p += 64u) top = fmaxf(top, sums[(uint64_t)p * R].x);
+    top = wave::max(top);
+    float all = 0.0f;
+    floatx4 x = floatx4{};
+    for (uint32_t p0 = 0; p0 < unit.parts; p0 += 64u) {
+      const uint32_t p = p0 + lane;
+      float factor = 0.0f;
+      if (p < unit.parts) {
+        const float2 own = sums[(uint64_t)p * R];
+        factor = own.x == top ? 1.0f : __builtin_amdgcn_exp2f(own.x - top);
+        all += own.y * factor;
+      }
+      const uint32_t count = min(64u, unit.parts - p0);
+      const float* from = work.outputs + ((uint64_t)(unit.slot + p0) * R + r) * dim + d;
+      for (uint32_t i = 0; i < count; i += 8u) {  // eight loads at a time
+        floatx4 some[8];
+#pragma unroll
+        for (uint32_t j = 0; j < 8u; ++j)
+          some[j] = *reinterpret_cast<const floatx4*>(from + (uint64_t)min(i + j, count - 1u) * R * dim);
+#pragma unroll
+        for (uint32_t j = 0; j < 8u; ++j) {
+          const uint32_t bits = (uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(factor), (int)min(i + j, 63u));
+          x += some[j] * (i + j < count ? __uint_as_float(bits) : 0.0f);
+        }
+      }
+    }
+    all = wave::sum(all);
+    x *= inverse(top, all);
+    const uint32_t i = unit.first + r, token = i / group;
+    T* to = static_cast<T*>(args.output) + (unit.row + token) * args.output_stride +
+            (uint64_t)(unit.head * group + (i - token * group)) * dim + d;
+    if (4u * lane < dim)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) to[e] = (T)x[e];
+  }
+}
+
+typedef void (*Kernel)(CacheAttentionArgs, Plan);
+struct Variant {
+  Kernel kernel, join;
+  uint32_t rows;  // of a unit
+};
+
+template <typename T, int DP, int RB>
+Variant few(bool whole) {
+  return {whole ? cache_attention_few_kernel<T, DP, RB, true> : cache_attention_few_kernel<T, DP, RB, false>,
+          cache_attention_join_kernel<T, 16 * RB>, 16 * RB};
+}
+
+// Blocks of 16 rows of a unit: as many as the rows of an average sequence need,
+// up to 4, and 2 for heads of more than 128 channels.
+uint32_t blocks_of(const CacheAttentionArgs& args) {
+  const uint64_t group = args.heads / args.cache.kv_heads;
+  const uint64_t rows = (args.cache.rows * group + args.cache.sequences - 1u) / args.cache.sequences;
+  return rows <= 16u ? 1u : rows <= 32u || args.cache.head_dim > 128u ? 2u : 4u;
+}
+
+template <typename T>
+Variant choose(const CacheAttentionArgs& args) {
+  const uint32_t dim = args.cache.head_dim, blocks = blocks_of(args);
+  if (dim <= 64u)
+    return blocks == 1u ? few<T, 64, 1>(dim == 64u) : blocks == 2u ? few<T, 64, 2>(dim == 64u) : few<T, 64, 4>(dim == 64u);
+  if (dim <= 128u)
+    return blocks == 1u   ? few<T, 128, 1>(dim == 128u)
+           : blocks == 2u ? few<T, 128, 2>(dim == 128u)
+                          : few<T, 128, 4>(dim == 128u);
+  return blocks == 1u ? few<T, 256, 1>(dim == 256u) : few<T, 256, 2>(dim == 256u);
+}
+
+constexpr uint32_t kShortest = 256;  // tokens of a part
+
+Plan plan_of(const CacheAttentionArgs& args, uint32_t R) {
+  const uint64_t group = args.heads / args.cache.kv_heads;
+  const uint32_t some = args.cache.sequences < args.cache.rows ? args.cache.sequences : args.cache.rows;
+  Plan plan;
+  // Full tiles of rows, and one that is not full for each sequence.
+  plan.most_units = (uint32_t)(args.cache.kv_heads * (args.cache.rows * group / R + some));
+  plan.more = args.cache.capacity() > kShortest ? (R > 32u ? 512u : 1024u) : 0u;
+  plan.shortest = kShortest;
+  return plan;
 }
 
 }  // namespace
 
+uint64_t cache_attention_workspace(const CacheAttentionArgs& args) {
+  // Any number of active sequences: the rows of a unit follow from it.
+  uint64_t most = 0;
+  for (uint32_t blocks : {1u, 2u, 4u}) {
+    if (blocks == 4u && args.cache.head_dim > 128u) continue;
+    const Plan plan = plan_of(args, 16u * blocks);
+    const uint64_t bytes = workspace_bytes(plan, 16u * blocks, args.cache.head_dim);
+    if (plan.more && bytes > most) most = bytes;
+  }
+  return most;
+}
+
 hipError_t launch_cache_attention(const CacheAttentionArgs& args, hipStream_t stream, hipEvent_t start,
                                   hipEvent_t stop) {
-  const auto kernel = args.f16 ? cache_attention_row_kernel<_Float16> : cache_attention_row_kernel<float>;
-  const dim3 grid(args.cache.rows, args.heads), block(kThreads);
-  if (start || stop)
-    hipExtLaunchKernelGGL(kernel, grid, block, 0, stream, start, stop, 0, args);
+  const Variant variant = args.f16 ? choose<_Float16>(args) : choose<float>(args);
+  const Plan plan = plan_of(args, variant.rows);
+  if (plan.more && workspace_bytes(plan, variant.rows, args.cache.head_dim) > args.workspace_bytes)
+    return hipErrorInvalidValue;
+  const dim3 grid(plan.most_units + plan.more), block(kThreads);
+  if (start || (stop && !plan.more))
+    hipExtLaunchKernelGGL(variant.kernel, grid, block, 0, stream, start, plan.more ? nullptr : stop, 0, args, plan);
   else
-    hipLaunchKernelGGL(kernel, grid, block, 0, stream, args);
+    hipLaunchKernelGGL(variant.kernel, grid, block, 0, stream, args, plan);
+  if (const hipError_t e = hipGetLastError()) return e;
+  if (!plan.more) return hipSuccess;
+  const dim3 units(plan.most_units, variant.rows / 16u);
+  if (stop)
+    hipExtLaunchKernelGGL(variant.join, units, block, 0, stream, nullptr, stop, 0, args, plan);
+  else
+    hipLaunchKernelGGL(variant.join, units, block, 0, stream, args, plan);
   return hipGetLastError();
 }
 

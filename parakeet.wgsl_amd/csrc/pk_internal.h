@@ -507,7 +507,13 @@ struct CacheAttentionArgs {
   float scale;
   float cap;        // of the scores, 0: none
   bool causal, f16;
+  bool wide_rows;   // queries and outputs in whole 16 byte pieces
+  // Memory of the op where long sequences are split over workgroups (null: never).
+  void* workspace;
+  uint64_t workspace_bytes;
 };
+// Bytes of workspace that launches of the op need.
+uint64_t cache_attention_workspace(const CacheAttentionArgs& args);
 hipError_t launch_cache_attention(const CacheAttentionArgs& args, hipStream_t stream, hipEvent_t start = nullptr,
                                   hipEvent_t stop = nullptr);
 
