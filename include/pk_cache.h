@@ -145,7 +145,7 @@ typedef struct pk_cache_attention_desc {
   int32_t causal;                /* 1: a row sees tokens up to its own position; 0: all */
   uint32_t window;               /* causal: the last so many tokens, its own among them; 0: all */
   int32_t has_scale;             /* 0: scale 1 / sqrt(head_dim) */
-  float scale;                   /* finite */
+  float scale;                   /* -2^60 to 2^60 */
   float score_cap;               /* 0: none; 2^-20 to 2^20 */
   const uint32_t *row_starts;    /* [sequences + 1] */
   uint64_t row_starts_bytes;

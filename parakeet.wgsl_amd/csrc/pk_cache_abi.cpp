@@ -186,7 +186,8 @@ int validate_attention(const pk_cache_attention_desc* d) {
   if (!d->queries || !d->output) return fail(PK_INVALID_ARGUMENT, "%s needs queries and an output", label);
   if (d->causal != 0 && d->causal != 1) return fail(PK_INVALID_ARGUMENT, "%s causal must be 0 or 1", label);
   if (d->window && !d->causal) return fail(PK_INVALID_ARGUMENT, "%s has a window without causal", label);
-  if (d->has_scale && !std::isfinite(d->scale)) return fail(PK_INVALID_ARGUMENT, "%s scale must be finite", label);
+  if (d->has_scale && !(std::fabs(d->scale) <= 0x1p60f))
+    return fail(PK_RANGE_ERROR, "%s scale must be at most 2^60 in magnitude", label);
   if (!(d->score_cap == 0.0f || (d->score_cap >= 0x1p-20f && d->score_cap <= 0x1p20f)))
     return fail(PK_RANGE_ERROR, "%s score cap must be 0 or in [2^-20, 2^20]", label);
   const uint64_t elem = d->precision == PK_PRECISION_F16 ? 2u : 4u;

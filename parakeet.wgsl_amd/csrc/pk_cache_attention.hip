@@ -31,6 +31,7 @@ constexpr float kMargin = 8.0f;
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef short short4v __attribute__((ext_vector_type(4)));
 
 // Tokens [low, high).
@@ -207,16 +208,17 @@ __device__ __forceinline__ float tanh_of(float x) {
   return fabsf(x) < 0.25f ? near : far;
 }
 
-// From the product of a query and a key to the score in log2 units.
+// From the product of a query and a key to the score in log2 units: a capped
+// product is the score over `factor`, any other the score itself, with factor > 0:
+// queries take the sign of the scale (and 0) with them, exactly.
 struct Score {
-  float before, after;
+  float factor, sign, before, after;
   bool capped;
   __device__ explicit Score(const CacheAttentionArgs& args)
-      : before(args.cap > 0.0f ? args.scale / args.cap : args.scale * kLog2E), after(args.cap * kLog2E),
-        capped(args.cap > 0.0f) {}
-  __device__ __forceinline__ float operator()(float dot) const {
-    return capped ? after * tanh_of(dot * before) : dot * before;
-  }
+      : factor(args.cap > 0.0f || args.scale == 0.0f ? 1.0f : fabsf(args.scale) * kLog2E),
+        sign(args.scale > 0.0f ? 1.0f : args.scale < 0.0f ? -1.0f : 0.0f), before(fabsf(args.scale) / args.cap),
+        after(args.cap * kLog2E), capped(args.cap > 0.0f) {}
+  __device__ __forceinline__ float cap(float dot) const { return after * tanh_of(dot * before); }
 };
 
 // Where the tokens of one kv head of a sequence lie, in pieces of 16 bytes
@@ -276,6 +278,12 @@ struct Result {
 // 1 / l, and 0 where no score counted.
 __device__ __forceinline__ float inverse(float m, float l) { return m == -kInf && l == 0.0f ? 0.0f : 1.0f / l; }
 
+// Of 64 tokens from t0 on, those below `end`.
+__device__ __forceinline__ uint64_t tokens_below(uint32_t t0, uint32_t end) {
+  const uint32_t n = end > t0 ? end - t0 : 0u;
+  return n >= 64u ? ~0ull : (1ull << n) - 1ull;
+}
+
 __device__ __forceinline__ float block_reduce(float x, bool largest, float* scratch) {
 #pragma unroll
   for (int off = 32; off; off >>= 1) {
@@ -313,7 +321,7 @@ __device__ __forceinline__ void careful_item(const CacheAttentionArgs& args, con
     const T* q = static_cast<const T*>(args.queries) + (item.row + token) * args.query_stride +
                  (uint64_t)(item.head * group + (i - token * group)) * dim;
     __syncthreads();
-    if (at < dim) query[at] = (float)q[at];
+    if (at < dim) query[at] = (float)q[at] * score.sign;
     float m = -kInf, l = 0.0f, out = 0.0f;
     for (uint32_t t0 = low; t0 < high; t0 += kThreads) {
       __syncthreads();
@@ -324,7 +332,7 @@ __device__ __forceinline__ void careful_item(const CacheAttentionArgs& args, con
         const T* k = static_cast<const T*>(args.key_cache) + (uint64_t)place * kPiece;
         float dot = 0.0f;
         for (uint32_t d = 0; d < dim; ++d) dot = __builtin_fmaf(query[d], (float)k[d], dot);
-        z = score(dot);
+        z = (score.capped ? score.cap(dot) : dot) * score.factor;
       }
       places[at] = place;
       const float top = fmaxf(m, block_reduce(z, true, scratch));
@@ -443,6 +451,7 @@ __global__ __launch_bounds__(kThreads) void cache_attention_few_kernel(CacheAtte
 #pragma unroll
             for (int e = 0; e < PIECE; ++e) query[b][k][e] = q[c * PIECE + e];
           }
+          query[b][k] *= (T)score.sign;
         }
       }
     }
@@ -549,19 +558,26 @@ __global__ __launch_bounds__(kThreads) void cache_attention_few_kernel(CacheAtte
     V weights[RB];
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
+      if (score.capped) {
+#pragma unroll
+        for (int t = 0; t < TB; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[b][t][j] = score.cap(s[b][t][j]);
+      }
+      if (!whole) {
+        const uint32_t seen =
+            (live_now & (uint32_t)(tokens_below(t0, high[b]) & ~tokens_below(t0, low[b]))) >> (4u * quarter);
+#pragma unroll
+        for (int t = 0; t < TB; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[b][t][j] = (seen & (1u << (16 * t + j))) ? s[b][t][j] : -kInf;
+      }
       float top = -kInf;
 #pragma unroll
       for (int t = 0; t < TB; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float z = score(s[b][t][j]);
-          if (!whole) {
-            const uint32_t at = 16u * t + 4u * quarter + j, token = t0 + at;
-            z = (live_now >> at & 1u) && token >= low[b] && token < high[b] ? z : -kInf;
-          }
-          s[b][t][j] = z;
-          top = fmaxf(top, z);
-        }
+        for (int j = 0; j < 4; ++j) top = fmaxf(top, s[b][t][j]);
+      top *= score.factor;
       if (__any(top > m[b] + kMargin)) {
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
@@ -577,7 +593,7 @@ __global__ __launch_bounds__(kThreads) void cache_attention_few_kernel(CacheAtte
       for (int t = 0; t < TB; ++t)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float p = __builtin_amdgcn_exp2f(s[b][t][j] - base);
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][t][j], score.factor, -base));
           l[b] += p;
           if constexpr (kHalf) weights[b][4 * t + j] = (_Float16)p;
           else weights[b][j] = p;
@@ -714,6 +730,267 @@ __global__ __launch_bounds__(kThreads) void cache_attention_few_kernel(CacheAtte
   }
 }
 
+// The kernel of many rows, f16: a workgroup of 4 wavefronts with 32 rows each,
+// which share tiles of 64 tokens in LDS, two of them: while one is used, the next one's
+// loads are on their way, in registers, and are written to the other at the
+// end of the step. Keys are read as operands of v_mfma_f32_32x32x16_f16, 16 bytes of
+// a token, values transposed, four tokens of a channel, in the order in which
+// the scores lie: scores 8u .. 8u + 7 of a lane are tokens 16u + 4 half + 0..3 and 8 more.
+// Both are laid out so that the lanes that read together read different banks: pieces
+// of 16 bytes of a key, and of 32 bytes of a value, are exchanged by a number of the row.
+template <int DP>
+struct ManyShape {
+  static constexpr int kTokens = 64, kRows = 128;
+  static constexpr int kTile = kTokens * DP;  // elements of a tile of keys or of values
+  static constexpr int kLds = 4 * kTile * 2 + 16;
+  static_assert(4 * kTile * 2 >= (int)(kMaxDim + kThreads + kWaves + kThreads) * 4, "the careful way's LDS");
+};
+
+template <int DP, bool WHOLE>
+__global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_many_kernel(CacheAttentionArgs args,
+                                                                                          Plan plan) {
+  typedef _Float16 T;
+  typedef ManyShape<DP> Shape;
+  constexpr int R = Shape::kRows, STEP = Shape::kTokens;
+  constexpr int KS = DP / 16, DB = DP / 32, VR = DP / 8;
+  constexpr int LOADS = STEP * VR / kThreads;  // pieces of keys, and of values, of a thread
+  __shared__ __attribute__((aligned(16))) uint8_t lds[Shape::kLds];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = lane & 31u, half = lane >> 5;
+  const CacheView& cache = args.cache;
+
+  uint32_t units;
+  const Item item = find_item<R>(args, plan, blockIdx.x, &units);
+  const Workspace work = bind(args.workspace, plan, R);
+  if (plan.more && blockIdx.x == 0 && threadIdx.x == 0) *work.units_count = min(units, plan.most_units);
+  if (!item.live) return;
+  if (plan.more && item.part == 0 && item.unit < plan.most_units && threadIdx.x == 0)
+    work.units[item.unit] = {item.slot, item.parts, item.row, item.rows, item.head, item.first};
+  const Seen part = part_of(args, item);
+  const uint32_t group = args.heads / cache.kv_heads, dim = cache.head_dim;
+  const Places<T> map(cache, item.sequence, item.head);
+  const Score score(args);
+  const uint32_t pieces = dim / 8u;
+
+  // This lane's query, what its row sees, what all rows of the wavefront see, and any.
+  half8 query[KS];
+  uint32_t low = 0, high = 0;
+  const uint32_t r = 32u * wave + col;
+#pragma unroll
+  for (int k = 0; k < KS; ++k) query[k] = half8{};
+  if (r < item.rows) {
+    const uint32_t i = item.first + r, token = i / group;
+    const Seen own = seen_by(args, item.length, item.position + token);
+    low = own.low;
+    high = own.high;
+    const T* q = static_cast<const T*>(args.queries) + (item.row + token) * args.query_stride +
+                 (uint64_t)(item.head * group + (i - token * group)) * dim;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const uint32_t c = 2u * k + half;
+      if (WHOLE || c < pieces) {
+        if (args.wide_rows) {
+          query[k] = *reinterpret_cast<const half8*>(q + c * 8u);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) query[k][e] = q[c * 8u + e];
+        }
+        query[k] *= (T)score.sign;
+      }
+    }
+  }
+  Seen any = {0, 0}, all = {0, 0};
+  if (32u * wave < item.rows) {
+    const uint32_t first = (item.first + 32u * wave) / group, last = (item.first + min(item.rows, 32u * wave + 32u) - 1u) / group;
+    const Seen a = seen_by(args, item.length, item.position + first), b = seen_by(args, item.length, item.position + last);
+    all = {b.low, a.high};
+    any = {a.low, b.high};
+  }
+
+  float m = -kInf, l = 0.0f;
+  floatx16 out[DB];
+#pragma unroll
+  for (int o = 0; o < DB; ++o) out[o] = floatx16{};
+
+  T* tiles = reinterpret_cast<T*>(lds);  // keys, values, keys, values
+  const auto key_turn = [](uint32_t row) { return DP == 64 ? row >> 1 & 7u : row & 15u; };
+  const auto value_turn = [](uint32_t row) { return (DP == 64 ? (row & 2u) : (row & 3u) << 1) | (row >> 2 & 1u); };
+
+  const uint8_t *keys = static_cast<const uint8_t*>(args.key_cache), *values = static_cast<const uint8_t*>(args.value_cache);
+  half8 key[LOADS], value[LOADS];
+  // Each wavefront stages 16 tokens of a tile, its lanes pieces of 64 / VR of them at a time.
+  const auto staged_token = [&](int i) { return 16u * wave + (uint32_t)i * (64u / VR) + lane / VR; };
+  const uint32_t staged_piece = lane % VR;
+  uint32_t entry = map.entry(part.low + lane, part.high);
+  uint64_t live_next = 0;
+  const auto load = [&](uint32_t t0) {
+    const bool held = entry < map.count;
+    live_next = __ballot(held);
+    const uint32_t places = held ? map.place(t0 + lane, entry) : 0u;
+    uint64_t from[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i)
+      from[i] = ((uint64_t)(uint32_t)__builtin_amdgcn_ds_bpermute((int)(staged_token(i) * 4u), (int)places) + staged_piece) * 16u;
+    if (WHOLE && live_next == ~0ull) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        key[i] = *reinterpret_cast<const half8*>(keys + from[i]);
+        value[i] = *reinterpret_cast<const half8*>(values + from[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        key[i] = value[i] = half8{};
+        if ((live_next >> staged_token(i) & 1u) && (WHOLE || staged_piece < pieces)) {
+          key[i] = *reinterpret_cast<const half8*>(keys + from[i]);
+          value[i] = *reinterpret_cast<const half8*>(values + from[i]);
+        }
+      }
+    }
+    entry = map.entry(t0 + STEP + lane, part.high);
+  };
+  const auto store = [&](uint32_t stage) {
+    T* k_to = tiles + stage * 2u * Shape::kTile;
+    T* v_to = k_to + Shape::kTile;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const uint32_t row = staged_token(i);
+      *reinterpret_cast<half8*>(k_to + row * DP + (staged_piece ^ key_turn(row)) * 8u) = key[i];
+      *reinterpret_cast<half8*>(v_to + row * DP + ((staged_piece >> 1) ^ value_turn(row)) * 16u + (staged_piece & 1u) * 8u) = value[i];
+    }
+  };
+  uint64_t live = 0;
+  if (part.low < part.high) {
+    load(part.low);
+    store(0);
+    live = live_next;
+  }
+  __syncthreads();
+  uint32_t stage = 0;
+  for (uint32_t t0 = part.low; t0 < part.high; t0 += STEP) {
+    const bool more = t0 + STEP < part.high;
+    if (more) load(t0 + STEP);
+    if (t0 < any.high && t0 + STEP > any.low) {
+      const T* k_from = tiles + stage * 2u * Shape::kTile;
+      const T* v_from = k_from + Shape::kTile;
+      floatx16 s[2];
+      s[0] = s[1] = floatx16{};
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const half8 x = *reinterpret_cast<const half8*>(k_from + (32u * t + col) * DP + ((2u * k + half) ^ key_turn(col)) * 8u);
+          s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, query[k], s[t], 0, 0, 0);
+        }
+      const bool whole = live == ~0ull && t0 >= all.low && t0 + STEP <= all.high;
+      if (score.capped) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) s[t][j] = score.cap(s[t][j]);
+      }
+      if (!whole) {
+        const uint64_t seen = (live & tokens_below(t0, high) & ~tokens_below(t0, low)) >> (4u * half);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            s[t][j] = ((uint32_t)(seen >> (32 * t)) & (1u << (8 * (j >> 2) + (j & 3)))) ? s[t][j] : -kInf;
+      }
+      float top = -kInf;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) top = fmaxf(top, s[t][j]);
+      top *= score.factor;
+      if (__any(top > m + kMargin)) {
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        top = fmaxf(top, m);
+        const float old = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+        m = top;
+        l *= old;
+#pragma unroll
+        for (int o = 0; o < DB; ++o) out[o] *= old;
+      }
+      const float base = m == -kInf ? 0.0f : m;
+      half8 weights[2][2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j], score.factor, -base));
+          l += p;
+          weights[t][j >> 3][j & 7] = (T)p;
+        }
+      const uint32_t row = 4u * half + (lane >> 2 & 3u), turn = value_turn(row);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int o = 0; o < DB; ++o) {
+            half8 v;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const T* from = v_from + (32u * t + 16u * u + 8u * j + row) * DP +
+                              ((2u * o + (lane >> 4 & 1u)) ^ turn) * 16u + (lane & 3u) * 4u;
+              const half4 four = __builtin_bit_cast(
+                  half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)from));
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[4 * j + e] = four[e];
+            }
+            out[o] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, weights[t][u], out[o], 0, 0, 0);
+          }
+    }
+    stage ^= 1u;
+    if (more) store(stage);
+    live = live_next;
+    __syncthreads();
+  }
+
+  uint32_t* strange = reinterpret_cast<uint32_t*>(lds + Shape::kLds - 16);
+  if (threadIdx.x == 0) *strange = 0;
+  l += __shfl_xor(l, 32, 64);
+  bool odd = false;
+#pragma unroll
+  for (int o = 0; o < DB; ++o)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) odd |= !(fabsf(out[o][j]) < kInf);
+  __syncthreads();
+  if (args.causal && item.new_tokens > 1u && __any(odd) && lane == 0) *strange = 1;
+  __syncthreads();
+  if (*strange) {
+    careful_item<T, R>(args, item, work, reinterpret_cast<float*>(lds));
+    return;
+  }
+  if (r >= item.rows) return;
+  const Result<T, R> result{args, item, work};
+  const float scale = item.parts > 1u ? 1.0f : inverse(m, l);
+  T* to = result.output(r);
+  float* part_to = result.partial(r);
+#pragma unroll
+  for (int o = 0; o < DB; ++o)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t d = 32u * o + 8u * j + 4u * half;
+      if (!WHOLE && d >= dim) continue;
+      const floatx4 x = {out[o][4 * j] * scale, out[o][4 * j + 1] * scale, out[o][4 * j + 2] * scale, out[o][4 * j + 3] * scale};
+      if (item.parts > 1u) {
+        *reinterpret_cast<floatx4*>(part_to + d) = x;
+      } else {
+        half4 four;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) four[e] = (T)x[e];
+        if (args.wide_rows) {
+          *reinterpret_cast<half4*>(to + d) = four;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) to[d + e] = four[e];
+        }
+      }
+    }
+  if (item.parts > 1u && half == 0) result.sums(r, m, l);
+}
+
 // Joins the parts of a unit: a wavefront takes a row, its lanes 4 channels each.
 template <typename T, int R>
 __global__ __launch_bounds__(kThreads) void cache_attention_join_kernel(CacheAttentionArgs args, Plan plan) {
@@ -775,24 +1052,34 @@ Variant few(bool whole) {
           cache_attention_join_kernel<T, 16 * RB>, 16 * RB};
 }
 
-// Blocks of 16 rows of a unit: as many as the rows of an average sequence need,
-// up to 4, and 2 for heads of more than 128 channels.
-uint32_t blocks_of(const CacheAttentionArgs& args) {
-  const uint64_t group = args.heads / args.cache.kv_heads;
-  const uint64_t rows = (args.cache.rows * group + args.cache.sequences - 1u) / args.cache.sequences;
-  return rows <= 16u ? 1u : rows <= 32u || args.cache.head_dim > 128u ? 2u : 4u;
+template <int DP>
+Variant many(bool whole) {
+  return {whole ? cache_attention_many_kernel<DP, true> : cache_attention_many_kernel<DP, false>,
+          cache_attention_join_kernel<_Float16, ManyShape<DP>::kRows>, ManyShape<DP>::kRows};
 }
 
+// Rows of a unit: 16 or 32 where the rows of an average sequence need no more, else
+// 128 (f16), 64 (f32), and 32 for f32 heads of more than 128 channels.
+uint32_t unit_rows(const CacheAttentionArgs& args) {
+  const uint64_t group = args.heads / args.cache.kv_heads;
+  const uint64_t rows = (args.cache.rows * group + args.cache.sequences - 1u) / args.cache.sequences;
+  if (rows <= 32u) return rows <= 16u ? 16u : 32u;
+  return args.f16 ? 128u : args.cache.head_dim > 128u ? 32u : 64u;
+}
+
+template <typename T, int DP>
+Variant choose(uint32_t rows, bool whole) {
+  if (rows == 16u) return few<T, DP, 1>(whole);
+  if (rows == 32u) return few<T, DP, 2>(whole);
+  if constexpr (sizeof(T) == 2) return many<DP>(whole);
+  else return few<T, DP, (DP > 128 ? 2 : 4)>(whole);
+}
 template <typename T>
 Variant choose(const CacheAttentionArgs& args) {
-  const uint32_t dim = args.cache.head_dim, blocks = blocks_of(args);
-  if (dim <= 64u)
-    return blocks == 1u ? few<T, 64, 1>(dim == 64u) : blocks == 2u ? few<T, 64, 2>(dim == 64u) : few<T, 64, 4>(dim == 64u);
-  if (dim <= 128u)
-    return blocks == 1u   ? few<T, 128, 1>(dim == 128u)
-           : blocks == 2u ? few<T, 128, 2>(dim == 128u)
-                          : few<T, 128, 4>(dim == 128u);
-  return blocks == 1u ? few<T, 256, 1>(dim == 256u) : few<T, 256, 2>(dim == 256u);
+  const uint32_t dim = args.cache.head_dim, rows = unit_rows(args);
+  if (dim <= 64u) return choose<T, 64>(rows, dim == 64u);
+  if (dim <= 128u) return choose<T, 128>(rows, dim == 128u);
+  return choose<T, 256>(rows, dim == 256u);
 }
 
 constexpr uint32_t kShortest = 256;  // tokens of a part
@@ -803,7 +1090,7 @@ Plan plan_of(const CacheAttentionArgs& args, uint32_t R) {
   Plan plan;
   // Full tiles of rows, and one that is not full for each sequence.
   plan.most_units = (uint32_t)(args.cache.kv_heads * (args.cache.rows * group / R + some));
-  plan.more = args.cache.capacity() > kShortest ? (R > 32u ? 512u : 1024u) : 0u;
+  plan.more = args.cache.capacity() > kShortest ? (R > 64u ? 256u : R > 32u ? 512u : 1024u) : 0u;
   plan.shortest = kShortest;
   return plan;
 }
@@ -813,10 +1100,9 @@ Plan plan_of(const CacheAttentionArgs& args, uint32_t R) {
 uint64_t cache_attention_workspace(const CacheAttentionArgs& args) {
   // Any number of active sequences: the rows of a unit follow from it.
   uint64_t most = 0;
-  for (uint32_t blocks : {1u, 2u, 4u}) {
-    if (blocks == 4u && args.cache.head_dim > 128u) continue;
-    const Plan plan = plan_of(args, 16u * blocks);
-    const uint64_t bytes = workspace_bytes(plan, 16u * blocks, args.cache.head_dim);
+  for (uint32_t rows : {16u, 32u, 64u, 128u}) {
+    const Plan plan = plan_of(args, rows);
+    const uint64_t bytes = workspace_bytes(plan, rows, args.cache.head_dim);
     if (plan.more && bytes > most) most = bytes;
   }
   return most;

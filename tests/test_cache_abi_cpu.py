@@ -154,7 +154,8 @@ def test_cache_attention_accepts(abi):
     (dict(heads=3), "PaletteRangeError", "step heads must be a multiple of the 2 kv heads"),
     (dict(queries=Fake(None, 0)), "PaletteError", "step needs queries and an output"),
     (dict(window=5, causal=False), "PaletteError", "step has a window without causal"),
-    (dict(scale=float("inf")), "PaletteError", "step scale must be finite"),
+    (dict(scale=float("-inf")), "PaletteRangeError", "step scale must be at most 2^60 in magnitude"),
+    (dict(scale=float("nan")), "PaletteRangeError", "step scale must be at most 2^60 in magnitude"),
     (dict(score_cap=-1.0), "PaletteRangeError", "step score cap must be 0 or in [2^-20, 2^20]"),
     (dict(score_cap=float("nan")), "PaletteRangeError", "step score cap must be 0 or in [2^-20, 2^20]"),
     (dict(output=Fake(0x400000, 5630)), "PaletteRangeError", "step output needs 5632 bytes"),
