@@ -115,10 +115,10 @@ __device__ __forceinline__ Item find_item(const CacheAttentionArgs& args, const 
   const CacheView& cache = args.cache;
   const uint32_t lane = threadIdx.x & 63u, group = args.heads / cache.kv_heads;
   struct Of {
-    uint32_t start, count, tiles, span;
+    uint32_t sequence, start, count, tiles, span;
   };
   const auto of = [&](uint32_t s) {
-    Of x = {0, 0, 0, 0};
+    Of x = {s, 0, 0, 0, 0};
     if (s < cache.sequences) {
       x.start = min(cache.row_starts[s], cache.rows);
       const uint32_t end = min(cache.row_starts[s + 1], cache.rows), length = cache.lengths[s];
@@ -157,6 +157,16 @@ __device__ __forceinline__ Item find_item(const CacheAttentionArgs& args, const 
   for (uint32_t base = 0; base < cache.sequences; base += 64u) {
     const uint32_t s = base + lane;
     if (cache.sequences > 64u) mine = of(s);
+    // The longest of these sequences first, so that the last workgroups are short ones.
+    uint32_t rank = 0;
+    const uint32_t here = min(64u, cache.sequences - base);
+    for (uint32_t j = 0; j < here; ++j) {
+      const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)mine.span, (int)j);
+      rank += other > mine.span || (other == mine.span && j < lane);
+    }
+    if (lane >= here) rank = lane;
+    const auto sorted = [&](uint32_t x) { return (uint32_t)__builtin_amdgcn_ds_permute((int)(rank * 4u), (int)x); };
+    mine = {sorted(s), sorted(mine.start), sorted(mine.count), sorted(mine.tiles), sorted(mine.span)};
     const uint32_t parts = mine.span ? (mine.span + longest - 1u) / longest : 0u;
     const uint32_t have = mine.tiles * cache.kv_heads, items = have * parts, slots = parts > 1u ? items : 0u;
     uint32_t items_to = items, units_to = have, slots_to = slots;
@@ -176,7 +186,7 @@ __device__ __forceinline__ Item find_item(const CacheAttentionArgs& args, const 
       const uint32_t before = items_before + __shfl(items_to, at, 64) - owned;
       const uint32_t local = index - before, unit = local / each;
       item.live = true;
-      item.sequence = base + at;
+      item.sequence = __shfl(mine.sequence, at, 64);
       item.parts = each;
       item.part = local - unit * each;
       item.head = unit / tiles;
@@ -393,8 +403,14 @@ struct FewShape {
   static constexpr int kJoinBytes = kWaves * RB * 16 * kSliceRow * 4;
   static constexpr int kCarefulBytes = (int)(kMaxDim + kThreads + kWaves + kThreads) * 4;
   static constexpr int kSums = 2 * kWaves * RB * 16 * 4;
+  // One block of f16 queries stays in registers; others are read from LDS for each step, rows
+  // 16 bytes longer than they are, so that 16 of them lie on different banks.
+  static constexpr bool kQueriesInLds = sizeof(T) == 4 || RB > 1;
+  static constexpr int kQueryRow = DP * (int)sizeof(T) + 16;
+  static constexpr int kQueryBytes = kQueriesInLds ? RB * 16 * kQueryRow : 0;
   static constexpr int largest(int a, int b) { return a > b ? a : b; }
-  static constexpr int kLds = kSums + 16 + largest(largest(kWaves * kValueBytes, kJoinBytes), kCarefulBytes);
+  static constexpr int kLds =
+      kSums + 16 + largest(largest(kWaves * kValueBytes + kQueryBytes, kJoinBytes), kCarefulBytes);
 };
 
 template <typename T, int DP, int RB, bool WHOLE>
@@ -426,35 +442,46 @@ __global__ __launch_bounds__(kThreads) void cache_attention_few_kernel(CacheAtte
   const uint32_t pieces = dim / PIECE;
 
   // Queries, and what their rows see.
-  V query[RB][KS];
+  constexpr bool kInLds = Shape::kQueriesInLds;
+  uint8_t* query_rows = lds + Shape::kSums + 16 + kWaves * Shape::kValueBytes;
+  const auto query_piece = [&](uint32_t r, uint32_t c) {
+    const uint32_t i = item.first + r, token = i / group;
+    const T* q = static_cast<const T*>(args.queries) + (item.row + token) * args.query_stride +
+                 (uint64_t)(item.head * group + (i - token * group)) * dim + c * PIECE;
+    V x = V{};
+    if (r < item.rows && (WHOLE || c < pieces)) {
+      if (args.wide_rows) {
+        x = *reinterpret_cast<const V*>(q);
+      } else {
+#pragma unroll
+        for (int e = 0; e < PIECE; ++e) x[e] = q[e];
+      }
+      x *= (T)score.sign;
+    }
+    return x;
+  };
+  V held[kInLds ? 1 : KS];
+  if constexpr (kInLds) {
+    for (uint32_t i = threadIdx.x; i < R * VR; i += kThreads)
+      *reinterpret_cast<V*>(query_rows + i / VR * Shape::kQueryRow + i % VR * 16u) = query_piece(i / VR, i % VR);
+    __syncthreads();
+  } else {
+#pragma unroll
+    for (int k = 0; k < KS; ++k) held[k] = query_piece(col, 4u * k + quarter);
+  }
+  const auto query = [&](int b, int k) {
+    if constexpr (kInLds)
+      return *reinterpret_cast<const V*>(query_rows + (16u * b + col) * Shape::kQueryRow + (4u * k + quarter) * 16u);
+    else
+      return held[k];
+  };
   uint32_t low[RB], high[RB];
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
     const uint32_t r = 16u * b + col;
-    low[b] = high[b] = 0;
-#pragma unroll
-    for (int k = 0; k < KS; ++k) query[b][k] = V{};
-    if (r < item.rows) {
-      const uint32_t i = item.first + r, token = i / group;
-      const Seen own = seen_by(args, item.length, item.position + token);
-      low[b] = own.low;
-      high[b] = own.high;
-      const T* q = static_cast<const T*>(args.queries) + (item.row + token) * args.query_stride +
-                   (uint64_t)(item.head * group + (i - token * group)) * dim;
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const uint32_t c = 4u * k + quarter;
-        if (WHOLE || c < pieces) {
-          if (args.wide_rows) {
-            query[b][k] = *reinterpret_cast<const V*>(q + c * PIECE);
-          } else {
-#pragma unroll
-            for (int e = 0; e < PIECE; ++e) query[b][k][e] = q[c * PIECE + e];
-          }
-          query[b][k] *= (T)score.sign;
-        }
-      }
-    }
+    const Seen own = seen_by(args, item.length, item.position + (item.first + r) / group);
+    low[b] = r < item.rows ? own.low : 0u;
+    high[b] = r < item.rows ? own.high : 0u;
   }
   // Tokens that all rows of the unit see.
   uint32_t common_low = 0, common_high = 0xffffffffu;
@@ -533,16 +560,20 @@ __global__ __launch_bounds__(kThreads) void cache_attention_few_kernel(CacheAtte
 #pragma unroll
     for (int b = 0; b < RB; ++b)
 #pragma unroll
-      for (int t = 0; t < TB; ++t) {
-        s[b][t] = floatx4{};
+      for (int t = 0; t < TB; ++t) s[b][t] = floatx4{};
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int b = 0; b < RB; ++b) {
+        const V q = query(b, k);
+#pragma unroll
+        for (int t = 0; t < TB; ++t) {
           if constexpr (kHalf) {
-            s[b][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key[t][k], query[b][k], s[b][t], 0, 0, 0);
+            s[b][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key[t][k], q, s[b][t], 0, 0, 0);
           } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              s[b][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(key[t][k][e], query[b][k][e], s[b][t], 0, 0, 0);
+              s[b][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(key[t][k][e], q[e], s[b][t], 0, 0, 0);
           }
         }
       }
@@ -1058,21 +1089,25 @@ Variant many(bool whole) {
           cache_attention_join_kernel<_Float16, ManyShape<DP>::kRows>, ManyShape<DP>::kRows};
 }
 
-// Rows of a unit: 16 or 32 where the rows of an average sequence need no more, else
-// 128 (f16), 64 (f32), and 32 for f32 heads of more than 128 channels.
+// Rows of a unit: 16, 32 or 64 where the rows of an average sequence need no more, else
+// 128 (f16) or 64 (f32). Heads of more than 128 channels take 16, 32 or 128 (f16), 16 or 32 (f32).
 uint32_t unit_rows(const CacheAttentionArgs& args) {
   const uint64_t group = args.heads / args.cache.kv_heads;
   const uint64_t rows = (args.cache.rows * group + args.cache.sequences - 1u) / args.cache.sequences;
+  const bool wide = args.cache.head_dim > 128u;
   if (rows <= 32u) return rows <= 16u ? 16u : 32u;
-  return args.f16 ? 128u : args.cache.head_dim > 128u ? 32u : 64u;
+  if (rows <= 64u && !wide) return 64u;
+  return args.f16 ? 128u : wide ? 32u : 64u;
 }
 
 template <typename T, int DP>
 Variant choose(uint32_t rows, bool whole) {
   if (rows == 16u) return few<T, DP, 1>(whole);
   if (rows == 32u) return few<T, DP, 2>(whole);
+  if constexpr (DP <= 128)
+    if (rows == 64u) return few<T, DP, 4>(whole);
   if constexpr (sizeof(T) == 2) return many<DP>(whole);
-  else return few<T, DP, (DP > 128 ? 2 : 4)>(whole);
+  else return few<T, DP, 2>(whole);
 }
 template <typename T>
 Variant choose(const CacheAttentionArgs& args) {
