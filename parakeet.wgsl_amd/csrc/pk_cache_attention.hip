@@ -414,7 +414,7 @@ struct FewShape {
 };
 
 template <typename T, int DP, int RB, bool WHOLE>
-__global__ __launch_bounds__(kThreads) void cache_attention_few_kernel(CacheAttentionArgs args, Plan plan) {
+__global__ __launch_bounds__(kThreads, DP <= 128 && DP * RB <= 256 ? 2 : 1) void cache_attention_few_kernel(CacheAttentionArgs args, Plan plan) {
   typedef FewShape<T, DP, RB> Shape;
   constexpr int R = 16 * RB, STEP = Shape::kTokens, TB = STEP / 16;  // token blocks of a step
   constexpr bool kHalf = sizeof(T) == 2;
@@ -461,14 +461,6 @@ __global__ __launch_bounds__(kThreads) void cache_attention_few_kernel(CacheAtte
     return x;
   };
   V held[kInLds ? 1 : KS];
-  if constexpr (kInLds) {
-    for (uint32_t i = threadIdx.x; i < R * VR; i += kThreads)
-      *reinterpret_cast<V*>(query_rows + i / VR * Shape::kQueryRow + i % VR * 16u) = query_piece(i / VR, i % VR);
-    __syncthreads();
-  } else {
-#pragma unroll
-    for (int k = 0; k < KS; ++k) held[k] = query_piece(col, 4u * k + quarter);
-  }
   const auto query = [&](int b, int k) {
     if constexpr (kInLds)
       return *reinterpret_cast<const V*>(query_rows + (16u * b + col) * Shape::kQueryRow + (4u * k + quarter) * 16u);
@@ -554,6 +546,14 @@ __global__ __launch_bounds__(kThreads) void cache_attention_few_kernel(CacheAtte
     load_keys(places);
     entry = map.entry(t0 + kStride + mine, part.high);
     load_values(places, live);
+  }
+  if constexpr (kInLds) {
+    for (uint32_t i = threadIdx.x; i < R * VR; i += kThreads)
+      *reinterpret_cast<V*>(query_rows + i / VR * Shape::kQueryRow + i % VR * 16u) = query_piece(i / VR, i % VR);
+    __syncthreads();
+  } else {
+#pragma unroll
+    for (int k = 0; k < KS; ++k) held[k] = query_piece(col, 4u * k + quarter);
   }
   for (; t0 < part.high; t0 += kStride) {
     floatx4 s[RB][TB];
@@ -1023,52 +1023,53 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
 }
 
 // Joins the parts of a unit: a wavefront takes a row, its lanes 4 channels each.
+constexpr int kJoinRows = 16;
 template <typename T, int R>
-__global__ __launch_bounds__(kThreads) void cache_attention_join_kernel(CacheAttentionArgs args, Plan plan) {
+__global__ __launch_bounds__(64 * kJoinRows) void cache_attention_join_kernel(CacheAttentionArgs args, Plan plan) {
   const Workspace work = bind(args.workspace, plan, R);
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   const Unit unit = work.units[blockIdx.x];
   if (blockIdx.x >= *work.units_count || unit.parts <= 1u) return;
   const uint32_t group = args.heads / args.cache.kv_heads, dim = args.cache.head_dim;
   const uint32_t d = 4u * lane < dim ? 4u * lane : 0u;  // all lanes take part in the exchange
-  for (uint32_t r = blockIdx.y * 16u + wave; r < min(unit.rows, blockIdx.y * 16u + 16u); r += kWaves) {
-    const float2* sums = work.sums + (uint64_t)unit.slot * R + r;
-    float top = -kInf;
-    for (uint32_t p = lane; p < unit.parts; p += 64u) top = fmaxf(top, sums[(uint64_t)p * R].x);
-    top = wave::max(top);
-    float all = 0.0f;
-    floatx4 x = floatx4{};
-    for (uint32_t p0 = 0; p0 < unit.parts; p0 += 64u) {
-      const uint32_t p = p0 + lane;
-      float factor = 0.0f;
-      if (p < unit.parts) {
-        const float2 own = sums[(uint64_t)p * R];
-        factor = own.x == top ? 1.0f : __builtin_amdgcn_exp2f(own.x - top);
-        all += own.y * factor;
-      }
-      const uint32_t count = min(64u, unit.parts - p0);
-      const float* from = work.outputs + ((uint64_t)(unit.slot + p0) * R + r) * dim + d;
-      for (uint32_t i = 0; i < count; i += 8u) {  // eight loads at a time
-        floatx4 some[8];
+  const uint32_t r = blockIdx.y * kJoinRows + wave;
+  if (r >= unit.rows) return;
+  const float2* sums = work.sums + (uint64_t)unit.slot * R + r;
+  float top = -kInf;
+  for (uint32_t p = lane; p < unit.parts; p += 64u) top = fmaxf(top, sums[(uint64_t)p * R].x);
+  top = wave::max(top);
+  float all = 0.0f;
+  floatx4 x = floatx4{};
+  for (uint32_t p0 = 0; p0 < unit.parts; p0 += 64u) {
+    const uint32_t p = p0 + lane;
+    float factor = 0.0f;
+    if (p < unit.parts) {
+      const float2 own = sums[(uint64_t)p * R];
+      factor = own.x == top ? 1.0f : __builtin_amdgcn_exp2f(own.x - top);
+      all += own.y * factor;
+    }
+    const uint32_t count = min(64u, unit.parts - p0);
+    const float* from = work.outputs + ((uint64_t)(unit.slot + p0) * R + r) * dim + d;
+    for (uint32_t i = 0; i < count; i += 8u) {  // eight loads at a time
+      floatx4 some[8];
 #pragma unroll
-        for (uint32_t j = 0; j < 8u; ++j)
-          some[j] = *reinterpret_cast<const floatx4*>(from + (uint64_t)min(i + j, count - 1u) * R * dim);
+      for (uint32_t j = 0; j < 8u; ++j)
+        some[j] = *reinterpret_cast<const floatx4*>(from + (uint64_t)min(i + j, count - 1u) * R * dim);
 #pragma unroll
-        for (uint32_t j = 0; j < 8u; ++j) {
-          const uint32_t bits = (uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(factor), (int)min(i + j, 63u));
-          x += some[j] * (i + j < count ? __uint_as_float(bits) : 0.0f);
-        }
+      for (uint32_t j = 0; j < 8u; ++j) {
+        const uint32_t bits = (uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(factor), (int)min(i + j, 63u));
+        x += some[j] * (i + j < count ? __uint_as_float(bits) : 0.0f);
       }
     }
-    all = wave::sum(all);
-    x *= inverse(top, all);
-    const uint32_t i = unit.first + r, token = i / group;
-    T* to = static_cast<T*>(args.output) + (unit.row + token) * args.output_stride +
-            (uint64_t)(unit.head * group + (i - token * group)) * dim + d;
-    if (4u * lane < dim)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) to[e] = (T)x[e];
   }
+  all = wave::sum(all);
+  x *= inverse(top, all);
+  const uint32_t i = unit.first + r, token = i / group;
+  T* to = static_cast<T*>(args.output) + (unit.row + token) * args.output_stride +
+          (uint64_t)(unit.head * group + (i - token * group)) * dim + d;
+  if (4u * lane < dim)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) to[e] = (T)x[e];
 }
 
 typedef void (*Kernel)(CacheAttentionArgs, Plan);
@@ -1090,24 +1091,26 @@ Variant many(bool whole) {
 }
 
 // Rows of a unit: 16, 32 or 64 where the rows of an average sequence need no more, else
-// 128 (f16) or 64 (f32). Heads of more than 128 channels take 16, 32 or 128 (f16), 16 or 32 (f32).
+// 128 (f16). f32 units end at 64, 32 and 16 rows for heads of up to 64, 128 and 256 channels, f16
+// units of 64 rows at 128 channels.
 uint32_t unit_rows(const CacheAttentionArgs& args) {
   const uint64_t group = args.heads / args.cache.kv_heads;
   const uint64_t rows = (args.cache.rows * group + args.cache.sequences - 1u) / args.cache.sequences;
-  const bool wide = args.cache.head_dim > 128u;
-  if (rows <= 32u) return rows <= 16u ? 16u : 32u;
-  if (rows <= 64u && !wide) return 64u;
-  return args.f16 ? 128u : wide ? 32u : 64u;
+  const uint32_t dim = args.cache.head_dim, most = args.f16 ? 128u : dim <= 64u ? 64u : dim <= 128u ? 32u : 16u;
+  const uint32_t wanted = rows <= 16u ? 16u : rows <= 32u ? 32u : rows <= 64u && dim <= 128u ? 64u : 128u;
+  return wanted < most ? wanted : most;
 }
 
 template <typename T, int DP>
 Variant choose(uint32_t rows, bool whole) {
-  if (rows == 16u) return few<T, DP, 1>(whole);
-  if (rows == 32u) return few<T, DP, 2>(whole);
-  if constexpr (DP <= 128)
+  constexpr bool kHalf = sizeof(T) == 2;
+  if constexpr (kHalf || DP <= 128)
+    if (rows == 32u) return few<T, DP, 2>(whole);
+  if constexpr (kHalf ? DP <= 128 : DP <= 64)
     if (rows == 64u) return few<T, DP, 4>(whole);
-  if constexpr (sizeof(T) == 2) return many<DP>(whole);
-  else return few<T, DP, 2>(whole);
+  if constexpr (kHalf)
+    if (rows == 128u) return many<DP>(whole);
+  return few<T, DP, 1>(whole);
 }
 template <typename T>
 Variant choose(const CacheAttentionArgs& args) {
@@ -1156,11 +1159,11 @@ hipError_t launch_cache_attention(const CacheAttentionArgs& args, hipStream_t st
     hipLaunchKernelGGL(variant.kernel, grid, block, 0, stream, args, plan);
   if (const hipError_t e = hipGetLastError()) return e;
   if (!plan.more) return hipSuccess;
-  const dim3 units(plan.most_units, variant.rows / 16u);
+  const dim3 units(plan.most_units, variant.rows / kJoinRows), joining(64 * kJoinRows);
   if (stop)
-    hipExtLaunchKernelGGL(variant.join, units, block, 0, stream, nullptr, stop, 0, args, plan);
+    hipExtLaunchKernelGGL(variant.join, units, joining, 0, stream, nullptr, stop, 0, args, plan);
   else
-    hipLaunchKernelGGL(variant.join, units, block, 0, stream, args, plan);
+    hipLaunchKernelGGL(variant.join, units, joining, 0, stream, args, plan);
   return hipGetLastError();
 }
 
