@@ -115,13 +115,14 @@ __device__ __forceinline__ Item find_item(const CacheAttentionArgs& args, const 
   const CacheView& cache = args.cache;
   const uint32_t lane = threadIdx.x & 63u, group = args.heads / cache.kv_heads;
   struct Of {
-    uint32_t sequence, start, count, tiles, span;
+    uint32_t sequence, start, count, tiles, span, length;
   };
   const auto of = [&](uint32_t s) {
-    Of x = {s, 0, 0, 0, 0};
+    Of x = {s, 0, 0, 0, 0, 0};
     if (s < cache.sequences) {
       x.start = min(cache.row_starts[s], cache.rows);
       const uint32_t end = min(cache.row_starts[s + 1], cache.rows), length = cache.lengths[s];
+      x.length = length;
       x.count = end > x.start ? end - x.start : 0u;
       x.tiles = (x.count * group + R - 1u) / R;
       const Seen seen = seen_by(args, length, (int64_t)length - x.count, x.count);
@@ -138,11 +139,8 @@ __device__ __forceinline__ Item find_item(const CacheAttentionArgs& args, const 
     units += mine.tiles * cache.kv_heads;
     tokens += (float)(mine.tiles * cache.kv_heads) * (float)mine.span;
   }
-#pragma unroll
-  for (int off = 32; off; off >>= 1) {
-    units += __shfl_xor(units, off, 64);
-    tokens += __shfl_xor(tokens, off, 64);
-  }
+  units = wave::reduce_bits(units, 0u, [](uint32_t a, uint32_t b) { return a + b; });
+  tokens = wave::sum(tokens);
   *units_count = units;
   // Parts of at most `longest` tokens: sum(ceil(span / longest)) over the units is at
   // most tokens / longest + units. The quotient is rounded up by more than its
@@ -158,51 +156,46 @@ __device__ __forceinline__ Item find_item(const CacheAttentionArgs& args, const 
     const uint32_t s = base + lane;
     if (cache.sequences > 64u) mine = of(s);
     // The longest of these sequences first, so that the last workgroups are short ones.
-    uint32_t rank = 0;
     const uint32_t here = min(64u, cache.sequences - base);
-    for (uint32_t j = 0; j < here; ++j) {
-      const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)mine.span, (int)j);
-      rank += other > mine.span || (other == mine.span && j < lane);
+    if (here > 1u) {
+      uint32_t rank = 0;
+      for (uint32_t j = 0; j < here; ++j) {
+        const uint32_t other = wave::of_lane(mine.span, j);
+        rank += other > mine.span || (other == mine.span && j < lane);
+      }
+      if (lane >= here) rank = lane;
+      const auto sorted = [&](uint32_t x) { return (uint32_t)__builtin_amdgcn_ds_permute((int)(rank * 4u), (int)x); };
+      mine = {sorted(s), sorted(mine.start), sorted(mine.count), sorted(mine.tiles), sorted(mine.span),
+              sorted(mine.length)};
     }
-    if (lane >= here) rank = lane;
-    const auto sorted = [&](uint32_t x) { return (uint32_t)__builtin_amdgcn_ds_permute((int)(rank * 4u), (int)x); };
-    mine = {sorted(s), sorted(mine.start), sorted(mine.count), sorted(mine.tiles), sorted(mine.span)};
     const uint32_t parts = mine.span ? (mine.span + longest - 1u) / longest : 0u;
     const uint32_t have = mine.tiles * cache.kv_heads, items = have * parts, slots = parts > 1u ? items : 0u;
-    uint32_t items_to = items, units_to = have, slots_to = slots;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const uint32_t a = __shfl_up(items_to, off, 64), b = __shfl_up(units_to, off, 64), c = __shfl_up(slots_to, off, 64);
-      if ((int)lane >= off) {
-        items_to += a;
-        units_to += b;
-        slots_to += c;
-      }
-    }
+    const uint32_t items_to = wave::running_sum(items), units_to = wave::running_sum(have),
+                   slots_to = wave::running_sum(slots);
     const uint64_t hit = __ballot(index < items_before + items_to);
     if (hit) {
-      const int at = __builtin_ctzll(hit);
-      const uint32_t owned = __shfl(items, at, 64), each = __shfl(parts, at, 64), tiles = __shfl(mine.tiles, at, 64);
-      const uint32_t before = items_before + __shfl(items_to, at, 64) - owned;
-      const uint32_t local = index - before, unit = local / each;
+      const uint32_t at = (uint32_t)__builtin_ctzll(hit);
+      const auto its = [&](uint32_t x) { return wave::of_lane(x, at); };
+      const uint32_t each = its(parts), tiles = its(mine.tiles);
+      const uint32_t local = index - (items_before + its(items_to - items)), unit = local / each;
       item.live = true;
-      item.sequence = __shfl(mine.sequence, at, 64);
+      item.sequence = its(mine.sequence);
       item.parts = each;
       item.part = local - unit * each;
       item.head = unit / tiles;
       item.first = (unit - item.head * tiles) * R;
-      item.row = __shfl(mine.start, at, 64);
-      item.new_tokens = __shfl(mine.count, at, 64);
+      item.row = its(mine.start);
+      item.new_tokens = its(mine.count);
       item.rows = min((uint32_t)R, item.new_tokens * group - item.first);
-      item.length = cache.lengths[item.sequence];
+      item.length = its(mine.length);
       item.position = (int64_t)item.length - item.new_tokens;
-      item.unit = units_before + __shfl(units_to, at, 64) - tiles * cache.kv_heads + unit;
-      item.slot = slots_before + __shfl(slots_to - slots, at, 64) + unit * each;
+      item.unit = units_before + its(units_to - have) + unit;
+      item.slot = slots_before + its(slots_to - slots) + unit * each;
       break;
     }
-    items_before += __shfl(items_to, 63, 64);
-    units_before += __shfl(units_to, 63, 64);
-    slots_before += __shfl(slots_to, 63, 64);
+    items_before += wave::of_lane(items_to, 63u);
+    units_before += wave::of_lane(units_to, 63u);
+    slots_before += wave::of_lane(slots_to, 63u);
   }
   return item;
 }
@@ -414,7 +407,7 @@ struct FewShape {
 };
 
 template <typename T, int DP, int RB, bool WHOLE>
-__global__ __launch_bounds__(kThreads, DP <= 128 && DP * RB <= 256 ? 2 : 1) void cache_attention_few_kernel(CacheAttentionArgs args, Plan plan) {
+__global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2 : 1) void cache_attention_few_kernel(CacheAttentionArgs args, Plan plan) {
   typedef FewShape<T, DP, RB> Shape;
   constexpr int R = 16 * RB, STEP = Shape::kTokens, TB = STEP / 16;  // token blocks of a step
   constexpr bool kHalf = sizeof(T) == 2;
@@ -1120,7 +1113,7 @@ Variant choose(const CacheAttentionArgs& args) {
   return choose<T, 256>(rows, dim == 256u);
 }
 
-constexpr uint32_t kShortest = 256;  // tokens of a part
+constexpr uint32_t kShortest = 512;  // tokens of a part
 
 Plan plan_of(const CacheAttentionArgs& args, uint32_t R) {
   const uint64_t group = args.heads / args.cache.kv_heads;
@@ -1128,7 +1121,7 @@ Plan plan_of(const CacheAttentionArgs& args, uint32_t R) {
   Plan plan;
   // Full tiles of rows, and one that is not full for each sequence.
   plan.most_units = (uint32_t)(args.cache.kv_heads * (args.cache.rows * group / R + some));
-  plan.more = args.cache.capacity() > kShortest ? (R > 64u ? 256u : R > 32u ? 512u : 1024u) : 0u;
+  plan.more = args.cache.capacity() > kShortest ? (R > 64u ? 256u : R > 32u ? 512u : R > 16u ? 1024u : 2048u) : 0u;
   plan.shortest = kShortest;
   return plan;
 }

@@ -16,16 +16,31 @@ __device__ __forceinline__ uint32_t dpp(uint32_t identity, uint32_t x) {
   return (uint32_t)__builtin_amdgcn_update_dpp((int)identity, (int)x, CTRL, ROWS, 0xf, false);
 }
 
-// op over the 64 lanes of x; lanes without a neighbour see the identity.
+// op over the lanes up to this one; lanes without a neighbour see the identity.
 template <typename Op>
-__device__ __forceinline__ uint32_t reduce_bits(uint32_t x, uint32_t identity, Op op) {
+__device__ __forceinline__ uint32_t scan_bits(uint32_t x, uint32_t identity, Op op) {
   x = op(x, dpp<0x111, 0xf>(identity, x));  // row_shr:1
   x = op(x, dpp<0x112, 0xf>(identity, x));
   x = op(x, dpp<0x114, 0xf>(identity, x));
   x = op(x, dpp<0x118, 0xf>(identity, x));  // lane 15 of each row of 16 holds the row
   x = op(x, dpp<0x142, 0xa>(identity, x));  // row_bcast:15 into rows 1 and 3
-  x = op(x, dpp<0x143, 0xc>(identity, x));  // row_bcast:31 into rows 2 and 3
-  return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+  return op(x, dpp<0x143, 0xc>(identity, x));  // row_bcast:31 into rows 2 and 3
+}
+
+// op over the 64 lanes of x.
+template <typename Op>
+__device__ __forceinline__ uint32_t reduce_bits(uint32_t x, uint32_t identity, Op op) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)scan_bits(x, identity, op), 63);
+}
+
+// x of one lane, the same for all.
+__device__ __forceinline__ uint32_t of_lane(uint32_t x, uint32_t lane) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, (int)lane);
+}
+
+// Sums over the lanes up to this one.
+__device__ __forceinline__ uint32_t running_sum(uint32_t x) {
+  return scan_bits(x, 0u, [](uint32_t a, uint32_t b) { return a + b; });
 }
 
 __device__ __forceinline__ float sum(float x) {
