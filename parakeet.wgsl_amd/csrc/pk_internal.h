@@ -532,7 +532,11 @@ struct VerifyArgs {
   uint32_t columns;
   double scale;        // log2(e) / temperature
   bool greedy, f16;
+  // Memory of the op for rows that are split over workgroups (null: never).
+  void* workspace;
 };
+// Bytes of workspace that launches of the op need.
+uint64_t verify_workspace(const VerifyArgs& args);
 hipError_t launch_verify(const VerifyArgs& args, hipStream_t stream, hipEvent_t start = nullptr,
                          hipEvent_t stop = nullptr);
 

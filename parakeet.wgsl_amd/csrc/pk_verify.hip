@@ -4,175 +4,601 @@
 //
 // Decisions are whole numbers, so probabilities and sums are f64: a sum of
 // 131072 f32 exponentials moves with its order by more than the gap between two
-// neighbouring tokens of a flat distribution.
+// neighbouring tokens of a flat distribution. An f64 operation takes the VALU no
+// longer than an f32 one; an exponential is some 20 of them, and bounds the
+// kernels: memory would feed twice as many.
+//
+// Short rows: one launch, a workgroup for each sequence. Its wavefronts take the
+// rows' sums, target and draft, side by side, the decisions are read from
+// them in turn, and all threads look for the next token. Long rows: a launch
+// for the sums of parts of all rows; one for each sequence and part that decides, every
+// workgroup for itself, and sums the part's weights; and one for each
+// sequence that finds the part and in it the token.
 #include "pk_internal.h"
+#include "pk_wave.h"
 
 namespace pk {
 namespace {
 
-constexpr int kThreads = 256;
 constexpr uint32_t kNoToken = 0xffffffffu;
 constexpr float kInf = __builtin_inff();
+constexpr int kThreads = 256;       // of a workgroup that holds a part of a row
+constexpr int kHeld = 4;            // pieces of 16 bytes of a part in a thread
+constexpr int kSequence = 1024;     // threads of a workgroup that holds a sequence
+template <typename T>
+constexpr uint32_t kSpan = kThreads * kHeld * 16 / sizeof(T);  // columns of a part
 
-// 2^x, x <= 0: the whole part goes to the exponent, and the Taylor series of
-// 2^f, |f| <= 1/2, is cut where its terms fall below 2^-53.
+// 2^x, x <= 0, within 2^-46 of it: the nearest whole number goes to the exponent, and the Taylor
+// series of 2^f, |f| <= 1/2, ends at f^11.
 __device__ __forceinline__ double exp2_of(double x) {
   x = x < -1100.0 ? -1100.0 : x;  // 0 from there on; a NaN passes
-  const double n = __builtin_rint(x), f = (x - n) * 0.6931471805599453;
-  double r = 1.0 / 6227020800.0;
-  constexpr double kInverse[13] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320,
-                                   1.0 / 362880, 1.0 / 3628800, 1.0 / 39916800, 1.0 / 479001600};
+  const double n = __builtin_rint(x), f = x - n;
+  constexpr double kLn2 = 0.6931471805599453;
+  constexpr double c2 = kLn2 * kLn2 / 2, c3 = c2 * kLn2 / 3, c4 = c3 * kLn2 / 4, c5 = c4 * kLn2 / 5, c6 = c5 * kLn2 / 6,
+                   c7 = c6 * kLn2 / 7, c8 = c7 * kLn2 / 8, c9 = c8 * kLn2 / 9, c10 = c9 * kLn2 / 10, c11 = c10 * kLn2 / 11;
+  double r = __builtin_fma(c11, f, c10);
+  constexpr double c[10] = {1.0, kLn2, c2, c3, c4, c5, c6, c7, c8, c9};
 #pragma unroll
-  for (int i = 12; i >= 0; --i) r = __builtin_fma(r, f, kInverse[i]);
+  for (int i = 9; i >= 0; --i) r = __builtin_fma(r, f, c[i]);
   return __builtin_ldexp(r, (int)n);
 }
 
-// Sums (or maxima) over the workgroup, in every thread, in a fixed order.
-template <typename V, typename Op>
-__device__ __forceinline__ V reduce(V x, V* scratch, Op op) {
+// Over the lanes of a wavefront, or over WIDTH neighbouring ones, in every lane and in a fixed order.
+template <int WIDTH, typename V, typename Op>
+__device__ __forceinline__ V reduce_lanes(V x, Op op) {
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) x = op(x, __shfl_xor(x, off, 64));
-  __syncthreads();
-  if ((threadIdx.x & 63u) == 0) scratch[threadIdx.x >> 6] = x;
-  __syncthreads();
-  x = scratch[0];
-#pragma unroll
-  for (int w = 1; w < kThreads / 64; ++w) x = op(x, scratch[w]);
+  for (int off = 1; off < WIDTH; off <<= 1) x = op(x, __shfl_xor(x, off, 64));
   return x;
 }
-
-// A row of logits: its maximum, the sum of 2^((z - m) scale), and whether
-// it has no probabilities.
-struct RowSum {
-  double m, sum;
-  bool bad;
+template <int THREADS, typename V, typename Op>
+__device__ __forceinline__ V reduce_group(V x, double* scratch, Op op) {
+  static_assert(sizeof(V) <= sizeof(double), "a word of scratch each");
+  x = reduce_lanes<64>(x, op);
+  V* all = reinterpret_cast<V*>(scratch);
+  __syncthreads();  // the readers of the one before
+  if ((threadIdx.x & 63u) == 0) all[threadIdx.x >> 6] = x;
+  __syncthreads();
+  x = all[0];
+#pragma unroll
+  for (int w = 1; w < THREADS / 64; ++w) x = op(x, all[w]);
+  return x;
+}
+struct Add {
+  __device__ double operator()(double a, double b) const { return a + b; }
+};
+struct Larger {
+  template <typename V>
+  __device__ V operator()(V a, V b) const { return a > b ? a : b; }
+};
+struct Smaller {
+  template <typename V>
+  __device__ V operator()(V a, V b) const { return a < b ? a : b; }
 };
 
+// Of a row of logits, or a part: the maximum m and the sum of 2^((z - m) scale);
+// greedy: the key of the best. A sum below 0: a NaN or plus infinity is among them.
+struct RowSum {
+  union {
+    double m;
+    uint64_t best;
+  };
+  double sum;
+};
+__device__ __forceinline__ bool has_none(const RowSum& r) { return !(r.sum > 0.0); }
+
+// Larger logits first, equal ones by index; 0 for what is none (NaN, minus infinity).
+__device__ __forceinline__ uint64_t key_of(float v, uint32_t index) {
+  const uint32_t bits = __float_as_uint(v + 0.0f), order = (bits & 0x80000000u) ? ~bits : bits | 0x80000000u;
+  return v > -kInf ? ((uint64_t)order << 32) | (uint32_t)~index : 0;
+}
+
+// Joins sums of parts whose maxima are `m` and sums `sum` to the whole's maximum.
+__device__ __forceinline__ double scaled(double m, double sum, double top, double scale) {
+  return sum > 0.0 ? sum * exp2_of((m - top) * scale) : 0.0;
+}
+
+// The rows of a sequence, and the draft that a row judges.
+struct Rows {
+  uint32_t start, end;
+  __device__ Rows(const VerifyArgs& args, uint32_t s)
+      : start(min(args.row_starts[s], args.rows)), end(min(args.row_starts[s + 1], args.rows)) {}
+  __device__ uint32_t draft(const VerifyArgs& args, uint32_t row) const {
+    return row + 1 < end ? args.tokens[row + 1] : kNoToken;
+  }
+};
+
+// What a sequence came to: accepted drafts, and the row that its next token is drawn from.
+struct End {
+  uint32_t accepted, row;
+  uint32_t draft;      // refused there; kNoToken: the row is the last
+  uint32_t token;      // decided already (kNoToken), or to be drawn (0)
+  RowSum p, q;
+};
+
+// Whether the draft of a row stands, given its sums.
 template <typename T>
-__device__ RowSum sum_row(const T* z, uint32_t columns, double scale, double* scratch) {
+__device__ __forceinline__ bool stands(const VerifyArgs& args, uint32_t row, uint32_t draft, const RowSum& p, const RowSum& q) {
+  const T* z = static_cast<const T*>(args.target) + row * args.target_stride;
+  const double pd = exp2_of(((double)(float)z[draft] - p.m) * args.scale) / p.sum;
+  double qd = 1.0;
+  if (args.draft) {
+    const T* y = static_cast<const T*>(args.draft) + row * args.draft_stride;
+    qd = exp2_of(((double)(float)y[draft] - q.m) * args.scale) / q.sum;
+  }
+  return (double)args.uniforms[row] * qd < pd;
+}
+
+// The weights that the next token is drawn by.
+template <typename T>
+struct Weights {
+  const T *z, *y;  // y null: no draft logits, or the last row
+  uint32_t refused;
+  double m, inverse, draft_m, draft_inverse, scale;
+  bool residual;
+  __device__ Weights(const VerifyArgs& args, const End& end, bool residual)
+      : z(static_cast<const T*>(args.target) + end.row * args.target_stride),
+        y(args.draft && residual ? static_cast<const T*>(args.draft) + end.row * args.draft_stride : nullptr),
+        refused(end.draft), m(end.p.m), inverse(1.0 / end.p.sum), draft_m(end.q.m), draft_inverse(1.0 / end.q.sum),
+        scale(args.scale), residual(residual) {}
+  __device__ double of(float target, float draft, uint32_t i) const {
+#pragma clang fp contract(off)  // equal probabilities leave 0
+    double w = exp2_of(((double)target - m) * scale) * inverse;
+    if (y) w -= exp2_of(((double)draft - draft_m) * scale) * draft_inverse;
+    else if (residual && i == refused) w -= 1.0;
+    return w > 0.0 ? w : 0.0;
+  }
+  __device__ double operator()(uint32_t i) const { return of((float)z[i], y ? (float)y[i] : 0.0f, i); }
+};
+
+// A draw of [0, 1) of the whole weight; below it none, above it all.
+__device__ __forceinline__ double wanted(float draw, double whole) {
+  return draw > 0.0f ? (draw < 1.0f ? (double)draw * whole : whole) : draw <= 0.0f ? 0.0 : whole;
+}
+
+// The first of the columns [first, last) whose running sum of weights, from `before`
+// on, exceeds `want`; the last with a weight if none does, kNoToken if none has one.
+// Each thread of the workgroup takes a run of columns.
+template <int THREADS, typename Weight>
+__device__ __forceinline__ uint32_t find_token(uint32_t first, uint32_t last, double before, double want, double* scratch,
+                                               Weight weight) {
+  const uint32_t at = threadIdx.x, lane = at & 63u, each = (last - first + THREADS - 1u) / THREADS;
+  const uint32_t from = min(last, first + at * each), to = min(last, from + each);
+  double mine = 0.0;
+  uint32_t behind = 0;  // one more than the last column with a weight
+  for (uint32_t i = from; i < to; ++i) {
+    const double w = weight(i);
+    mine += w;
+    if (w > 0.0) behind = i + 1u;
+  }
+  double running = mine;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const double other = __shfl_up(running, off, 64);
+    if ((int)lane >= off) running += other;
+  }
+  __syncthreads();
+  if (lane == 63u) scratch[at >> 6] = running;
+  __syncthreads();
+  double base = before;
+  for (uint32_t w = 0; w < (at >> 6); ++w) base += scratch[w];
+  uint32_t hit = kNoToken;
+  if (base + running > want) {
+    double sum = base + (running - mine);
+    for (uint32_t i = from; i < to && hit == kNoToken; ++i) {
+      const double w = weight(i);
+      sum += w;
+      if (w > 0.0 && sum > want) hit = i;
+    }
+  }
+  hit = reduce_group<THREADS>(hit, scratch, Smaller());
+  behind = reduce_group<THREADS>(behind, scratch, Larger());
+  return hit != kNoToken ? hit : behind ? behind - 1u : kNoToken;
+}
+
+// ------------------------------------------------------------- short rows
+
+// A wavefront's sum of a whole row.
+template <typename T>
+__device__ __forceinline__ RowSum sum_row(const T* z, uint32_t columns, double scale, bool greedy) {
+  const uint32_t lane = threadIdx.x & 63u;
+  RowSum row;
+  if (greedy) {
+    unsigned long long best = 0;
+    for (uint32_t i = lane; i < columns; i += 64u) best = Larger()(best, (unsigned long long)key_of((float)z[i], i));
+    row.best = reduce_lanes<64>(best, Larger());
+    row.sum = row.best ? 1.0 : 0.0;
+    return row;
+  }
   float m = -kInf;
-  int strange = 0;
-  for (uint32_t i = threadIdx.x; i < columns; i += kThreads) {
+  bool strange = false;
+#pragma unroll 4
+  for (uint32_t i = lane; i < columns; i += 64u) {
     const float v = (float)z[i];
     strange |= !(v < kInf);
     m = fmaxf(m, v);
   }
-  float* f = reinterpret_cast<float*>(scratch);
-  m = reduce(m, f, [](float a, float b) { return fmaxf(a, b); });
-  strange = reduce(strange, reinterpret_cast<int*>(scratch), [](int a, int b) { return a | b; });
-  RowSum row = {m, 0.0, strange || m == -kInf};
-  if (row.bad) return row;
+  m = wave::max(m);
+  row.m = m;
+  row.sum = -1.0;
+  if (__any(strange)) return row;
   double sum = 0.0;
-  for (uint32_t i = threadIdx.x; i < columns; i += kThreads) sum += exp2_of(((double)(float)z[i] - row.m) * scale);
-  row.sum = reduce(sum, scratch, [](double a, double b) { return a + b; });
+  if (m > -kInf)
+#pragma unroll 4
+    for (uint32_t i = lane; i < columns; i += 64u) sum += exp2_of(((double)(float)z[i] - row.m) * scale);
+  row.sum = reduce_lanes<64>(sum, Add());
   return row;
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs args) {
-  __shared__ double scratch[kThreads / 64];
-  const uint32_t s = blockIdx.x, at = threadIdx.x, columns = args.columns;
-  const uint32_t start = min(args.row_starts[s], args.rows), end = min(args.row_starts[s + 1], args.rows);
-  uint32_t accepted = 0, token = kNoToken;
-  for (uint32_t row = start; row < end; ++row) {
-    const T* z = static_cast<const T*>(args.target) + row * args.target_stride;
-    const uint32_t draft = row + 1 < end ? args.tokens[row + 1] : kNoToken;
-    const bool last = draft >= columns;
-    if (args.greedy) {
-      // The largest, the lowest index of equal ones; 0 where there is none.
-      uint64_t best = 0;
-      for (uint32_t i = at; i < columns; i += kThreads) {
-        const float v = (float)z[i] + 0.0f;
-        const uint32_t bits = __float_as_uint(v), order = (bits & 0x80000000u) ? ~bits : bits | 0x80000000u;
-        const uint64_t key = v > -kInf ? ((uint64_t)order << 32) | (uint32_t)~i : 0;
-        best = key > best ? key : best;
+__global__ __launch_bounds__(kSequence) void verify_sequence_kernel(VerifyArgs args) {
+  constexpr uint32_t kWaves = kSequence / 64;
+  __shared__ double scratch[kWaves];
+  __shared__ RowSum sums[kWaves];
+  const uint32_t s = blockIdx.x, wave = threadIdx.x >> 6;
+  const Rows rows(args, s);
+  const bool two = args.draft && !args.greedy;
+  const uint32_t together = two ? kWaves / 2 : kWaves;
+  End end = {0, rows.start, kNoToken, kNoToken, {}, {}};
+  bool done = rows.start >= rows.end;
+  for (uint32_t first = rows.start; !done; first += together) {
+    const uint32_t row = first + (two ? wave / 2 : wave);
+    RowSum sum = {{0.0}, 0.0};
+    if (row < rows.end) {
+      // The row of a sequence's last token has no draft.
+      const bool of_draft = two && (wave & 1u), needed = !of_draft || rows.draft(args, row) < args.columns;
+      const T* z = of_draft ? static_cast<const T*>(args.draft) + row * args.draft_stride
+                            : static_cast<const T*>(args.target) + row * args.target_stride;
+      if (needed) sum = sum_row(z, args.columns, args.scale, args.greedy);
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63u) == 0) sums[wave] = sum;
+    __syncthreads();
+    for (uint32_t i = 0; i < together && !done; ++i) {
+      const uint32_t at = first + i;
+      const RowSum p = sums[two ? 2 * i : i], q = sums[two ? 2 * i + 1 : i];
+      const uint32_t draft = rows.draft(args, at);
+      const bool last = draft >= args.columns;
+      end.row = at;
+      end.draft = last ? kNoToken : draft;
+      end.p = p;
+      end.q = q;
+      done = true;
+      if (args.greedy) {
+        end.token = has_none(p) ? kNoToken : ~(uint32_t)p.best;
+        if (!last && end.token == draft) done = false;
+      } else if (has_none(p) || (!last && args.draft && has_none(q))) {
+        end.token = kNoToken;
+      } else {
+        end.token = 0;
+        if (!last && stands<T>(args, at, draft, p, q)) done = false;
       }
-      unsigned long long all = best;
-      all = reduce(all, reinterpret_cast<unsigned long long*>(scratch),
-                   [](unsigned long long a, unsigned long long b) { return a > b ? a : b; });
-      token = all ? ~(uint32_t)all : kNoToken;
-      if (last || token != draft) break;
-      ++accepted;
-      continue;
+      end.accepted += !done;
     }
-    const T* y = args.draft ? static_cast<const T*>(args.draft) + row * args.draft_stride : nullptr;
-    const RowSum p = sum_row(z, columns, args.scale, scratch);
-    RowSum q = {0.0, 1.0, false};
-    if (!last && y) q = sum_row(y, columns, args.scale, scratch);
-    if (p.bad || q.bad) {
-      token = kNoToken;
-      break;
-    }
-    const auto target_of = [&](uint32_t i) { return exp2_of(((double)(float)z[i] - p.m) * args.scale) / p.sum; };
-    const auto draft_of = [&](uint32_t i) {
-      return y ? exp2_of(((double)(float)y[i] - q.m) * args.scale) / q.sum : i == draft ? 1.0 : 0.0;
-    };
-    if (!last && (double)args.uniforms[row] * draft_of(draft) < target_of(draft)) {
-      ++accepted;
-      continue;
-    }
-    bool residual = !last;
-    const auto weight = [&](uint32_t i) {
-      if (i >= columns) return 0.0;
-      const double w = target_of(i) - (residual ? draft_of(i) : 0.0);
-      return w > 0.0 ? w : 0.0;
-    };
-    const auto add = [](double a, double b) { return a + b; };
+  }
+  if (!args.greedy && end.token != kNoToken) {
+    bool residual = end.draft != kNoToken;
     double whole = 0.0;
     for (;;) {
-      whole = 0.0;
-      for (uint32_t i = 0; i < columns; i += kThreads) whole += reduce(weight(i + at), scratch, add);
+      const Weights<T> weights(args, end, residual);
+      double mine = 0.0;
+      for (uint32_t i = threadIdx.x; i < args.columns; i += kSequence) mine += weights(i);
+      whole = reduce_group<kSequence>(mine, scratch, Add());
       if (whole > 0.0 || !residual) break;
-      residual = false;
+      residual = false;  // p nowhere above q
     }
-    const float draw = args.draws[s];
-    const double want = draw > 0.0f ? (draw < 1.0f ? (double)draw * whole : whole) : draw <= 0.0f ? 0.0 : whole;
-    double before = 0.0;
-    uint32_t behind = 0;  // the last token with a weight
-    token = kNoToken;
-    for (uint32_t i = 0; i < columns && token == kNoToken; i += kThreads) {
-      const double mine = weight(i + at);
-      double running = mine;  // of the wavefront up to this lane, then of the workgroup
+    end.token = find_token<kSequence>(0, args.columns, 0.0, wanted(args.draws[s], whole), scratch,
+                                      Weights<T>(args, end, residual));
+  }
+  if (threadIdx.x == 0) {
+    args.accepted[s] = end.accepted;
+    args.next_tokens[s] = end.token;
+  }
+}
+
+// -------------------------------------------------------------- long rows
+
+// Memory of the op: for each row of target and draft the sums of its parts;
+// for each sequence where it ended, and the weights of the parts of that row.
+struct Workspace {
+  RowSum* sums;     // [rows][2][parts]
+  End* ends;        // [sequences]
+  double* weights;  // [sequences][parts]
+};
+template <typename T>
+__host__ __device__ uint32_t parts_of(uint32_t columns) {
+  return (columns + kSpan<T> - 1u) / kSpan<T>;
+}
+__host__ __device__ Workspace bind(const VerifyArgs& args, uint64_t parts, uint64_t sequences) {
+  Workspace w;
+  w.sums = static_cast<RowSum*>(args.workspace);
+  w.ends = reinterpret_cast<End*>(w.sums + 2u * args.rows * parts);
+  w.weights = reinterpret_cast<double*>(w.ends + sequences);
+  return w;
+}
+
+// The columns of a part as a thread holds them: pieces of 16 bytes from the first
+// boundary on, and a single one of those before and behind.
+template <typename T>
+struct Part {
+  static constexpr int VEC = 16 / sizeof(T);
+  typedef T V __attribute__((ext_vector_type(VEC)));
+  uint32_t first, head, vectors, tail;
+  __device__ Part(const T* row, uint32_t columns, uint32_t part) : first(part * kSpan<T>) {
+    const uint32_t size = min(kSpan<T>, columns - first);
+    head = min(size, (uint32_t)(-reinterpret_cast<uintptr_t>(row + first) % 16u / sizeof(T)));
+    vectors = (size - head) / VEC;
+    tail = size - head - vectors * VEC;
+  }
+};
+
+// The sums of a part of a row.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs args, uint32_t parts) {
+  typedef typename Part<T>::V V;
+  constexpr int VEC = Part<T>::VEC;
+  __shared__ double scratch[kThreads / 64];
+  __shared__ uint32_t needed;
+  const uint32_t at = threadIdx.x, row = blockIdx.x, which = blockIdx.y / parts, part_index = blockIdx.y - which * parts;
+  const T* z = which ? static_cast<const T*>(args.draft) + row * args.draft_stride
+                     : static_cast<const T*>(args.target) + row * args.target_stride;
+  const Part<T> part(z, args.columns, part_index);
+  const V* body = reinterpret_cast<const V*>(z + part.first + part.head);
+  V held[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const uint32_t v = at + i * kThreads;
+    if (v < part.vectors) held[i] = body[v];
+    else
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) held[i][c] = (T)-kInf;
+  }
+  const uint32_t edge = part.first + (at < part.head ? at : part.head + part.vectors * VEC + (at - part.head));
+  const float single = at < part.head + part.tail ? (float)z[edge] : -kInf;
+  // A row of no sequence, or the draft's of a last one, is not asked for.
+  if (at == 0) needed = 0;
+  __syncthreads();
+  for (uint32_t s = at; s < args.sequences; s += kThreads) {
+    const Rows rows(args, s);
+    if (row >= rows.start && row < rows.end && (!which || rows.draft(args, row) < args.columns)) needed = 1;
+  }
+  __syncthreads();
+  if (!needed) return;
+  RowSum sum;
+  if (args.greedy) {
+    unsigned long long best = at < part.head + part.tail ? key_of(single, edge) : 0;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+#pragma unroll
+      for (int c = 0; c < VEC; ++c)
+        best = Larger()(best, (unsigned long long)key_of((float)held[i][c], part.first + part.head + (at + i * kThreads) * VEC + c));
+    sum.best = reduce_group<kThreads>(best, scratch, Larger());
+    sum.sum = sum.best ? 1.0 : 0.0;
+  } else {
+    float m = single;
+    bool strange = !(single < kInf);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) {
+        strange |= !((float)held[i][c] < kInf);
+        m = fmaxf(m, (float)held[i][c]);
+      }
+    // Plus infinity stands for what is no number.
+    m = reduce_group<kThreads>(__any(strange) ? kInf : wave::max(m), scratch, Larger());
+    sum.m = m;
+    double mine = 0.0;
+    if (m > -kInf && m < kInf) {
+      mine = exp2_of(((double)single - sum.m) * args.scale);
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i)
+        if (at + i * kThreads < part.vectors)
+#pragma unroll
+          for (int c = 0; c < VEC; ++c) mine += exp2_of(((double)(float)held[i][c] - sum.m) * args.scale);
+    }
+    sum.sum = reduce_group<kThreads>(mine, scratch, Add());
+    if (m == kInf) sum.sum = -1.0;
+  }
+  if (at == 0) bind(args, parts, 0).sums[((uint64_t)row * 2 + which) * parts + part_index] = sum;
+}
+
+// Where a sequence ends: groups of 16 lanes join the parts of a row each, 8 rows at a time,
+// and the decisions are read from them in turn.
+template <typename T>
+__device__ __forceinline__ End find_end(const VerifyArgs& args, const Workspace& work, uint32_t s, uint32_t parts, RowSum* sums) {
+  constexpr uint32_t kTogether = kThreads / 32;
+  const Rows rows(args, s);
+  const uint32_t group = threadIdx.x / 16, lane = threadIdx.x % 16;
+  End end = {0, rows.start, kNoToken, kNoToken, {}, {}};
+  bool done = rows.start >= rows.end;
+  for (uint32_t first = rows.start; !done; first += kTogether) {
+    const uint32_t row = first + group / 2, which = group & 1u;
+    const bool needed = row < rows.end && (!which || (args.draft && !args.greedy && rows.draft(args, row) < args.columns));
+    RowSum sum = {{0.0}, 0.0};
+    const RowSum* from = work.sums + ((uint64_t)row * 2 + which) * parts;
+    if (args.greedy) {
+      unsigned long long best = 0;
+      if (needed)
+        for (uint32_t i = lane; i < parts; i += 16u) best = Larger()(best, (unsigned long long)from[i].best);
+      sum.best = reduce_lanes<16>(best, Larger());
+      sum.sum = sum.best ? 1.0 : 0.0;
+    } else {
+      double m = -(double)kInf, all = 0.0;
+      bool strange = false;
+      if (needed)
+        for (uint32_t i = lane; i < parts; i += 16u) {
+          m = Larger()(m, from[i].m);
+          strange |= from[i].sum < 0.0;
+        }
+      m = reduce_lanes<16>(m, Larger());
+      if (needed)
+        for (uint32_t i = lane; i < parts; i += 16u) all += scaled(from[i].m, from[i].sum, m, args.scale);
+      sum.m = m;
+      sum.sum = reduce_lanes<16>(all, Add());
+      strange = reduce_lanes<16>((int)strange, Larger());
+      if (strange) sum.sum = -1.0;
+    }
+    __syncthreads();
+    if (lane == 0) sums[group] = sum;
+    __syncthreads();
+    for (uint32_t i = 0; i < kTogether && !done; ++i) {
+      const uint32_t at = first + i;
+      const uint32_t draft = rows.draft(args, at);
+      const bool last = draft >= args.columns;
+      end.row = at;
+      end.draft = last ? kNoToken : draft;
+      end.p = sums[2 * i];
+      end.q = sums[2 * i + 1];
+      done = true;
+      if (args.greedy) {
+        end.token = has_none(end.p) ? kNoToken : ~(uint32_t)end.p.best;
+        if (!last && end.token == draft) done = false;
+      } else if (has_none(end.p) || (!last && args.draft && has_none(end.q))) {
+        end.token = kNoToken;
+      } else {
+        end.token = 0;
+        if (!last && stands<T>(args, at, draft, end.p, end.q)) done = false;
+      }
+      end.accepted += !done;
+    }
+  }
+  return end;
+}
+
+// Decides a sequence, and sums the weights of a part of the row where it ends.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void verify_weights_kernel(VerifyArgs args, uint32_t parts, uint32_t sequences) {
+  __shared__ double scratch[kThreads / 64];
+  __shared__ RowSum sums[kThreads / 16];
+  const uint32_t s = blockIdx.x, part_index = blockIdx.y, at = threadIdx.x;
+  const Workspace work = bind(args, parts, sequences);
+  const End end = find_end<T>(args, work, s, parts, sums);
+  if (part_index == 0 && at == 0) {
+    args.accepted[s] = end.accepted;
+    if (args.greedy || end.token == kNoToken) args.next_tokens[s] = end.token;
+    work.ends[s] = end;
+  }
+  if (args.greedy || end.token == kNoToken) return;
+  const Weights<T> weights(args, end, end.draft != kNoToken);
+  const uint32_t first = part_index * kSpan<T>, last = min(args.columns, first + kSpan<T>);
+  double mine = 0.0;
+#pragma unroll 4
+  for (uint32_t i = first + at; i < last; i += kThreads) mine += weights(i);
+  mine = reduce_group<kThreads>(mine, scratch, Add());
+  if (at == 0) work.weights[(uint64_t)s * parts + part_index] = mine;
+}
+
+// Finds the part of the row whose weights the draw ends in, and in it the token.
+template <typename T>
+__global__ __launch_bounds__(kSequence) void verify_token_kernel(VerifyArgs args, uint32_t parts, uint32_t sequences) {
+  __shared__ double scratch[kSequence / 64];
+  __shared__ double found_before;
+  __shared__ uint32_t found_part;
+  const uint32_t s = blockIdx.x, at = threadIdx.x;
+  const Workspace work = bind(args, parts, sequences);
+  const End end = work.ends[s];
+  if (end.token == kNoToken) return;
+  bool residual = end.draft != kNoToken;
+  // The parts' weights: of p - q, or of p where that is nothing.
+  double whole = 0.0;
+  const auto part_weight = [&](uint32_t i) {
+    if (residual || end.draft == kNoToken) return work.weights[(uint64_t)s * parts + i];
+    const RowSum p = work.sums[(uint64_t)end.row * 2 * parts + i];
+    return scaled(p.m, p.sum, end.p.m, args.scale) / end.p.sum;
+  };
+  for (;;) {
+    double mine = 0.0;
+    for (uint32_t i = at; i < parts; i += kSequence) mine += part_weight(i);
+    whole = reduce_group<kSequence>(mine, scratch, Add());
+    if (whole > 0.0 || !residual) break;
+    residual = false;
+  }
+  const double want = wanted(args.draws[s], whole);
+  if (at < 64u) {  // the first wavefront, 64 parts at a time
+    double before = 0.0, last_before = 0.0;
+    uint32_t part = kNoToken, last = kNoToken;
+    for (uint32_t base = 0; base < parts && part == kNoToken; base += 64u) {
+      const double w = base + at < parts ? part_weight(base + at) : 0.0;
+      double running = w;
+#pragma unroll
       for (int off = 1; off < 64; off <<= 1) {
         const double other = __shfl_up(running, off, 64);
-        if ((int)(at & 63u) >= off) running += other;
+        if ((int)at >= off) running += other;
       }
-      __syncthreads();
-      if ((at & 63u) == 63u) scratch[at >> 6] = running;
-      __syncthreads();
-      double base = before, total = 0.0;
-      for (uint32_t w = 0; w < kThreads / 64; ++w) {
-        if (w < (at >> 6)) base += scratch[w];
-        total += scratch[w];
+      const uint64_t hit = __ballot(w > 0.0 && before + running > want), live = __ballot(w > 0.0);
+      const int lane = hit ? __builtin_ctzll(hit) : live ? 63 - __builtin_clzll(live) : 0;
+      const double to = before + __shfl(running - w, lane, 64);
+      if (hit) part = base + lane;
+      if (live) {
+        last = base + lane;
+        last_before = to;
       }
-      uint32_t hit = mine > 0.0 && base + running > want ? i + at : kNoToken;
-      __syncthreads();
-      hit = reduce(hit, reinterpret_cast<uint32_t*>(scratch), [](uint32_t a, uint32_t b) { return a < b ? a : b; });
-      const uint32_t live = reduce(mine > 0.0 ? i + at : 0u, reinterpret_cast<uint32_t*>(scratch),
-                                   [](uint32_t a, uint32_t b) { return a > b ? a : b; });
-      token = hit;
-      behind = live > behind ? live : behind;
-      before += total;
+      before += __shfl(running, 63, 64);
     }
-    if (token == kNoToken) token = behind;
-    break;
+    if (at == 0) {
+      found_part = part != kNoToken ? part : last;
+      found_before = last_before;
+    }
   }
-  if (at == 0) {
-    args.accepted[s] = accepted;
-    args.next_tokens[s] = token;
+  __syncthreads();
+  if (found_part == kNoToken) {  // no weight at all
+    if (at == 0) args.next_tokens[s] = kNoToken;
+    return;
   }
+  const uint32_t first = found_part * kSpan<T>;
+  const uint32_t token = find_token<kSequence>(first, min(args.columns, first + kSpan<T>), found_before, want, scratch,
+                                               Weights<T>(args, end, residual));
+  if (at == 0) args.next_tokens[s] = token;
+}
+
+// Rows of a part each are read by one workgroup for a sequence, unless it has many.
+template <typename T>
+bool together(const VerifyArgs& args) {
+  return parts_of<T>(args.columns) == 1u && args.rows <= 64ull * args.sequences;
+}
+
+template <typename Kernel, typename... Args>
+hipError_t launch(Kernel kernel, dim3 grid, dim3 block, hipStream_t stream, hipEvent_t start, hipEvent_t stop, Args... args) {
+  if (start || stop)
+    hipExtLaunchKernelGGL(kernel, grid, block, 0, stream, start, stop, 0, args...);
+  else
+    hipLaunchKernelGGL(kernel, grid, block, 0, stream, args...);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_typed(const VerifyArgs& args, hipStream_t stream, hipEvent_t start, hipEvent_t stop) {
+  if (together<T>(args))
+    return launch(verify_sequence_kernel<T>, dim3(args.sequences), dim3(kSequence), stream, start, stop, args);
+  if (!args.workspace) return hipErrorInvalidValue;
+  const uint32_t parts = parts_of<T>(args.columns), sequences = args.sequences;
+  const bool two = args.draft && !args.greedy;
+  if (const hipError_t e = launch(verify_sums_kernel<T>, dim3(args.rows, parts * (two ? 2u : 1u)), dim3(kThreads), stream,
+                                  start, nullptr, args, parts))
+    return e;
+  const hipError_t e = launch(verify_weights_kernel<T>, dim3(sequences, args.greedy ? 1u : parts), dim3(kThreads), stream,
+                              nullptr, args.greedy ? stop : nullptr, args, parts, sequences);
+  if (e || args.greedy) return e;
+  return launch(verify_token_kernel<T>, dim3(sequences), dim3(kSequence), stream, nullptr, stop, args, parts, sequences);
+}
+
+template <typename T>
+uint64_t workspace_typed(const VerifyArgs& args) {
+  // Fewer active sequences may no longer be together.
+  VerifyArgs one = args;
+  one.sequences = 1;
+  if (together<T>(one)) return 0;
+  const uint64_t parts = parts_of<T>(args.columns);
+  return 2u * args.rows * parts * sizeof(RowSum) + args.sequences * (sizeof(End) + parts * sizeof(double));
 }
 
 }  // namespace
 
+uint64_t verify_workspace(const VerifyArgs& args) {
+  return args.f16 ? workspace_typed<_Float16>(args) : workspace_typed<float>(args);
+}
+
 hipError_t launch_verify(const VerifyArgs& args, hipStream_t stream, hipEvent_t start, hipEvent_t stop) {
-  const auto kernel = args.f16 ? verify_kernel<_Float16> : verify_kernel<float>;
-  const dim3 grid(args.sequences), block(kThreads);
-  if (start || stop)
-    hipExtLaunchKernelGGL(kernel, grid, block, 0, stream, start, stop, 0, args);
-  else
-    hipLaunchKernelGGL(kernel, grid, block, 0, stream, args);
-  return hipGetLastError();
+  return args.f16 ? launch_typed<_Float16>(args, stream, start, stop) : launch_typed<float>(args, stream, start, stop);
 }
 
 }  // namespace pk

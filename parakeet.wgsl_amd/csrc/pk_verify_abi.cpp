@@ -16,6 +16,7 @@ struct pk_verify_op {
   std::string label;
   uint32_t sequences = 0;
   pk::VerifyArgs args{};
+  void* workspace = nullptr;
   bool destroyed = false;
 };
 
@@ -106,12 +107,28 @@ int pk_verify_create(pk_context* ctx, const pk_verify_desc* d, pk_verify_op** ou
   a.scale = 1.4426950408889634 / (d->has_temperature ? (double)d->temperature : 1.0);
   a.greedy = d->mode == PK_VERIFY_GREEDY;
   a.f16 = d->precision == PK_PRECISION_F16;
+  void* workspace = nullptr;
+  if (const uint64_t bytes = pk::verify_workspace(a)) {
+    DeviceScope device(ctx->device);
+    PK_HIP(device.status(), "hipSetDevice");
+    const hipError_t e = hipMalloc(&workspace, bytes);
+    if (e != hipSuccess) {
+      (void)hipGetLastError();
+      return fail(PK_ALLOCATION_FAILURE, "%s: cannot allocate %llu bytes of workspace: %s", label.c_str(),
+                  (unsigned long long)bytes, hipGetErrorString(e));
+    }
+    a.workspace = workspace;
+  }
   auto* op = new (std::nothrow) pk_verify_op();
-  if (!op) return fail(PK_ALLOCATION_FAILURE, "%s: out of host memory", label.c_str());
+  if (!op) {
+    free_on(ctx->device, workspace);
+    return fail(PK_ALLOCATION_FAILURE, "%s: out of host memory", label.c_str());
+  }
   op->ctx = ctx;
   op->label.swap(label);
   op->sequences = d->sequences;
   op->args = a;
+  op->workspace = workspace;
   *out = op;
   return ok();
 } catch (const std::bad_alloc&) {
@@ -139,7 +156,10 @@ int pk_verify_enqueue_timed(pk_verify_op* op, uint32_t active_sequences, void* s
 }
 
 int pk_verify_destroy(pk_verify_op* op) {
-  if (op) op->destroyed = true;
+  if (!op || op->destroyed) return ok();
+  op->destroyed = true;
+  free_on(op->ctx->device, op->workspace);
+  op->workspace = nullptr;
   return ok();
 }
 
