@@ -28,19 +28,47 @@ constexpr int kSequence = 1024;     // threads of a workgroup that holds a seque
 template <typename T>
 constexpr uint32_t kSpan = kThreads * kHeld * 16 / sizeof(T);  // columns of a part
 
-// 2^x, x <= 0, within 2^-46 of it: the nearest whole number goes to the exponent, and the Taylor
-// series of 2^f, |f| <= 1/2, ends at f^11.
+// 2^x, x <= 0 but for roundings, within 2^-45 of it: x less its nearest whole number goes
+// through a polynomial that meets 2^f at the 10 Chebyshev points of [-1/2, 1/2]; the whole number is
+// in the low bits of x + 1.5 * 2^52 and is added to the exponent. 0 below 2^-1000.
 __device__ __forceinline__ double exp2_of(double x) {
-  x = x < -1100.0 ? -1100.0 : x;  // 0 from there on; a NaN passes
-  const double n = __builtin_rint(x), f = x - n;
-  constexpr double kLn2 = 0.6931471805599453;
-  constexpr double c2 = kLn2 * kLn2 / 2, c3 = c2 * kLn2 / 3, c4 = c3 * kLn2 / 4, c5 = c4 * kLn2 / 5, c6 = c5 * kLn2 / 6,
-                   c7 = c6 * kLn2 / 7, c8 = c7 * kLn2 / 8, c9 = c8 * kLn2 / 9, c10 = c9 * kLn2 / 10, c11 = c10 * kLn2 / 11;
-  double r = __builtin_fma(c11, f, c10);
-  constexpr double c[10] = {1.0, kLn2, c2, c3, c4, c5, c6, c7, c8, c9};
+#pragma clang fp contract(off)
+  constexpr double kWhole = 6755399441055744.0;
+  const double shifted = x + kWhole, f = x - (shifted - kWhole);
+  constexpr double c[10] = {1.0000000000000135, 0.6931471805599462, 0.2402265069564034, 0.05550410866465166,
+                            0.00961812919393429, 0.0013333558200796013, 0.0001540343375126647, 1.5252672924257465e-05,
+                            1.3259645241948732e-06, 1.020590550210069e-07};
+  double r = c[9];
 #pragma unroll
-  for (int i = 9; i >= 0; --i) r = __builtin_fma(r, f, c[i]);
-  return __builtin_ldexp(r, (int)n);
+  for (int i = 8; i >= 0; --i) r = __builtin_fma(r, f, c[i]);
+  const uint64_t bits = __builtin_bit_cast(uint64_t, r);
+  const uint32_t high = (uint32_t)(bits >> 32) + ((uint32_t)__builtin_bit_cast(uint64_t, shifted) << 20);
+  const double all = __builtin_bit_cast(double, ((uint64_t)high << 32) | (uint32_t)bits);
+  return x > -1000.0 ? all : 0.0;
+}
+
+// 2^((z - m) scale). The difference comes first: z * scale - m * scale in one operation less
+// loses all digits where logits of the size of f32's largest meet.
+struct Powers {
+  double m, scale;
+  __device__ __forceinline__ double at(float z) const { return exp2_of(((double)z - m) * scale); }
+};
+
+// Up to N elements from `row` on, `count` of them there: 16 bytes at a time where they lie so.
+template <int N, typename T>
+__device__ __forceinline__ void load_run(const T* row, uint32_t count, float (&to)[N]) {
+  constexpr int VEC = 16 / sizeof(T);
+  typedef T V __attribute__((ext_vector_type(VEC)));
+  if (count >= (uint32_t)N && reinterpret_cast<uintptr_t>(row) % 16u == 0) {
+    V v[N / VEC];
+#pragma unroll
+    for (int i = 0; i < N / VEC; ++i) v[i] = reinterpret_cast<const V*>(row)[i];
+#pragma unroll
+    for (int i = 0; i < N; ++i) to[i] = (float)v[i / VEC][i % VEC];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) to[i] = (uint32_t)i < count ? (float)row[i] : -kInf;
+  }
 }
 
 // Over the lanes of a wavefront, or over WIDTH neighbouring ones, in every lane and in a fixed order.
@@ -131,23 +159,33 @@ __device__ __forceinline__ bool stands(const VerifyArgs& args, uint32_t row, uin
 // The weights that the next token is drawn by.
 template <typename T>
 struct Weights {
+  static constexpr int kRun = kSpan<T> / kSequence;  // columns of a thread, of those that hold a sequence
   const T *z, *y;  // y null: no draft logits, or the last row
   uint32_t refused;
-  double m, inverse, draft_m, draft_inverse, scale;
+  Powers p, q;
+  double inverse, draft_inverse;
   bool residual;
   __device__ Weights(const VerifyArgs& args, const End& end, bool residual)
       : z(static_cast<const T*>(args.target) + end.row * args.target_stride),
         y(args.draft && residual ? static_cast<const T*>(args.draft) + end.row * args.draft_stride : nullptr),
-        refused(end.draft), m(end.p.m), inverse(1.0 / end.p.sum), draft_m(end.q.m), draft_inverse(1.0 / end.q.sum),
-        scale(args.scale), residual(residual) {}
-  __device__ double of(float target, float draft, uint32_t i) const {
+        refused(end.draft), p{end.p.m, args.scale}, q{end.q.m, args.scale}, inverse(1.0 / end.p.sum),
+        draft_inverse(y ? 1.0 / end.q.sum : 0.0), residual(residual) {}
+  __device__ __forceinline__ double of(float target, float draft, uint32_t i) const {
 #pragma clang fp contract(off)  // equal probabilities leave 0
-    double w = exp2_of(((double)target - m) * scale) * inverse;
-    if (y) w -= exp2_of(((double)draft - draft_m) * scale) * draft_inverse;
+    double w = p.at(target) * inverse;
+    if (y) w -= q.at(draft) * draft_inverse;
     else if (residual && i == refused) w -= 1.0;
     return w > 0.0 ? w : 0.0;
   }
-  __device__ double operator()(uint32_t i) const { return of((float)z[i], y ? (float)y[i] : 0.0f, i); }
+  // Of N columns from `first` on, `count` of them there; the others' are 0.
+  template <int N>
+  __device__ __forceinline__ void run(uint32_t first, uint32_t count, double (&w)[N]) const {
+    float target[N], draft[N];
+    load_run<N>(z + first, count, target);
+    if (y) load_run<N>(y + first, count, draft);
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = (uint32_t)i < count ? of(target[i], y ? draft[i] : 0.0f, first + i) : 0.0;
+  }
 };
 
 // A draw of [0, 1) of the whole weight; below it none, above it all.
@@ -155,22 +193,13 @@ __device__ __forceinline__ double wanted(float draw, double whole) {
   return draw > 0.0f ? (draw < 1.0f ? (double)draw * whole : whole) : draw <= 0.0f ? 0.0 : whole;
 }
 
-// The first of the columns [first, last) whose running sum of weights, from `before`
-// on, exceeds `want`; the last with a weight if none does, kNoToken if none has one.
-// Each thread of the workgroup takes a run of columns.
-template <int THREADS, typename Weight>
-__device__ __forceinline__ uint32_t find_token(uint32_t first, uint32_t last, double before, double want, double* scratch,
-                                               Weight weight) {
-  const uint32_t at = threadIdx.x, lane = at & 63u, each = (last - first + THREADS - 1u) / THREADS;
-  const uint32_t from = min(last, first + at * each), to = min(last, from + each);
-  double mine = 0.0;
-  uint32_t behind = 0;  // one more than the last column with a weight
-  for (uint32_t i = from; i < to; ++i) {
-    const double w = weight(i);
-    mine += w;
-    if (w > 0.0) behind = i + 1u;
-  }
-  double running = mine;
+// Of a workgroup of kSequence threads: the sum of x over the threads before this one, and over all.
+struct Running {
+  double before, whole;
+};
+__device__ __forceinline__ Running running_sum(double x, double* scratch) {
+  const uint32_t at = threadIdx.x, lane = at & 63u;
+  double running = x;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
     const double other = __shfl_up(running, off, 64);
@@ -179,52 +208,119 @@ __device__ __forceinline__ uint32_t find_token(uint32_t first, uint32_t last, do
   __syncthreads();
   if (lane == 63u) scratch[at >> 6] = running;
   __syncthreads();
-  double base = before;
-  for (uint32_t w = 0; w < (at >> 6); ++w) base += scratch[w];
-  uint32_t hit = kNoToken;
-  if (base + running > want) {
-    double sum = base + (running - mine);
-    for (uint32_t i = from; i < to && hit == kNoToken; ++i) {
-      const double w = weight(i);
-      sum += w;
-      if (w > 0.0 && sum > want) hit = i;
+  Running r = {0.0, 0.0};
+#pragma unroll
+  for (uint32_t w = 0; w < kSequence / 64; ++w) {
+    if (w == (at >> 6)) r.before = r.whole + (running - x);
+    r.whole += scratch[w];
+  }
+  return r;
+}
+
+// The first column whose running sum of weights exceeds `want`, `before` being the sum in front of
+// this thread's run of N from `first` on; the last with a weight if none does, kNoToken if none has one.
+template <int N>
+__device__ __forceinline__ uint32_t find_token(const double (&w)[N], uint32_t first, double before, double want,
+                                               double* scratch) {
+  uint32_t hit = kNoToken, behind = 0;  // one more than the last column with a weight
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    before += w[i];
+    if (w[i] > 0.0) {
+      behind = first + i + 1u;
+      if (before > want && hit == kNoToken) hit = first + i;
     }
   }
-  hit = reduce_group<THREADS>(hit, scratch, Smaller());
-  behind = reduce_group<THREADS>(behind, scratch, Larger());
+  hit = reduce_group<kSequence>(hit, scratch, Smaller());
+  behind = reduce_group<kSequence>(behind, scratch, Larger());
   return hit != kNoToken ? hit : behind ? behind - 1u : kNoToken;
+}
+
+// The rows [first, first + count) of a sequence in turn, from their sums (`each` apart: of the target, and of the
+// draft behind it): where it ends, if it does. Threads decide a row each first.
+template <typename T>
+__device__ __forceinline__ bool decide(const VerifyArgs& args, const Rows& rows, uint32_t first, uint32_t count, const RowSum* sums,
+                                       uint32_t each, uint32_t* states, End* end) {
+  enum { kStands = 0, kDraws = 1, kNone = 2 };
+  if (threadIdx.x < count && first + threadIdx.x < rows.end) {
+    const uint32_t row = first + threadIdx.x, draft = rows.draft(args, row);
+    const RowSum p = sums[threadIdx.x * each], q = sums[threadIdx.x * each + each - 1u];
+    const bool last = draft >= args.columns;
+    uint32_t state;
+    if (args.greedy) {
+      state = !has_none(p) && !last && ~(uint32_t)p.best == draft ? kStands : kDraws;
+    } else if (has_none(p) || (!last && args.draft && has_none(q))) {
+      state = kNone;
+    } else {
+      state = !last && stands<T>(args, row, draft, p, q) ? kStands : kDraws;
+    }
+    states[threadIdx.x] = state;
+  }
+  __syncthreads();
+  for (uint32_t i = 0; i < count; ++i) {
+    const uint32_t state = states[i];
+    if (state == kStands) continue;
+    const uint32_t draft = rows.draft(args, first + i);
+    end->p = sums[i * each];
+    end->q = sums[i * each + each - 1u];
+    end->row = first + i;
+    end->accepted = end->row - rows.start;
+    end->draft = draft >= args.columns ? kNoToken : draft;
+    end->token = args.greedy ? (has_none(end->p) ? kNoToken : ~(uint32_t)end->p.best) : state == kNone ? kNoToken : 0u;
+    return true;
+  }
+  return false;
 }
 
 // ------------------------------------------------------------- short rows
 
-// A wavefront's sum of a whole row.
+// A wavefront's sum of a whole row: pieces of kRun columns a lane, the row read
+// twice, the second time from the cache.
 template <typename T>
 __device__ __forceinline__ RowSum sum_row(const T* z, uint32_t columns, double scale, bool greedy) {
+  constexpr int kRun = 16 / sizeof(T), kPieces = 4;
   const uint32_t lane = threadIdx.x & 63u;
+  // Calls use(value, column) for the columns that there are.
+  const auto each = [&](auto use) {
+    for (uint32_t base = 0; base < columns; base += 64u * kRun * kPieces) {
+      float v[kPieces][kRun];
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const uint32_t from = base + (i * 64u + lane) * kRun;
+        load_run<kRun>(z + from, columns > from ? columns - from : 0u, v[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const uint32_t from = base + (i * 64u + lane) * kRun;
+        if (from < columns)
+#pragma unroll
+          for (int c = 0; c < kRun; ++c) use(v[i][c], from + c);
+      }
+    }
+  };
   RowSum row;
   if (greedy) {
     unsigned long long best = 0;
-    for (uint32_t i = lane; i < columns; i += 64u) best = Larger()(best, (unsigned long long)key_of((float)z[i], i));
+    each([&](float v, uint32_t i) { best = Larger()(best, (unsigned long long)key_of(v, i)); });
     row.best = reduce_lanes<64>(best, Larger());
     row.sum = row.best ? 1.0 : 0.0;
     return row;
   }
   float m = -kInf;
   bool strange = false;
-#pragma unroll 4
-  for (uint32_t i = lane; i < columns; i += 64u) {
-    const float v = (float)z[i];
+  each([&](float v, uint32_t) {
     strange |= !(v < kInf);
     m = fmaxf(m, v);
-  }
+  });
   m = wave::max(m);
   row.m = m;
   row.sum = -1.0;
   if (__any(strange)) return row;
   double sum = 0.0;
-  if (m > -kInf)
-#pragma unroll 4
-    for (uint32_t i = lane; i < columns; i += 64u) sum += exp2_of(((double)(float)z[i] - row.m) * scale);
+  if (m > -kInf) {
+    const Powers powers = {row.m, scale};
+    each([&](float v, uint32_t) { sum += powers.at(v); });
+  }
   row.sum = reduce_lanes<64>(sum, Add());
   return row;
 }
@@ -232,62 +328,43 @@ __device__ __forceinline__ RowSum sum_row(const T* z, uint32_t columns, double s
 template <typename T>
 __global__ __launch_bounds__(kSequence) void verify_sequence_kernel(VerifyArgs args) {
   constexpr uint32_t kWaves = kSequence / 64;
+  constexpr int kRun = Weights<T>::kRun;
   __shared__ double scratch[kWaves];
   __shared__ RowSum sums[kWaves];
+  __shared__ uint32_t states[kWaves];
   const uint32_t s = blockIdx.x, wave = threadIdx.x >> 6;
   const Rows rows(args, s);
   const bool two = args.draft && !args.greedy;
-  const uint32_t together = two ? kWaves / 2 : kWaves;
+  const uint32_t each = two ? 2u : 1u;
   End end = {0, rows.start, kNoToken, kNoToken, {}, {}};
-  bool done = rows.start >= rows.end;
-  for (uint32_t first = rows.start; !done; first += together) {
-    const uint32_t row = first + (two ? wave / 2 : wave);
+  for (uint32_t first = rows.start; first < rows.end; first += kWaves / each) {
+    const uint32_t row = first + wave / each;
     RowSum sum = {{0.0}, 0.0};
     if (row < rows.end) {
       // The row of a sequence's last token has no draft.
-      const bool of_draft = two && (wave & 1u), needed = !of_draft || rows.draft(args, row) < args.columns;
+      const bool of_draft = two && (wave & 1u);
       const T* z = of_draft ? static_cast<const T*>(args.draft) + row * args.draft_stride
                             : static_cast<const T*>(args.target) + row * args.target_stride;
-      if (needed) sum = sum_row(z, args.columns, args.scale, args.greedy);
+      if (!of_draft || rows.draft(args, row) < args.columns) sum = sum_row(z, args.columns, args.scale, args.greedy);
     }
     __syncthreads();
     if ((threadIdx.x & 63u) == 0) sums[wave] = sum;
     __syncthreads();
-    for (uint32_t i = 0; i < together && !done; ++i) {
-      const uint32_t at = first + i;
-      const RowSum p = sums[two ? 2 * i : i], q = sums[two ? 2 * i + 1 : i];
-      const uint32_t draft = rows.draft(args, at);
-      const bool last = draft >= args.columns;
-      end.row = at;
-      end.draft = last ? kNoToken : draft;
-      end.p = p;
-      end.q = q;
-      done = true;
-      if (args.greedy) {
-        end.token = has_none(p) ? kNoToken : ~(uint32_t)p.best;
-        if (!last && end.token == draft) done = false;
-      } else if (has_none(p) || (!last && args.draft && has_none(q))) {
-        end.token = kNoToken;
-      } else {
-        end.token = 0;
-        if (!last && stands<T>(args, at, draft, p, q)) done = false;
-      }
-      end.accepted += !done;
-    }
+    if (decide<T>(args, rows, first, min(kWaves / each, rows.end - first), sums, each, states, &end)) break;
   }
   if (!args.greedy && end.token != kNoToken) {
-    bool residual = end.draft != kNoToken;
-    double whole = 0.0;
-    for (;;) {
-      const Weights<T> weights(args, end, residual);
+    const uint32_t first = threadIdx.x * kRun, count = args.columns > first ? args.columns - first : 0u;
+    double w[kRun];
+    Running running;
+    for (bool residual = end.draft != kNoToken;; residual = false) {
+      Weights<T>(args, end, residual).run(first, count, w);
       double mine = 0.0;
-      for (uint32_t i = threadIdx.x; i < args.columns; i += kSequence) mine += weights(i);
-      whole = reduce_group<kSequence>(mine, scratch, Add());
-      if (whole > 0.0 || !residual) break;
-      residual = false;  // p nowhere above q
+#pragma unroll
+      for (int i = 0; i < kRun; ++i) mine += w[i];
+      running = running_sum(mine, scratch);
+      if (running.whole > 0.0 || !residual) break;  // or p is nowhere above q
     }
-    end.token = find_token<kSequence>(0, args.columns, 0.0, wanted(args.draws[s], whole), scratch,
-                                      Weights<T>(args, end, residual));
+    end.token = find_token(w, first, running.before, wanted(args.draws[s], running.whole), scratch);
   }
   if (threadIdx.x == 0) {
     args.accepted[s] = end.accepted;
@@ -388,12 +465,13 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs args, 
     sum.m = m;
     double mine = 0.0;
     if (m > -kInf && m < kInf) {
-      mine = exp2_of(((double)single - sum.m) * args.scale);
+      const Powers powers = {sum.m, args.scale};
+      mine = powers.at(single);
 #pragma unroll
       for (int i = 0; i < kHeld; ++i)
         if (at + i * kThreads < part.vectors)
 #pragma unroll
-          for (int c = 0; c < VEC; ++c) mine += exp2_of(((double)(float)held[i][c] - sum.m) * args.scale);
+          for (int c = 0; c < VEC; ++c) mine += powers.at((float)held[i][c]);
     }
     sum.sum = reduce_group<kThreads>(mine, scratch, Add());
     if (m == kInf) sum.sum = -1.0;
@@ -404,13 +482,13 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs args, 
 // Where a sequence ends: groups of 16 lanes join the parts of a row each, 8 rows at a time,
 // and the decisions are read from them in turn.
 template <typename T>
-__device__ __forceinline__ End find_end(const VerifyArgs& args, const Workspace& work, uint32_t s, uint32_t parts, RowSum* sums) {
+__device__ __forceinline__ End find_end(const VerifyArgs& args, const Workspace& work, uint32_t s, uint32_t parts, RowSum* sums,
+                                        uint32_t* states) {
   constexpr uint32_t kTogether = kThreads / 32;
   const Rows rows(args, s);
   const uint32_t group = threadIdx.x / 16, lane = threadIdx.x % 16;
   End end = {0, rows.start, kNoToken, kNoToken, {}, {}};
-  bool done = rows.start >= rows.end;
-  for (uint32_t first = rows.start; !done; first += kTogether) {
+  for (uint32_t first = rows.start; first < rows.end; first += kTogether) {
     const uint32_t row = first + group / 2, which = group & 1u;
     const bool needed = row < rows.end && (!which || (args.draft && !args.greedy && rows.draft(args, row) < args.columns));
     RowSum sum = {{0.0}, 0.0};
@@ -440,26 +518,7 @@ __device__ __forceinline__ End find_end(const VerifyArgs& args, const Workspace&
     __syncthreads();
     if (lane == 0) sums[group] = sum;
     __syncthreads();
-    for (uint32_t i = 0; i < kTogether && !done; ++i) {
-      const uint32_t at = first + i;
-      const uint32_t draft = rows.draft(args, at);
-      const bool last = draft >= args.columns;
-      end.row = at;
-      end.draft = last ? kNoToken : draft;
-      end.p = sums[2 * i];
-      end.q = sums[2 * i + 1];
-      done = true;
-      if (args.greedy) {
-        end.token = has_none(end.p) ? kNoToken : ~(uint32_t)end.p.best;
-        if (!last && end.token == draft) done = false;
-      } else if (has_none(end.p) || (!last && args.draft && has_none(end.q))) {
-        end.token = kNoToken;
-      } else {
-        end.token = 0;
-        if (!last && stands<T>(args, at, draft, end.p, end.q)) done = false;
-      }
-      end.accepted += !done;
-    }
+    if (decide<T>(args, rows, first, min(kTogether, rows.end - first), sums, 2u, states, &end)) break;
   }
   return end;
 }
@@ -469,9 +528,10 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void verify_weights_kernel(VerifyArgs args, uint32_t parts, uint32_t sequences) {
   __shared__ double scratch[kThreads / 64];
   __shared__ RowSum sums[kThreads / 16];
+  __shared__ uint32_t states[kThreads / 32];
   const uint32_t s = blockIdx.x, part_index = blockIdx.y, at = threadIdx.x;
   const Workspace work = bind(args, parts, sequences);
-  const End end = find_end<T>(args, work, s, parts, sums);
+  const End end = find_end<T>(args, work, s, parts, sums, states);
   if (part_index == 0 && at == 0) {
     args.accepted[s] = end.accepted;
     if (args.greedy || end.token == kNoToken) args.next_tokens[s] = end.token;
@@ -479,10 +539,16 @@ __global__ __launch_bounds__(kThreads) void verify_weights_kernel(VerifyArgs arg
   }
   if (args.greedy || end.token == kNoToken) return;
   const Weights<T> weights(args, end, end.draft != kNoToken);
-  const uint32_t first = part_index * kSpan<T>, last = min(args.columns, first + kSpan<T>);
+  constexpr int kRun = 16 / sizeof(T);
   double mine = 0.0;
-#pragma unroll 4
-  for (uint32_t i = first + at; i < last; i += kThreads) mine += weights(i);
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j) {
+    const uint32_t first = part_index * kSpan<T> + (j * kThreads + at) * kRun;
+    double w[kRun];
+    weights.run(first, args.columns > first ? args.columns - first : 0u, w);
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) mine += w[i];
+  }
   mine = reduce_group<kThreads>(mine, scratch, Add());
   if (at == 0) work.weights[(uint64_t)s * parts + part_index] = mine;
 }
@@ -544,9 +610,13 @@ __global__ __launch_bounds__(kSequence) void verify_token_kernel(VerifyArgs args
     if (at == 0) args.next_tokens[s] = kNoToken;
     return;
   }
-  const uint32_t first = found_part * kSpan<T>;
-  const uint32_t token = find_token<kSequence>(first, min(args.columns, first + kSpan<T>), found_before, want, scratch,
-                                               Weights<T>(args, end, residual));
+  constexpr int kRun = Weights<T>::kRun;
+  const uint32_t first = found_part * kSpan<T> + at * kRun;
+  double w[kRun], mine = 0.0;
+  Weights<T>(args, end, residual).run(first, args.columns > first ? args.columns - first : 0u, w);
+#pragma unroll
+  for (int i = 0; i < kRun; ++i) mine += w[i];
+  const uint32_t token = find_token(w, first, found_before + running_sum(mine, scratch).before, want, scratch);
   if (at == 0) args.next_tokens[s] = token;
 }
 
