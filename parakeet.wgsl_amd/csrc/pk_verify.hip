@@ -23,10 +23,14 @@ namespace {
 constexpr uint32_t kNoToken = 0xffffffffu;
 constexpr float kInf = __builtin_inff();
 constexpr int kThreads = 256;       // of a workgroup that holds a part of a row
-constexpr int kHeld = 4;            // pieces of 16 bytes of a part in a thread
+// Pieces of 16 bytes in a thread that sums a part of a row, and one that sums the
+// weights of a smaller part: those launches have fewer rows.
+constexpr int kSumsHeld = 8, kHeld = 4;
 constexpr int kSequence = 1024;     // threads of a workgroup that holds a sequence
 template <typename T>
-constexpr uint32_t kSpan = kThreads * kHeld * 16 / sizeof(T);  // columns of a part
+constexpr uint32_t kSumsSpan = kThreads * kSumsHeld * 16 / sizeof(T);  // columns of a part for the sums
+template <typename T>
+constexpr uint32_t kSpan = kThreads * kHeld * 16 / sizeof(T);          // and for the weights
 
 // 2^x, x <= 0 but for roundings, within 2^-45 of it: x less its nearest whole number goes
 // through a polynomial that meets 2^f at the 10 Chebyshev points of [-1/2, 1/2]; the whole number is
@@ -47,11 +51,46 @@ __device__ __forceinline__ double exp2_of(double x) {
   return x > -1000.0 ? all : 0.0;
 }
 
-// 2^((z - m) scale). The difference comes first: z * scale - m * scale in one operation less
-// loses all digits where logits of the size of f32's largest meet.
+// The many exponentials of a row, 2^((z - m) scale) within 2^-45: the whole number k of 512ths of
+// the exponent goes to the table of 2^(j / 512) in LDS, j = k mod 512, and to the exponent of what
+// it finds there, the rest, at most a 1024th, through the Taylor series up to its third power. The
+// table has j taken from its exponents already, so that k as it is can be added.
+constexpr int kTable = 512;
+// What is below stands for 0: a masked token has 2^-1000.
+constexpr double kLeast = 0x1p-990;
+template <int THREADS>
+__device__ __forceinline__ void make_table(double* table) {
+  for (int j = threadIdx.x; j < kTable; j += THREADS) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, 2.0 * exp2_of((double)(j - kTable) / kTable));
+    table[j] = __builtin_bit_cast(double, bits - ((uint64_t)j << 43));
+  }
+  __syncthreads();
+}
+template <typename T>
 struct Powers {
-  double m, scale;
-  __device__ __forceinline__ double at(float z) const { return exp2_of(((double)z - m) * scale); }
+  const double* table;
+  double m, scale, c;
+  double right;  // of the true power over at()
+  // f16: the exponent is one operation, z * scale - c, c the product of m and scale
+  // rounded, the same for every z; what that rounding left, below 2^-16, is put right for the
+  // whole row. f32: z - m first, since where logits are as large as f32's largest, c has no digits left.
+  __device__ Powers(const double* table, double m, double scale_of_one)
+      : table(table), m(m), scale(scale_of_one * kTable), c(m * scale) {
+    right = sizeof(T) == 2 ? exp2_of(-__builtin_fma(m, scale, -c) / kTable) : 1.0;
+  }
+  __device__ __forceinline__ double at(float z) const {
+#pragma clang fp contract(off)
+    const double exponent = sizeof(T) == 2 ? __builtin_fma((double)z, scale, -c) : ((double)z - m) * scale;
+    const double x = __builtin_fmax(exponent, -1000.0 * kTable);
+    constexpr double kWhole = 6755399441055744.0, kLn2 = 0.6931471805599453 / kTable;
+    const double shifted = x + kWhole, f = x - (shifted - kWhole);
+    const uint32_t k = (uint32_t)__builtin_bit_cast(uint64_t, shifted);
+    const uint64_t bits = __builtin_bit_cast(uint64_t, table[k % kTable]);
+    const uint32_t high = (uint32_t)(bits >> 32) + (k << 11);
+    const double power = __builtin_bit_cast(double, ((uint64_t)high << 32) | (uint32_t)bits);
+    const double rest = f * __builtin_fma(__builtin_fma(kLn2 * kLn2 * kLn2 / 6, f, kLn2 * kLn2 / 2), f, kLn2);
+    return __builtin_fma(power, rest, power);
+  }
 };
 
 // Up to N elements from `row` on, `count` of them there: 16 bytes at a time where they lie so.
@@ -143,18 +182,25 @@ struct End {
   RowSum p, q;
 };
 
-// Whether the draft of a row stands, given its sums.
-template <typename T>
-__device__ __forceinline__ bool stands(const VerifyArgs& args, uint32_t row, uint32_t draft, const RowSum& p, const RowSum& q) {
-  const T* z = static_cast<const T*>(args.target) + row * args.target_stride;
-  const double pd = exp2_of(((double)(float)z[draft] - p.m) * args.scale) / p.sum;
-  double qd = 1.0;
-  if (args.draft) {
-    const T* y = static_cast<const T*>(args.draft) + row * args.draft_stride;
-    qd = exp2_of(((double)(float)y[draft] - q.m) * args.scale) / q.sum;
+// What decides about a row but for its sums, which are on their way meanwhile.
+struct Judged {
+  uint32_t draft;
+  float uniform, target, drafted;  // and the draft's logits
+  template <typename T>
+  __device__ void load(const VerifyArgs& args, const Rows& rows, uint32_t row, T) {
+    uniform = target = drafted = 0.0f;
+    draft = row < rows.end ? rows.draft(args, row) : kNoToken;
+    if (draft >= args.columns || args.greedy) return;
+    uniform = args.uniforms[row];
+    target = (float)(static_cast<const T*>(args.target) + row * args.target_stride)[draft];
+    if (args.draft) drafted = (float)(static_cast<const T*>(args.draft) + row * args.draft_stride)[draft];
   }
-  return (double)args.uniforms[row] * qd < pd;
-}
+  __device__ bool stands(const VerifyArgs& args, const RowSum& p, const RowSum& q) const {
+    const double pd = exp2_of(((double)target - p.m) * args.scale) / p.sum;
+    const double qd = args.draft ? exp2_of(((double)drafted - q.m) * args.scale) / q.sum : 1.0;
+    return (double)uniform * qd < pd;
+  }
+};
 
 // The weights that the next token is drawn by.
 template <typename T>
@@ -162,29 +208,35 @@ struct Weights {
   static constexpr int kRun = kSpan<T> / kSequence;  // columns of a thread, of those that hold a sequence
   const T *z, *y;  // y null: no draft logits, or the last row
   uint32_t refused;
-  Powers p, q;
+  Powers<T> p, q;
   double inverse, draft_inverse;
   bool residual;
-  __device__ Weights(const VerifyArgs& args, const End& end, bool residual)
+  __device__ Weights(const VerifyArgs& args, const double* table, const End& end, bool residual)
       : z(static_cast<const T*>(args.target) + end.row * args.target_stride),
         y(args.draft && residual ? static_cast<const T*>(args.draft) + end.row * args.draft_stride : nullptr),
-        refused(end.draft), p{end.p.m, args.scale}, q{end.q.m, args.scale}, inverse(1.0 / end.p.sum),
-        draft_inverse(y ? 1.0 / end.q.sum : 0.0), residual(residual) {}
-  __device__ __forceinline__ double of(float target, float draft, uint32_t i) const {
+        refused(end.draft), p(table, end.p.m, args.scale), q(table, y ? end.q.m : 0.0, args.scale), inverse(p.right / end.p.sum),
+        draft_inverse(y ? q.right / end.q.sum : 0.0), residual(residual) {}
+  // `whole` gets the target's probability.
+  __device__ __forceinline__ double of(float target, float draft, uint32_t i, double* whole) const {
 #pragma clang fp contract(off)  // equal probabilities leave 0
     double w = p.at(target) * inverse;
+    *whole = w;
     if (y) w -= q.at(draft) * draft_inverse;
     else if (residual && i == refused) w -= 1.0;
-    return w > 0.0 ? w : 0.0;
+    return w > kLeast ? w : 0.0;
   }
   // Of N columns from `first` on, `count` of them there; the others' are 0.
   template <int N>
-  __device__ __forceinline__ void run(uint32_t first, uint32_t count, double (&w)[N]) const {
+  __device__ __forceinline__ void run(uint32_t first, uint32_t count, double (&w)[N], double* whole = nullptr) const {
     float target[N], draft[N];
     load_run<N>(z + first, count, target);
     if (y) load_run<N>(y + first, count, draft);
 #pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = (uint32_t)i < count ? of(target[i], y ? draft[i] : 0.0f, first + i) : 0.0;
+    for (int i = 0; i < N; ++i) {
+      double p = 0.0;
+      w[i] = (uint32_t)i < count ? of(target[i], y ? draft[i] : 0.0f, first + i, &p) : 0.0;
+      if (whole) *whole += p;
+    }
   }
 };
 
@@ -238,12 +290,11 @@ __device__ __forceinline__ uint32_t find_token(const double (&w)[N], uint32_t fi
 
 // The rows [first, first + count) of a sequence in turn, from their sums (`each` apart: of the target, and of the
 // draft behind it): where it ends, if it does. Threads decide a row each first.
-template <typename T>
-__device__ __forceinline__ bool decide(const VerifyArgs& args, const Rows& rows, uint32_t first, uint32_t count, const RowSum* sums,
-                                       uint32_t each, uint32_t* states, End* end) {
+__device__ __forceinline__ bool decide(const VerifyArgs& args, const Rows& rows, const Judged& judged, uint32_t first, uint32_t count,
+                                       const RowSum* sums, uint32_t each, uint32_t* states, End* end) {
   enum { kStands = 0, kDraws = 1, kNone = 2 };
-  if (threadIdx.x < count && first + threadIdx.x < rows.end) {
-    const uint32_t row = first + threadIdx.x, draft = rows.draft(args, row);
+  if (threadIdx.x < count) {
+    const uint32_t draft = judged.draft;
     const RowSum p = sums[threadIdx.x * each], q = sums[threadIdx.x * each + each - 1u];
     const bool last = draft >= args.columns;
     uint32_t state;
@@ -252,7 +303,7 @@ __device__ __forceinline__ bool decide(const VerifyArgs& args, const Rows& rows,
     } else if (has_none(p) || (!last && args.draft && has_none(q))) {
       state = kNone;
     } else {
-      state = !last && stands<T>(args, row, draft, p, q) ? kStands : kDraws;
+      state = !last && judged.stands(args, p, q) ? kStands : kDraws;
     }
     states[threadIdx.x] = state;
   }
@@ -277,7 +328,7 @@ __device__ __forceinline__ bool decide(const VerifyArgs& args, const Rows& rows,
 // A wavefront's sum of a whole row: pieces of kRun columns a lane, the row read
 // twice, the second time from the cache.
 template <typename T>
-__device__ __forceinline__ RowSum sum_row(const T* z, uint32_t columns, double scale, bool greedy) {
+__device__ __forceinline__ RowSum sum_row(const T* z, const double* table, uint32_t columns, double scale, bool greedy) {
   constexpr int kRun = 16 / sizeof(T), kPieces = 4;
   const uint32_t lane = threadIdx.x & 63u;
   // Calls use(value, column) for the columns that there are.
@@ -318,8 +369,9 @@ __device__ __forceinline__ RowSum sum_row(const T* z, uint32_t columns, double s
   if (__any(strange)) return row;
   double sum = 0.0;
   if (m > -kInf) {
-    const Powers powers = {row.m, scale};
+    const Powers<T> powers(table, row.m, scale);
     each([&](float v, uint32_t) { sum += powers.at(v); });
+    sum *= powers.right;
   }
   row.sum = reduce_lanes<64>(sum, Add());
   return row;
@@ -328,36 +380,40 @@ __device__ __forceinline__ RowSum sum_row(const T* z, uint32_t columns, double s
 template <typename T>
 __global__ __launch_bounds__(kSequence) void verify_sequence_kernel(VerifyArgs args) {
   constexpr uint32_t kWaves = kSequence / 64;
-  constexpr int kRun = Weights<T>::kRun;
+  constexpr int kRun = 16384 / sizeof(T) / kSequence;
   __shared__ double scratch[kWaves];
   __shared__ RowSum sums[kWaves];
   __shared__ uint32_t states[kWaves];
+  __shared__ double table[kTable];
   const uint32_t s = blockIdx.x, wave = threadIdx.x >> 6;
+  if (!args.greedy) make_table<kSequence>(table);
   const Rows rows(args, s);
   const bool two = args.draft && !args.greedy;
   const uint32_t each = two ? 2u : 1u;
   End end = {0, rows.start, kNoToken, kNoToken, {}, {}};
   for (uint32_t first = rows.start; first < rows.end; first += kWaves / each) {
     const uint32_t row = first + wave / each;
+    Judged judged;
+    judged.load(args, rows, threadIdx.x < kWaves / each ? first + threadIdx.x : rows.end, T());
     RowSum sum = {{0.0}, 0.0};
     if (row < rows.end) {
       // The row of a sequence's last token has no draft.
       const bool of_draft = two && (wave & 1u);
       const T* z = of_draft ? static_cast<const T*>(args.draft) + row * args.draft_stride
                             : static_cast<const T*>(args.target) + row * args.target_stride;
-      if (!of_draft || rows.draft(args, row) < args.columns) sum = sum_row(z, args.columns, args.scale, args.greedy);
+      if (!of_draft || rows.draft(args, row) < args.columns) sum = sum_row(z, table, args.columns, args.scale, args.greedy);
     }
     __syncthreads();
     if ((threadIdx.x & 63u) == 0) sums[wave] = sum;
     __syncthreads();
-    if (decide<T>(args, rows, first, min(kWaves / each, rows.end - first), sums, each, states, &end)) break;
+    if (decide(args, rows, judged, first, min(kWaves / each, rows.end - first), sums, each, states, &end)) break;
   }
   if (!args.greedy && end.token != kNoToken) {
     const uint32_t first = threadIdx.x * kRun, count = args.columns > first ? args.columns - first : 0u;
     double w[kRun];
     Running running;
     for (bool residual = end.draft != kNoToken;; residual = false) {
-      Weights<T>(args, end, residual).run(first, count, w);
+      Weights<T>(args, table, end, residual).run(first, count, w);
       double mine = 0.0;
 #pragma unroll
       for (int i = 0; i < kRun; ++i) mine += w[i];
@@ -377,19 +433,24 @@ __global__ __launch_bounds__(kSequence) void verify_sequence_kernel(VerifyArgs a
 // Memory of the op: for each row of target and draft the sums of its parts;
 // for each sequence where it ended, and the weights of the parts of that row.
 struct Workspace {
-  RowSum* sums;     // [rows][2][parts]
+  RowSum* sums;     // [rows][2][sums parts]
   End* ends;        // [sequences]
-  double* weights;  // [sequences][parts]
+  double2* weights;  // [sequences][parts]: of max(p - q, 0), and of p
 };
 template <typename T>
 __host__ __device__ uint32_t parts_of(uint32_t columns) {
   return (columns + kSpan<T> - 1u) / kSpan<T>;
 }
-__host__ __device__ Workspace bind(const VerifyArgs& args, uint64_t parts, uint64_t sequences) {
+template <typename T>
+__host__ __device__ uint32_t sums_parts_of(uint32_t columns) {
+  return (columns + kSumsSpan<T> - 1u) / kSumsSpan<T>;
+}
+template <typename T>
+__host__ __device__ Workspace bind(const VerifyArgs& args, uint64_t sequences) {
   Workspace w;
   w.sums = static_cast<RowSum*>(args.workspace);
-  w.ends = reinterpret_cast<End*>(w.sums + 2u * args.rows * parts);
-  w.weights = reinterpret_cast<double*>(w.ends + sequences);
+  w.ends = reinterpret_cast<End*>(w.sums + 2ull * args.rows * sums_parts_of<T>(args.columns));
+  w.weights = reinterpret_cast<double2*>(w.ends + sequences);
   return w;
 }
 
@@ -400,13 +461,29 @@ struct Part {
   static constexpr int VEC = 16 / sizeof(T);
   typedef T V __attribute__((ext_vector_type(VEC)));
   uint32_t first, head, vectors, tail;
-  __device__ Part(const T* row, uint32_t columns, uint32_t part) : first(part * kSpan<T>) {
-    const uint32_t size = min(kSpan<T>, columns - first);
+  __device__ Part(const T* row, uint32_t columns, uint32_t part) : first(part * kSumsSpan<T>) {
+    const uint32_t size = min(kSumsSpan<T>, columns - first);
     head = min(size, (uint32_t)(-reinterpret_cast<uintptr_t>(row + first) % 16u / sizeof(T)));
     vectors = (size - head) / VEC;
     tail = size - head - vectors * VEC;
   }
 };
+
+// Whether a row belongs to a sequence, and, of the draft's, is not a last one. Lanes look for the
+// last sequence that starts at or before it.
+__device__ __forceinline__ bool is_needed(const VerifyArgs& args, uint32_t row, bool of_draft) {
+  const uint32_t lane = threadIdx.x & 63u;
+  uint32_t low = 0, count = args.sequences;
+  while (count > 1u) {
+    const uint32_t step = (count + 63u) / 64u, at = lane * step;
+    const bool before = at < count && args.row_starts[low + at] <= row;
+    const uint32_t last = 63u - (uint32_t)__builtin_clzll(__ballot(before) | 1ull);
+    low += last * step;
+    count = min(step, count - last * step);
+  }
+  const Rows rows(args, low);
+  return row >= rows.start && row < rows.end && (!of_draft || rows.draft(args, row) < args.columns);
+}
 
 // The sums of a part of a row.
 template <typename T>
@@ -414,15 +491,15 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs args, 
   typedef typename Part<T>::V V;
   constexpr int VEC = Part<T>::VEC;
   __shared__ double scratch[kThreads / 64];
-  __shared__ uint32_t needed;
+  __shared__ double table[kTable];
   const uint32_t at = threadIdx.x, row = blockIdx.x, which = blockIdx.y / parts, part_index = blockIdx.y - which * parts;
   const T* z = which ? static_cast<const T*>(args.draft) + row * args.draft_stride
                      : static_cast<const T*>(args.target) + row * args.target_stride;
   const Part<T> part(z, args.columns, part_index);
   const V* body = reinterpret_cast<const V*>(z + part.first + part.head);
-  V held[kHeld];
+  V held[kSumsHeld];
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) {
+  for (int i = 0; i < kSumsHeld; ++i) {
     const uint32_t v = at + i * kThreads;
     if (v < part.vectors) held[i] = body[v];
     else
@@ -431,20 +508,14 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs args, 
   }
   const uint32_t edge = part.first + (at < part.head ? at : part.head + part.vectors * VEC + (at - part.head));
   const float single = at < part.head + part.tail ? (float)z[edge] : -kInf;
-  // A row of no sequence, or the draft's of a last one, is not asked for.
-  if (at == 0) needed = 0;
-  __syncthreads();
-  for (uint32_t s = at; s < args.sequences; s += kThreads) {
-    const Rows rows(args, s);
-    if (row >= rows.start && row < rows.end && (!which || rows.draft(args, row) < args.columns)) needed = 1;
-  }
-  __syncthreads();
+  const bool needed = is_needed(args, row, which);
+  make_table<kThreads>(table);
   if (!needed) return;
   RowSum sum;
   if (args.greedy) {
     unsigned long long best = at < part.head + part.tail ? key_of(single, edge) : 0;
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i)
+    for (int i = 0; i < kSumsHeld; ++i)
 #pragma unroll
       for (int c = 0; c < VEC; ++c)
         best = Larger()(best, (unsigned long long)key_of((float)held[i][c], part.first + part.head + (at + i * kThreads) * VEC + c));
@@ -454,29 +525,35 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs args, 
     float m = single;
     bool strange = !(single < kInf);
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i)
+    for (int i = 0; i < kSumsHeld; ++i)
 #pragma unroll
       for (int c = 0; c < VEC; ++c) {
         strange |= !((float)held[i][c] < kInf);
         m = fmaxf(m, (float)held[i][c]);
       }
     // Plus infinity stands for what is no number.
-    m = reduce_group<kThreads>(__any(strange) ? kInf : wave::max(m), scratch, Larger());
+    float* tops = reinterpret_cast<float*>(scratch);
+    m = __any(strange) ? kInf : wave::max(m);
+    if ((at & 63u) == 0) tops[at >> 6] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) m = fmaxf(m, tops[w]);
     sum.m = m;
     double mine = 0.0;
     if (m > -kInf && m < kInf) {
-      const Powers powers = {sum.m, args.scale};
+      const Powers<T> powers(table, sum.m, args.scale);
       mine = powers.at(single);
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i)
+      for (int i = 0; i < kSumsHeld; ++i)
         if (at + i * kThreads < part.vectors)
 #pragma unroll
           for (int c = 0; c < VEC; ++c) mine += powers.at((float)held[i][c]);
+      mine *= powers.right;
     }
     sum.sum = reduce_group<kThreads>(mine, scratch, Add());
     if (m == kInf) sum.sum = -1.0;
   }
-  if (at == 0) bind(args, parts, 0).sums[((uint64_t)row * 2 + which) * parts + part_index] = sum;
+  if (at == 0) bind<T>(args, 0).sums[((uint64_t)row * 2 + which) * parts + part_index] = sum;
 }
 
 // Where a sequence ends: groups of 16 lanes join the parts of a row each, 8 rows at a time,
@@ -491,6 +568,8 @@ __device__ __forceinline__ End find_end(const VerifyArgs& args, const Workspace&
   for (uint32_t first = rows.start; first < rows.end; first += kTogether) {
     const uint32_t row = first + group / 2, which = group & 1u;
     const bool needed = row < rows.end && (!which || (args.draft && !args.greedy && rows.draft(args, row) < args.columns));
+    Judged judged;
+    judged.load(args, rows, threadIdx.x < kTogether ? first + threadIdx.x : rows.end, T());
     RowSum sum = {{0.0}, 0.0};
     const RowSum* from = work.sums + ((uint64_t)row * 2 + which) * parts;
     if (args.greedy) {
@@ -518,7 +597,7 @@ __device__ __forceinline__ End find_end(const VerifyArgs& args, const Workspace&
     __syncthreads();
     if (lane == 0) sums[group] = sum;
     __syncthreads();
-    if (decide<T>(args, rows, first, min(kTogether, rows.end - first), sums, 2u, states, &end)) break;
+    if (decide(args, rows, judged, first, min(kTogether, rows.end - first), sums, 2u, states, &end)) break;
   }
   return end;
 }
@@ -529,28 +608,31 @@ __global__ __launch_bounds__(kThreads) void verify_weights_kernel(VerifyArgs arg
   __shared__ double scratch[kThreads / 64];
   __shared__ RowSum sums[kThreads / 16];
   __shared__ uint32_t states[kThreads / 32];
+  __shared__ double table[kTable];
+  make_table<kThreads>(table);
   const uint32_t s = blockIdx.x, part_index = blockIdx.y, at = threadIdx.x;
-  const Workspace work = bind(args, parts, sequences);
-  const End end = find_end<T>(args, work, s, parts, sums, states);
+  const Workspace work = bind<T>(args, sequences);
+  const End end = find_end<T>(args, work, s, sums_parts_of<T>(args.columns), sums, states);
   if (part_index == 0 && at == 0) {
     args.accepted[s] = end.accepted;
     if (args.greedy || end.token == kNoToken) args.next_tokens[s] = end.token;
     work.ends[s] = end;
   }
   if (args.greedy || end.token == kNoToken) return;
-  const Weights<T> weights(args, end, end.draft != kNoToken);
+  const Weights<T> weights(args, table, end, end.draft != kNoToken);
   constexpr int kRun = 16 / sizeof(T);
-  double mine = 0.0;
+  double mine = 0.0, all = 0.0;
 #pragma unroll
   for (int j = 0; j < kHeld; ++j) {
     const uint32_t first = part_index * kSpan<T> + (j * kThreads + at) * kRun;
     double w[kRun];
-    weights.run(first, args.columns > first ? args.columns - first : 0u, w);
+    weights.run(first, args.columns > first ? args.columns - first : 0u, w, &all);
 #pragma unroll
     for (int i = 0; i < kRun; ++i) mine += w[i];
   }
   mine = reduce_group<kThreads>(mine, scratch, Add());
-  if (at == 0) work.weights[(uint64_t)s * parts + part_index] = mine;
+  all = reduce_group<kThreads>(all, scratch, Add());
+  if (at == 0) work.weights[(uint64_t)s * parts + part_index] = make_double2(mine, all);
 }
 
 // Finds the part of the row whose weights the draw ends in, and in it the token.
@@ -559,17 +641,18 @@ __global__ __launch_bounds__(kSequence) void verify_token_kernel(VerifyArgs args
   __shared__ double scratch[kSequence / 64];
   __shared__ double found_before;
   __shared__ uint32_t found_part;
+  __shared__ double table[kTable];
+  make_table<kSequence>(table);
   const uint32_t s = blockIdx.x, at = threadIdx.x;
-  const Workspace work = bind(args, parts, sequences);
+  const Workspace work = bind<T>(args, sequences);
   const End end = work.ends[s];
   if (end.token == kNoToken) return;
   bool residual = end.draft != kNoToken;
   // The parts' weights: of p - q, or of p where that is nothing.
   double whole = 0.0;
   const auto part_weight = [&](uint32_t i) {
-    if (residual || end.draft == kNoToken) return work.weights[(uint64_t)s * parts + i];
-    const RowSum p = work.sums[(uint64_t)end.row * 2 * parts + i];
-    return scaled(p.m, p.sum, end.p.m, args.scale) / end.p.sum;
+    const double2 w = work.weights[(uint64_t)s * parts + i];
+    return residual ? w.x : w.y;
   };
   for (;;) {
     double mine = 0.0;
@@ -613,17 +696,17 @@ __global__ __launch_bounds__(kSequence) void verify_token_kernel(VerifyArgs args
   constexpr int kRun = Weights<T>::kRun;
   const uint32_t first = found_part * kSpan<T> + at * kRun;
   double w[kRun], mine = 0.0;
-  Weights<T>(args, end, residual).run(first, args.columns > first ? args.columns - first : 0u, w);
+  Weights<T>(args, table, end, residual).run(first, args.columns > first ? args.columns - first : 0u, w);
 #pragma unroll
   for (int i = 0; i < kRun; ++i) mine += w[i];
   const uint32_t token = find_token(w, first, found_before + running_sum(mine, scratch).before, want, scratch);
   if (at == 0) args.next_tokens[s] = token;
 }
 
-// Rows of a part each are read by one workgroup for a sequence, unless it has many.
+// Rows of up to 16 KiB are read by one workgroup for a sequence, unless it has many.
 template <typename T>
 bool together(const VerifyArgs& args) {
-  return parts_of<T>(args.columns) == 1u && args.rows <= 64ull * args.sequences;
+  return args.columns * sizeof(T) <= 16384u && args.rows <= 64ull * args.sequences;
 }
 
 template <typename Kernel, typename... Args>
@@ -642,8 +725,9 @@ hipError_t launch_typed(const VerifyArgs& args, hipStream_t stream, hipEvent_t s
   if (!args.workspace) return hipErrorInvalidValue;
   const uint32_t parts = parts_of<T>(args.columns), sequences = args.sequences;
   const bool two = args.draft && !args.greedy;
-  if (const hipError_t e = launch(verify_sums_kernel<T>, dim3(args.rows, parts * (two ? 2u : 1u)), dim3(kThreads), stream,
-                                  start, nullptr, args, parts))
+  const uint32_t sums_parts = sums_parts_of<T>(args.columns);
+  if (const hipError_t e = launch(verify_sums_kernel<T>, dim3(args.rows, sums_parts * (two ? 2u : 1u)), dim3(kThreads), stream,
+                                  start, nullptr, args, sums_parts))
     return e;
   const hipError_t e = launch(verify_weights_kernel<T>, dim3(sequences, args.greedy ? 1u : parts), dim3(kThreads), stream,
                               nullptr, args.greedy ? stop : nullptr, args, parts, sequences);
@@ -658,7 +742,7 @@ uint64_t workspace_typed(const VerifyArgs& args) {
   one.sequences = 1;
   if (together<T>(one)) return 0;
   const uint64_t parts = parts_of<T>(args.columns);
-  return 2u * args.rows * parts * sizeof(RowSum) + args.sequences * (sizeof(End) + parts * sizeof(double));
+  return 2ull * args.rows * sums_parts_of<T>(args.columns) * sizeof(RowSum) + args.sequences * (sizeof(End) + parts * sizeof(double2));
 }
 
 }  // namespace
