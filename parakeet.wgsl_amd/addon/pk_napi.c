@@ -5,8 +5,9 @@
  * (include/pk_attention.h), the row LayerNorm (include/pk_layernorm.h), the
  * subsampling convolutions (include/pk_subsampling.h), the encoder graph
  * (include/pk_encoder.h), the norms around a block (include/pk_block_norm.h),
- * the 4-bit product (include/pk_q4.h) and token scores
- * (include/pk_score.h). It is the thin native layer under the JavaScript
+ * the 4-bit product (include/pk_q4.h), token scores
+ * (include/pk_score.h), the paged cache (include/pk_cache.h) and the
+ * verification of drafted tokens (include/pk_verify.h). It is the thin native layer under the JavaScript
  * host in ../host: every function forwards to one pk_* call, converts device
  * pointers to BigInt, and turns a failing pk_status into a thrown Error
  * (RangeError for PK_RANGE_ERROR, as the reference throws RangeError for
@@ -27,6 +28,7 @@
 
 #include "pk_attention.h"
 #include "pk_block_norm.h"
+#include "pk_cache.h"
 #include "pk_conv.h"
 #include "pk_encoder.h"
 #include "pk_layernorm.h"
@@ -35,6 +37,7 @@
 #include "pk_score.h"
 #include "pk_subsampling.h"
 #include "pk_tdt.h"
+#include "pk_verify.h"
 
 #define NAPI_CALL(env, call)                                              \
   do {                                                                    \
@@ -876,6 +879,12 @@ static int optional_u32(napi_env env, napi_value o, const char *name, uint32_t *
   return bad_field(env, name, "a non-negative 32-bit integer");
 }
 
+static int optional_u64(napi_env env, napi_value o, const char *name, uint64_t *out) {
+  napi_value v;
+  if (!prop(env, o, name, &v) || get_u64(env, v, out)) return 1;
+  return bad_field(env, name, "a non-negative integer");
+}
+
 /* *has tells whether it is there. */
 static int optional_float(napi_env env, napi_value o, const char *name, int32_t *has, float *out) {
   napi_value v;
@@ -1001,8 +1010,116 @@ static int parse_score_desc(napi_env env, napi_value o, pk_score_desc *d, char *
   return 1;
 }
 
+/* The fields that cache append and cache attention share: {rows, sequences,
+   heads?, kvHeads, headDim, queries?, queryStride?, rowStarts, lengths,
+   pageTable, pagesPerSequence, pages, pageSize, pageStride?, keyCache,
+   valueCache}, each binding with its Bytes */
+#define PARSE_CACHE(env, o, d)                                                                     \
+  (optional_u32(env, o, "heads", &(d)->heads) &&                                                   \
+   optional_binding(env, o, "queries", &(d)->queries, &(d)->queries_bytes) &&                      \
+   optional_u32(env, o, "queryStride", &(d)->query_stride) &&                                      \
+   optional_binding(env, o, "rowStarts", &(d)->row_starts, &(d)->row_starts_bytes) &&              \
+   optional_binding(env, o, "lengths", &(d)->lengths, &(d)->lengths_bytes) &&                      \
+   optional_binding(env, o, "pageTable", &(d)->page_table, &(d)->page_table_bytes) &&              \
+   optional_u64(env, o, "pageStride", &(d)->page_stride) &&                                        \
+   optional_binding(env, o, "keyCache", &(d)->key_cache, &(d)->key_cache_bytes) &&                 \
+   optional_binding(env, o, "valueCache", &(d)->value_cache, &(d)->value_cache_bytes))
+#define HAS_CACHE_SHAPE(env, o, d)                                                                 \
+  (prop_u32(env, o, "rows", &(d)->rows) && prop_u32(env, o, "sequences", &(d)->sequences) &&       \
+   prop_u32(env, o, "kvHeads", &(d)->kv_heads) && prop_u32(env, o, "headDim", &(d)->head_dim) &&   \
+   prop_u32(env, o, "pagesPerSequence", &(d)->pages_per_sequence) &&                               \
+   prop_u32(env, o, "pages", &(d)->pages) && prop_u32(env, o, "pageSize", &(d)->page_size))
+
+/* {label, precision, the cache's fields, queryOutput?, queryOutputStride?,
+   keys, keyStride?, values, valueStride?, rotaryDim?, rotary?, frequencies?,
+   positions?}, each binding with its Bytes */
+static int parse_cache_append_desc(napi_env env, napi_value o, pk_cache_append_desc *d, char **label) {
+  memset(d, 0, sizeof *d);
+  d->struct_size = sizeof *d;
+  *label = NULL;
+  parse_precision(env, o, &d->precision);
+  if (!HAS_CACHE_SHAPE(env, o, d)) {
+    bad_argument(env, "cache append descriptor is missing a required field");
+    return 0;
+  }
+  uint32_t rotary = 0;
+  if (!PARSE_CACHE(env, o, d) ||
+      !optional_binding(env, o, "queryOutput", &d->query_output, &d->query_output_bytes) ||
+      !optional_u32(env, o, "queryOutputStride", &d->query_output_stride) ||
+      !optional_binding(env, o, "keys", &d->keys, &d->keys_bytes) ||
+      !optional_u32(env, o, "keyStride", &d->key_stride) ||
+      !optional_binding(env, o, "values", &d->values, &d->values_bytes) ||
+      !optional_u32(env, o, "valueStride", &d->value_stride) ||
+      !optional_u32(env, o, "rotaryDim", &d->rotary_dim) || !optional_u32(env, o, "rotary", &rotary) ||
+      !optional_binding(env, o, "frequencies", &d->frequencies, &d->frequencies_bytes) ||
+      !optional_binding(env, o, "positions", &d->positions, &d->positions_bytes))
+    return 0;
+  d->rotary = (int32_t)rotary;
+  *label = prop_string(env, o, "label");
+  d->label = *label;
+  return 1;
+}
+
+/* {label, precision, the cache's fields, output, outputStride?, causal?,
+   window?, scale?, scoreCap?}, each binding with its Bytes */
+static int parse_cache_attention_desc(napi_env env, napi_value o, pk_cache_attention_desc *d, char **label) {
+  memset(d, 0, sizeof *d);
+  d->struct_size = sizeof *d;
+  *label = NULL;
+  parse_precision(env, o, &d->precision);
+  if (!HAS_CACHE_SHAPE(env, o, d)) {
+    bad_argument(env, "cache attention descriptor is missing a required field");
+    return 0;
+  }
+  uint32_t causal = 1;
+  int32_t capped = 0;
+  if (!PARSE_CACHE(env, o, d) || !optional_binding(env, o, "output", &d->output, &d->output_bytes) ||
+      !optional_u32(env, o, "outputStride", &d->output_stride) || !optional_u32(env, o, "causal", &causal) ||
+      !optional_u32(env, o, "window", &d->window) || !optional_float(env, o, "scale", &d->has_scale, &d->scale) ||
+      !optional_float(env, o, "scoreCap", &capped, &d->score_cap))
+    return 0;
+  d->causal = causal > 1 ? -1 : (int32_t)causal;
+  *label = prop_string(env, o, "label");
+  d->label = *label;
+  return 1;
+}
+
+/* {label, precision, mode?, rows, sequences, columns, target, targetStride?,
+   draft?, draftStride?, temperature?, rowStarts, tokens, uniforms?, draws?,
+   accepted, nextTokens}, each binding with its Bytes */
+static int parse_verify_desc(napi_env env, napi_value o, pk_verify_desc *d, char **label) {
+  memset(d, 0, sizeof *d);
+  d->struct_size = sizeof *d;
+  *label = NULL;
+  parse_precision(env, o, &d->precision);
+  if (!prop_u32(env, o, "rows", &d->rows) || !prop_u32(env, o, "sequences", &d->sequences) ||
+      !prop_u32(env, o, "columns", &d->columns)) {
+    bad_argument(env, "draft verification descriptor is missing a required field");
+    return 0;
+  }
+  uint32_t mode = 0;
+  if (!optional_u32(env, o, "mode", &mode) ||
+      !optional_binding(env, o, "target", &d->target, &d->target_bytes) ||
+      !optional_u32(env, o, "targetStride", &d->target_stride) ||
+      !optional_binding(env, o, "draft", &d->draft, &d->draft_bytes) ||
+      !optional_u32(env, o, "draftStride", &d->draft_stride) ||
+      !optional_float(env, o, "temperature", &d->has_temperature, &d->temperature) ||
+      !optional_binding(env, o, "rowStarts", &d->row_starts, &d->row_starts_bytes) ||
+      !optional_binding(env, o, "tokens", &d->tokens, &d->tokens_bytes) ||
+      !optional_binding(env, o, "uniforms", &d->uniforms, &d->uniforms_bytes) ||
+      !optional_binding(env, o, "draws", &d->draws, &d->draws_bytes) ||
+      !optional_binding(env, o, "accepted", &d->accepted, &d->accepted_bytes) ||
+      !optional_binding(env, o, "nextTokens", &d->next_tokens, &d->next_tokens_bytes))
+    return 0;
+  d->mode = mode > 1 ? -1 : (int32_t)mode;
+  *label = prop_string(env, o, "label");
+  d->label = *label;
+  return 1;
+}
+
 /* finalize, validate(desc), enqueue(op, activeRows, stream?, startEvent?,
-   endEvent?) and destroy(op) of the ops above */
+   endEvent?) and destroy(op) of the ops above (of the paged cache and the
+   verification: activeSequences) */
 #define ROWS_OP(name)                                                                              \
   static void name##_finalize(napi_env env, void *data, void *hint) {                              \
     (void)env;                                                                                     \
@@ -1025,7 +1142,7 @@ static int parse_score_desc(napi_env env, napi_value o, pk_score_desc *d, char *
     uint32_t rows = 0;                                                                             \
     if (!get_args(env, info, 5, argv)) return NULL;                                                \
     if (!is_nullish(env, argv[1]) && !get_u32(env, argv[1], &rows))                                \
-      return bad_argument(env, "active rows must be a non-negative integer");                      \
+      return bad_argument(env, "active " ACTIVE_##name " must be a non-negative integer");         \
     PK_CALL(env, pk_##name##_enqueue_timed((pk_##name##_op *)get_external(env, argv[0]), rows,     \
                                            get_external(env, argv[2]), get_external(env, argv[3]), \
                                            get_external(env, argv[4])));                           \
@@ -1054,9 +1171,21 @@ static int parse_score_desc(napi_env env, napi_value o, pk_score_desc *d, char *
 #define CREATE_block_norm(ctx, d, op) pk_block_norm_create(ctx, d, op)
 #define CREATE_q4(ctx, d, op) pk_q4_create(ctx, d, NULL, op)
 #define CREATE_score(ctx, d, op) pk_score_create(ctx, d, op)
+#define CREATE_cache_append(ctx, d, op) pk_cache_append_create(ctx, d, op)
+#define CREATE_cache_attention(ctx, d, op) pk_cache_attention_create(ctx, d, op)
+#define CREATE_verify(ctx, d, op) pk_verify_create(ctx, d, op)
+#define ACTIVE_block_norm "rows"
+#define ACTIVE_q4 "rows"
+#define ACTIVE_score "rows"
+#define ACTIVE_cache_append "sequences"
+#define ACTIVE_cache_attention "sequences"
+#define ACTIVE_verify "sequences"
 ROWS_OP(block_norm)
 ROWS_OP(q4)
 ROWS_OP(score)
+ROWS_OP(cache_append)
+ROWS_OP(cache_attention)
+ROWS_OP(verify)
 
 /* ---- row LayerNorm ------------------------------------------------------- */
 
@@ -1820,6 +1949,18 @@ static napi_value init(napi_env env, napi_value exports) {
       {"scoreCreate", js_score_create},
       {"scoreEnqueue", js_score_enqueue},
       {"scoreDestroy", js_score_destroy},
+      {"cacheAppendValidate", js_cache_append_validate},
+      {"cacheAppendCreate", js_cache_append_create},
+      {"cacheAppendEnqueue", js_cache_append_enqueue},
+      {"cacheAppendDestroy", js_cache_append_destroy},
+      {"cacheAttentionValidate", js_cache_attention_validate},
+      {"cacheAttentionCreate", js_cache_attention_create},
+      {"cacheAttentionEnqueue", js_cache_attention_enqueue},
+      {"cacheAttentionDestroy", js_cache_attention_destroy},
+      {"verifyValidate", js_verify_validate},
+      {"verifyCreate", js_verify_create},
+      {"verifyEnqueue", js_verify_enqueue},
+      {"verifyDestroy", js_verify_destroy},
       {"subsamplingOutputDimension", js_subsampling_output_dimension},
       {"subsamplingValidLength", js_subsampling_valid_length},
       {"subsamplingValidate", js_subsampling_validate},

@@ -515,6 +515,142 @@ export declare class TokenScoreKernel {
 
 export declare const SCORE_NO_TOKEN: number;
 
+/* ---- Paged cache, draft verification (no counterpart in the reference) ---- */
+
+/** A dispatch over the rows of sequences; shape.batchSize selects the active sequences. */
+export declare class SequencesDispatch extends RowsDispatch {}
+
+/** A cache [pages][kvHeads][pageSize][headDim], and where its sequences lie in it. */
+export interface PagedCache {
+  /** u32 [sequences + 1]: the first row of each sequence of the batch. */
+  readonly rowStarts: ArenaSlice;
+  /** u32 [sequences]: tokens of each, its rows of this batch among them. */
+  readonly lengths: ArenaSlice;
+  /** u32 [sequences, pagesPerSequence]; CACHE_NO_PAGE: none. */
+  readonly pageTable: ArenaSlice;
+  readonly pagesPerSequence: number;
+  readonly pages: number;
+  /** Tokens, 1 to 65536. */
+  readonly pageSize: number;
+  /** Elements from page to page, a multiple of 8; default packed. */
+  readonly pageStride?: number;
+  /** Aligned to 16 bytes. */
+  readonly keys: ArenaSlice;
+  readonly values: ArenaSlice;
+}
+
+/** Rotated queries to queryOutput, rotated keys and values of new tokens into the cache. */
+export interface CacheAppendDescriptor {
+  readonly label: string;
+  /** Rows that the bindings hold. */
+  readonly rows: number;
+  readonly sequences: number;
+  /** Of the queries; default 0: none. */
+  readonly heads?: number;
+  readonly kvHeads: number;
+  /** A multiple of 8 up to 256. */
+  readonly headDim: number;
+  readonly queries?: ArenaSlice;
+  readonly queryStride?: number;
+  /** May be the queries' slice. */
+  readonly queryOutput?: ArenaSlice;
+  readonly queryOutputStride?: number;
+  readonly keys: ArenaSlice;
+  readonly keyStride?: number;
+  readonly values: ArenaSlice;
+  readonly valueStride?: number;
+  /** Default 0: no rotation. */
+  readonly rotaryDim?: number;
+  /** Elements j and rotaryDim / 2 + j, or 2 j and 2 j + 1, are a pair; default "halves". */
+  readonly rotary?: "halves" | "neighbours";
+  /** f32 [rotaryDim / 2] radians per position. */
+  readonly frequencies?: ArenaSlice | GpuTensor;
+  /** u32 [rows]; default: the positions in the sequences. */
+  readonly positions?: ArenaSlice;
+  readonly cache: PagedCache;
+}
+
+export declare class CacheAppendKernel {
+  static create(device: HipGpuDevice, arena: GpuActivationArena,
+                executionProfile?: { precision: "fp16" | "fp32" }): Promise<CacheAppendKernel>;
+  validateDescriptor(descriptor: CacheAppendDescriptor): void;
+  createDispatch(descriptor: CacheAppendDescriptor): SequencesDispatch;
+  destroy(): void;
+}
+
+/** Attention of new tokens over the cache: softmax(scale q . k, capped) . v. */
+export interface CacheAttentionDescriptor {
+  readonly label: string;
+  readonly rows: number;
+  readonly sequences: number;
+  /** A multiple of kvHeads. */
+  readonly heads: number;
+  readonly kvHeads: number;
+  readonly headDim: number;
+  readonly queries: ArenaSlice;
+  readonly queryStride?: number;
+  readonly output: ArenaSlice;
+  readonly outputStride?: number;
+  /** Default true: a row sees tokens up to its own position; false: all. */
+  readonly causal?: boolean;
+  /** Of these the last so many; default 0: all. */
+  readonly window?: number;
+  /** Default 1 / sqrt(headDim). */
+  readonly scale?: number;
+  /** Scores become scoreCap * tanh(score / scoreCap); default 0: they do not. */
+  readonly scoreCap?: number;
+  readonly cache: PagedCache;
+}
+
+export declare class CacheAttentionKernel {
+  static create(device: HipGpuDevice, arena: GpuActivationArena,
+                executionProfile?: { precision: "fp16" | "fp32" }): Promise<CacheAttentionKernel>;
+  validateDescriptor(descriptor: CacheAttentionDescriptor): void;
+  createDispatch(descriptor: CacheAttentionDescriptor): SequencesDispatch;
+  destroy(): void;
+}
+
+export declare const CACHE_NO_PAGE: number;
+
+/** How many drafted tokens stand against the target's logits, and the token that follows. */
+export interface DraftVerifyDescriptor {
+  readonly label: string;
+  /** Default "sample". */
+  readonly mode?: "sample" | "greedy";
+  readonly rows: number;
+  readonly sequences: number;
+  readonly columns: number;
+  readonly target: ArenaSlice;
+  readonly targetStride?: number;
+  /** What the token of the next row was drawn from; default: drafts that were not drawn. */
+  readonly draft?: ArenaSlice;
+  readonly draftStride?: number;
+  /** Default 1. */
+  readonly temperature?: number;
+  /** u32 [sequences + 1]. */
+  readonly rowStarts: ArenaSlice;
+  /** u32 [rows]; each row but a sequence's last judges the next one's token. */
+  readonly tokens: ArenaSlice;
+  /** f32 [rows] of [0, 1), with mode "sample". */
+  readonly uniforms?: ArenaSlice;
+  /** f32 [sequences] of [0, 1), with mode "sample". */
+  readonly draws?: ArenaSlice;
+  /** u32 [sequences]. */
+  readonly accepted: ArenaSlice;
+  /** u32 [sequences]; VERIFY_NO_TOKEN where a row has no probabilities. */
+  readonly nextTokens: ArenaSlice;
+}
+
+export declare class DraftVerifyKernel {
+  static create(device: HipGpuDevice, arena: GpuActivationArena,
+                executionProfile?: { precision: "fp16" | "fp32" }): Promise<DraftVerifyKernel>;
+  validateDescriptor(descriptor: DraftVerifyDescriptor): void;
+  createDispatch(descriptor: DraftVerifyDescriptor): SequencesDispatch;
+  destroy(): void;
+}
+
+export declare const VERIFY_NO_TOKEN: number;
+
 /* ---- Subsampling front end (src/webgpu/kernels/subsampling.ts) ---- */
 
 /** subsampling.ts:119-122 */

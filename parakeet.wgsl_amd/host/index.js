@@ -35,6 +35,11 @@
  *                                      block with gate and residual, products
  *                                      with 4-bit weights, token scores
  *                                      (include/pk_block_norm.h, pk_q4.h, pk_score.h)
+ *   CacheAppendKernel, CacheAttentionKernel, DraftVerifyKernel, SequencesDispatch
+ *                                      no counterpart: keys and values of new
+ *                                      tokens into a paged cache, attention
+ *                                      over it, the verification of drafted
+ *                                      tokens (include/pk_cache.h, pk_verify.h)
  *   FusedSubsamplingConv0Depthwise2Kernel, DepthwiseSubsamplingKernel,
  *   SubsamplingTimeMaskKernel, SubsamplingDispatch,
  *   subsamplingOutputDimension / subsamplingValidLength
@@ -1323,6 +1328,111 @@ class TokenScoreKernel extends RowsKernel {
 /** A token of a padded position, and of a place behind the last alternative. */
 const SCORE_NO_TOKEN = 0xffffffff;
 
+/** A dispatch over the rows of sequences. */
+class SequencesDispatch extends RowsDispatch {
+  /** shape.batchSize selects the active sequences. */
+  encode(encoder, timestampWrites, shape) {
+    if (this.destroyed) throw new Error(`${this.label} was destroyed`);
+    const active = shape === undefined || shape.batchSize === undefined ? this.rows : shape.batchSize;
+    if (!isSafe(active) || active <= 0 || active > this.rows)
+      throw new RangeError(`${this.label} active sequences must be in [1, ${this.rows}]`);
+    super.encode(encoder, timestampWrites, { rows: active });
+  }
+}
+
+/** A kernel whose dispatches are SequencesDispatch. */
+class SequencesKernel extends RowsKernel {
+  createDispatch(descriptor) {
+    if (this.destroyed) throw new Error(`Parakeet ${this.what} kernel was destroyed`);
+    const op = native()[`${this.prefix}Create`](this.device.context, this.nativeDescriptor(descriptor));
+    return new SequencesDispatch(descriptor.label, this.result(descriptor), op, descriptor.sequences, this.prefix);
+  }
+
+  /** The fields of `descriptor.cache` and of the rows over it. */
+  cacheOf(descriptor) {
+    const { label } = descriptor, cache = descriptor.cache || {};
+    const sizes = Object.assign({ label }, cache), pageStride = cache.pageStride;
+    if (pageStride !== undefined && (!isSafe(pageStride) || pageStride < 0))
+      throw new RangeError(`${label} pageStride must be a non-negative integer`);
+    return Object.assign(
+      this.sizesOf(descriptor, ["rows", "sequences", "heads", "kvHeads", "headDim", "queryStride"]),
+      this.sizesOf(sizes, ["pagesPerSequence", "pages", "pageSize"]), pageStride === undefined ? {} : { pageStride },
+      this.bindingOf("queries", descriptor.queries), this.bindingOf("rowStarts", cache.rowStarts),
+      this.bindingOf("lengths", cache.lengths), this.bindingOf("pageTable", cache.pageTable),
+      this.bindingOf("keyCache", cache.keys), this.bindingOf("valueCache", cache.values));
+  }
+}
+
+class CacheAppendKernel extends SequencesKernel {
+  static create(device, arena, executionProfile) {
+    return Promise.resolve(new CacheAppendKernel(device, arena, executionProfile));
+  }
+
+  get prefix() { return "cacheAppend"; }
+  get what() { return "cache append"; }
+  result(descriptor) { return descriptor.queryOutput; }
+
+  nativeDescriptor(descriptor) {
+    const { label } = descriptor;
+    const rotary = { halves: 0, neighbours: 1 }[descriptor.rotary === undefined ? "halves" : descriptor.rotary];
+    if (rotary === undefined) throw new Error(`${label} has an unsupported rotary kind ${descriptor.rotary}`);
+    return Object.assign(
+      { label, precision: this.precision, rotary }, this.cacheOf(descriptor),
+      this.sizesOf(descriptor, ["queryOutputStride", "keyStride", "valueStride", "rotaryDim"]),
+      this.bindingOf("queryOutput", descriptor.queryOutput), this.bindingOf("keys", descriptor.keys),
+      this.bindingOf("values", descriptor.values), this.bindingOf("frequencies", descriptor.frequencies),
+      this.bindingOf("positions", descriptor.positions));
+  }
+}
+
+class CacheAttentionKernel extends SequencesKernel {
+  static create(device, arena, executionProfile) {
+    return Promise.resolve(new CacheAttentionKernel(device, arena, executionProfile));
+  }
+
+  get prefix() { return "cacheAttention"; }
+  get what() { return "cache attention"; }
+  result(descriptor) { return descriptor.output; }
+
+  nativeDescriptor(descriptor) {
+    const { label, causal } = descriptor;
+    if (causal !== undefined && typeof causal !== "boolean") throw new Error(`${label} causal must be a boolean`);
+    return Object.assign(
+      { label, precision: this.precision, causal: causal === false ? 0 : 1 }, this.cacheOf(descriptor),
+      this.sizesOf(descriptor, ["outputStride", "window"]), this.bindingOf("output", descriptor.output),
+      this.numberOf(descriptor, "scale"), this.numberOf(descriptor, "scoreCap"));
+  }
+}
+
+class DraftVerifyKernel extends SequencesKernel {
+  static create(device, arena, executionProfile) {
+    return Promise.resolve(new DraftVerifyKernel(device, arena, executionProfile));
+  }
+
+  get prefix() { return "verify"; }
+  get what() { return "draft verification"; }
+  result(descriptor) { return descriptor.nextTokens; }
+
+  nativeDescriptor(descriptor) {
+    const { label } = descriptor;
+    const mode = { sample: 0, greedy: 1 }[descriptor.mode === undefined ? "sample" : descriptor.mode];
+    if (mode === undefined) throw new Error(`${label} has an unsupported mode ${descriptor.mode}`);
+    return Object.assign(
+      { label, precision: this.precision, mode },
+      this.sizesOf(descriptor, ["rows", "sequences", "columns", "targetStride", "draftStride"]),
+      this.bindingOf("target", descriptor.target), this.bindingOf("draft", descriptor.draft),
+      this.bindingOf("rowStarts", descriptor.rowStarts), this.bindingOf("tokens", descriptor.tokens),
+      this.bindingOf("uniforms", descriptor.uniforms), this.bindingOf("draws", descriptor.draws),
+      this.bindingOf("accepted", descriptor.accepted), this.bindingOf("nextTokens", descriptor.nextTokens),
+      this.numberOf(descriptor, "temperature"));
+  }
+}
+
+/** A page table's entry without a page. */
+const CACHE_NO_PAGE = 0xffffffff;
+/** A row without a draft, and the next token of a sequence that has none. */
+const VERIFY_NO_TOKEN = 0xffffffff;
+
 /** Records of a 4-bit weight: packed codes and the tables of scales and
  * offsets ([groups, columns] of the profile's element). */
 function q4TensorRecords({ inner, columns, groupSize, dtype }) {
@@ -2152,6 +2262,12 @@ module.exports = {
   RowsDispatch,
   q4TensorRecords,
   SCORE_NO_TOKEN,
+  CacheAppendKernel,
+  CacheAttentionKernel,
+  DraftVerifyKernel,
+  SequencesDispatch,
+  CACHE_NO_PAGE,
+  VERIFY_NO_TOKEN,
   subsamplingOutputDimension,
   subsamplingValidLength,
   subsamplingTensorRecords,
