@@ -840,59 +840,51 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
   const auto value_turn = [](uint32_t row) { return (DP == 64 ? (row & 2u) : (row & 3u) << 1) | (row >> 2 & 1u); };
 
   const uint8_t *keys = static_cast<const uint8_t*>(args.key_cache), *values = static_cast<const uint8_t*>(args.value_cache);
-  half8 key[LOADS], value[LOADS];
-  // Each wavefront stages 16 tokens of a tile, its lanes pieces of 64 / VR of them at a time.
+  // Each wavefront stages 16 tokens of a tile, its lanes pieces of 64 / VR of them at a time, each
+  // lane the piece that belongs where lanes in their order put 16 bytes each.
   const auto staged_token = [&](int i) { return 16u * wave + (uint32_t)i * (64u / VR) + lane / VR; };
-  const uint32_t staged_piece = lane % VR;
+  const uint32_t slot = lane % VR;
   uint32_t entry = map.entry(part.low + lane, part.high);
   uint64_t live_next = 0;
-  const auto load = [&](uint32_t t0) {
+  const auto load = [&](uint32_t t0, uint32_t stage) {
     const bool held = entry < map.count;
     live_next = __ballot(held);
     const uint32_t places = held ? map.place(t0 + lane, entry) : 0u;
-    uint64_t from[LOADS];
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i)
-      from[i] = ((uint64_t)(uint32_t)__builtin_amdgcn_ds_bpermute((int)(staged_token(i) * 4u), (int)places) + staged_piece) * 16u;
-    if (WHOLE && live_next == ~0ull) {
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        key[i] = *reinterpret_cast<const half8*>(keys + from[i]);
-        value[i] = *reinterpret_cast<const half8*>(values + from[i]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        key[i] = value[i] = half8{};
-        if ((live_next >> staged_token(i) & 1u) && (WHOLE || staged_piece < pieces)) {
-          key[i] = *reinterpret_cast<const half8*>(keys + from[i]);
-          value[i] = *reinterpret_cast<const half8*>(values + from[i]);
-        }
-      }
-    }
-    entry = map.entry(t0 + STEP + lane, part.high);
-  };
-  const auto store = [&](uint32_t stage) {
-    T* k_to = tiles + stage * 2u * Shape::kTile;
+    T* k_to = tiles + stage * 2u * Shape::kTile + 16u * wave * DP;
     T* v_to = k_to + Shape::kTile;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const uint32_t row = staged_token(i);
-      *reinterpret_cast<half8*>(k_to + row * DP + (staged_piece ^ key_turn(row)) * 8u) = key[i];
-      *reinterpret_cast<half8*>(v_to + row * DP + ((staged_piece >> 1) ^ value_turn(row)) * 16u + (staged_piece & 1u) * 8u) = value[i];
+      const uint32_t place = (uint32_t)__builtin_amdgcn_ds_bpermute((int)(row * 4u), (int)places);
+      const uint32_t k_piece = slot ^ key_turn(row), v_piece = (((slot >> 1) ^ value_turn(row)) << 1) | (slot & 1u);
+      if (WHOLE && live_next == ~0ull) {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(keys + ((uint64_t)place + k_piece) * 16u),
+                                         (__attribute__((address_space(3))) void*)(k_to + i * 512), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(values + ((uint64_t)place + v_piece) * 16u),
+                                         (__attribute__((address_space(3))) void*)(v_to + i * 512), 16, 0, 0);
+      } else {
+        half8 key = half8{}, value = half8{};
+        if (live_next >> row & 1u) {
+          if (WHOLE || k_piece < pieces) key = *reinterpret_cast<const half8*>(keys + ((uint64_t)place + k_piece) * 16u);
+          if (WHOLE || v_piece < pieces) value = *reinterpret_cast<const half8*>(values + ((uint64_t)place + v_piece) * 16u);
+        }
+        *reinterpret_cast<half8*>(k_to + i * 512 + lane * 8u) = key;
+        *reinterpret_cast<half8*>(v_to + i * 512 + lane * 8u) = value;
+      }
     }
+    entry = map.entry(t0 + STEP + lane, part.high);
   };
   uint64_t live = 0;
   if (part.low < part.high) {
-    load(part.low);
-    store(0);
+    load(part.low, 0);
     live = live_next;
   }
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // what this wavefront loads to LDS is there
   __syncthreads();
   uint32_t stage = 0;
   for (uint32_t t0 = part.low; t0 < part.high; t0 += STEP) {
     const bool more = t0 + STEP < part.high;
-    if (more) load(t0 + STEP);
+    if (more) load(t0 + STEP, stage ^ 1u);
     if (t0 < any.high && t0 + STEP > any.low) {
       const T* k_from = tiles + stage * 2u * Shape::kTile;
       const T* v_from = k_from + Shape::kTile;
@@ -966,8 +958,8 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
           }
     }
     stage ^= 1u;
-    if (more) store(stage);
     live = live_next;
+    __builtin_amdgcn_s_waitcnt(0x0f70);
     __syncthreads();
   }
 
