@@ -108,6 +108,13 @@ struct Item {
   bool live;
 };
 
+// The item of a workgroup. Workgroups go to the 8 XCDs in turn; 8 neighbouring items, blocks of rows
+// of one kv head, go to one, whose L2 has their keys and values then.
+__device__ __forceinline__ uint32_t item_index() {
+  const uint32_t i = blockIdx.x, base = i & ~63u, j = i & 63u;
+  return base + 64u <= gridDim.x ? base + (j & 7u) * 8u + (j >> 3) : i;
+}
+
 // Finds item `index`; every wavefront for itself, lanes over the sequences.
 template <int R>
 __device__ __forceinline__ Item find_item(const CacheAttentionArgs& args, const Plan& plan, uint32_t index,
@@ -422,7 +429,7 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
   const CacheView& cache = args.cache;
 
   uint32_t units;
-  const Item item = find_item<R>(args, plan, blockIdx.x, &units);
+  const Item item = find_item<R>(args, plan, item_index(), &units);
   const Workspace work = bind(args.workspace, plan, R);
   if (plan.more && blockIdx.x == 0 && threadIdx.x == 0) *work.units_count = min(units, plan.most_units);
   if (!item.live) return;
@@ -783,7 +790,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
   const CacheView& cache = args.cache;
 
   uint32_t units;
-  const Item item = find_item<R>(args, plan, blockIdx.x, &units);
+  const Item item = find_item<R>(args, plan, item_index(), &units);
   const Workspace work = bind(args.workspace, plan, R);
   if (plan.more && blockIdx.x == 0 && threadIdx.x == 0) *work.units_count = min(units, plan.most_units);
   if (!item.live) return;
