@@ -786,7 +786,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
   constexpr int KS = DP / 16, DB = DP / 32, VR = DP / 8;
   constexpr int LOADS = STEP * VR / kThreads;  // pieces of keys, and of values, of a thread
   __shared__ __attribute__((aligned(16))) uint8_t lds[Shape::kLds];
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = lane & 31u, half = lane >> 5;
+  const uint32_t lane = threadIdx.x & 63u, col = lane & 31u, half = lane >> 5;
   const CacheView& cache = args.cache;
 
   uint32_t units;
@@ -805,7 +805,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
   // This lane's query, what its row sees, what all rows of the wavefront see, and any.
   half8 query[KS];
   uint32_t low = 0, high = 0;
-  const uint32_t r = 32u * wave + col;
+  const uint32_t wave = wave::of_lane(threadIdx.x >> 6, 0u), r = 32u * wave + col;
 #pragma unroll
   for (int k = 0; k < KS; ++k) query[k] = half8{};
   if (r < item.rows) {
@@ -849,47 +849,82 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
   const uint8_t *keys = static_cast<const uint8_t*>(args.key_cache), *values = static_cast<const uint8_t*>(args.value_cache);
   // Each wavefront stages 16 tokens of a tile, its lanes pieces of 64 / VR of them at a time, each
   // lane the piece that belongs where lanes in their order put 16 bytes each.
-  const auto staged_token = [&](int i) { return 16u * wave + (uint32_t)i * (64u / VR) + lane / VR; };
+  const auto staged_row = [&](int i) { return (uint32_t)i * (64u / VR) + lane / VR; };
   const uint32_t slot = lane % VR;
-  uint32_t entry = map.entry(part.low + lane, part.high);
+  // A key's and a value's piece for this lane, of row `row` of the 16: rows turn alike in each 16.
+  const auto key_piece = [&](uint32_t row) { return slot ^ key_turn(row); };
+  const auto value_piece = [&](uint32_t row) { return (((slot >> 1) ^ value_turn(row)) << 1) | (slot & 1u); };
+  // Tiles start at multiples of 16. Where pages hold a multiple of 16 tokens, the wavefront's 16 lie side by
+  // side, and what differs from lane to lane is the same for all tiles.
+  const bool runs = WHOLE && cache.page_size % 16u == 0;
+  const uint32_t begin = part.low & ~15u;
+  uint32_t key_offset[LOADS], value_offset[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    key_offset[i] = (staged_row(i) * VR + key_piece(staged_row(i))) * 16u;
+    value_offset[i] = (staged_row(i) * VR + value_piece(staged_row(i))) * 16u;
+  }
+  // The entries of the next tile's tokens, or, of runs, of its four 16s in lanes 0 to 3.
+  const auto next_entry = [&](uint32_t t0) { return map.entry(runs ? t0 + 16u * (lane & 3u) : t0 + lane, part.high); };
+  uint32_t entry = next_entry(begin);
   uint64_t live_next = 0;
   const auto load = [&](uint32_t t0, uint32_t stage) {
-    const bool held = entry < map.count;
-    live_next = __ballot(held);
-    const uint32_t places = held ? map.place(t0 + lane, entry) : 0u;
     T* k_to = tiles + stage * 2u * Shape::kTile + 16u * wave * DP;
     T* v_to = k_to + Shape::kTile;
+    const uint32_t ours = t0 + 16u * wave;
+    uint32_t places = 0;
+    bool whole;
+    if (runs) {
+      const uint32_t held = (uint32_t)__ballot(entry < map.count) & 15u;
+      const uint32_t spread = (held | held << 15) & 0x10001u, more = (held >> 2 | held << 13) & 0x10001u;
+      live_next = (((uint64_t)(more * 0xffffu) << 32) | (spread * 0xffffu)) & tokens_below(t0, part.high) &
+                  ~tokens_below(t0, part.low);
+      whole = (held >> wave & 1u) && ours >= part.low && ours + 16u <= part.high;
+      if (whole) {
+        const uint64_t from = (uint64_t)map.place(ours, wave::of_lane(entry, wave)) * 16u;
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const uint32_t row = staged_token(i);
-      const uint32_t place = (uint32_t)__builtin_amdgcn_ds_bpermute((int)(row * 4u), (int)places);
-      const uint32_t k_piece = slot ^ key_turn(row), v_piece = (((slot >> 1) ^ value_turn(row)) << 1) | (slot & 1u);
-      if (WHOLE && live_next == ~0ull) {
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(keys + ((uint64_t)place + k_piece) * 16u),
-                                         (__attribute__((address_space(3))) void*)(k_to + i * 512), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(values + ((uint64_t)place + v_piece) * 16u),
-                                         (__attribute__((address_space(3))) void*)(v_to + i * 512), 16, 0, 0);
+        for (int i = 0; i < LOADS; ++i) {
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(keys + from + key_offset[i]),
+                                           (__attribute__((address_space(3))) void*)(k_to + i * 512), 16, 0, 0);
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(values + from + value_offset[i]),
+                                           (__attribute__((address_space(3))) void*)(v_to + i * 512), 16, 0, 0);
+        }
       } else {
+        places = held >> wave & 1u ? map.place(ours, wave::of_lane(entry, wave)) : 0u;
+      }
+    } else {
+      const bool held = entry < map.count && t0 + lane >= part.low;
+      live_next = __ballot(held);
+      whole = false;
+      places = held ? map.place(t0 + lane, entry) : 0u;
+    }
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const uint32_t row = staged_row(i), at = 16u * wave + row;
+        const uint32_t place = runs ? places + row * map.row : (uint32_t)__builtin_amdgcn_ds_bpermute((int)(at * 4u), (int)places);
         half8 key = half8{}, value = half8{};
-        if (live_next >> row & 1u) {
-          if (WHOLE || k_piece < pieces) key = *reinterpret_cast<const half8*>(keys + ((uint64_t)place + k_piece) * 16u);
-          if (WHOLE || v_piece < pieces) value = *reinterpret_cast<const half8*>(values + ((uint64_t)place + v_piece) * 16u);
+        if (live_next >> at & 1u) {
+          if (WHOLE || key_piece(row) < pieces)
+            key = *reinterpret_cast<const half8*>(keys + ((uint64_t)place + key_piece(row)) * 16u);
+          if (WHOLE || value_piece(row) < pieces)
+            value = *reinterpret_cast<const half8*>(values + ((uint64_t)place + value_piece(row)) * 16u);
         }
         *reinterpret_cast<half8*>(k_to + i * 512 + lane * 8u) = key;
         *reinterpret_cast<half8*>(v_to + i * 512 + lane * 8u) = value;
       }
     }
-    entry = map.entry(t0 + STEP + lane, part.high);
+    entry = next_entry(t0 + STEP);
   };
   uint64_t live = 0;
-  if (part.low < part.high) {
-    load(part.low, 0);
+  if (begin < part.high) {
+    load(begin, 0);
     live = live_next;
   }
   __builtin_amdgcn_s_waitcnt(0x0f70);  // what this wavefront loads to LDS is there
   __syncthreads();
   uint32_t stage = 0;
-  for (uint32_t t0 = part.low; t0 < part.high; t0 += STEP) {
+  for (uint32_t t0 = begin; t0 < part.high; t0 += STEP) {
     const bool more = t0 + STEP < part.high;
     if (more) load(t0 + STEP, stage ^ 1u);
     if (t0 < any.high && t0 + STEP > any.low) {
