@@ -207,10 +207,13 @@ __device__ __forceinline__ Item find_item(const CacheAttentionArgs& args, const 
   return item;
 }
 
-// tanh: by the exponential, and near 0, where that loses digits, by its series.
+// tanh: by the exponential, within 2^-23, which is enough beside the f16 rounding of the weights; f32: near 0,
+// where that has lost digits, by its series.
+template <typename T>
 __device__ __forceinline__ float tanh_of(float x) {
   const float e = __builtin_amdgcn_exp2f(2.0f * kLog2E * x);
-  const float far = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + e);
+  const float far = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f);
+  if constexpr (sizeof(T) == 2) return far;
   const float x2 = x * x;
   const float near = __builtin_fmaf(
       x * x2, __builtin_fmaf(x2, __builtin_fmaf(x2, __builtin_fmaf(x2, 0.021869489f, -0.053968254f), 0.13333333f),
@@ -221,6 +224,7 @@ __device__ __forceinline__ float tanh_of(float x) {
 // From the product of a query and a key to the score in log2 units: a capped
 // product is the score over `factor`, any other the score itself, with factor > 0:
 // queries take the sign of the scale (and 0) with them, exactly.
+template <typename T>
 struct Score {
   float factor, sign, before, after;
   bool capped;
@@ -228,7 +232,7 @@ struct Score {
       : factor(args.cap > 0.0f || args.scale == 0.0f ? 1.0f : fabsf(args.scale) * kLog2E),
         sign(args.scale > 0.0f ? 1.0f : args.scale < 0.0f ? -1.0f : 0.0f), before(fabsf(args.scale) / args.cap),
         after(args.cap * kLog2E), capped(args.cap > 0.0f) {}
-  __device__ __forceinline__ float cap(float dot) const { return after * tanh_of(dot * before); }
+  __device__ __forceinline__ float cap(float dot) const { return after * tanh_of<T>(dot * before); }
 };
 
 // Where the tokens of one kv head of a sequence lie, in pieces of 16 bytes
@@ -321,7 +325,7 @@ __device__ __forceinline__ void careful_item(const CacheAttentionArgs& args, con
   const uint32_t at = threadIdx.x, dim = cache.head_dim, group = args.heads / cache.kv_heads;
   const Seen part = part_of(args, item);
   const Places<T> map(cache, item.sequence, item.head);
-  const Score score(args);
+  const Score<T> score(args);
   const Result<T, R> result{args, item, work};
   constexpr uint32_t kPiece = 16 / sizeof(T);
   for (uint32_t r = 0; r < item.rows; ++r) {
@@ -438,7 +442,7 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
   const Seen part = part_of(args, item);
   const uint32_t group = args.heads / cache.kv_heads, dim = cache.head_dim;
   const Places<T> map(cache, item.sequence, item.head);
-  const Score score(args);
+  const Score<T> score(args);
   const uint32_t pieces = dim / PIECE;
 
   // Queries, and what their rows see.
@@ -799,7 +803,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
   const Seen part = part_of(args, item);
   const uint32_t group = args.heads / cache.kv_heads, dim = cache.head_dim;
   const Places<T> map(cache, item.sequence, item.head);
-  const Score score(args);
+  const Score<T> score(args);
   const uint32_t pieces = dim / 8u;
 
   // This lane's query, what its row sees, what all rows of the wavefront see, and any.
