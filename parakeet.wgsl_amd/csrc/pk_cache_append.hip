@@ -2,12 +2,17 @@
 // (include/pk_cache.h has the formulas and what the arrays may hold).
 //
 // Bound by memory, each element read and written once, and by the launch where
-// rows are few. A workgroup holds whole rows. Its threads first turn the
-// angles of their rows into sines and cosines in LDS, once for all heads; the
-// position times the frequency is a product of 32 by 24 bits, exact in f64 but
-// for 3 bits that a second fma gives, and nothing is rounded to f32 before the
-// sines and cosines are. Then a thread takes VEC pairs of a head at
-// a time: 16 bytes of each half, or 32 together.
+// rows are few: 8192 rows of 32 + 2 * 8 heads of 128 f16 channels 44.5 us, 4.5 TB/s where a
+// large copy reaches 5.1; 1616 of 8 + 2 * 8 6.5 us; one row 3.5 to 4.
+//
+// A workgroup holds whole rows. Where a row's token goes takes three loads in turn (row
+// starts, length, page table), so the first elements are loaded before it, the rest of the chain is gone
+// through once for a workgroup, and of many rows a workgroup takes several: 1 row each
+// was 46 us in the first case, two workgroups for each row 52. Sines and cosines are made in LDS, once for all
+// heads; the position times the frequency is a product of 32 by 24 bits, exact in
+// f64 but for 3 bits that a second fma gives, and nothing is rounded to f32 before the
+// sines and cosines are. A thread takes VEC pairs of a head at a time: 16 bytes of each half, or 32
+// together; narrower where strides or head sizes ask for it.
 #include "pk_internal.h"
 
 namespace pk {
@@ -15,6 +20,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxRows = 8;        // rows of a workgroup
+constexpr int kHeld = 2;           // items of a thread at a time, where it has several
+constexpr uint32_t kMany = 2048;   // workgroups that many rows are left to
 constexpr uint32_t kMaxPairs = 128;
 
 // cos and sin of position * frequency radians, each within a step of f32: the
@@ -54,73 +61,118 @@ __device__ __forceinline__ void store_run(T* p, const Run<T, VEC>& r) {
   *reinterpret_cast<Run<T, VEC>*>(p) = r;
 }
 
-template <typename T, int VEC>
+// An item of a row: VEC pairs of a head that are rotated, or 2 VEC elements that are not.
+struct Item {
+  uint32_t row, head, x, y;  // of the workgroup's rows; of all heads; elements of the head where its runs start
+  bool live, turn;
+};
+
+// Of a row: whether it has a position, the one of its rotation, and its token's place in the caches.
+struct Where {
+  bool live;
+  uint32_t position;
+  uint64_t place;
+};
+
+template <typename T, int VEC, int HELD>
 __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheAppendArgs args, uint32_t group_rows) {
   __shared__ float2 units[kMaxRows * kMaxPairs];
-  __shared__ uint32_t sequence_of[kMaxRows];
+  __shared__ uint32_t sequence_of[kMaxRows], behind_of[kMaxRows];
+  __shared__ Where where[kMaxRows];
   const CacheView& cache = args.cache;
   const uint32_t at = threadIdx.x, first = blockIdx.x * group_rows;
+  const uint32_t pairs = args.rotary_dim / 2, dim = cache.head_dim;
+  // A head has `turned` items that are rotated and then those that are copied.
+  const uint32_t turned = pairs / VEC, each = dim / (2 * VEC);
+  const uint32_t row_items = (args.heads + 2 * cache.kv_heads) * each;
+  const uint32_t items = min(group_rows, cache.rows - first) * row_items;
+  const auto item_of = [&](uint32_t i) {
+    Item t;
+    t.live = i < items;
+    t.row = i / row_items;
+    const uint32_t rest = i - t.row * row_items;
+    t.head = rest / each;
+    const uint32_t index = rest - t.head * each;
+    const bool value = t.head >= args.heads + cache.kv_heads;
+    t.turn = !value && index < turned;
+    const bool halves = t.turn && !args.neighbours;
+    t.x = halves ? index * VEC : value || t.turn ? index * 2 * VEC : args.rotary_dim + (index - turned) * 2 * VEC;
+    t.y = halves ? t.x + pairs : t.x + VEC;
+    return t;
+  };
+  const auto source = [&](const Item& t) {
+    const uint64_t row = first + t.row;
+    const uint32_t kv = t.head - args.heads;
+    return t.head < args.heads ? static_cast<const T*>(args.queries) + row * args.query_stride + (uint64_t)t.head * dim
+           : kv < cache.kv_heads
+               ? static_cast<const T*>(args.keys) + row * args.key_stride + (uint64_t)kv * dim
+               : static_cast<const T*>(args.values) + row * args.value_stride + (uint64_t)(kv - cache.kv_heads) * dim;
+  };
+  // HELD items at a time; the first ones' elements are loaded before it is known where they go.
+  Item held[HELD];
+  Run<T, VEC> x[HELD], y[HELD];
+  const auto load = [&](uint32_t from_item) {
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+      held[h] = item_of(from_item + h * kThreads);
+      if (held[h].live) {
+        const T* from = source(held[h]);
+        x[h] = load_run<T, VEC>(from + held[h].x);
+        y[h] = load_run<T, VEC>(from + held[h].y);
+      }
+    }
+  };
+  load(at);
+
   if (at < kMaxRows) sequence_of[at] = ~0u;
   __syncthreads();
   for (uint32_t s = at; s < cache.sequences; s += kThreads) {
     const uint32_t from = min(cache.row_starts[s], cache.rows), to = min(cache.row_starts[s + 1], cache.rows);
     for (uint32_t r = 0; r < group_rows; ++r)
-      if (first + r >= from && first + r < to) sequence_of[r] = s;
+      if (first + r >= from && first + r < to) {
+        sequence_of[r] = s;
+        behind_of[r] = to - (first + r);
+      }
   }
   __syncthreads();
-
-  const uint32_t pairs = args.rotary_dim / 2, dim = cache.head_dim;
-  // The position of row `first + r` in its sequence; false: none, or before the first.
-  const auto position_of = [&](uint32_t r, uint32_t* sequence, uint32_t* position) {
-    const uint32_t s = sequence_of[r];
-    *sequence = s;
-    if (s >= cache.sequences) return false;
-    const uint32_t behind = min(cache.row_starts[s + 1], cache.rows) - (first + r), length = cache.lengths[s];
-    *position = length - behind;
-    return length >= behind;
-  };
+  // Of each row whether it has a position, which, and where its token lies.
+  if (at < group_rows) {
+    const uint32_t s = sequence_of[at];
+    Where w = {false, 0, CacheView::no_place};
+    if (s < cache.sequences) {
+      const uint32_t behind = behind_of[at], length = cache.lengths[s];
+      w.live = length >= behind;
+      w.position = length - behind;
+      if (w.live && w.position < cache.capacity()) w.place = cache.place(s, w.position);
+      if (args.positions) w.position = args.positions[first + at];
+    }
+    where[at] = w;
+  }
+  __syncthreads();
   for (uint32_t i = at; i < group_rows * pairs; i += kThreads) {
-    const uint32_t r = i / pairs, j = i - r * pairs;
-    uint32_t s, position = 0;
-    if (!position_of(r, &s, &position)) continue;
-    units[i] = unit_of(args.positions ? args.positions[first + r] : position, args.frequencies[j]);
+    const uint32_t r = i / pairs;
+    if (where[r].live) units[i] = unit_of(where[r].position, args.frequencies[i - r * pairs]);
   }
-  __syncthreads();
+  if (pairs) __syncthreads();
 
-  // A head is `turned` items of VEC pairs that are rotated and `copied` of 2 VEC elements that are not.
-  const uint32_t turned = pairs / VEC, each = dim / (2 * VEC);
-  const uint32_t heads = args.heads + 2 * cache.kv_heads, row_items = heads * each;
-  for (uint32_t i = at; i < group_rows * row_items; i += kThreads) {
-    const uint32_t r = i / row_items, rest = i - r * row_items, h = rest / each, item = rest - h * each;
-    uint32_t s, position;
-    if (!position_of(r, &s, &position)) continue;
-    const uint64_t row = first + r;
-    const T* from;
+  const auto store = [&](const Item& item, const Run<T, VEC>& x, const Run<T, VEC>& y) {
+    const Where w = where[item.row];
+    if (!w.live) return;
     T* to;
-    const bool value = h >= args.heads + cache.kv_heads;
-    if (h < args.heads) {
-      from = static_cast<const T*>(args.queries) + row * args.query_stride + (uint64_t)h * dim;
-      to = static_cast<T*>(args.query_output) + row * args.query_output_stride + (uint64_t)h * dim;
+    if (item.head < args.heads) {
+      to = static_cast<T*>(args.query_output) + (uint64_t)(first + item.row) * args.query_output_stride + (uint64_t)item.head * dim;
     } else {
-      const uint32_t kv = h - args.heads - (value ? cache.kv_heads : 0u);
-      const uint64_t place = position < cache.capacity() ? cache.place(s, position) : CacheView::no_place;
-      if (place == CacheView::no_place) continue;
-      from = (value ? static_cast<const T*>(args.values) + row * args.value_stride
-                    : static_cast<const T*>(args.keys) + row * args.key_stride) + (uint64_t)kv * dim;
-      to = static_cast<T*>(value ? args.value_cache : args.key_cache) + place + (uint64_t)kv * cache.page_size * dim;
+      if (w.place == CacheView::no_place) return;
+      const bool value = item.head >= args.heads + cache.kv_heads;
+      const uint32_t kv = item.head - args.heads - (value ? cache.kv_heads : 0u);
+      to = static_cast<T*>(value ? args.value_cache : args.key_cache) + w.place + (uint64_t)kv * cache.page_size * dim;
     }
-    const bool turn = !value && item < turned;
-    // The elements of the item: two runs, side by side but for rotated halves.
-    const uint32_t x_at = turn && !args.neighbours ? item * VEC : value || turn ? item * 2 * VEC
-                                                                : args.rotary_dim + (item - turned) * 2 * VEC;
-    const uint32_t y_at = turn && !args.neighbours ? x_at + pairs : x_at + VEC;
-    const Run<T, VEC> x = load_run<T, VEC>(from + x_at), y = load_run<T, VEC>(from + y_at);
-    if (!turn) {
-      store_run<T, VEC>(to + x_at, x);
-      store_run<T, VEC>(to + y_at, y);
-      continue;
+    if (!item.turn) {
+      store_run<T, VEC>(to + item.x, x);
+      store_run<T, VEC>(to + item.y, y);
+      return;
     }
-    const float2* unit = units + r * pairs + item * VEC;
+    const float2* unit = units + item.row * pairs + (args.neighbours ? item.x / 2 : item.x);
     Run<T, VEC> a, b;
     if (!args.neighbours) {
 #pragma unroll
@@ -148,8 +200,15 @@ __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheAppendArgs 
         b.v[c] = out[VEC + c];
       }
     }
-    store_run<T, VEC>(to + x_at, a);
-    store_run<T, VEC>(to + y_at, b);
+    store_run<T, VEC>(to + item.x, a);
+    store_run<T, VEC>(to + item.y, b);
+  };
+  for (uint32_t from_item = at;; load(from_item)) {
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+      if (held[h].live) store(held[h], x[h], y[h]);
+    from_item += HELD * kThreads;
+    if (from_item - at >= items) break;
   }
 }
 
@@ -171,19 +230,18 @@ bool fits(const CacheAppendArgs& a, uint32_t vec) {
 }  // namespace
 
 hipError_t launch_cache_append(const CacheAppendArgs& args, hipStream_t stream, hipEvent_t start, hipEvent_t stop) {
-  uint32_t vec = 1;
-  Kernel kernel = args.f16 ? cache_append_kernel<_Float16, 1> : cache_append_kernel<float, 1>;
-  if (args.f16 && fits(args, 8)) {
-    vec = 8;
-    kernel = cache_append_kernel<_Float16, 8>;
-  } else if (fits(args, 4)) {
-    vec = 4;
-    kernel = args.f16 ? cache_append_kernel<_Float16, 4> : cache_append_kernel<float, 4>;
-  }
-  // Rows of a workgroup: as many as give each thread an item.
+  const uint32_t vec = args.f16 && fits(args, 8) ? 8u : fits(args, 4) ? 4u : 1u;
+  // Rows of a workgroup: as many as give each thread an item, or, of many rows, as many as
+  // leave kMany workgroups, whose threads then go through several items.
   const uint32_t items = (args.heads + 2u * args.cache.kv_heads) * (args.cache.head_dim / (2u * vec));
-  uint32_t rows = (kThreads + items - 1u) / items;
-  rows = rows > (uint32_t)kMaxRows ? (uint32_t)kMaxRows : rows;
+  const uint32_t few = kThreads / items, many = args.cache.rows / kMany;
+  uint32_t rows = many > few ? many : few;
+  rows = rows > (uint32_t)kMaxRows ? (uint32_t)kMaxRows : rows ? rows : 1u;
+  const bool one = rows * items <= (uint32_t)kThreads;
+  const Kernel kernel = vec == 8u   ? (one ? cache_append_kernel<_Float16, 8, 1> : cache_append_kernel<_Float16, 8, kHeld>)
+                        : args.f16  ? (vec == 4u ? cache_append_kernel<_Float16, 4, 1> : cache_append_kernel<_Float16, 1, 1>)
+                        : vec == 4u ? (one ? cache_append_kernel<float, 4, 1> : cache_append_kernel<float, 4, kHeld>)
+                                    : cache_append_kernel<float, 1, 1>;
   const dim3 grid((args.cache.rows + rows - 1u) / rows), block(kThreads);
   if (start || stop)
     hipExtLaunchKernelGGL(kernel, grid, block, 0, stream, start, stop, 0, args, rows);
