@@ -32,6 +32,8 @@ constexpr uint32_t kSumsSpan = kThreads * kSumsHeld * 16 / sizeof(T);  // column
 template <typename T>
 constexpr uint32_t kSpan = kThreads * kHeld * 16 / sizeof(T);          // and for the weights
 
+typedef uint32_t Words __attribute__((ext_vector_type(2)));  // of a double, the low one first
+
 // 2^x, x <= 0 but for roundings, within 2^-45 of it: x less its nearest whole number goes
 // through a polynomial that meets 2^f at the 10 Chebyshev points of [-1/2, 1/2]; the whole number is
 // in the low bits of x + 1.5 * 2^52 and is added to the exponent. 0 below 2^-1000.
@@ -45,10 +47,9 @@ __device__ __forceinline__ double exp2_of(double x) {
   double r = c[9];
 #pragma unroll
   for (int i = 8; i >= 0; --i) r = __builtin_fma(r, f, c[i]);
-  const uint64_t bits = __builtin_bit_cast(uint64_t, r);
-  const uint32_t high = (uint32_t)(bits >> 32) + ((uint32_t)__builtin_bit_cast(uint64_t, shifted) << 20);
-  const double all = __builtin_bit_cast(double, ((uint64_t)high << 32) | (uint32_t)bits);
-  return x > -1000.0 ? all : 0.0;
+  const Words w = __builtin_bit_cast(Words, r), k = __builtin_bit_cast(Words, shifted);
+  const Words all = {w.x, w.y + (k.x << 20)};
+  return x > -1000.0 ? __builtin_bit_cast(double, all) : 0.0;
 }
 
 // The many exponentials of a row, 2^((z - m) scale) within 2^-45: the whole number k of 512ths of
@@ -84,10 +85,9 @@ struct Powers {
     const double x = __builtin_fmax(exponent, -1000.0 * kTable);
     constexpr double kWhole = 6755399441055744.0, kLn2 = 0.6931471805599453 / kTable;
     const double shifted = x + kWhole, f = x - (shifted - kWhole);
-    const uint32_t k = (uint32_t)__builtin_bit_cast(uint64_t, shifted);
-    const uint64_t bits = __builtin_bit_cast(uint64_t, table[k % kTable]);
-    const uint32_t high = (uint32_t)(bits >> 32) + (k << 11);
-    const double power = __builtin_bit_cast(double, ((uint64_t)high << 32) | (uint32_t)bits);
+    const uint32_t k = __builtin_bit_cast(Words, shifted).x;
+    const Words found = __builtin_bit_cast(Words, table[k % kTable]), moved = {found.x, found.y + (k << 11)};
+    const double power = __builtin_bit_cast(double, moved);
     const double rest = f * __builtin_fma(__builtin_fma(kLn2 * kLn2 * kLn2 / 6, f, kLn2 * kLn2 / 2), f, kLn2);
     return __builtin_fma(power, rest, power);
   }
@@ -120,7 +120,8 @@ __device__ __forceinline__ V reduce_lanes(V x, Op op) {
 template <int THREADS, typename V, typename Op>
 __device__ __forceinline__ V reduce_group(V x, double* scratch, Op op) {
   static_assert(sizeof(V) <= sizeof(double), "a word of scratch each");
-  x = reduce_lanes<64>(x, op);
+  if constexpr (sizeof(V) == 8 && Op::kSum) x = wave::sum(x);
+  else x = reduce_lanes<64>(x, op);
   V* all = reinterpret_cast<V*>(scratch);
   __syncthreads();  // the readers of the one before
   if ((threadIdx.x & 63u) == 0) all[threadIdx.x >> 6] = x;
@@ -131,15 +132,13 @@ __device__ __forceinline__ V reduce_group(V x, double* scratch, Op op) {
   return x;
 }
 struct Add {
+  static constexpr bool kSum = true;
   __device__ double operator()(double a, double b) const { return a + b; }
 };
 struct Larger {
+  static constexpr bool kSum = false;
   template <typename V>
   __device__ V operator()(V a, V b) const { return a > b ? a : b; }
-};
-struct Smaller {
-  template <typename V>
-  __device__ V operator()(V a, V b) const { return a < b ? a : b; }
 };
 
 // Of a row of logits, or a part: the maximum m and the sum of 2^((z - m) scale);
@@ -251,12 +250,7 @@ struct Running {
 };
 __device__ __forceinline__ Running running_sum(double x, double* scratch) {
   const uint32_t at = threadIdx.x, lane = at & 63u;
-  double running = x;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const double other = __shfl_up(running, off, 64);
-    if ((int)lane >= off) running += other;
-  }
+  const double running = wave::running_sum(x);
   __syncthreads();
   if (lane == 63u) scratch[at >> 6] = running;
   __syncthreads();
@@ -270,22 +264,34 @@ __device__ __forceinline__ Running running_sum(double x, double* scratch) {
 }
 
 // The first column whose running sum of weights exceeds `want`, `before` being the sum in front of
-// this thread's run of N from `first` on; the last with a weight if none does, kNoToken if none has one.
+// this thread's run of N from `first` on; the last with a weight if none does, kNoToken if none has
+// one. Threads have their runs in order, so the first lane of the first wavefront with one has it.
 template <int N>
 __device__ __forceinline__ uint32_t find_token(const double (&w)[N], uint32_t first, double before, double want,
                                                double* scratch) {
-  uint32_t hit = kNoToken, behind = 0;  // one more than the last column with a weight
+  uint32_t hit = kNoToken, behind = kNoToken;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     before += w[i];
     if (w[i] > 0.0) {
-      behind = first + i + 1u;
+      behind = first + i;
       if (before > want && hit == kNoToken) hit = first + i;
     }
   }
-  hit = reduce_group<kSequence>(hit, scratch, Smaller());
-  behind = reduce_group<kSequence>(behind, scratch, Larger());
-  return hit != kNoToken ? hit : behind ? behind - 1u : kNoToken;
+  const uint64_t hits = __ballot(hit != kNoToken), weights = __ballot(behind != kNoToken);
+  hit = hits ? wave::of_lane(hit, (uint32_t)__builtin_ctzll(hits)) : kNoToken;
+  behind = weights ? wave::of_lane(behind, 63u - (uint32_t)__builtin_clzll(weights)) : kNoToken;
+  uint2* found = reinterpret_cast<uint2*>(scratch);
+  __syncthreads();
+  if ((threadIdx.x & 63u) == 0) found[threadIdx.x >> 6] = make_uint2(hit, behind);
+  __syncthreads();
+  hit = behind = kNoToken;
+#pragma unroll
+  for (int i = 0; i < kSequence / 64; ++i) {
+    hit = hit == kNoToken ? found[i].x : hit;
+    behind = found[i].y == kNoToken ? behind : found[i].y;
+  }
+  return hit != kNoToken ? hit : behind;
 }
 
 // The rows [first, first + count) of a sequence in turn, from their sums (`each` apart: of the target, and of the
@@ -325,21 +331,25 @@ __device__ __forceinline__ bool decide(const VerifyArgs& args, const Rows& rows,
 
 // ------------------------------------------------------------- short rows
 
-// A wavefront's sum of a whole row: pieces of kRun columns a lane, the row read
-// twice, the second time from the cache.
+// A wavefront's sum of a whole row, pieces of kRun columns a lane. Rows of up to kAll columns stay
+// in registers, longer ones are read a second time from the cache.
 template <typename T>
 __device__ __forceinline__ RowSum sum_row(const T* z, const double* table, uint32_t columns, double scale, bool greedy) {
   constexpr int kRun = 16 / sizeof(T), kPieces = 4;
+  constexpr uint32_t kAll = 64 * kRun * kPieces;
   const uint32_t lane = threadIdx.x & 63u;
-  // Calls use(value, column) for the columns that there are.
-  const auto each = [&](auto use) {
-    for (uint32_t base = 0; base < columns; base += 64u * kRun * kPieces) {
-      float v[kPieces][kRun];
+  float v[kPieces][kRun];
+  const auto load = [&](uint32_t base) {
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) {
-        const uint32_t from = base + (i * 64u + lane) * kRun;
-        load_run<kRun>(z + from, columns > from ? columns - from : 0u, v[i]);
-      }
+    for (int i = 0; i < kPieces; ++i) {
+      const uint32_t from = base + (i * 64u + lane) * kRun;
+      load_run<kRun>(z + from, columns > from ? columns - from : 0u, v[i]);
+    }
+  };
+  // Calls use(value, column) for the columns that there are.
+  const auto each = [&](bool loaded, auto use) {
+    for (uint32_t base = 0; base < columns; base += kAll) {
+      if (!loaded) load(base);
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
         const uint32_t from = base + (i * 64u + lane) * kRun;
@@ -352,16 +362,16 @@ __device__ __forceinline__ RowSum sum_row(const T* z, const double* table, uint3
   RowSum row;
   if (greedy) {
     unsigned long long best = 0;
-    each([&](float v, uint32_t i) { best = Larger()(best, (unsigned long long)key_of(v, i)); });
+    each(false, [&](float x, uint32_t i) { best = Larger()(best, (unsigned long long)key_of(x, i)); });
     row.best = reduce_lanes<64>(best, Larger());
     row.sum = row.best ? 1.0 : 0.0;
     return row;
   }
   float m = -kInf;
   bool strange = false;
-  each([&](float v, uint32_t) {
-    strange |= !(v < kInf);
-    m = fmaxf(m, v);
+  each(false, [&](float x, uint32_t) {
+    strange |= !(x < kInf);
+    m = fmaxf(m, x);
   });
   m = wave::max(m);
   row.m = m;
@@ -370,10 +380,10 @@ __device__ __forceinline__ RowSum sum_row(const T* z, const double* table, uint3
   double sum = 0.0;
   if (m > -kInf) {
     const Powers<T> powers(table, row.m, scale);
-    each([&](float v, uint32_t) { sum += powers.at(v); });
+    each(columns <= kAll, [&](float x, uint32_t) { sum += powers.at(x); });
     sum *= powers.right;
   }
-  row.sum = reduce_lanes<64>(sum, Add());
+  row.sum = wave::sum(sum);
   return row;
 }
 
@@ -667,21 +677,16 @@ __global__ __launch_bounds__(kSequence) void verify_token_kernel(VerifyArgs args
     uint32_t part = kNoToken, last = kNoToken;
     for (uint32_t base = 0; base < parts && part == kNoToken; base += 64u) {
       const double w = base + at < parts ? part_weight(base + at) : 0.0;
-      double running = w;
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const double other = __shfl_up(running, off, 64);
-        if ((int)at >= off) running += other;
-      }
+      const double running = wave::running_sum(w);
       const uint64_t hit = __ballot(w > 0.0 && before + running > want), live = __ballot(w > 0.0);
       const int lane = hit ? __builtin_ctzll(hit) : live ? 63 - __builtin_clzll(live) : 0;
-      const double to = before + __shfl(running - w, lane, 64);
+      const double to = before + wave::of_lane(running - w, (uint32_t)lane);
       if (hit) part = base + lane;
       if (live) {
         last = base + lane;
         last_before = to;
       }
-      before += __shfl(running, 63, 64);
+      before += wave::of_lane(running, 63u);
     }
     if (at == 0) {
       found_part = part != kNoToken ? part : last;

@@ -49,6 +49,27 @@ __device__ __forceinline__ float sum(float x) {
   }));
 }
 
+// f64: the halves of a register pair take the same way.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double plus_dpp(double x) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, x);
+  const uint64_t other = ((uint64_t)dpp<CTRL, ROWS>(0u, (uint32_t)(bits >> 32)) << 32) | dpp<CTRL, ROWS>(0u, (uint32_t)bits);
+  return x + __builtin_bit_cast(double, other);
+}
+__device__ __forceinline__ double running_sum(double x) {
+  x = plus_dpp<0x111, 0xf>(x);
+  x = plus_dpp<0x112, 0xf>(x);
+  x = plus_dpp<0x114, 0xf>(x);
+  x = plus_dpp<0x118, 0xf>(x);
+  x = plus_dpp<0x142, 0xa>(x);
+  return plus_dpp<0x143, 0xc>(x);
+}
+__device__ __forceinline__ double of_lane(double x, uint32_t lane) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, x);
+  return __builtin_bit_cast(double, ((uint64_t)of_lane((uint32_t)(bits >> 32), lane) << 32) | of_lane((uint32_t)bits, lane));
+}
+__device__ __forceinline__ double sum(double x) { return of_lane(running_sum(x), 63u); }
+
 // The largest lane, NaN left out; minus infinity if every lane is NaN.
 __device__ __forceinline__ float max(float x) {
   return __uint_as_float(reduce_bits(__float_as_uint(x), 0xff800000u, [](uint32_t a, uint32_t b) {
