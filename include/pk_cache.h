@@ -39,7 +39,10 @@
  * exponentials are f32; f16 rows round the exponentials, relative to a running
  * maximum, to f16 for their product with the values. A row that sees
  * nothing, or only scores of minus infinity, gives zeros. What a row does not
- * see, infinities and NaN included, does not touch it.
+ * see, infinities and NaN included, does not touch it; values that it does see
+ * and that are infinite or NaN make its block of rows many times slower.
+ * How the work is shared out follows rows / sequences, which the host knows,
+ * and not from row_starts: hold one op for single tokens and one for chunks.
  */
 #ifndef PK_CACHE_H
 #define PK_CACHE_H
@@ -58,6 +61,7 @@ extern "C" {
 #define PK_CACHE_MAX_PAGE_SIZE 65536u
 #define PK_CACHE_MAX_TOKENS 1073741824u           /* page_size * pages_per_sequence */
 #define PK_CACHE_MAX_BYTES (64ull << 30)          /* of one cache binding's extent */
+#define PK_CACHE_MAX_UNITS 4000000u               /* attention: rows * heads / 16 + kv_heads * sequences */
 
 typedef enum pk_rotary_kind {
   PK_ROTARY_HALVES = 0,
@@ -168,8 +172,8 @@ int pk_cache_attention_validate(const pk_cache_attention_desc *desc);
 int pk_cache_attention_create(pk_context *ctx, const pk_cache_attention_desc *desc, pk_cache_attention_op **out);
 /* The rows of the first `active_sequences` sequences (0 = all); rows behind
    them are left as they were. May be captured into graphs. Long sequences
-   are split over workgroups, which meet in memory of the op: launches of one
-   op, eager or replayed, must be ordered by the caller, as their outputs ask
+   are split over workgroups, which meet in memory of the op, where lists of
+   more than 64 sequences lie as well: launches of one op, eager or replayed, must be ordered by the caller, as their outputs ask
    for anyway. */
 int pk_cache_attention_enqueue(pk_cache_attention_op *op, uint32_t active_sequences, void *stream);
 int pk_cache_attention_enqueue_timed(pk_cache_attention_op *op, uint32_t active_sequences, void *stream,

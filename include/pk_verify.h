@@ -20,7 +20,8 @@
  * or at the last row from w = p: the first whose running sum of w, in the order
  * of the columns, exceeds draws[s] times the whole sum. So drafts that were
  * drawn from q give tokens distributed as p. Probabilities and their sums are
- * f64, so that these decisions do not hang on the order of the sums.
+ * f64, so that these decisions do not hang on the order of the sums. A
+ * probability under 2^-990 counts as 0.
  * PK_VERIFY_GREEDY: d is accepted if it is the row's best logit, the lowest
  * of equal ones, and the next token is the best of the row that ends; draft
  * logits, the temperature, uniforms and draws are not read.

@@ -183,6 +183,10 @@ int validate_attention(const pk_cache_attention_desc* d) {
   if (int s = check_cache(d, label, cache)) return s;
   if (d->heads == 0 || d->heads % d->kv_heads)
     return fail(PK_RANGE_ERROR, "%s heads must be a multiple of the %u kv heads", label, d->kv_heads);
+  // Workgroups of the smallest units, 16 rows of a kv head: as many as a launch holds.
+  const uint64_t some = d->sequences < d->rows ? d->sequences : d->rows;
+  if ((uint64_t)d->rows * d->heads / 16u + d->kv_heads * some > PK_CACHE_MAX_UNITS)
+    return fail(PK_RANGE_ERROR, "%s has more than %u blocks of 16 rows", label, PK_CACHE_MAX_UNITS);
   if (!d->queries || !d->output) return fail(PK_INVALID_ARGUMENT, "%s needs queries and an output", label);
   if (d->causal != 0 && d->causal != 1) return fail(PK_INVALID_ARGUMENT, "%s causal must be 0 or 1", label);
   if (d->window && !d->causal) return fail(PK_INVALID_ARGUMENT, "%s has a window without causal", label);

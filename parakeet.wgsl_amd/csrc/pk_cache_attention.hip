@@ -66,30 +66,42 @@ struct Plan {
   uint32_t most_units;
   uint32_t more;      // 0: no unit is split
   uint32_t shortest;  // tokens of a part, at least
+  uint32_t listed;    // sequences of the list that a launch of its own makes; 0: none
 };
-// Memory of the op: the number of units, the units, then a record of each
+// A sequence in the order of the items: its number, first row, rows, blocks of rows, tokens that any of its rows
+// sees, length; and, up to and with it, the items, the units, and the records of split units.
+struct Listed {
+  uint32_t sequence, start, count, tiles, span, length;
+  uint32_t parts, items_to, units_to, slots_to;
+};
+// Memory of the op: the number of units, the list, the units, then a record of each
 // item of a split unit: maxima and sums of its rows, then their outputs before the division.
 // A unit of more than `longest` tokens has less than 2 span / longest parts, and all
 // spans add up to at most `more` times longest: 2 * more records.
 struct Workspace {
   uint32_t* units_count;
+  Listed* list;
   Unit* units;
   float2* sums;    // [records][R]
   float* outputs;  // [records][R][dim]
 };
 constexpr uint64_t kHeader = 256;
+__host__ __device__ constexpr uint64_t list_bytes(const Plan& p) {
+  return (p.listed * sizeof(Listed) + 255u) / 256u * 256u;
+}
 __host__ __device__ constexpr uint64_t units_bytes(const Plan& p) {
   return (p.most_units * sizeof(Unit) + 255u) / 256u * 256u;
 }
 uint64_t workspace_bytes(const Plan& p, uint32_t R, uint32_t dim) {
-  return kHeader + units_bytes(p) + 2ull * p.more * R * (sizeof(float2) + 4u * dim);
+  return kHeader + list_bytes(p) + units_bytes(p) + 2ull * p.more * R * (sizeof(float2) + 4u * dim);
 }
 __device__ inline Workspace bind(void* memory, const Plan& plan, uint32_t R) {
   uint8_t* p = static_cast<uint8_t*>(memory);
   Workspace w;
   w.units_count = reinterpret_cast<uint32_t*>(p);
-  w.units = reinterpret_cast<Unit*>(p + kHeader);
-  w.sums = reinterpret_cast<float2*>(p + kHeader + units_bytes(plan));
+  w.list = reinterpret_cast<Listed*>(p + kHeader);
+  w.units = reinterpret_cast<Unit*>(p + kHeader + list_bytes(plan));
+  w.sums = reinterpret_cast<float2*>(p + kHeader + list_bytes(plan) + units_bytes(plan));
   w.outputs = reinterpret_cast<float*>(w.sums + 2ull * plan.more * R);
   return w;
 }
@@ -115,96 +127,211 @@ __device__ __forceinline__ uint32_t item_index() {
   return base + 64u <= gridDim.x ? base + (j & 7u) * 8u + (j >> 3) : i;
 }
 
-// Finds item `index`; every wavefront for itself, lanes over the sequences.
+// Sequence s; one behind the last has nothing.
 template <int R>
-__device__ __forceinline__ Item find_item(const CacheAttentionArgs& args, const Plan& plan, uint32_t index,
-                                          uint32_t* units_count) {
+__device__ __forceinline__ Listed look_at(const CacheAttentionArgs& args, uint32_t s) {
   const CacheView& cache = args.cache;
-  const uint32_t lane = threadIdx.x & 63u, group = args.heads / cache.kv_heads;
-  struct Of {
-    uint32_t sequence, start, count, tiles, span, length;
-  };
-  const auto of = [&](uint32_t s) {
-    Of x = {s, 0, 0, 0, 0, 0};
-    if (s < cache.sequences) {
-      x.start = min(cache.row_starts[s], cache.rows);
-      const uint32_t end = min(cache.row_starts[s + 1], cache.rows), length = cache.lengths[s];
-      x.length = length;
-      x.count = end > x.start ? end - x.start : 0u;
-      x.tiles = (x.count * group + R - 1u) / R;
-      const Seen seen = seen_by(args, length, (int64_t)length - x.count, x.count);
-      x.span = x.count ? max(1u, seen.high - seen.low) : 0u;
-    }
-    return x;
-  };
-  // All units, and all their tokens.
-  uint32_t units = 0;
-  float tokens = 0.0f;
-  Of mine = of(lane);
-  for (uint32_t s = lane; s < cache.sequences; s += 64u) {
-    if (s != lane) mine = of(s);
-    units += mine.tiles * cache.kv_heads;
-    tokens += (float)(mine.tiles * cache.kv_heads) * (float)mine.span;
+  Listed x = {s, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+  if (s < cache.sequences) {
+    x.start = min(cache.row_starts[s], cache.rows);
+    const uint32_t end = min(cache.row_starts[s + 1], cache.rows), length = cache.lengths[s];
+    x.length = length;
+    x.count = end > x.start ? end - x.start : 0u;
+    x.tiles = (x.count * (args.heads / cache.kv_heads) + R - 1u) / R;
+    const Seen seen = seen_by(args, length, (int64_t)length - x.count, x.count);
+    x.span = x.count ? max(1u, seen.high - seen.low) : 0u;
   }
-  units = wave::reduce_bits(units, 0u, [](uint32_t a, uint32_t b) { return a + b; });
-  tokens = wave::sum(tokens);
-  *units_count = units;
-  // Parts of at most `longest` tokens: sum(ceil(span / longest)) over the units is at
-  // most tokens / longest + units. The quotient is rounded up by more than its
-  // and the sum's roundings. More units than there can be come from row starts
-  // that decrease: those are not split.
-  uint32_t longest = 0x7fffffffu;
-  if (plan.more && units <= plan.most_units)
-    longest = max(plan.shortest, (uint32_t)min(tokens / (float)plan.more * 1.0001f + 1.0f, 2e9f));
+  return x;
+}
+// Parts of at most so many tokens, from all units and all their tokens: sum(ceil(span /
+// longest)) over the units is at most tokens / longest + units. The quotient is rounded up by
+// more than its and the sum's roundings. More units than there can be come from row starts
+// that decrease: those are not split, and none is joined.
+__device__ __forceinline__ uint32_t longest_part(const Plan& plan, uint32_t units, float tokens) {
+  if (!plan.more || units > plan.most_units) return 0x7fffffffu;
+  return max(plan.shortest, (uint32_t)min(tokens / (float)plan.more * 1.0001f + 1.0f, 2e9f));
+}
+__device__ __forceinline__ uint32_t parts_of(uint32_t span, uint32_t longest) {
+  return span ? (span + longest - 1u) / longest : 0u;
+}
+
+// Item `index` of a sequence whose sums count it: the sums of those before it are these less its own.
+template <int R>
+__device__ __forceinline__ Item item_in(const CacheAttentionArgs& args, const Listed& x, uint32_t index) {
+  const uint32_t units = x.tiles * args.cache.kv_heads, items = units * x.parts, group = args.heads / args.cache.kv_heads;
+  const uint32_t local = index - (x.items_to - items), unit = local / x.parts;
   Item item;
-  item.live = false;
-  uint32_t items_before = 0, units_before = 0, slots_before = 0;
-  for (uint32_t base = 0; base < cache.sequences; base += 64u) {
-    const uint32_t s = base + lane;
-    if (cache.sequences > 64u) mine = of(s);
-    // The longest of these sequences first, so that the last workgroups are short ones.
-    const uint32_t here = min(64u, cache.sequences - base);
-    if (here > 1u) {
-      uint32_t rank = 0;
-      for (uint32_t j = 0; j < here; ++j) {
-        const uint32_t other = wave::of_lane(mine.span, j);
-        rank += other > mine.span || (other == mine.span && j < lane);
-      }
-      if (lane >= here) rank = lane;
-      const auto sorted = [&](uint32_t x) { return (uint32_t)__builtin_amdgcn_ds_permute((int)(rank * 4u), (int)x); };
-      mine = {sorted(s), sorted(mine.start), sorted(mine.count), sorted(mine.tiles), sorted(mine.span),
-              sorted(mine.length)};
-    }
-    const uint32_t parts = mine.span ? (mine.span + longest - 1u) / longest : 0u;
-    const uint32_t have = mine.tiles * cache.kv_heads, items = have * parts, slots = parts > 1u ? items : 0u;
-    const uint32_t items_to = wave::running_sum(items), units_to = wave::running_sum(have),
-                   slots_to = wave::running_sum(slots);
-    const uint64_t hit = __ballot(index < items_before + items_to);
-    if (hit) {
-      const uint32_t at = (uint32_t)__builtin_ctzll(hit);
-      const auto its = [&](uint32_t x) { return wave::of_lane(x, at); };
-      const uint32_t each = its(parts), tiles = its(mine.tiles);
-      const uint32_t local = index - (items_before + its(items_to - items)), unit = local / each;
-      item.live = true;
-      item.sequence = its(mine.sequence);
-      item.parts = each;
-      item.part = local - unit * each;
-      item.head = unit / tiles;
-      item.first = (unit - item.head * tiles) * R;
-      item.row = its(mine.start);
-      item.new_tokens = its(mine.count);
-      item.rows = min((uint32_t)R, item.new_tokens * group - item.first);
-      item.length = its(mine.length);
-      item.position = (int64_t)item.length - item.new_tokens;
-      item.unit = units_before + its(units_to - have) + unit;
-      item.slot = slots_before + its(slots_to - slots) + unit * each;
-      break;
-    }
-    items_before += wave::of_lane(items_to, 63u);
-    units_before += wave::of_lane(units_to, 63u);
-    slots_before += wave::of_lane(slots_to, 63u);
-  }
+  item.live = local < items;  // else from sums past 32 bits: of row starts that decrease
+  item.sequence = x.sequence;
+  item.parts = x.parts;
+  item.part = local - unit * x.parts;
+  item.head = unit / x.tiles;
+  item.first = (unit - item.head * x.tiles) * R;
+  item.row = x.start;
+  item.new_tokens = x.count;
+  item.rows = min((uint32_t)R, x.count * group - item.first);
+  item.length = x.length;
+  item.position = (int64_t)x.length - x.count;
+  item.unit = x.units_to - units + unit;
+  item.slot = x.slots_to - (x.parts > 1u ? items : 0u) + unit * x.parts;
   return item;
+}
+
+// Finds item `index`; every wavefront for itself, lanes over up to 64 sequences, or over the list.
+constexpr uint32_t kUnlisted = 64;
+template <int R>
+__device__ __forceinline__ Item find_item(const CacheAttentionArgs& args, const Plan& plan, const Workspace& work,
+                                          uint32_t index) {
+  const CacheView& cache = args.cache;
+  const uint32_t lane = threadIdx.x & 63u;
+  Item none;
+  none.live = false;
+  if (plan.listed) {
+    // The 64 sequences that the item is in, by the last of each 64, then the one.
+    uint32_t at = min((lane + 1u) * 64u, plan.listed) - 1u;
+    uint64_t hit = __ballot(index < work.list[at].items_to);
+    if (!hit) return none;
+    const uint32_t base = (uint32_t)__builtin_ctzll(hit) * 64u;
+    at = min(base + lane, plan.listed - 1u);
+    hit = __ballot(index < work.list[at].items_to);
+    at = base + (uint32_t)__builtin_ctzll(hit);
+    return item_in<R>(args, work.list[at], index);
+  }
+  Listed mine = look_at<R>(args, lane);
+  const uint32_t units = wave::reduce_bits(mine.tiles * cache.kv_heads, 0u, [](uint32_t a, uint32_t b) { return a + b; });
+  const float tokens = wave::sum((float)(mine.tiles * cache.kv_heads) * (float)mine.span);
+  if (plan.more && blockIdx.x == 0 && threadIdx.x == 0) *work.units_count = units > plan.most_units ? 0u : units;
+  // The longest of the sequences first, so that the last workgroups are short ones.
+  if (cache.sequences > 1u) {
+    uint32_t rank = 0;
+    for (uint32_t j = 0; j < cache.sequences; ++j) {
+      const uint32_t other = wave::of_lane(mine.span, j);
+      rank += other > mine.span || (other == mine.span && j < lane);
+    }
+    if (lane >= cache.sequences) rank = lane;
+    const auto sorted = [&](uint32_t x) { return (uint32_t)__builtin_amdgcn_ds_permute((int)(rank * 4u), (int)x); };
+    mine = {sorted(lane), sorted(mine.start), sorted(mine.count), sorted(mine.tiles), sorted(mine.span),
+            sorted(mine.length), 0, 0, 0, 0};
+  }
+  mine.parts = parts_of(mine.span, longest_part(plan, units, tokens));
+  const uint32_t have = mine.tiles * cache.kv_heads, items = have * mine.parts;
+  mine.items_to = wave::running_sum(items);
+  mine.units_to = wave::running_sum(have);
+  mine.slots_to = wave::running_sum(mine.parts > 1u ? items : 0u);
+  const uint64_t hit = __ballot(index < mine.items_to);
+  if (!hit) return none;
+  const uint32_t at = (uint32_t)__builtin_ctzll(hit);
+  const auto its = [&](uint32_t x) { return wave::of_lane(x, at); };
+  const Listed found = {its(mine.sequence), its(mine.start), its(mine.count), its(mine.tiles), its(mine.span),
+                        its(mine.length), its(mine.parts), its(mine.items_to), its(mine.units_to), its(mine.slots_to)};
+  return item_in<R>(args, found, index);
+}
+
+// The list of more than kUnlisted sequences, by one workgroup, instead of a pass of every item over all of
+// them: 32 query heads over 8, one token each of up to 500 in f16, take 14.2 us without and 17
+// with it at 32 sequences, 20.1 and 21 at 64, 36.8 and 29.4 at 96, 122 and 69 at 256. In
+// descending order of the spans, as far as 8 classes to an octave go; which of a class
+// comes first may change, and with it who works on what, but no sum.
+constexpr int kListThreads = 1024;
+constexpr uint32_t kEach = 4;  // sequences of a thread: 4096
+template <int R>
+__global__ __launch_bounds__(kListThreads) void cache_attention_list_kernel(CacheAttentionArgs args, Plan plan) {
+  __shared__ uint32_t order[kListThreads * kEach], classes[256], totals[4][kListThreads / 64];
+  __shared__ float all_tokens[kListThreads / 64];
+  const Workspace work = bind(args.workspace, plan, R);
+  const uint32_t at = threadIdx.x, lane = at & 63u, wave_at = at >> 6, kv = args.cache.kv_heads, n = plan.listed;
+  const auto class_of = [](uint32_t span) {
+    if (span < 8u) return 255u - span;
+    const uint32_t octave = 31u - (uint32_t)__builtin_clz(span);
+    return 255u - (octave * 8u + (span >> (octave - 3u) & 7u) - 16u);
+  };
+  if (at < 256u) classes[at] = 0;
+  __syncthreads();
+  uint32_t units = 0, place[kEach], kind[kEach];
+  float tokens = 0.0f;
+#pragma unroll
+  for (uint32_t i = 0; i < kEach; ++i) {
+    const uint32_t s = at + i * kListThreads;
+    if (s >= n) continue;
+    const Listed x = look_at<R>(args, s);
+    units += x.tiles * kv;
+    tokens += (float)(x.tiles * kv) * (float)x.span;
+    kind[i] = class_of(x.span);
+    place[i] = atomicAdd(&classes[kind[i]], 1u);
+  }
+  units = wave::reduce_bits(min(units, plan.most_units + 1u), 0u, [](uint32_t a, uint32_t b) { return a + b; });
+  units = min(units, plan.most_units + 1u);  // decreasing row starts: no sum past 32 bits
+  tokens = wave::sum(tokens);
+  if (lane == 0) {
+    totals[3][wave_at] = units;
+    all_tokens[wave_at] = tokens;
+  }
+  __syncthreads();
+  if (at < 64u) {  // classes before each class
+    uint32_t here[4], sum = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      here[c] = sum;
+      sum += classes[at * 4u + c];
+    }
+    const uint32_t before = wave::running_sum(sum) - sum;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) classes[at * 4u + c] = before + here[c];
+  }
+  __syncthreads();
+#pragma unroll
+  for (uint32_t i = 0; i < kEach; ++i)
+    if (at + i * kListThreads < n) order[classes[kind[i]] + place[i]] = at + i * kListThreads;
+  units = 0;
+  tokens = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kListThreads / 64; ++w) {
+    units += totals[3][w];
+    tokens += all_tokens[w];
+  }
+  __syncthreads();
+  const uint32_t longest = longest_part(plan, units, tokens);
+  // A thread's neighbours in this order, and the sums over those before them.
+  Listed mine[kEach];
+  uint32_t items = 0, have = 0, slots = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < kEach; ++i) {
+    const uint32_t p = at * kEach + i;
+    if (p < n) {
+      mine[i] = look_at<R>(args, order[p]);
+      mine[i].parts = parts_of(mine[i].span, longest);
+      const uint32_t own = mine[i].tiles * kv;
+      items += own * mine[i].parts;
+      have += own;
+      slots += mine[i].parts > 1u ? own * mine[i].parts : 0u;
+    }
+    if (p < n) {
+      mine[i].items_to = items;
+      mine[i].units_to = have;
+      mine[i].slots_to = slots;
+    }
+  }
+  const uint32_t items_to = wave::running_sum(items), units_to = wave::running_sum(have), slots_to = wave::running_sum(slots);
+  if (lane == 63u) {
+    totals[0][wave_at] = items_to;
+    totals[1][wave_at] = units_to;
+    totals[2][wave_at] = slots_to;
+  }
+  __syncthreads();
+  uint32_t before[3] = {items_to - items, units_to - have, slots_to - slots};
+  for (uint32_t w = 0; w < wave_at; ++w)
+#pragma unroll
+    for (int c = 0; c < 3; ++c) before[c] += totals[c][w];
+#pragma unroll
+  for (uint32_t i = 0; i < kEach; ++i) {
+    const uint32_t p = at * kEach + i;
+    if (p >= n) continue;
+    mine[i].items_to += before[0];
+    mine[i].units_to += before[1];
+    mine[i].slots_to += before[2];
+    work.list[p] = mine[i];
+  }
+  if (at == 0) *work.units_count = units > plan.most_units ? 0u : units;
 }
 
 // tanh: by the exponential, within 2^-23, which is enough beside the f16 rounding of the weights; f32: near 0,
@@ -432,10 +559,8 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = lane & 15u, quarter = lane >> 4;
   const CacheView& cache = args.cache;
 
-  uint32_t units;
-  const Item item = find_item<R>(args, plan, item_index(), &units);
   const Workspace work = bind(args.workspace, plan, R);
-  if (plan.more && blockIdx.x == 0 && threadIdx.x == 0) *work.units_count = min(units, plan.most_units);
+  const Item item = find_item<R>(args, plan, work, item_index());
   if (!item.live) return;
   if (plan.more && item.part == 0 && item.unit < plan.most_units && threadIdx.x == 0)
     work.units[item.unit] = {item.slot, item.parts, item.row, item.rows, item.head, item.first};
@@ -793,10 +918,8 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
   const uint32_t lane = threadIdx.x & 63u, col = lane & 31u, half = lane >> 5;
   const CacheView& cache = args.cache;
 
-  uint32_t units;
-  const Item item = find_item<R>(args, plan, item_index(), &units);
   const Workspace work = bind(args.workspace, plan, R);
-  if (plan.more && blockIdx.x == 0 && threadIdx.x == 0) *work.units_count = min(units, plan.most_units);
+  const Item item = find_item<R>(args, plan, work, item_index());
   if (!item.live) return;
   if (plan.more && item.part == 0 && item.unit < plan.most_units && threadIdx.x == 0)
     work.units[item.unit] = {item.slot, item.parts, item.row, item.rows, item.head, item.first};
@@ -1105,20 +1228,21 @@ __global__ __launch_bounds__(64 * kJoinRows) void cache_attention_join_kernel(Ca
 
 typedef void (*Kernel)(CacheAttentionArgs, Plan);
 struct Variant {
-  Kernel kernel, join;
+  Kernel kernel, list, join;
   uint32_t rows;  // of a unit
 };
 
 template <typename T, int DP, int RB>
 Variant few(bool whole) {
   return {whole ? cache_attention_few_kernel<T, DP, RB, true> : cache_attention_few_kernel<T, DP, RB, false>,
-          cache_attention_join_kernel<T, 16 * RB>, 16 * RB};
+          cache_attention_list_kernel<16 * RB>, cache_attention_join_kernel<T, 16 * RB>, 16 * RB};
 }
 
 template <int DP>
 Variant many(bool whole) {
   return {whole ? cache_attention_many_kernel<DP, true> : cache_attention_many_kernel<DP, false>,
-          cache_attention_join_kernel<_Float16, ManyShape<DP>::kRows>, ManyShape<DP>::kRows};
+          cache_attention_list_kernel<ManyShape<DP>::kRows>, cache_attention_join_kernel<_Float16, ManyShape<DP>::kRows>,
+          ManyShape<DP>::kRows};
 }
 
 // Rows of a unit: 16, 32 or 64 where the rows of an average sequence need no more, else
@@ -1161,6 +1285,7 @@ Plan plan_of(const CacheAttentionArgs& args, uint32_t R) {
   plan.most_units = (uint32_t)(args.cache.kv_heads * (args.cache.rows * group / R + some));
   plan.more = args.cache.capacity() > kShortest ? (R > 64u ? 256u : R > 32u ? 512u : R > 16u ? 1024u : 2048u) : 0u;
   plan.shortest = kShortest;
+  plan.listed = args.cache.sequences > kUnlisted ? args.cache.sequences : 0u;
   return plan;
 }
 
@@ -1172,7 +1297,7 @@ uint64_t cache_attention_workspace(const CacheAttentionArgs& args) {
   for (uint32_t rows : {16u, 32u, 64u, 128u}) {
     const Plan plan = plan_of(args, rows);
     const uint64_t bytes = workspace_bytes(plan, rows, args.cache.head_dim);
-    if (plan.more && bytes > most) most = bytes;
+    if ((plan.more || plan.listed) && bytes > most) most = bytes;
   }
   return most;
 }
@@ -1181,9 +1306,17 @@ hipError_t launch_cache_attention(const CacheAttentionArgs& args, hipStream_t st
                                   hipEvent_t stop) {
   const Variant variant = args.f16 ? choose<_Float16>(args) : choose<float>(args);
   const Plan plan = plan_of(args, variant.rows);
-  if (plan.more && workspace_bytes(plan, variant.rows, args.cache.head_dim) > args.workspace_bytes)
+  if ((plan.more || plan.listed) && workspace_bytes(plan, variant.rows, args.cache.head_dim) > args.workspace_bytes)
     return hipErrorInvalidValue;
   const dim3 grid(plan.most_units + plan.more), block(kThreads);
+  if (plan.listed) {
+    if (start)
+      hipExtLaunchKernelGGL(variant.list, dim3(1), dim3(kListThreads), 0, stream, start, nullptr, 0, args, plan);
+    else
+      hipLaunchKernelGGL(variant.list, dim3(1), dim3(kListThreads), 0, stream, args, plan);
+    if (const hipError_t e = hipGetLastError()) return e;
+    start = nullptr;
+  }
   if (start || (stop && !plan.more))
     hipExtLaunchKernelGGL(variant.kernel, grid, block, 0, stream, start, plan.more ? nullptr : stop, 0, args, plan);
   else

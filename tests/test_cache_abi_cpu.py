@@ -152,6 +152,7 @@ def test_cache_attention_accepts(abi):
 @pytest.mark.parametrize("over,error,message", CACHE_REFUSALS + [
     (dict(heads=0), "PaletteRangeError", "step heads must be a multiple of the 2 kv heads"),
     (dict(heads=3), "PaletteRangeError", "step heads must be a multiple of the 2 kv heads"),
+    (dict(rows=1 << 20, heads=64), "PaletteRangeError", "step has more than 4000000 blocks of 16 rows"),
     (dict(queries=Fake(None, 0)), "PaletteError", "step needs queries and an output"),
     (dict(window=5, causal=False), "PaletteError", "step has a window without causal"),
     (dict(scale=float("-inf")), "PaletteRangeError", "step scale must be at most 2^60 in magnitude"),

@@ -508,6 +508,43 @@ def test_long(abi, ctx, scope, dtype, counts, lengths, width):
 
 
 @DTYPES
+@pytest.mark.parametrize("sequences,most_rows,longest", [(64, 1, 700), (65, 1, 700), (65, 40, 90), (130, 3, 400), (1100, 1, 60)])
+def test_many_sequences(abi, ctx, scope, dtype, sequences, most_rows, longest):
+    """More sequences than a wavefront has lanes are listed by a launch of their own; some have no rows."""
+    rng = np.random.default_rng(sequences)
+    counts = rng.integers(0, most_rows + 1, sequences)
+    lengths = np.maximum(counts, np.exp(rng.uniform(0, np.log(longest), sequences)).astype(int))
+    for width in (0, 100):
+        run_attention(abi, ctx, scope, rng, dtype, list(counts), list(lengths), 2, 1, 32, 16, width=width)
+    run_attention(abi, ctx, scope, rng, dtype, list(counts), list(lengths), 2, 1, 32, 16, active=sequences - 3)
+
+
+@DTYPES
+def test_long_among_many_sequences(abi, ctx, scope, dtype):
+    rng = np.random.default_rng(20)
+    lengths = [9000 if s % 30 == 7 else 1 + s for s in range(100)]
+    run_attention(abi, ctx, scope, rng, dtype, [1] * 100, lengths, 2, 1, 64, 16)
+
+
+@DTYPES
+@pytest.mark.parametrize("sequences,length", [(4, 60), (4, 3000), (70, 60), (70, 3000)])
+def test_starts_that_decrease(abi, ctx, scope, dtype, sequences, length):
+    """Rows that only the first sequence has are right, whatever those of several
+    hold; to the bit they need not be, as too many rows in all are not split."""
+    counts = [8] + [0] * (sequences - 1)
+    lengths = [length] + [40] * (sequences - 1)
+
+    def decrease(cache, queries):
+        cache.starts[2:] = [2 if s % 2 == 0 else 6 for s in range(2, sequences + 1)]
+
+    run = lambda **kw: run_attention(abi, ctx, scope, np.random.default_rng(3), dtype, counts, lengths, 4, 2, 64, 16, **kw)
+    cache, want, queries = run()
+    got = run(spoil=decrease, check=False)[1]
+    got[2:6] = want[2:6]
+    check_attention(cache, got, queries, 4)
+
+
+@DTYPES
 def test_offsets_past_32_bits(abi, ctx, scope, dtype):
     """Pages whose elements, and bytes, lie beyond 2^32."""
     rng, page, dim = np.random.default_rng(18), 16, 128
