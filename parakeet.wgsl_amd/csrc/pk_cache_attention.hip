@@ -1246,13 +1246,19 @@ Variant many(bool whole) {
 }
 
 // Rows of a unit: 16, 32 or 64 where the rows of an average sequence need no more, else
-// 128 (f16). f32 units end at 64, 32 and 16 rows for heads of up to 64, 128 and 256 channels, f16
-// units of 64 rows at 128 channels.
+// 128 (f16). The kernel of 64 rows holds heads of up to 64 channels; 33 to 64 rows of wider heads go
+// to the kernel of 128, or, where that fills the registers of a wavefront alone, beyond 128
+// channels, to two units of 32. f32 units end at 64, 32 and 16 rows for heads of up to 64, 128
+// and 256 channels. 16 sequences with 32 to 64 rows of 64 channels, 1500 to 6000 tokens: 64 rows
+// 22.2 us, 128 30.1. 8 sequences with 48 to 64 rows, up to 8192 tokens: 128 channels 47 us by
+// 64 rows (their outputs and keys fill the registers), 29 by 128, 41 by 32; 24 to 32 rows 25.8 by 32
+// rows, 25.6 by 128, and 64 such sequences of up to 1000 24.6 and 28.7. 8 with 64 rows of 256
+// channels, up to 4000: 56 by 32 rows, 63 by 128; with 128 rows 82 and 69.
 uint32_t unit_rows(const CacheAttentionArgs& args) {
   const uint64_t group = args.heads / args.cache.kv_heads;
   const uint64_t rows = (args.cache.rows * group + args.cache.sequences - 1u) / args.cache.sequences;
   const uint32_t dim = args.cache.head_dim, most = args.f16 ? 128u : dim <= 64u ? 64u : dim <= 128u ? 32u : 16u;
-  const uint32_t wanted = rows <= 16u ? 16u : rows <= 32u ? 32u : rows <= 64u && dim <= 128u ? 64u : 128u;
+  const uint32_t wanted = rows <= 16u ? 16u : rows <= 32u ? 32u : rows > 64u ? 128u : dim <= 64u ? 64u : dim <= 128u ? 128u : 32u;
   return wanted < most ? wanted : most;
 }
 
@@ -1261,7 +1267,7 @@ Variant choose(uint32_t rows, bool whole) {
   constexpr bool kHalf = sizeof(T) == 2;
   if constexpr (kHalf || DP <= 128)
     if (rows == 32u) return few<T, DP, 2>(whole);
-  if constexpr (kHalf ? DP <= 128 : DP <= 64)
+  if constexpr (DP <= 64)
     if (rows == 64u) return few<T, DP, 4>(whole);
   if constexpr (kHalf)
     if (rows == 128u) return many<DP>(whole);
@@ -1275,7 +1281,14 @@ Variant choose(const CacheAttentionArgs& args) {
   return choose<T, 256>(rows, dim == 256u);
 }
 
-constexpr uint32_t kShortest = 512;  // tokens of a part
+// Tokens of a part at least, and workgroups beside one for each unit, of which parts are made: a
+// part costs its start, and its record's way to the join. Parts of 256, 512 and 1024: one token of 32 over 8
+// heads of 128 channels in f16 over 2000 tokens takes 12, 14.9 and 20.6 us, 8 such over 500 to 2000
+// 16.7, 15.5 and 20.5; 16 drafts over up to 6000 22.8, 22.4 and 27.5. Twice as many workgroups: one token over 131072 132
+// us and not 113, 64 over up to 16384 187 and not 183 (half as many 198); of 32 rows, 4 drafts over 32768
+// 71 and not 61 (60); of 64 rows 82 and not 67 (117). Of 128 rows half as many: two chunks of 512
+// over 16000 206 us and not 181 (twice as many 199), eight of 100 to 300 over up to 8192 52 and not 59.
+constexpr uint32_t kShortest = 512;
 
 Plan plan_of(const CacheAttentionArgs& args, uint32_t R) {
   const uint64_t group = args.heads / args.cache.kv_heads;
@@ -1283,7 +1296,7 @@ Plan plan_of(const CacheAttentionArgs& args, uint32_t R) {
   Plan plan;
   // Full tiles of rows, and one that is not full for each sequence.
   plan.most_units = (uint32_t)(args.cache.kv_heads * (args.cache.rows * group / R + some));
-  plan.more = args.cache.capacity() > kShortest ? (R > 64u ? 256u : R > 32u ? 512u : R > 16u ? 1024u : 2048u) : 0u;
+  plan.more = args.cache.capacity() > kShortest ? (R == 16u ? 1024u : R == 64u ? 256u : 512u) : 0u;
   plan.shortest = kShortest;
   plan.listed = args.cache.sequences > kUnlisted ? args.cache.sequences : 0u;
   return plan;
@@ -1293,8 +1306,10 @@ Plan plan_of(const CacheAttentionArgs& args, uint32_t R) {
 
 uint64_t cache_attention_workspace(const CacheAttentionArgs& args) {
   // Any number of active sequences: the rows of a unit follow from it.
+  CacheAttentionArgs one = args;
+  one.cache.sequences = 1;
   uint64_t most = 0;
-  for (uint32_t rows : {16u, 32u, 64u, 128u}) {
+  for (uint32_t rows = unit_rows(args); rows <= unit_rows(one); rows *= 2) {
     const Plan plan = plan_of(args, rows);
     const uint64_t bytes = workspace_bytes(plan, rows, args.cache.head_dim);
     if ((plan.more || plan.listed) && bytes > most) most = bytes;
