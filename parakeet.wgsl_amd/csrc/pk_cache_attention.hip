@@ -10,6 +10,10 @@
 // among short ones fills the device too. Parts meet in memory of the op and a second
 // launch joins them in their order.
 //
+// Single tokens and drafts are bound by memory where sequences are long, else by the chain of
+// loads to a unit's first keys and the launches; chunks by the matrix instructions and the exponentials
+// beside them. Each kernel has its figures.
+//
 // Scores are computed transposed, S^T = K Q^T: a lane then holds scores of
 // one row, its running maximum and sum stay in that lane, and the exponentials
 // are at once the operand of O^T = V^T P^T.
@@ -121,7 +125,8 @@ struct Item {
 };
 
 // The item of a workgroup. Workgroups go to the 8 XCDs in turn; 8 neighbouring items, blocks of rows
-// of one kv head, go to one, whose L2 has their keys and values then.
+// of one kv head, go to one, whose L2 has their keys and values then: 4 chunks of 1024 rows 268 us
+// and not 272, 16 of up to 188 in f32 44 and not 46.
 __device__ __forceinline__ uint32_t item_index() {
   const uint32_t i = blockIdx.x, base = i & ~63u, j = i & 63u;
   return base + 64u <= gridDim.x ? base + (j & 7u) * 8u + (j >> 3) : i;
@@ -514,7 +519,15 @@ __device__ __forceinline__ void careful_item(const CacheAttentionArgs& args, con
 //
 // The loads of a step's keys are issued when the step before has used its own, those of
 // its values likewise, and the entries of the page table a step ahead of the keys, before
-// the values: loads return in their order, and nothing waits for more than it needs.
+// the values: loads return in their order, and nothing waits for more than it needs. Keys two
+// steps ahead, in registers or in a ring of LDS, gained nothing.
+//
+// f16, 32 heads over 8 of 128 channels: 4 sequences with 131072 tokens 368 us, 5.8 TB/s of keys and
+// values, 64 with 200 to 16384 182, 5.3; one token of 8 heads over 376 9.5 us, of which the launch is 3 and
+// the chain row starts, length, page, key, value most of the rest. 16 drafts of 4 to 8 tokens over
+// up to 6000 (16 heads over 2 of 64 channels, a window, capped scores) 21.3 us: 10 before the first step, 1.7 a step, 4
+// for the join. f32, 16 chunks of up to 188 rows with windows of 376: 42 us, 23 of them the
+// matrix instructions, of which a SIMD has one wavefront or two.
 template <typename T>
 struct Step;
 template <>
@@ -891,13 +904,19 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
 }
 
 // The kernel of many rows, f16: a workgroup of 4 wavefronts with 32 rows each,
-// which share tiles of 64 tokens in LDS, two of them: while one is used, the next one's
-// loads are on their way, in registers, and are written to the other at the
-// end of the step. Keys are read as operands of v_mfma_f32_32x32x16_f16, 16 bytes of
+// which share tiles of 64 tokens in LDS, two of them: while one is used, the next one
+// is loaded straight to the other, 16 tokens by each wavefront; where some of these 16 are hidden or
+// have no page they go through registers, zeros in their places. Keys are read as operands of v_mfma_f32_32x32x16_f16, 16 bytes of
 // a token, values transposed, four tokens of a channel, in the order in which
 // the scores lie: scores 8u .. 8u + 7 of a lane are tokens 16u + 4 half + 0..3 and 8 more.
 // Both are laid out so that the lanes that read together read different banks: pieces
 // of 16 bytes of a key, and of 32 bytes of a value, are exchanged by a number of the row.
+//
+// 4 chunks of 700 to 1024 rows over up to 8192 tokens, 32 heads over 8 of 128 channels: 252 to 260 us, 780
+// TF where a large product reaches 1032; blocks of 64 rows by the kernel above took 1024. Matrix
+// instructions and exponentials hardly overlap: two wavefronts share a SIMD, and their sum is
+// the time. Pages of 8, 24 or 100 tokens take 275 to 277 us (through registers 378), heads of 96 and 80
+// channels 259 and 250 (361).
 template <int DP>
 struct ManyShape {
   static constexpr int kTokens = 64, kRows = 128;
@@ -982,15 +1001,29 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
   const auto key_piece = [&](uint32_t row) { return slot ^ key_turn(row); };
   const auto value_piece = [&](uint32_t row) { return (((slot >> 1) ^ value_turn(row)) << 1) | (slot & 1u); };
   // Tiles start at multiples of 16. Where pages hold a multiple of 16 tokens, the wavefront's 16 lie side by
-  // side, and what differs from lane to lane is the same for all tiles.
-  const bool runs = WHOLE && cache.page_size % 16u == 0;
+  // side, and what differs from lane to lane is the same for all tiles (4 chunks of 1024: 252 and not 268 us). Not
+  // beyond 128 channels, where its registers are not left: two chunks of 1024 131 us and not 241.
+  const bool runs = DP <= 128 && cache.page_size % 16u == 0;
   const uint32_t begin = part.low & ~15u;
   uint32_t key_offset[LOADS], value_offset[LOADS];
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
-    key_offset[i] = (staged_row(i) * VR + key_piece(staged_row(i))) * 16u;
-    value_offset[i] = (staged_row(i) * VR + value_piece(staged_row(i))) * 16u;
+    const uint32_t row = staged_row(i);
+    key_offset[i] = (row * map.row + key_piece(row)) * 16u;
+    value_offset[i] = (row * map.row + value_piece(row)) * 16u;
+    if constexpr (!WHOLE)  // pieces behind a head are never loaded
+#pragma unroll
+      for (int stage = 0; stage < 2; ++stage) {
+        T* k_to = tiles + stage * 2 * Shape::kTile + 16u * wave * DP + i * 512 + lane * 8u;
+        if (key_piece(row) >= pieces) *reinterpret_cast<half8*>(k_to) = half8{};
+        if (value_piece(row) >= pieces) *reinterpret_cast<half8*>(k_to + Shape::kTile) = half8{};
+      }
   }
+  const auto to_lds = [&](const uint8_t* from, T* to, bool there) {
+    if (WHOLE || there)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                       (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+  };
   // The entries of the next tile's tokens, or, of runs, of its four 16s in lanes 0 to 3.
   const auto next_entry = [&](uint32_t t0) { return map.entry(runs ? t0 + 16u * (lane & 3u) : t0 + lane, part.high); };
   uint32_t entry = next_entry(begin);
@@ -1011,10 +1044,8 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
         const uint64_t from = (uint64_t)map.place(ours, wave::of_lane(entry, wave)) * 16u;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(keys + from + key_offset[i]),
-                                           (__attribute__((address_space(3))) void*)(k_to + i * 512), 16, 0, 0);
-          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(values + from + value_offset[i]),
-                                           (__attribute__((address_space(3))) void*)(v_to + i * 512), 16, 0, 0);
+          to_lds(keys + from + key_offset[i], k_to + i * 512, key_piece(staged_row(i)) < pieces);
+          to_lds(values + from + value_offset[i], v_to + i * 512, value_piece(staged_row(i)) < pieces);
         }
       } else {
         places = held >> wave & 1u ? map.place(ours, wave::of_lane(entry, wave)) : 0u;
@@ -1022,8 +1053,17 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
     } else {
       const bool held = entry < map.count && t0 + lane >= part.low;
       live_next = __ballot(held);
-      whole = false;
+      whole = (live_next >> (16u * wave) & 0xffffu) == 0xffffu;
       places = held ? map.place(t0 + lane, entry) : 0u;
+      if (whole) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+          const uint32_t row = staged_row(i);
+          const uint64_t place = (uint32_t)__builtin_amdgcn_ds_bpermute((int)((16u * wave + row) * 4u), (int)places);
+          to_lds(keys + (place + key_piece(row)) * 16u, k_to + i * 512, key_piece(row) < pieces);
+          to_lds(values + (place + value_piece(row)) * 16u, v_to + i * 512, value_piece(row) < pieces);
+        }
+      }
     }
     if (!whole) {
 #pragma unroll
@@ -1176,8 +1216,10 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
   if (item.parts > 1u && half == 0) result.sums(r, m, l);
 }
 
-// Joins the parts of a unit: a wavefront takes a row, its lanes 4 channels each.
-constexpr int kJoinRows = 16;
+// Joins the parts of a unit: a wavefront takes a row, its lanes 4 channels each, 8 parts' loads at a
+// time. Some 5 us, the launch among them; 16 rows a workgroup instead of 4
+// cost 16 drafts 0.8 us.
+constexpr int kJoinRows = 4;
 template <typename T, int R>
 __global__ __launch_bounds__(64 * kJoinRows) void cache_attention_join_kernel(CacheAttentionArgs args, Plan plan) {
   const Workspace work = bind(args.workspace, plan, R);
@@ -1246,19 +1288,18 @@ Variant many(bool whole) {
 }
 
 // Rows of a unit: 16, 32 or 64 where the rows of an average sequence need no more, else
-// 128 (f16). The kernel of 64 rows holds heads of up to 64 channels; 33 to 64 rows of wider heads go
-// to the kernel of 128, or, where that fills the registers of a wavefront alone, beyond 128
-// channels, to two units of 32. f32 units end at 64, 32 and 16 rows for heads of up to 64, 128
-// and 256 channels. 16 sequences with 32 to 64 rows of 64 channels, 1500 to 6000 tokens: 64 rows
-// 22.2 us, 128 30.1. 8 sequences with 48 to 64 rows, up to 8192 tokens: 128 channels 47 us by
-// 64 rows (their outputs and keys fill the registers), 29 by 128, 41 by 32; 24 to 32 rows 25.8 by 32
-// rows, 25.6 by 128, and 64 such sequences of up to 1000 24.6 and 28.7. 8 with 64 rows of 256
-// channels, up to 4000: 56 by 32 rows, 63 by 128; with 128 rows 82 and 69.
+// 128 (f16). f16 units have 64 rows for heads of up to 64 channels: beyond, their outputs and keys
+// fill the registers. f32 units end at 64, 32 and 16 rows for heads of up to 64, 128 and 256
+// channels. 16 sequences with 32 to 64 rows of 64 channels, 1500 to 6000 tokens: 64 rows 22.2 us,
+// 128 30.1. 8 sequences with 48 to 64 rows of 128 channels, up to 8192 tokens: 47 us by 64 rows, 29
+// by 128, 41 by 32; 24 to 32 rows 25.8 by 32 rows, 25.6 by 128, and 64 such sequences of up to
+// 1000 24.6 and 28.7. Of 256 channels, 8 with 64 rows, up to 4000 tokens: 55.7 by 32, 38.7 by 128; with
+// 32 rows 32 and 36.5.
 uint32_t unit_rows(const CacheAttentionArgs& args) {
   const uint64_t group = args.heads / args.cache.kv_heads;
   const uint64_t rows = (args.cache.rows * group + args.cache.sequences - 1u) / args.cache.sequences;
   const uint32_t dim = args.cache.head_dim, most = args.f16 ? 128u : dim <= 64u ? 64u : dim <= 128u ? 32u : 16u;
-  const uint32_t wanted = rows <= 16u ? 16u : rows <= 32u ? 32u : rows > 64u ? 128u : dim <= 64u ? 64u : dim <= 128u ? 128u : 32u;
+  const uint32_t wanted = rows <= 16u ? 16u : rows <= 32u ? 32u : rows > 64u ? 128u : dim <= 64u ? 64u : 128u;
   return wanted < most ? wanted : most;
 }
 
@@ -1296,7 +1337,9 @@ Plan plan_of(const CacheAttentionArgs& args, uint32_t R) {
   Plan plan;
   // Full tiles of rows, and one that is not full for each sequence.
   plan.most_units = (uint32_t)(args.cache.kv_heads * (args.cache.rows * group / R + some));
-  plan.more = args.cache.capacity() > kShortest ? (R == 16u ? 1024u : R == 64u ? 256u : 512u) : 0u;
+  // Tokens that the rows of a unit see: of a window those before its first row's, and the unit's own.
+  const uint64_t own = (R - 1u) / group + 2u, seen = args.causal && args.window ? args.window + own : ~0ull;
+  plan.more = args.cache.capacity() > kShortest && seen > kShortest ? (R == 16u ? 1024u : R == 64u ? 256u : 512u) : 0u;
   plan.shortest = kShortest;
   plan.listed = args.cache.sequences > kUnlisted ? args.cache.sequences : 0u;
   return plan;

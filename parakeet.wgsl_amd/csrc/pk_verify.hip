@@ -4,16 +4,18 @@
 //
 // Decisions are whole numbers, so probabilities and sums are f64: a sum of
 // 131072 f32 exponentials moves with its order by more than the gap between two
-// neighbouring tokens of a flat distribution. An f64 operation takes the VALU no
-// longer than an f32 one; an exponential is some 20 of them, and bounds the
-// kernels: memory would feed twice as many.
+// neighbouring tokens of a flat distribution. An exponential through the table is
+// 10 operations of f64 and 7 others, and they bound the sums: 64 logits take a SIMD 115
+// cycles, where memory would feed twice as many.
 //
 // Short rows: one launch, a workgroup for each sequence. Its wavefronts take the
 // rows' sums, target and draft, side by side, the decisions are read from
 // them in turn, and all threads look for the next token. Long rows: a launch
 // for the sums of parts of all rows; one for each sequence and part that decides, every
 // workgroup for itself, and sums the part's weights; and one for each
-// sequence that finds the part and in it the token.
+// sequence that finds the part and in it the token. f16: a chunk of 5 rows of 1025 columns
+// 10.5 us; 32 chunks of 3 to 8 rows of 131072 with as many of the draft model's 50.5, of which the
+// sums of 36 million logits are 28, the weights 11 and the token 5, these two chains of dependent loads.
 #include "pk_internal.h"
 #include "pk_wave.h"
 
@@ -24,9 +26,11 @@ constexpr uint32_t kNoToken = 0xffffffffu;
 constexpr float kInf = __builtin_inff();
 constexpr int kThreads = 256;       // of a workgroup that holds a part of a row
 // Pieces of 16 bytes in a thread that sums a part of a row, and one that sums the
-// weights of a smaller part: those launches have fewer rows.
+// weights of a smaller part: those launches have fewer rows. 4 pieces for the sums take 53.5 us and not
+// 52.4 (32 x 8 x 131072), 8 for the weights 61.4.
 constexpr int kSumsHeld = 8, kHeld = 4;
 constexpr int kSequence = 1024;     // threads of a workgroup that holds a sequence
+constexpr uint32_t kShort = 4096;   // columns of a row that is short
 template <typename T>
 constexpr uint32_t kSumsSpan = kThreads * kSumsHeld * 16 / sizeof(T);  // columns of a part for the sums
 template <typename T>
@@ -390,7 +394,8 @@ __device__ __forceinline__ RowSum sum_row(const T* z, const double* table, uint3
 template <typename T>
 __global__ __launch_bounds__(kSequence) void verify_sequence_kernel(VerifyArgs args) {
   constexpr uint32_t kWaves = kSequence / 64;
-  constexpr int kRun = 16384 / sizeof(T) / kSequence;
+  constexpr int kRun = 16 / sizeof(T);
+  static_assert(kRun * kSequence >= (int)kShort, "a thread's columns");
   __shared__ double scratch[kWaves];
   __shared__ RowSum sums[kWaves];
   __shared__ uint32_t states[kWaves];
@@ -708,11 +713,11 @@ __global__ __launch_bounds__(kSequence) void verify_token_kernel(VerifyArgs args
   if (at == 0) args.next_tokens[s] = token;
 }
 
-// Rows of up to 16 KiB are read by one workgroup for a sequence, unless it has many.
-template <typename T>
-bool together(const VerifyArgs& args) {
-  return args.columns * sizeof(T) <= 16384u && args.rows <= 64ull * args.sequences;
-}
+// One workgroup for a sequence, or its rows in parts over many: the exponentials of 16 rows at a time, 8
+// with drafts, against two launches more. 12 rows of 1025 f16 columns, refused early or accepted to
+// the end: 14.6 and 20 us by one, 20.2 either way by many; 5 rows of 4096 16.8 and 19.8, 12 of 4096 19.1 to
+// 27.7 and 20.4, 30 of 4096 up to 56 and 25; 5 of 8192 26.8 and 23.1. f32: 5 of 4096 16 and 18.
+bool together(const VerifyArgs& args) { return args.columns <= kShort && args.rows <= 16ull * args.sequences; }
 
 template <typename Kernel, typename... Args>
 hipError_t launch(Kernel kernel, dim3 grid, dim3 block, hipStream_t stream, hipEvent_t start, hipEvent_t stop, Args... args) {
@@ -725,7 +730,7 @@ hipError_t launch(Kernel kernel, dim3 grid, dim3 block, hipStream_t stream, hipE
 
 template <typename T>
 hipError_t launch_typed(const VerifyArgs& args, hipStream_t stream, hipEvent_t start, hipEvent_t stop) {
-  if (together<T>(args))
+  if (together(args))
     return launch(verify_sequence_kernel<T>, dim3(args.sequences), dim3(kSequence), stream, start, stop, args);
   if (!args.workspace) return hipErrorInvalidValue;
   const uint32_t parts = parts_of<T>(args.columns), sequences = args.sequences;
@@ -745,7 +750,7 @@ uint64_t workspace_typed(const VerifyArgs& args) {
   // Fewer active sequences may no longer be together.
   VerifyArgs one = args;
   one.sequences = 1;
-  if (together<T>(one)) return 0;
+  if (together(one)) return 0;
   const uint64_t parts = parts_of<T>(args.columns);
   return 2ull * args.rows * sums_parts_of<T>(args.columns) * sizeof(RowSum) + args.sequences * (sizeof(End) + parts * sizeof(double2));
 }

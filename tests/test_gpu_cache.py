@@ -374,6 +374,24 @@ def test_chunks(abi, ctx, scope, dtype, counts, lengths, heads, kv_heads, dim, c
 
 
 @DTYPES
+@pytest.mark.parametrize("dim", [8, 40, 64, 80, 96, 128, 192, 256])
+@pytest.mark.parametrize("page_size", [1, 7, 16, 24, 48, 100])
+def test_pages_of_chunks(abi, ctx, scope, dtype, dim, page_size):
+    """Pages that end inside a tile, or hold some of its tokens, a page that is missing, and what lies behind a sequence."""
+    def spoil(cache, queries):
+        held = np.zeros(cache.pages * page_size, bool)
+        for s in range(cache.sequences):
+            for t in range(int(cache.lengths[s])):
+                held[cache.table[s, t // page_size] * page_size + t % page_size] = True
+        for x in (cache.keys, cache.values):
+            rows = x.reshape(cache.pages, 2, page_size, dim)
+            rows[~np.repeat(held.reshape(cache.pages, 1, page_size), 2, 1)] = np.nan
+        cache.table[0, 30 // page_size] = NO_PAGE
+    run_attention(abi, ctx, scope, np.random.default_rng(dim + page_size), dtype, [140, 66, 3], [150, 200, 77], 4, 2, dim,
+                  page_size, spoil=spoil)
+
+
+@DTYPES
 @pytest.mark.parametrize("counts", [[1, 1, 1], [6, 3, 1], [90, 40, 3]])
 @pytest.mark.parametrize("window", [1, 5, 32, 100, 10000])
 def test_windows(abi, ctx, scope, dtype, counts, window):
