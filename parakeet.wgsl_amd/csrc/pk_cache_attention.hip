@@ -915,8 +915,9 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
 // 4 chunks of 700 to 1024 rows over up to 8192 tokens, 32 heads over 8 of 128 channels: 252 to 260 us, 780
 // TF where a large product reaches 1032; blocks of 64 rows by the kernel above took 1024. Matrix
 // instructions and exponentials hardly overlap: two wavefronts share a SIMD, and their sum is
-// the time. Pages of 8, 24 or 100 tokens take 275 to 277 us (through registers 378), heads of 96 and 80
-// channels 259 and 250 (361).
+// the time. Pages of 8, 24 or 100 tokens take 270 to 274 us (through registers 378). Of DP channels of a tile
+// USED take part in the products, all or three quarters: heads of 96 and 80 channels 236 and 224 us, of
+// 192 among 256 380; with all 259, 250 and 447.
 template <int DP>
 struct ManyShape {
   static constexpr int kTokens = 64, kRows = 128;
@@ -925,13 +926,13 @@ struct ManyShape {
   static_assert(4 * kTile * 2 >= (int)(kMaxDim + kThreads + kWaves + kThreads) * 4, "the careful way's LDS");
 };
 
-template <int DP, bool WHOLE>
+template <int DP, int USED, bool WHOLE>
 __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_many_kernel(CacheAttentionArgs args,
                                                                                           Plan plan) {
   typedef _Float16 T;
   typedef ManyShape<DP> Shape;
   constexpr int R = Shape::kRows, STEP = Shape::kTokens;
-  constexpr int KS = DP / 16, DB = DP / 32, VR = DP / 8;
+  constexpr int KS = USED / 16, DB = USED / 32, VR = DP / 8;
   constexpr int LOADS = STEP * VR / kThreads;  // pieces of keys, and of values, of a thread
   __shared__ __attribute__((aligned(16))) uint8_t lds[Shape::kLds];
   const uint32_t lane = threadIdx.x & 63u, col = lane & 31u, half = lane >> 5;
@@ -1281,8 +1282,11 @@ Variant few(bool whole) {
 }
 
 template <int DP>
-Variant many(bool whole) {
-  return {whole ? cache_attention_many_kernel<DP, true> : cache_attention_many_kernel<DP, false>,
+Variant many(uint32_t dim) {
+  constexpr int kNarrow = DP > 64 ? DP / 4 * 3 : DP;
+  return {dim == (uint32_t)DP           ? cache_attention_many_kernel<DP, DP, true>
+          : dim <= (uint32_t)kNarrow ? cache_attention_many_kernel<DP, kNarrow, false>
+                                     : cache_attention_many_kernel<DP, DP, false>,
           cache_attention_list_kernel<ManyShape<DP>::kRows>, cache_attention_join_kernel<_Float16, ManyShape<DP>::kRows>,
           ManyShape<DP>::kRows};
 }
@@ -1304,22 +1308,22 @@ uint32_t unit_rows(const CacheAttentionArgs& args) {
 }
 
 template <typename T, int DP>
-Variant choose(uint32_t rows, bool whole) {
+Variant choose(uint32_t rows, uint32_t dim) {
   constexpr bool kHalf = sizeof(T) == 2;
   if constexpr (kHalf || DP <= 128)
-    if (rows == 32u) return few<T, DP, 2>(whole);
+    if (rows == 32u) return few<T, DP, 2>(dim == (uint32_t)DP);
   if constexpr (DP <= 64)
-    if (rows == 64u) return few<T, DP, 4>(whole);
+    if (rows == 64u) return few<T, DP, 4>(dim == (uint32_t)DP);
   if constexpr (kHalf)
-    if (rows == 128u) return many<DP>(whole);
-  return few<T, DP, 1>(whole);
+    if (rows == 128u) return many<DP>(dim);
+  return few<T, DP, 1>(dim == (uint32_t)DP);
 }
 template <typename T>
 Variant choose(const CacheAttentionArgs& args) {
   const uint32_t dim = args.cache.head_dim, rows = unit_rows(args);
-  if (dim <= 64u) return choose<T, 64>(rows, dim == 64u);
-  if (dim <= 128u) return choose<T, 128>(rows, dim == 128u);
-  return choose<T, 256>(rows, dim == 256u);
+  if (dim <= 64u) return choose<T, 64>(rows, dim);
+  if (dim <= 128u) return choose<T, 128>(rows, dim);
+  return choose<T, 256>(rows, dim);
 }
 
 // Tokens of a part at least, and workgroups beside one for each unit, of which parts are made: a
