@@ -1218,18 +1218,18 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
 }
 
 // Joins the parts of a unit: a wavefront takes a row, its lanes 4 channels each, 8 parts' loads at a
-// time. Some 5 us, the launch among them; 16 rows a workgroup instead of 4
-// cost 16 drafts 0.8 us.
-constexpr int kJoinRows = 4;
+// time. 4 to 6 us, the launch among them, whether there are parts or not. 4 rows a workgroup, 0.8 us less
+// for 16 drafts than 16 rows; units of 128 rows keep 16, as few of them are split (4 chunks of 1024 5.8 and 7.7).
+__host__ __device__ constexpr int join_rows(int R) { return R > 64 ? 16 : 4; }
 template <typename T, int R>
-__global__ __launch_bounds__(64 * kJoinRows) void cache_attention_join_kernel(CacheAttentionArgs args, Plan plan) {
+__global__ __launch_bounds__(64 * join_rows(R)) void cache_attention_join_kernel(CacheAttentionArgs args, Plan plan) {
   const Workspace work = bind(args.workspace, plan, R);
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   const Unit unit = work.units[blockIdx.x];
   if (blockIdx.x >= *work.units_count || unit.parts <= 1u) return;
   const uint32_t group = args.heads / args.cache.kv_heads, dim = args.cache.head_dim;
   const uint32_t d = 4u * lane < dim ? 4u * lane : 0u;  // all lanes take part in the exchange
-  const uint32_t r = blockIdx.y * kJoinRows + wave;
+  const uint32_t r = blockIdx.y * join_rows(R) + wave;
   if (r >= unit.rows) return;
   const float2* sums = work.sums + (uint64_t)unit.slot * R + r;
   float top = -kInf;
@@ -1385,7 +1385,9 @@ hipError_t launch_cache_attention(const CacheAttentionArgs& args, hipStream_t st
     hipLaunchKernelGGL(variant.kernel, grid, block, 0, stream, args, plan);
   if (const hipError_t e = hipGetLastError()) return e;
   if (!plan.more) return hipSuccess;
-  const dim3 units(plan.most_units, variant.rows / kJoinRows), joining(64 * kJoinRows);
+  // Each unit that is split has one of the workgroups beside the units' at least; of sorted sequences its units come first.
+  const uint32_t split = plan.listed || plan.most_units < plan.more ? plan.most_units : plan.more;
+  const dim3 units(split, variant.rows / join_rows(variant.rows)), joining(64 * join_rows(variant.rows));
   if (stop)
     hipExtLaunchKernelGGL(variant.join, units, joining, 0, stream, nullptr, stop, 0, args, plan);
   else
