@@ -519,15 +519,17 @@ __device__ __forceinline__ void careful_item(const CacheAttentionArgs& args, con
 //
 // The loads of a step's keys are issued when the step before has used its own, those of
 // its values likewise, and the entries of the page table a step ahead of the keys, before
-// the values: loads return in their order, and nothing waits for more than it needs. Keys two
-// steps ahead, in registers or in a ring of LDS, gained nothing.
+// the values: loads return in their order, and nothing waits for more than it needs. Keys and values
+// two steps ahead leave one wavefront a SIMD and twice the code: 201 us for 64 sequences below and
+// not 182, 10.2 for one token and not 9.5. Eight wavefronts a workgroup: 197, and 9.7.
 //
 // f16, 32 heads over 8 of 128 channels: 4 sequences with 131072 tokens 368 us, 5.8 TB/s of keys and
-// values, 64 with 200 to 16384 182, 5.3; one token of 8 heads over 376 9.5 us, of which the launch is 3 and
-// the chain row starts, length, page, key, value most of the rest. 16 drafts of 4 to 8 tokens over
-// up to 6000 (16 heads over 2 of 64 channels, a window, capped scores) 21.3 us: 10 before the first step, 1.7 a step, 4
-// for the join. f32, 16 chunks of up to 188 rows with windows of 376: 42 us, 23 of them the
-// matrix instructions, of which a SIMD has one wavefront or two.
+// values, 64 with 200 to 16384 182, 5.3. One token of 8 heads over 376 9.5 us, by the clock from the
+// first instruction on: 1.0 for the item, 0.5 for the pages, 2.1 for keys, values and queries, 3.1 for
+// three steps, 1.4 for the end; the launch is the rest. 16 drafts of 4 to 8 tokens over up to 6000 (16
+// heads over 2 of 64 channels, a window, capped scores) 21.3 us: 1.8, 0.9, 1.8, 8 for four steps,
+// 2.7, then the join. f32, 16 chunks of up to 188 rows with windows of 376: 42 us, 23 of them
+// the matrix instructions, of which a SIMD has one wavefront or two.
 template <typename T>
 struct Step;
 template <>
