@@ -306,6 +306,7 @@ int pk_cache_attention_create(pk_context* ctx, const pk_cache_attention_desc* d,
   a.query_stride = stride_of(d->query_stride, d->heads, d->head_dim);
   a.output_stride = stride_of(d->output_stride, d->heads, d->head_dim);
   a.heads = d->heads;
+  a.group.set(d->heads / d->kv_heads);
   a.window = d->window;
   a.scale = d->has_scale ? d->scale : (float)(1.0 / std::sqrt((double)d->head_dim));
   a.cap = d->score_cap;

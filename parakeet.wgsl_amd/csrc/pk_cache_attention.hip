@@ -142,7 +142,7 @@ __device__ __forceinline__ Listed look_at(const CacheAttentionArgs& args, uint32
     const uint32_t end = min(cache.row_starts[s + 1], cache.rows), length = cache.lengths[s];
     x.length = length;
     x.count = end > x.start ? end - x.start : 0u;
-    x.tiles = (x.count * (args.heads / cache.kv_heads) + R - 1u) / R;
+    x.tiles = (x.count * args.group.by + R - 1u) / R;
     const Seen seen = seen_by(args, length, (int64_t)length - x.count, x.count);
     x.span = x.count ? max(1u, seen.high - seen.low) : 0u;
   }
@@ -163,7 +163,7 @@ __device__ __forceinline__ uint32_t parts_of(uint32_t span, uint32_t longest) {
 // Item `index` of a sequence whose sums count it: the sums of those before it are these less its own.
 template <int R>
 __device__ __forceinline__ Item item_in(const CacheAttentionArgs& args, const Listed& x, uint32_t index) {
-  const uint32_t units = x.tiles * args.cache.kv_heads, items = units * x.parts, group = args.heads / args.cache.kv_heads;
+  const uint32_t units = x.tiles * args.cache.kv_heads, items = units * x.parts, group = args.group.by;
   const uint32_t local = index - (x.items_to - items), unit = local / x.parts;
   Item item;
   item.live = local < items;  // else from sums past 32 bits: of row starts that decrease
@@ -378,7 +378,7 @@ struct Places {
       : table(c.page_table + (uint64_t)sequence * c.pages_per_sequence),
         row((uint32_t)(c.head_dim * sizeof(T) / 16u)), page((uint32_t)(c.page_stride * sizeof(T) / 16u)),
         head(kv * c.page_size * (uint32_t)(c.head_dim * sizeof(T) / 16u)), count(c.pages), size(c.page_size),
-        magic(c.page_magic), shift(c.page_shift) {}
+        magic(c.page.magic), shift(c.page.shift) {}
   static constexpr uint32_t none = 0xffffffffu;
   __device__ __forceinline__ uint32_t at(uint32_t token) const {
     return (uint32_t)(((uint64_t)token * magic) >> shift);
@@ -394,8 +394,7 @@ struct Places {
 
 // The part [from, to) of the tokens that an item works on.
 __device__ __forceinline__ Seen part_of(const CacheAttentionArgs& args, const Item& item) {
-  const uint32_t group = args.heads / args.cache.kv_heads;
-  const uint32_t token = item.first / group, last = (item.first + item.rows - 1u) / group;
+  const uint32_t token = args.group.under(item.first), last = args.group.under(item.first + item.rows - 1u);
   const Seen all = seen_by(args, item.length, item.position + token, last - token + 1u);
   if (item.parts == 1u) return all;
   const uint32_t each = ((all.high - all.low) / item.parts + 32u) & ~31u;
@@ -410,7 +409,7 @@ struct Result {
   const Item& item;
   const Workspace& work;
   __device__ T* output(uint32_t r) const {
-    const uint32_t group = args.heads / args.cache.kv_heads, i = item.first + r, token = i / group;
+    const uint32_t group = args.group.by, i = item.first + r, token = args.group.under(i);
     return static_cast<T*>(args.output) + (item.row + token) * args.output_stride +
            (uint64_t)(item.head * group + (i - token * group)) * args.cache.head_dim;
   }
@@ -454,14 +453,14 @@ __device__ __forceinline__ void careful_item(const CacheAttentionArgs& args, con
   float *query = lds, *weight = lds + kMaxDim, *scratch = weight + kThreads;
   uint32_t* places = reinterpret_cast<uint32_t*>(scratch + kWaves);
   const CacheView& cache = args.cache;
-  const uint32_t at = threadIdx.x, dim = cache.head_dim, group = args.heads / cache.kv_heads;
+  const uint32_t at = threadIdx.x, dim = cache.head_dim, group = args.group.by;
   const Seen part = part_of(args, item);
   const Places<T> map(cache, item.sequence, item.head);
   const Score<T> score(args);
   const Result<T, R> result{args, item, work};
   constexpr uint32_t kPiece = 16 / sizeof(T);
   for (uint32_t r = 0; r < item.rows; ++r) {
-    const uint32_t i = item.first + r, token = i / group;
+    const uint32_t i = item.first + r, token = args.group.under(i);
     const Seen own = seen_by(args, item.length, item.position + token);
     const uint32_t low = max(own.low, part.low), high = min(own.high, part.high);
     const T* q = static_cast<const T*>(args.queries) + (item.row + token) * args.query_stride +
@@ -580,7 +579,7 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
   if (plan.more && item.part == 0 && item.unit < plan.most_units && threadIdx.x == 0)
     work.units[item.unit] = {item.slot, item.parts, item.row, item.rows, item.head, item.first};
   const Seen part = part_of(args, item);
-  const uint32_t group = args.heads / cache.kv_heads, dim = cache.head_dim;
+  const uint32_t group = args.group.by, dim = cache.head_dim;
   const Places<T> map(cache, item.sequence, item.head);
   const Score<T> score(args);
   const uint32_t pieces = dim / PIECE;
@@ -589,7 +588,7 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
   constexpr bool kInLds = Shape::kQueriesInLds;
   uint8_t* query_rows = lds + Shape::kSums + 16 + kWaves * Shape::kValueBytes;
   const auto query_piece = [&](uint32_t r, uint32_t c) {
-    const uint32_t i = item.first + r, token = i / group;
+    const uint32_t i = item.first + r, token = args.group.under(i);
     const T* q = static_cast<const T*>(args.queries) + (item.row + token) * args.query_stride +
                  (uint64_t)(item.head * group + (i - token * group)) * dim + c * PIECE;
     V x = V{};
@@ -615,14 +614,14 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
     const uint32_t r = 16u * b + col;
-    const Seen own = seen_by(args, item.length, item.position + (item.first + r) / group);
+    const Seen own = seen_by(args, item.length, item.position + args.group.under(item.first + r));
     low[b] = r < item.rows ? own.low : 0u;
     high[b] = r < item.rows ? own.high : 0u;
   }
   // Tokens that all rows of the unit see.
   uint32_t common_low = 0, common_high = 0xffffffffu;
   {
-    const uint32_t t0 = item.first / group, t1 = (item.first + item.rows - 1u) / group;
+    const uint32_t t0 = args.group.under(item.first), t1 = args.group.under(item.first + item.rows - 1u);
     common_high = seen_by(args, item.length, item.position + t0).high;
     common_low = seen_by(args, item.length, item.position + t1).low;
   }
@@ -946,7 +945,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
   if (plan.more && item.part == 0 && item.unit < plan.most_units && threadIdx.x == 0)
     work.units[item.unit] = {item.slot, item.parts, item.row, item.rows, item.head, item.first};
   const Seen part = part_of(args, item);
-  const uint32_t group = args.heads / cache.kv_heads, dim = cache.head_dim;
+  const uint32_t group = args.group.by, dim = cache.head_dim;
   const Places<T> map(cache, item.sequence, item.head);
   const Score<T> score(args);
   const uint32_t pieces = dim / 8u;
@@ -958,7 +957,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
 #pragma unroll
   for (int k = 0; k < KS; ++k) query[k] = half8{};
   if (r < item.rows) {
-    const uint32_t i = item.first + r, token = i / group;
+    const uint32_t i = item.first + r, token = args.group.under(i);
     const Seen own = seen_by(args, item.length, item.position + token);
     low = own.low;
     high = own.high;
@@ -980,7 +979,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
   }
   Seen any = {0, 0}, all = {0, 0};
   if (32u * wave < item.rows) {
-    const uint32_t first = (item.first + 32u * wave) / group, last = (item.first + min(item.rows, 32u * wave + 32u) - 1u) / group;
+    const uint32_t first = args.group.under(item.first + 32u * wave), last = args.group.under(item.first + min(item.rows, 32u * wave + 32u) - 1u);
     const Seen a = seen_by(args, item.length, item.position + first), b = seen_by(args, item.length, item.position + last);
     all = {b.low, a.high};
     any = {a.low, b.high};
@@ -1229,7 +1228,7 @@ __global__ __launch_bounds__(64 * join_rows(R)) void cache_attention_join_kernel
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   const Unit unit = work.units[blockIdx.x];
   if (blockIdx.x >= *work.units_count || unit.parts <= 1u) return;
-  const uint32_t group = args.heads / args.cache.kv_heads, dim = args.cache.head_dim;
+  const uint32_t group = args.group.by, dim = args.cache.head_dim;
   const uint32_t d = 4u * lane < dim ? 4u * lane : 0u;  // all lanes take part in the exchange
   const uint32_t r = blockIdx.y * join_rows(R) + wave;
   if (r >= unit.rows) return;
@@ -1263,7 +1262,7 @@ __global__ __launch_bounds__(64 * join_rows(R)) void cache_attention_join_kernel
   }
   all = wave::sum(all);
   x *= inverse(top, all);
-  const uint32_t i = unit.first + r, token = i / group;
+  const uint32_t i = unit.first + r, token = args.group.under(i);
   T* to = static_cast<T*>(args.output) + (unit.row + token) * args.output_stride +
           (uint64_t)(unit.head * group + (i - token * group)) * dim + d;
   if (4u * lane < dim)
@@ -1302,7 +1301,7 @@ Variant many(uint32_t dim) {
 // 1000 24.6 and 28.7. Of 256 channels, 8 with 64 rows, up to 4000 tokens: 55.7 by 32, 38.7 by 128; with
 // 32 rows 32 and 36.5.
 uint32_t unit_rows(const CacheAttentionArgs& args) {
-  const uint64_t group = args.heads / args.cache.kv_heads;
+  const uint64_t group = args.group.by;
   const uint64_t rows = (args.cache.rows * group + args.cache.sequences - 1u) / args.cache.sequences;
   const uint32_t dim = args.cache.head_dim, most = args.f16 ? 128u : dim <= 64u ? 64u : dim <= 128u ? 32u : 16u;
   const uint32_t wanted = rows <= 16u ? 16u : rows <= 32u ? 32u : rows > 64u ? 128u : dim <= 64u ? 64u : 128u;
@@ -1338,7 +1337,7 @@ Variant choose(const CacheAttentionArgs& args) {
 constexpr uint32_t kShortest = 512;
 
 Plan plan_of(const CacheAttentionArgs& args, uint32_t R) {
-  const uint64_t group = args.heads / args.cache.kv_heads;
+  const uint64_t group = args.group.by;
   const uint32_t some = args.cache.sequences < args.cache.rows ? args.cache.sequences : args.cache.rows;
   Plan plan;
   // Full tiles of rows, and one that is not full for each sequence.

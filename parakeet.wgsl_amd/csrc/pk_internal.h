@@ -440,6 +440,20 @@ hipError_t launch_q4_layout(const Q4Args& args, const uint32_t* packed, const vo
 uint64_t q4_workspace(const Q4Args& args);
 hipError_t launch_q4(const Q4Args& args, hipStream_t stream, hipEvent_t start = nullptr, hipEvent_t stop = nullptr);
 
+// x / by = x * magic >> shift, up to 2^30: with s = floor(log2 by), magic = floor(2^(31 + s) / by) + 1 is
+// off by less than 2^-(31 + s) of 1 / by, less than 1 / by in all.
+struct Divisor {
+  uint32_t by, magic, shift;
+  __host__ void set(uint32_t x) {
+    uint32_t s = 0;
+    while ((x >> s) > 1u) ++s;
+    by = x;
+    shift = 31u + s;
+    magic = (uint32_t)((1ull << shift) / x + 1u);
+  }
+  __device__ uint32_t under(uint32_t x) const { return (uint32_t)(((uint64_t)x * magic) >> shift); }
+};
+
 // The paged cache of include/pk_cache.h: what append and attention share.
 // Strides in elements.
 struct CacheView {
@@ -452,28 +466,21 @@ struct CacheView {
   uint32_t pages_per_sequence;
   uint32_t pages;
   uint32_t page_size;
-  uint32_t page_magic;         // t / page_size = t * page_magic >> page_shift
-  uint32_t page_shift;
+  Divisor page;
   uint32_t kv_heads;
   uint32_t head_dim;
 
-  // With s = floor(log2 size), magic = floor(2^(31 + s) / size) + 1 is off by
-  // less than 2^(s + 1) / 2^(31 + s) of a page a token: exact below 2^30 tokens.
   __host__ void set_page_size(uint32_t size) {
-    uint32_t s = 0;
-    while ((size >> s) > 1u) ++s;
     page_size = size;
-    page_shift = 31u + s;
-    page_magic = (uint32_t)((1ull << page_shift) / size + 1u);
+    page.set(size);
   }
-  __device__ uint32_t page_of(uint32_t token) const { return (uint32_t)(((uint64_t)token * page_magic) >> page_shift); }
   // Tokens that the tables have places for.
   __host__ __device__ uint32_t capacity() const { return pages_per_sequence * page_size; }
   // Element of a token's row for kv head 0 (others follow page_size * head_dim
   // elements apart), or no_place.
   static constexpr uint64_t no_place = ~0ull;
   __device__ uint64_t place(uint32_t sequence, uint32_t token) const {
-    const uint32_t at = page_of(token);
+    const uint32_t at = page.under(token);
     const uint32_t page = page_table[(uint64_t)sequence * pages_per_sequence + at];
     return page < pages ? page * page_stride + (uint64_t)(token - at * page_size) * head_dim : no_place;
   }
@@ -503,6 +510,7 @@ struct CacheAttentionArgs {
   const void *key_cache, *value_cache;
   uint64_t query_stride, output_stride;
   uint32_t heads;
+  Divisor group;    // heads / kv_heads
   uint32_t window;  // tokens a row sees, 0: all
   float scale;
   float cap;        // of the scores, 0: none
