@@ -518,16 +518,17 @@ __device__ __forceinline__ void careful_item(const CacheAttentionArgs& args, con
 //
 // The loads of a step's keys are issued when the step before has used its own, those of
 // its values likewise, and the entries of the page table a step ahead of the keys, before
-// the values: loads return in their order, and nothing waits for more than it needs. Keys and values
+// the values: loads return in their order, and nothing waits for more than it needs; of the first
+// step the queries come between keys and values (f32 chunks below 40 us, behind them 41). Keys and values
 // two steps ahead leave one wavefront a SIMD and twice the code: 201 us for 64 sequences below and
-// not 182, 10.2 for one token and not 9.5. Eight wavefronts a workgroup: 197, and 9.7.
+// not 182, 10.2 for one token where one was 9.5. Eight wavefronts a workgroup: 197, and 9.7.
 //
 // f16, 32 heads over 8 of 128 channels: 4 sequences with 131072 tokens 368 us, 5.8 TB/s of keys and
-// values, 64 with 200 to 16384 182, 5.3. One token of 8 heads over 376 9.5 us, by the clock from the
+// values, 64 with 200 to 16384 182, 5.3. One token of 8 heads over 376 9.3 us, by the clock from the
 // first instruction on: 1.0 for the item, 0.5 for the pages, 2.1 for keys, values and queries, 3.1 for
 // three steps, 1.4 for the end; the launch is the rest. 16 drafts of 4 to 8 tokens over up to 6000 (16
-// heads over 2 of 64 channels, a window, capped scores) 21.3 us: 1.8, 0.9, 1.8, 8 for four steps,
-// 2.7, then the join. f32, 16 chunks of up to 188 rows with windows of 376: 42 us, 23 of them
+// heads over 2 of 64 channels, a window, capped scores) 20.7 us: 1.8, 0.9, 1.8, 8 for four steps,
+// 2.7, then the join. f32, 16 chunks of up to 188 rows with windows of 376: 40 us, 23 of them
 // the matrix instructions, of which a SIMD has one wavefront or two.
 template <typename T>
 struct Step;
@@ -599,11 +600,12 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
 #pragma unroll
         for (int e = 0; e < PIECE; ++e) x[e] = q[e];
       }
-      x *= (T)score.sign;
     }
     return x;
   };
-  V held[kInLds ? 1 : KS];
+  constexpr int QUERIES = kInLds ? R * VR / kThreads : KS;  // pieces of a thread; on their way to LDS
+  static_assert(!kInLds || R * VR % kThreads == 0, "whole rounds of pieces");
+  V held[QUERIES];
   const auto query = [&](int b, int k) {
     if constexpr (kInLds)
       return *reinterpret_cast<const V*>(query_rows + (16u * b + col) * Shape::kQueryRow + (4u * k + quarter) * 16u);
@@ -688,15 +690,22 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
     places = places_of(t0, &live);
     load_keys(places);
     entry = map.entry(t0 + kStride + mine, part.high);
-    load_values(places, live);
   }
-  if constexpr (kInLds) {
-    for (uint32_t i = threadIdx.x; i < R * VR; i += kThreads)
-      *reinterpret_cast<V*>(query_rows + i / VR * Shape::kQueryRow + i % VR * 16u) = query_piece(i / VR, i % VR);
-    __syncthreads();
-  } else {
 #pragma unroll
-    for (int k = 0; k < KS; ++k) held[k] = query_piece(col, 4u * k + quarter);
+  for (int i = 0; i < QUERIES; ++i) {
+    const uint32_t at = threadIdx.x + i * kThreads;
+    held[i] = kInLds ? query_piece(at / VR, at % VR) : query_piece(col, 4u * i + quarter);
+  }
+  if (t0 < part.high) load_values(places, live);
+#pragma unroll
+  for (int i = 0; i < QUERIES; ++i) held[i] *= (T)score.sign;
+  if constexpr (kInLds) {
+#pragma unroll
+    for (int i = 0; i < QUERIES; ++i) {
+      const uint32_t at = threadIdx.x + i * kThreads;
+      *reinterpret_cast<V*>(query_rows + at / VR * Shape::kQueryRow + at % VR * 16u) = held[i];
+    }
+    __syncthreads();
   }
   for (; t0 < part.high; t0 += kStride) {
     floatx4 s[RB][TB];
