@@ -545,6 +545,40 @@ def test_long_among_many_sequences(abi, ctx, scope, dtype):
 
 
 @DTYPES
+@pytest.mark.parametrize("sequences,longest", [(3, 2000), (90, 100), (90, 900)])
+def test_replays_follow_lengths(abi, ctx, scope, dtype, sequences, longest):
+    """One graph, lengths and rows of each replay its own; eager and timed launches between them."""
+    rng = np.random.default_rng(21)
+    counts = list(rng.integers(1, 5, sequences))
+    cache = Cache(rng, dtype, counts, [longest] * sequences, 2, 64, 16)
+    queries = rng.standard_normal((cache.rows, 4 * 64)).astype(dtype)
+    output = scope.put(np.zeros((cache.rows, 4 * 64), dtype))
+    op = abi.CacheAttentionOp(ctx, queries=scope.put(queries), output=output, heads=4, **cache.put(scope))
+    graph = abi.Graph.capture(ctx, ctx.stream)
+    with graph:
+        op.enqueue(0, ctx.stream)
+    start, end = abi.Event(ctx), abi.Event(ctx)
+    for i in range(4):
+        cache.lengths = rng.integers(4, longest + 1, sequences).astype(np.uint32)
+        cache.counts = list(rng.permutation(cache.counts))
+        cache.starts = np.concatenate([[0], np.cumsum(cache.counts)]).astype(np.uint32)
+        cache.device["lengths"].upload(cache.lengths)
+        cache.device["row_starts"].upload(cache.starts)
+        output.upload(np.zeros((cache.rows, 4 * 64), dtype))
+        ctx.synchronize()
+        if i % 2:
+            op.enqueue(0, start=start, end=end)
+        else:
+            graph.launch()
+        ctx.synchronize()
+        if i % 2:
+            assert 0 < start.elapsed_ms(end) < 100
+        check_attention(cache, output.download(), queries, 4)
+    graph.release()
+    op.release()
+
+
+@DTYPES
 @pytest.mark.parametrize("sequences,length", [(4, 60), (4, 3000), (70, 60), (70, 3000)])
 def test_starts_that_decrease(abi, ctx, scope, dtype, sequences, length):
     """Rows that only the first sequence has are right, whatever those of several
