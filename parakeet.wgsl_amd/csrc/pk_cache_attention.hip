@@ -528,7 +528,7 @@ __device__ __forceinline__ void careful_item(const CacheAttentionArgs& args, con
 // first instruction on: 1.0 for the item, 0.5 for the pages, 2.1 for keys, values and queries, 3.1 for
 // three steps, 1.4 for the end; the launch is the rest. 16 drafts of 4 to 8 tokens over up to 6000 (16
 // heads over 2 of 64 channels, a window, capped scores) 20.7 us: 1.8, 0.9, 1.8, 8 for four steps,
-// 2.7, then the join. f32, 16 chunks of up to 188 rows with windows of 376: 40 us, 23 of them
+// 2.7, then the join. f32, 16 chunks of up to 188 rows with windows of 376: 40 to 42 us, 23 of them
 // the matrix instructions, of which a SIMD has one wavefront or two.
 template <typename T>
 struct Step;
@@ -1312,7 +1312,7 @@ Variant many(uint32_t dim) {
 // 128 30.1. 8 sequences with 48 to 64 rows of 128 channels, up to 8192 tokens: 47 us by 64 rows, 29
 // by 128, 41 by 32; 24 to 32 rows 25.8 by 32 rows, 25.6 by 128, and 64 such sequences of up to
 // 1000 24.6 and 28.7. Of 256 channels, 8 with 64 rows, up to 4000 tokens: 55.7 by 32, 38.7 by 128; with
-// 32 rows 32 and 36.5.
+// 32 rows 32 and 36.5. f32, 256 channels, 4 chunks of 512: 937 us by 16 rows, 1402 by 32, which spill.
 uint32_t unit_rows(const CacheAttentionArgs& args) {
   const uint64_t group = args.group.by;
   const uint64_t rows = (args.cache.rows * group + args.cache.sequences - 1u) / args.cache.sequences;
