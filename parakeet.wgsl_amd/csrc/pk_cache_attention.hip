@@ -202,6 +202,16 @@ __device__ __forceinline__ Item find_item(const CacheAttentionArgs& args, const 
     at = base + (uint32_t)__builtin_ctzll(hit);
     return item_in<R>(args, work.list[at], index);
   }
+  if (cache.sequences == 1u) {  // no sums over lanes: one token over 300 to 2000 0.4 us less
+    Listed only = look_at<R>(args, 0);
+    const uint32_t units = only.tiles * cache.kv_heads;
+    only.parts = parts_of(only.span, longest_part(plan, units, (float)units * (float)only.span));
+    only.units_to = units;
+    only.items_to = units * only.parts;
+    only.slots_to = only.parts > 1u ? only.items_to : 0u;
+    if (plan.more && blockIdx.x == 0 && threadIdx.x == 0) *work.units_count = units > plan.most_units ? 0u : units;
+    return index < only.items_to ? item_in<R>(args, only, index) : none;
+  }
   Listed mine = look_at<R>(args, lane);
   const uint32_t units = wave::reduce_bits(mine.tiles * cache.kv_heads, 0u, [](uint32_t a, uint32_t b) { return a + b; });
   const float tokens = wave::sum((float)(mine.tiles * cache.kv_heads) * (float)mine.span);
@@ -524,8 +534,8 @@ __device__ __forceinline__ void careful_item(const CacheAttentionArgs& args, con
 // not 182, 10.2 for one token where one was 9.5. Eight wavefronts a workgroup: 197, and 9.7.
 //
 // f16, 32 heads over 8 of 128 channels: 4 sequences with 131072 tokens 368 us, 5.8 TB/s of keys and
-// values, 64 with 200 to 16384 182, 5.3. One token of 8 heads over 376 9.3 us, by the clock from the
-// first instruction on: 1.0 for the item, 0.5 for the pages, 2.1 for keys, values and queries, 3.1 for
+// values, 64 with 200 to 16384 182, 5.3. One token of 8 heads over 376 9.0 us, by the clock from the
+// first instruction on: 0.7 for the item, 0.5 for the pages, 2.1 for keys, values and queries, 3.1 for
 // three steps, 1.4 for the end; the launch is the rest. 16 drafts of 4 to 8 tokens over up to 6000 (16
 // heads over 2 of 64 channels, a window, capped scores) 20.7 us: 1.8, 0.9, 1.8, 8 for four steps,
 // 2.7, then the join. f32, 16 chunks of up to 188 rows with windows of 376: 40 to 42 us, 23 of them
