@@ -61,7 +61,7 @@ extern "C" {
 #define PK_CACHE_MAX_PAGE_SIZE 65536u
 #define PK_CACHE_MAX_TOKENS 1073741824u           /* page_size * pages_per_sequence */
 #define PK_CACHE_MAX_BYTES (64ull << 30)          /* of one cache binding's extent */
-#define PK_CACHE_MAX_UNITS 4000000u               /* attention: rows * heads / 16 + kv_heads * sequences */
+#define PK_CACHE_MAX_UNITS 4000000u               /* attention: rows * heads / 16 + kv_heads * min(sequences, rows) */
 
 typedef enum pk_rotary_kind {
   PK_ROTARY_HALVES = 0,
