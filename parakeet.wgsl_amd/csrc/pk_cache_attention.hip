@@ -1277,10 +1277,9 @@ __global__ __launch_bounds__(64 * join_rows(R)) void cache_attention_join_kernel
       for (uint32_t j = 0; j < 8u; ++j)
         some[j] = *reinterpret_cast<const floatx4*>(from + (uint64_t)min(i + j, count - 1u) * R * dim);
 #pragma unroll
-      for (uint32_t j = 0; j < 8u; ++j) {
-        const uint32_t bits = (uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(factor), (int)min(i + j, 63u));
-        x += some[j] * (i + j < count ? __uint_as_float(bits) : 0.0f);
-      }
+      for (uint32_t j = 0; j < 8u; ++j)
+        if (i + j < count)  // and no product with 0 else, which an infinity would spoil
+          x += some[j] * __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(factor), (int)(i + j)));
     }
   }
   all = wave::sum(all);
