@@ -223,7 +223,7 @@ struct Weights {
   __device__ __forceinline__ double of(float target, float draft, uint32_t i, double* whole) const {
 #pragma clang fp contract(off)  // equal probabilities leave 0
     double w = p.at(target) * inverse;
-    *whole = w;
+    *whole = w > kLeast ? w : 0.0;  // as it counts where p is drawn from: a part that is masked whole has none
     if (y) w -= q.at(draft) * draft_inverse;
     else if (residual && i == refused) w -= 1.0;
     return w > kLeast ? w : 0.0;
