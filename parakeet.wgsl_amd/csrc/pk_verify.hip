@@ -243,9 +243,10 @@ struct Weights {
   }
 };
 
-// A draw of [0, 1) of the whole weight; below it none, above it all.
+// A draw of [0, 1) of the whole weight; below it none. Above it, or NaN, more than all: not the whole
+// itself, which a running sum, taken in another order, may pass by a rounding before the last token.
 __device__ __forceinline__ double wanted(float draw, double whole) {
-  return draw > 0.0f ? (draw < 1.0f ? (double)draw * whole : whole) : draw <= 0.0f ? 0.0 : whole;
+  return draw <= 0.0f ? 0.0 : draw < 1.0f ? (double)draw * whole : (double)kInf;
 }
 
 // Of a workgroup of kSequence threads: the sum of x over the threads before this one, and over all.

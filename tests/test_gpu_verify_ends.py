@@ -38,3 +38,16 @@ def test_masked_parts(abi, ctx, scope, dtype, columns, rows_each, lowest, residu
     want = verify.check(abi, ctx, scope, case)
     assert (want[0] == 0).all() and ((want[1] >= first) & (want[1] < last)).all()
     assert want[1][0] == first and want[1][2] == last - 1
+
+
+@DTYPES
+@pytest.mark.parametrize("columns", [70, 1025, 4096, 20000, 131072])
+def test_draws_from_one_on(abi, ctx, scope, dtype, columns):
+    """The last token with a weight, be that far below the sum's last digit."""
+    rng = np.random.default_rng(columns)
+    case = single_rows(rng, dtype, 48, columns)
+    case["target"][:, -1] = -45
+    case["target"][::3, columns // 2 + 1:] = -40
+    case["draws"][:] = np.resize(np.array([1.0, np.nan, 2.0, np.inf], np.float32), 48)
+    want = verify.check(abi, ctx, scope, case)
+    assert (want[1] == columns - 1).all()
