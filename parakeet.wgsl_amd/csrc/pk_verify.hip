@@ -199,7 +199,7 @@ struct Judged {
     if (args.draft) drafted = (float)(static_cast<const T*>(args.draft) + row * args.draft_stride)[draft];
   }
   __device__ bool stands(const VerifyArgs& args, const RowSum& p, const RowSum& q) const {
-    const double pd = exp2_of(((double)target - p.m) * args.scale) / p.sum;
+    const double power = exp2_of(((double)target - p.m) * args.scale) / p.sum, pd = power > kLeast ? power : 0.0;
     const double qd = args.draft ? exp2_of(((double)drafted - q.m) * args.scale) / q.sum : 1.0;
     return (double)uniform * qd < pd;
   }

@@ -51,3 +51,19 @@ def test_draws_from_one_on(abi, ctx, scope, dtype, columns):
     case["draws"][:] = np.resize(np.array([1.0, np.nan, 2.0, np.inf], np.float32), 48)
     want = verify.check(abi, ctx, scope, case)
     assert (want[1] == columns - 1).all()
+
+
+@pytest.mark.parametrize("columns", [100, 9000])
+def test_probabilities_that_count_as_zero(abi, ctx, scope, columns):
+    """Below 2^-990: a draft of that probability is refused, even by a uniform of 0, and is not drawn."""
+    case = verify.make(np.random.default_rng(1), np.float32, [2, 2], columns, drafted=False)
+    case["target"][:] = -1e30
+    case["target"][:, 7] = 0
+    case["target"][0, 50] = -685          # 2^-988
+    case["target"][2, 50] = -690          # 2^-995
+    case["tokens"][:] = 50
+    case["uniforms"][:] = 0
+    case["draws"][:] = [1.0, 1.0]
+    got = verify.run(abi, ctx, scope, case)
+    assert list(got[0]) == [1, 0]
+    assert list(got[1]) == [7, 7]
