@@ -525,7 +525,7 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs args, 
   const uint32_t edge = part.first + (at < part.head ? at : part.head + part.vectors * VEC + (at - part.head));
   const float single = at < part.head + part.tail ? (float)z[edge] : -kInf;
   const bool needed = is_needed(args, row, which);
-  make_table<kThreads>(table);
+  if (!args.greedy) make_table<kThreads>(table);
   if (!needed) return;
   RowSum sum;
   if (args.greedy) {
@@ -625,7 +625,7 @@ __global__ __launch_bounds__(kThreads) void verify_weights_kernel(VerifyArgs arg
   __shared__ RowSum sums[kThreads / 16];
   __shared__ uint32_t states[kThreads / 32];
   __shared__ double table[kTable];
-  make_table<kThreads>(table);
+  if (!args.greedy) make_table<kThreads>(table);
   const uint32_t s = blockIdx.x, part_index = blockIdx.y, at = threadIdx.x;
   const Workspace work = bind<T>(args, sequences);
   const End end = find_end<T>(args, work, s, sums_parts_of<T>(args.columns), sums, states);
