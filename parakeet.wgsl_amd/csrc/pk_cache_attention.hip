@@ -349,13 +349,13 @@ __global__ __launch_bounds__(kListThreads) void cache_attention_list_kernel(Cach
   if (at == 0) *work.units_count = units > plan.most_units ? 0u : units;
 }
 
-// tanh: by the exponential, within 2^-23, which is enough beside the f16 rounding of the weights; f32: near 0,
-// where that has lost digits, by its series.
-template <typename T>
+// tanh: by the exponential, within 2^-23 of 1; NEAR: near 0, where that has lost digits, by its
+// series, relative to it.
+template <bool NEAR>
 __device__ __forceinline__ float tanh_of(float x) {
   const float e = __builtin_amdgcn_exp2f(2.0f * kLog2E * x);
   const float far = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f);
-  if constexpr (sizeof(T) == 2) return far;
+  if constexpr (!NEAR) return far;
   const float x2 = x * x;
   const float near = __builtin_fmaf(
       x * x2, __builtin_fmaf(x2, __builtin_fmaf(x2, __builtin_fmaf(x2, 0.021869489f, -0.053968254f), 0.13333333f),
@@ -365,8 +365,12 @@ __device__ __forceinline__ float tanh_of(float x) {
 
 // From the product of a query and a key to the score in log2 units: a capped
 // product is the score over `factor`, any other the score itself, with factor > 0:
-// queries take the sign of the scale (and 0) with them, exactly.
-template <typename T>
+// queries take the sign of the scale (and 0) with them, exactly. NEAR: any cap. Without, as f16 kernels are
+// but for those of large caps, caps up to kNearCap, of which 2^-23 is a tenth of what the rounding of the
+// weights to f16 comes to (16 drafts 22.6 us and not 24); of larger ones it is most of the error, and in the end the score.
+// Both ways in one kernel cost its registers: 4 chunks of 1024 444 us and not 274, without a cap.
+constexpr float kNearCap = 256.0f;
+template <bool NEAR>
 struct Score {
   float factor, sign, before, after;
   bool capped;
@@ -374,7 +378,7 @@ struct Score {
       : factor(args.cap > 0.0f || args.scale == 0.0f ? 1.0f : fabsf(args.scale) * kLog2E),
         sign(args.scale > 0.0f ? 1.0f : args.scale < 0.0f ? -1.0f : 0.0f), before(fabsf(args.scale) / args.cap),
         after(args.cap * kLog2E), capped(args.cap > 0.0f) {}
-  __device__ __forceinline__ float cap(float dot) const { return after * tanh_of<T>(dot * before); }
+  __device__ __forceinline__ float cap(float dot) const { return after * tanh_of<NEAR>(dot * before); }
 };
 
 // Where the tokens of one kv head of a sequence lie, in pieces of 16 bytes
@@ -466,7 +470,7 @@ __device__ __forceinline__ void careful_item(const CacheAttentionArgs& args, con
   const uint32_t at = threadIdx.x, dim = cache.head_dim, group = args.group.by;
   const Seen part = part_of(args, item);
   const Places<T> map(cache, item.sequence, item.head);
-  const Score<T> score(args);
+  const Score<true> score(args);
   const Result<T, R> result{args, item, work};
   constexpr uint32_t kPiece = 16 / sizeof(T);
   for (uint32_t r = 0; r < item.rows; ++r) {
@@ -569,8 +573,9 @@ struct FewShape {
       kSums + 16 + largest(largest(kWaves * kValueBytes + kQueryBytes, kJoinBytes), kCarefulBytes);
 };
 
-template <typename T, int DP, int RB, bool WHOLE>
-__global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2 : 1) void cache_attention_few_kernel(CacheAttentionArgs args, Plan plan) {
+template <typename T, int DP, int RB, bool WHOLE, bool NEAR>
+__global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2 : 1) void cache_attention_few_kernel(
+    CacheAttentionArgs args, Plan plan) {
   typedef FewShape<T, DP, RB> Shape;
   constexpr int R = 16 * RB, STEP = Shape::kTokens, TB = STEP / 16;  // token blocks of a step
   constexpr bool kHalf = sizeof(T) == 2;
@@ -592,7 +597,7 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
   const Seen part = part_of(args, item);
   const uint32_t group = args.group.by, dim = cache.head_dim;
   const Places<T> map(cache, item.sequence, item.head);
-  const Score<T> score(args);
+  const Score<NEAR> score(args);
   const uint32_t pieces = dim / PIECE;
 
   // Queries, and what their rows see.
@@ -950,7 +955,7 @@ struct ManyShape {
   static_assert(4 * kTile * 2 >= (int)(kMaxDim + kThreads + kWaves + kThreads) * 4, "the careful way's LDS");
 };
 
-template <int DP, int USED, bool WHOLE>
+template <int DP, int USED, bool WHOLE, bool NEAR>
 __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_many_kernel(CacheAttentionArgs args,
                                                                                           Plan plan) {
   typedef _Float16 T;
@@ -970,7 +975,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
   const Seen part = part_of(args, item);
   const uint32_t group = args.group.by, dim = cache.head_dim;
   const Places<T> map(cache, item.sequence, item.head);
-  const Score<T> score(args);
+  const Score<NEAR> score(args);
   const uint32_t pieces = dim / 8u;
 
   // This lane's query, what its row sees, what all rows of the wavefront see, and any.
@@ -1298,18 +1303,23 @@ struct Variant {
   uint32_t rows;  // of a unit
 };
 
+// Of large caps in f16 one kernel for heads of any width.
 template <typename T, int DP, int RB>
-Variant few(bool whole) {
-  return {whole ? cache_attention_few_kernel<T, DP, RB, true> : cache_attention_few_kernel<T, DP, RB, false>,
+Variant few(bool whole, bool near) {
+  constexpr bool kNear = sizeof(T) == 4;
+  return {near && !kNear ? cache_attention_few_kernel<T, DP, RB, false, true>
+          : whole        ? cache_attention_few_kernel<T, DP, RB, true, kNear>
+                         : cache_attention_few_kernel<T, DP, RB, false, kNear>,
           cache_attention_list_kernel<16 * RB>, cache_attention_join_kernel<T, 16 * RB>, 16 * RB};
 }
 
 template <int DP>
-Variant many(uint32_t dim) {
+Variant many(uint32_t dim, bool near) {
   constexpr int kNarrow = DP > 64 ? DP / 4 * 3 : DP;
-  return {dim == (uint32_t)DP           ? cache_attention_many_kernel<DP, DP, true>
-          : dim <= (uint32_t)kNarrow ? cache_attention_many_kernel<DP, kNarrow, false>
-                                     : cache_attention_many_kernel<DP, DP, false>,
+  return {near                       ? cache_attention_many_kernel<DP, DP, false, true>
+          : dim == (uint32_t)DP      ? cache_attention_many_kernel<DP, DP, true, false>
+          : dim <= (uint32_t)kNarrow ? cache_attention_many_kernel<DP, kNarrow, false, false>
+                                     : cache_attention_many_kernel<DP, DP, false, false>,
           cache_attention_list_kernel<ManyShape<DP>::kRows>, cache_attention_join_kernel<_Float16, ManyShape<DP>::kRows>,
           ManyShape<DP>::kRows};
 }
@@ -1331,22 +1341,23 @@ uint32_t unit_rows(const CacheAttentionArgs& args) {
 }
 
 template <typename T, int DP>
-Variant choose(uint32_t rows, uint32_t dim) {
+Variant choose(uint32_t rows, uint32_t dim, bool near) {
   constexpr bool kHalf = sizeof(T) == 2;
   if constexpr (kHalf || DP <= 128)
-    if (rows == 32u) return few<T, DP, 2>(dim == (uint32_t)DP);
+    if (rows == 32u) return few<T, DP, 2>(dim == (uint32_t)DP, near);
   if constexpr (DP <= 64)
-    if (rows == 64u) return few<T, DP, 4>(dim == (uint32_t)DP);
+    if (rows == 64u) return few<T, DP, 4>(dim == (uint32_t)DP, near);
   if constexpr (kHalf)
-    if (rows == 128u) return many<DP>(dim);
-  return few<T, DP, 1>(dim == (uint32_t)DP);
+    if (rows == 128u) return many<DP>(dim, near);
+  return few<T, DP, 1>(dim == (uint32_t)DP, near);
 }
 template <typename T>
 Variant choose(const CacheAttentionArgs& args) {
   const uint32_t dim = args.cache.head_dim, rows = unit_rows(args);
-  if (dim <= 64u) return choose<T, 64>(rows, dim);
-  if (dim <= 128u) return choose<T, 128>(rows, dim);
-  return choose<T, 256>(rows, dim);
+  const bool near = args.cap > kNearCap;
+  if (dim <= 64u) return choose<T, 64>(rows, dim, near);
+  if (dim <= 128u) return choose<T, 128>(rows, dim, near);
+  return choose<T, 256>(rows, dim, near);
 }
 
 // Tokens of a part at least, and workgroups beside one for each unit, of which parts are made: a
