@@ -1276,15 +1276,25 @@ __global__ __launch_bounds__(64 * join_rows(R)) void cache_attention_join_kernel
     }
     const uint32_t count = min(64u, unit.parts - p0);
     const float* from = work.outputs + ((uint64_t)(unit.slot + p0) * R + r) * dim + d;
-    for (uint32_t i = 0; i < count; i += 8u) {  // eight loads at a time
+    const auto add = [&](const floatx4& part, uint32_t lane_of) {
+      x += part * __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(factor), (int)lane_of));
+    };
+    uint32_t i = 0;
+    for (; i + 8u <= count; i += 8u) {  // eight loads at a time
       floatx4 some[8];
 #pragma unroll
-      for (uint32_t j = 0; j < 8u; ++j)
+      for (uint32_t j = 0; j < 8u; ++j) some[j] = *reinterpret_cast<const floatx4*>(from + (uint64_t)(i + j) * R * dim);
+#pragma unroll
+      for (uint32_t j = 0; j < 8u; ++j) add(some[j], i + j);
+    }
+    if (i < count) {  // those behind the last are loaded and not added: 0 times an infinity is none
+      floatx4 some[7];
+#pragma unroll
+      for (uint32_t j = 0; j < 7u; ++j)
         some[j] = *reinterpret_cast<const floatx4*>(from + (uint64_t)min(i + j, count - 1u) * R * dim);
 #pragma unroll
-      for (uint32_t j = 0; j < 8u; ++j)
-        if (i + j < count)  // and no product with 0 else, which an infinity would spoil
-          x += some[j] * __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(factor), (int)(i + j)));
+      for (uint32_t j = 0; j < 7u; ++j)
+        if (i + j < count) add(some[j], i + j);
     }
   }
   all = wave::sum(all);
