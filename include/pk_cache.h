@@ -36,8 +36,9 @@
  *   output = sum exp(z) v / sum exp(z)
  * over the tokens that the row sees: of the first lengths[s], those up to its
  * own position if causal, and of these the last `window`. Sums, maxima and
- * exponentials are f32; f16 rows round the exponentials, relative to a running
- * maximum, to f16 for their product with the values. A row that sees
+ * exponentials are f32; f16 rows round the exponentials to f16 for their
+ * product with the values, where those below 2^-32 of the largest so far
+ * are 0, in the sum they are not. A row that sees
  * nothing, or only scores of minus infinity, gives zeros. What a row does not
  * see, infinities and NaN included, does not touch it; values that it does see
  * and that are infinite or NaN make its block of rows many times slower.
