@@ -466,7 +466,7 @@ __device__ __forceinline__ float block_reduce(float x, bool largest, float* scra
 // A product of matrices multiplies every value of a tile by every row's exponential, so that an
 // infinity or a NaN that only a later row sees would reach the earlier ones as
 // 0 * inf: items whose output is not finite come here.
-template <typename T, int R>
+template <typename T, int R, bool NEAR>
 __device__ __forceinline__ void careful_item(const CacheAttentionArgs& args, const Item& item, const Workspace& work,
                                              float* lds) {
   float *query = lds, *weight = lds + kMaxDim, *scratch = weight + kThreads;
@@ -475,7 +475,7 @@ __device__ __forceinline__ void careful_item(const CacheAttentionArgs& args, con
   const uint32_t at = threadIdx.x, dim = cache.head_dim, group = args.group.by;
   const Seen part = part_of(args, item);
   const Places<T> map(cache, item.sequence, item.head);
-  const Score<true> score(args);
+  const Score<NEAR> score(args);
   const Result<T, R> result{args, item, work};
   constexpr uint32_t kPiece = 16 / sizeof(T);
   for (uint32_t r = 0; r < item.rows; ++r) {
@@ -877,7 +877,7 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
   }
   __syncthreads();
   if (*strange) {
-    careful_item<T, R>(args, item, work, reinterpret_cast<float*>(lds + Shape::kSums + 16));
+    careful_item<T, R, NEAR>(args, item, work, reinterpret_cast<float*>(lds + Shape::kSums + 16));
     return;
   }
   float* slices = reinterpret_cast<float*>(lds + Shape::kSums + 16);
@@ -1219,7 +1219,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
   if (args.causal && item.new_tokens > 1u && __any(odd) && lane == 0) *strange = 1;
   __syncthreads();
   if (*strange) {
-    careful_item<T, R>(args, item, work, reinterpret_cast<float*>(lds));
+    careful_item<T, R, NEAR>(args, item, work, reinterpret_cast<float*>(lds));
     return;
   }
   if (r >= item.rows) return;
