@@ -41,7 +41,8 @@
  * are 0, in the sum they are not. A row that sees
  * nothing, or only scores of minus infinity, gives zeros. What a row does not
  * see, infinities and NaN included, does not touch it; values that it does see
- * and that are infinite or NaN make its block of rows many times slower.
+ * and that are infinite or NaN, and scores beyond 2^23, make its block of rows
+ * many times slower.
  * How the work is shared out follows rows / sequences, which the host knows,
  * and not from row_starts: hold one op for single tokens and one for chunks.
  */

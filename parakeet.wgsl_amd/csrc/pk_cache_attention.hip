@@ -36,6 +36,11 @@ constexpr uint32_t kMaxDim = 256;
 constexpr float kMargin = 8.0f;
 template <typename T>
 constexpr float kLift = sizeof(T) == 2 ? 7.0f : 0.0f;
+// The exponent of the kernels is fma(product, factor, -base): exact, where the maximum was rounded. From scores
+// of 2^24 on that rounding is a factor of 2 and more, in the end beyond the type: items with such a base
+// go to the plain loop, which takes the rounded score of all.
+constexpr float kFar = 16777216.0f;
+__device__ __forceinline__ bool is_far(float base) { return !(fabsf(base) < kFar) && base != -kInf; }
 
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -465,7 +470,7 @@ __device__ __forceinline__ float block_reduce(float x, bool largest, float* scra
 // An item without matrix instructions: a thread scores a token, then sums an element.
 // A product of matrices multiplies every value of a tile by every row's exponential, so that an
 // infinity or a NaN that only a later row sees would reach the earlier ones as
-// 0 * inf: items whose output is not finite come here.
+// 0 * inf: items whose output is not finite come here, and those of far scores.
 template <typename T, int R, bool NEAR>
 __device__ __forceinline__ void careful_item(const CacheAttentionArgs& args, const Item& item, const Workspace& work,
                                              float* lds) {
@@ -649,6 +654,7 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
   }
 
   float m[RB], l[RB];
+  bool far = false;
   floatx4 out[RB][OB];
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
@@ -789,6 +795,7 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         top = fmaxf(top - kLift<T>, m[b]);
+        far |= is_far(top);
         const float old = m[b] == top ? 1.0f : __builtin_amdgcn_exp2f(m[b] - top);
         m[b] = top;
         l[b] *= old;
@@ -851,7 +858,14 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
   float* sums = reinterpret_cast<float*>(lds);
   uint32_t* strange = reinterpret_cast<uint32_t*>(lds + Shape::kSums);
   if (threadIdx.x == 0) *strange = 0;
-  bool odd = false;
+  bool odd = far;
+  if (args.causal && item.new_tokens > 1u)  // rows that do not all see the same
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+      for (int o = 0; o < OB; ++o)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) odd |= !(fabsf(out[b][o][j]) < kInf);
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
     l[b] += __shfl_xor(l[b], 16, 64);
@@ -860,13 +874,9 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
       sums[wave * R + 16 * b + col] = m[b];
       sums[kWaves * R + wave * R + 16 * b + col] = l[b];
     }
-#pragma unroll
-    for (int o = 0; o < OB; ++o)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) odd |= !(fabsf(out[b][o][j]) < kInf);
   }
   __syncthreads();
-  if (args.causal && item.new_tokens > 1u && __any(odd) && lane == 0) *strange = 1;
+  if (__any(odd) && lane == 0) *strange = 1;
   float scale[RB];
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
@@ -1019,6 +1029,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
   }
 
   float m = -kInf, l = 0.0f;
+  bool far = false;
   floatx16 out[DB];
 #pragma unroll
   for (int o = 0; o < DB; ++o) out[o] = floatx16{};
@@ -1165,6 +1176,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
       if (__any(top > m + (kMargin + kLift<T>))) {
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         top = fmaxf(top - kLift<T>, m);
+        far |= is_far(top);
         const float old = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
         m = top;
         l *= old;
@@ -1210,13 +1222,14 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
   uint32_t* strange = reinterpret_cast<uint32_t*>(lds + Shape::kLds - 16);
   if (threadIdx.x == 0) *strange = 0;
   l += __shfl_xor(l, 32, 64);
-  bool odd = false;
+  bool odd = far;
+  if (args.causal && item.new_tokens > 1u)
 #pragma unroll
-  for (int o = 0; o < DB; ++o)
+    for (int o = 0; o < DB; ++o)
 #pragma unroll
-    for (int j = 0; j < 16; ++j) odd |= !(fabsf(out[o][j]) < kInf);
+      for (int j = 0; j < 16; ++j) odd |= !(fabsf(out[o][j]) < kInf);
   __syncthreads();
-  if (args.causal && item.new_tokens > 1u && __any(odd) && lane == 0) *strange = 1;
+  if (__any(odd) && lane == 0) *strange = 1;
   __syncthreads();
   if (*strange) {
     careful_item<T, R, NEAR>(args, item, work, reinterpret_cast<float*>(lds));
