@@ -38,9 +38,11 @@ template <typename T>
 constexpr float kLift = sizeof(T) == 2 ? 7.0f : 0.0f;
 // The exponent of the kernels is fma(product, factor, -base): exact, where the maximum was rounded. From scores
 // of 2^24 on that rounding is a factor of 2 and more, in the end beyond the type: items with such a base
-// go to the plain loop, which takes the rounded score of all.
+// go to the plain loop, which takes the rounded score of all. Their sums are minus infinity till then.
 constexpr float kFar = 16777216.0f;
-__device__ __forceinline__ bool is_far(float base) { return !(fabsf(base) < kFar) && base != -kInf; }
+__device__ __forceinline__ float moved(float l, float old, float base) {
+  return l < 0.0f || (!(fabsf(base) < kFar) && base != -kInf) ? -kInf : l * old;
+}
 
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -654,7 +656,6 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
   }
 
   float m[RB], l[RB];
-  bool far = false;
   floatx4 out[RB][OB];
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
@@ -795,10 +796,9 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         top = fmaxf(top - kLift<T>, m[b]);
-        far |= is_far(top);
         const float old = m[b] == top ? 1.0f : __builtin_amdgcn_exp2f(m[b] - top);
         m[b] = top;
-        l[b] *= old;
+        l[b] = moved(l[b], old, top);
 #pragma unroll
         for (int o = 0; o < OB; ++o) out[b][o] *= old;
       }
@@ -858,7 +858,7 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
   float* sums = reinterpret_cast<float*>(lds);
   uint32_t* strange = reinterpret_cast<uint32_t*>(lds + Shape::kSums);
   if (threadIdx.x == 0) *strange = 0;
-  bool odd = far;
+  bool odd = false;
   if (args.causal && item.new_tokens > 1u)  // rows that do not all see the same
 #pragma unroll
     for (int b = 0; b < RB; ++b)
@@ -868,6 +868,7 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
         for (int j = 0; j < 4; ++j) odd |= !(fabsf(out[b][o][j]) < kInf);
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
+    odd |= l[b] < 0.0f;
     l[b] += __shfl_xor(l[b], 16, 64);
     l[b] += __shfl_xor(l[b], 32, 64);
     if (quarter == 0) {
@@ -1029,7 +1030,6 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
   }
 
   float m = -kInf, l = 0.0f;
-  bool far = false;
   floatx16 out[DB];
 #pragma unroll
   for (int o = 0; o < DB; ++o) out[o] = floatx16{};
@@ -1176,10 +1176,9 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
       if (__any(top > m + (kMargin + kLift<T>))) {
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         top = fmaxf(top - kLift<T>, m);
-        far |= is_far(top);
         const float old = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
         m = top;
-        l *= old;
+        l = moved(l, old, top);
 #pragma unroll
         for (int o = 0; o < DB; ++o) out[o] *= old;
       }
@@ -1221,8 +1220,8 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
 
   uint32_t* strange = reinterpret_cast<uint32_t*>(lds + Shape::kLds - 16);
   if (threadIdx.x == 0) *strange = 0;
+  bool odd = l < 0.0f;
   l += __shfl_xor(l, 32, 64);
-  bool odd = far;
   if (args.causal && item.new_tokens > 1u)
 #pragma unroll
     for (int o = 0; o < DB; ++o)
