@@ -449,6 +449,22 @@ struct Result {
 // 1 / l, and 0 where no score counted.
 __device__ __forceinline__ float inverse(float m, float l) { return m == -kInf && l == 0.0f ? 0.0f : 1.0f / l; }
 
+// Outputs before they are rounded. Weights that were rounded up, and a sum that was not, put a mean of f16's
+// largest values beyond the type; a number stays one, and an infinity an infinity.
+template <typename T, typename V>
+__device__ __forceinline__ V kept_finite(V x, int count) {
+  constexpr float kMost = 65504.0f;
+  if constexpr (sizeof(T) == 2) {
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < count; ++i) most = fmaxf(most, fabsf(x[i]));
+    if (most > kMost)
+#pragma unroll
+      for (int i = 0; i < count; ++i) x[i] = fabsf(x[i]) < kInf ? __builtin_amdgcn_fmed3f(x[i], -kMost, kMost) : x[i];
+  }
+  return x;
+}
+
 // Of 64 tokens from t0 on, those below `end`.
 __device__ __forceinline__ uint64_t tokens_below(uint32_t t0, uint32_t end) {
   const uint32_t n = end > t0 ? end - t0 : 0u;
@@ -523,7 +539,8 @@ __device__ __forceinline__ void careful_item(const CacheAttentionArgs& args, con
       }
     }
     if (item.parts == 1u) {
-      if (at < dim) result.output(r)[at] = (T)(out * inverse(m, l));
+      const floatx4 x = {out * inverse(m, l)};
+      if (at < dim) result.output(r)[at] = (T)kept_finite<T>(x, 1)[0];
     } else {
       if (at < dim) result.partial(r)[at] = out;
       if (at == 0) result.sums(r, m, l);
@@ -932,7 +949,7 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
         if (at + d == 0) result.sums(r, top, all);
         continue;
       }
-      x *= inverse(top, all);
+      x = kept_finite<T>(x * inverse(top, all), 4);
       T* to = result.output(r) + at + d;
       if (args.wide_rows) {
         typedef T T4 __attribute__((ext_vector_type(4)));
@@ -1240,12 +1257,14 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
   T* to = result.output(r);
   float* part_to = result.partial(r);
 #pragma unroll
-  for (int o = 0; o < DB; ++o)
+  for (int o = 0; o < DB; ++o) {
+    out[o] *= scale;
+    if (item.parts == 1u) out[o] = kept_finite<T>(out[o], 16);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint32_t d = 32u * o + 8u * j + 4u * half;
       if (!WHOLE && d >= dim) continue;
-      const floatx4 x = {out[o][4 * j] * scale, out[o][4 * j + 1] * scale, out[o][4 * j + 2] * scale, out[o][4 * j + 3] * scale};
+      const floatx4 x = {out[o][4 * j], out[o][4 * j + 1], out[o][4 * j + 2], out[o][4 * j + 3]};
       if (item.parts > 1u) {
         *reinterpret_cast<floatx4*>(part_to + d) = x;
       } else {
@@ -1260,6 +1279,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
         }
       }
     }
+  }
   if (item.parts > 1u && half == 0) result.sums(r, m, l);
 }
 
@@ -1315,7 +1335,7 @@ __global__ __launch_bounds__(64 * join_rows(R)) void cache_attention_join_kernel
     }
   }
   all = wave::sum(all);
-  x *= inverse(top, all);
+  x = kept_finite<T>(x * inverse(top, all), 4);
   const uint32_t i = unit.first + r, token = args.group.under(i);
   T* to = static_cast<T*>(args.output) + (unit.row + token) * args.output_stride +
           (uint64_t)(unit.head * group + (i - token * group)) * dim + d;

@@ -36,3 +36,28 @@ def test_small_weights(abi, ctx, scope, count, heads, kv_heads, dim, gap, rising
     bound = half * np.abs(want) + (1 + half) * (weights * size + least * 2.0 ** -32) + 2.0 ** -24
     off = np.abs(got.reshape(want.shape).astype(np.float64) - want) / bound
     assert off.max() <= 1, off.max()
+
+
+@pytest.mark.parametrize("counts,heads,kv_heads,dim", [([1, 1], 2, 2, 64), ([7, 3], 4, 2, 128), ([50, 20], 2, 1, 64),
+                                                       ([140, 90], 2, 1, 96), ([1, 2], 1, 1, 256)])
+@pytest.mark.parametrize("length", [500, 3000])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_values_of_the_largest_number(abi, ctx, scope, counts, heads, kv_heads, dim, length, sign):
+    """A mean of f16's largest number is that number, and no infinity, also where nearly all weights are rounded
+    up: of scores 0.00055 above those of the first tokens, by 0.00043."""
+    largest = float(np.finfo(np.float16).max)
+
+    def spoil(cache, queries):
+        cache.values[:] = sign * largest
+        queries[:] = 0
+        queries[:, ::dim] = 1
+        for s, n in enumerate(cache.lengths):
+            for t in range(int(n)):
+                for h in range(kv_heads):
+                    cache.keys[cache.place(s, t) + h * 16 * dim] = 0.00055 if t >= 128 else 0
+    cache, got, queries = run_attention(abi, ctx, scope, np.random.default_rng(dim), np.float16, counts, [length, 500], heads,
+                                        kv_heads, dim, 16, scale=1.0, spoil=spoil, check=False)
+    got = got.astype(np.float64)
+    assert np.isfinite(got).all()
+    # the weights' rounding, half a step, and the sums'
+    assert (np.abs(got - sign * largest) <= largest * (2.0 ** -10 + 2.0 ** -16)).all()
