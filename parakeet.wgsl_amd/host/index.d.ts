@@ -517,8 +517,12 @@ export declare const SCORE_NO_TOKEN: number;
 
 /* ---- Paged cache, draft verification (no counterpart in the reference) ---- */
 
-/** A dispatch over the rows of sequences; shape.batchSize selects the active sequences. */
-export declare class SequencesDispatch extends RowsDispatch {}
+/** A dispatch over the rows of sequences; batchSize, or sequences, selects the active ones: no shape stands for all, a
+ * shape without either is refused. */
+export declare class SequencesDispatch extends RowsDispatch {
+  encode(encoder: HipCommandEncoder, timestampWrites?: TimestampWrites,
+         shape?: { batchSize?: number; sequences?: number; rows?: number }): void;
+}
 
 /** A cache [pages][kvHeads][pageSize][headDim], and where its sequences lie in it. */
 export interface PagedCache {

@@ -1330,10 +1330,15 @@ const SCORE_NO_TOKEN = 0xffffffff;
 
 /** A dispatch over the rows of sequences. */
 class SequencesDispatch extends RowsDispatch {
-  /** shape.batchSize selects the active sequences. */
+  /** shape.batchSize, or shape.sequences, selects the active sequences; no shape: all. */
   encode(encoder, timestampWrites, shape) {
     if (this.destroyed) throw new Error(`${this.label} was destroyed`);
-    const active = shape === undefined || shape.batchSize === undefined ? this.rows : shape.batchSize;
+    const { batchSize, sequences } = shape === undefined ? { batchSize: this.rows } : shape;
+    if (batchSize === undefined && sequences === undefined)
+      throw new Error(`${this.label} needs batchSize or sequences in its shape`);
+    if (batchSize !== undefined && sequences !== undefined && batchSize !== sequences)
+      throw new Error(`${this.label} has a batchSize and sequences that differ`);
+    const active = batchSize === undefined ? sequences : batchSize;
     if (!isSafe(active) || active <= 0 || active > this.rows)
       throw new RangeError(`${this.label} active sequences must be in [1, ${this.rows}]`);
     super.encode(encoder, timestampWrites, { rows: active });
