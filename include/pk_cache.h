@@ -28,8 +28,9 @@
  * at j and rotary_dim / 2 + j (PK_ROTARY_HALVES) or at 2j and 2j + 1
  * (PK_ROTARY_NEIGHBOURS) become
  *   x cos a - y sin a,  y cos a + x sin a
- * in f32, rounded once; the angle is reduced exactly, at any position. The
- * other elements, and the values, are copied.
+ * in f32, rounded once; the angle is reduced exactly, at any position and for
+ * frequencies of up to 2^36 in magnitude. The other elements, and the values,
+ * are copied.
  *
  * cache attention: head h reads the kv head h / (heads / kv_heads);
  *   z = scale * q . k, or cap * tanh(scale * q . k / cap),
@@ -100,7 +101,7 @@ typedef struct pk_cache_append_desc {
   uint32_t value_stride;
   uint32_t rotary_dim;           /* even, up to head_dim; 0: no rotation */
   int32_t rotary;                /* pk_rotary_kind */
-  const float *frequencies;      /* [rotary_dim / 2] radians per position, with rotary_dim; finite */
+  const float *frequencies;      /* [rotary_dim / 2] radians per position, with rotary_dim; up to 2^36 */
   uint64_t frequencies_bytes;
   const uint32_t *positions;     /* [rows] of the rotation, NULL: those in the sequence */
   uint64_t positions_bytes;
