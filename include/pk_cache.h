@@ -18,10 +18,11 @@
  * These arrays lie on the device and are read by every launch: a replayed
  * graph follows what they hold then. What they hold is kept within the
  * bindings: row_starts are cut to `rows` and should not decrease; a row before
- * position 0 (n above the length) is neither appended nor rotated and attends
- * to nothing; a token whose page is PK_CACHE_NO_PAGE or any other number of
- * `pages` or more, or that lies behind pages_per_sequence pages, is not stored
- * and is hidden from every row.
+ * position 0 (n above the length) is neither appended nor rotated, its query
+ * output is left as it was, and it attends to nothing if causal, or else, as
+ * all rows of its sequence, to what that holds; a token whose page is
+ * PK_CACHE_NO_PAGE or any other number of `pages` or more, or that lies behind
+ * pages_per_sequence pages, is not stored and is hidden from every row.
  *
  * cache append: with j < rotary_dim / 2 and the angle a = position *
  * frequencies[j], the elements x, y of a head of the queries and keys that lie
