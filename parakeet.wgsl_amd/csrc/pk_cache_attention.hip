@@ -37,12 +37,11 @@ constexpr float kMargin = 8.0f;
 template <typename T>
 constexpr float kLift = sizeof(T) == 2 ? 7.0f : 0.0f;
 // The exponent of the kernels is fma(product, factor, -base): exact, where the maximum was rounded. From scores
-// of 2^24 on that rounding is a factor of 2 and more, in the end beyond the type: items with such a base
-// go to the plain loop, which takes the rounded score of all. Their sums are minus infinity till then.
-constexpr float kFar = 16777216.0f;
-__device__ __forceinline__ float moved(float l, float old, float base) {
-  return l < 0.0f || (!(fabsf(base) < kFar) && base != -kInf) ? -kInf : l * old;
-}
+// of 2^24 on that rounding is a factor of 2 and more, in the end beyond the type: a base that far becomes
+// kLost, for which every exponential is 0 and which no score passes, and its item goes to the
+// plain loop, which takes the rounded score of all.
+constexpr float kFar = 16777216.0f, kLost = 3.0e38f;
+__device__ __forceinline__ float base_at(float base) { return fabsf(base) < kFar || base == -kInf ? base : kLost; }
 
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -812,10 +811,10 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
       if (__any(top > m[b] + (kMargin + kLift<T>))) {
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
-        top = fmaxf(top - kLift<T>, m[b]);
+        top = base_at(fmaxf(top - kLift<T>, m[b]));
         const float old = m[b] == top ? 1.0f : __builtin_amdgcn_exp2f(m[b] - top);
         m[b] = top;
-        l[b] = moved(l[b], old, top);
+        l[b] *= old;
 #pragma unroll
         for (int o = 0; o < OB; ++o) out[b][o] *= old;
       }
@@ -885,7 +884,7 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
         for (int j = 0; j < 4; ++j) odd |= !(fabsf(out[b][o][j]) < kInf);
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
-    odd |= l[b] < 0.0f;
+    odd |= m[b] == kLost;
     l[b] += __shfl_xor(l[b], 16, 64);
     l[b] += __shfl_xor(l[b], 32, 64);
     if (quarter == 0) {
@@ -1192,10 +1191,10 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
       top *= score.factor;
       if (__any(top > m + (kMargin + kLift<T>))) {
         top = fmaxf(top, __shfl_xor(top, 32, 64));
-        top = fmaxf(top - kLift<T>, m);
+        top = base_at(fmaxf(top - kLift<T>, m));
         const float old = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
         m = top;
-        l = moved(l, old, top);
+        l *= old;
 #pragma unroll
         for (int o = 0; o < DB; ++o) out[o] *= old;
       }
@@ -1237,7 +1236,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
 
   uint32_t* strange = reinterpret_cast<uint32_t*>(lds + Shape::kLds - 16);
   if (threadIdx.x == 0) *strange = 0;
-  bool odd = l < 0.0f;
+  bool odd = m == kLost;
   l += __shfl_xor(l, 32, 64);
   if (args.causal && item.new_tokens > 1u)
 #pragma unroll
