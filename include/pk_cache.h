@@ -45,8 +45,10 @@
  * see, infinities and NaN included, does not touch it; values that it does see
  * and that are infinite or NaN, and scores beyond 2^23, make its block of rows
  * many times slower.
- * How the work is shared out follows rows / sequences, which the host knows,
- * and not from row_starts: hold one op for single tokens and one for chunks.
+ * Scores beyond f32 and sums of f32 values beyond 2^119 overflow.
+ * How the work is shared out follows the op's rows over the launch's active
+ * sequences, which the host knows, and not row_starts: hold one op for single
+ * tokens and one for chunks.
  */
 #ifndef PK_CACHE_H
 #define PK_CACHE_H
@@ -177,8 +179,8 @@ int pk_cache_attention_create(pk_context *ctx, const pk_cache_attention_desc *de
 /* The rows of the first `active_sequences` sequences (0 = all); rows behind
    them are left as they were. May be captured into graphs. Long sequences
    are split over workgroups, which meet in memory of the op, where lists of
-   more than 64 sequences lie as well: launches of one op, eager or replayed, must be ordered by the caller, as their outputs ask
-   for anyway. */
+   more than 64 sequences lie as well: launches of one op, eager or replayed,
+   must be ordered by the caller, as their outputs ask for anyway. */
 int pk_cache_attention_enqueue(pk_cache_attention_op *op, uint32_t active_sequences, void *stream);
 int pk_cache_attention_enqueue_timed(pk_cache_attention_op *op, uint32_t active_sequences, void *stream,
                                      void *start_event, void *end_event);

@@ -160,7 +160,8 @@ __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheAppendArgs 
     if (!w.live) return;
     T* to;
     if (item.head < args.heads) {
-      to = static_cast<T*>(args.query_output) + (uint64_t)(first + item.row) * args.query_output_stride + (uint64_t)item.head * dim;
+      to = static_cast<T*>(args.query_output) + (uint64_t)(first + item.row) * args.query_output_stride +
+           (uint64_t)item.head * dim;
     } else {
       if (w.place == CacheView::no_place) return;
       const bool value = item.head >= args.heads + cache.kv_heads;

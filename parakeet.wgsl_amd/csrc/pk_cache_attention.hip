@@ -337,7 +337,8 @@ __global__ __launch_bounds__(kListThreads) void cache_attention_list_kernel(Cach
       mine[i].slots_to = slots;
     }
   }
-  const uint32_t items_to = wave::running_sum(items), units_to = wave::running_sum(have), slots_to = wave::running_sum(slots);
+  const uint32_t items_to = wave::running_sum(items), units_to = wave::running_sum(have),
+                 slots_to = wave::running_sum(slots);
   if (lane == 63u) {
     totals[0][wave_at] = items_to;
     totals[1][wave_at] = units_to;
@@ -532,9 +533,10 @@ __device__ __forceinline__ void careful_item(const CacheAttentionArgs& args, con
         out *= old;
         const uint32_t count = min((uint32_t)kThreads, high - t0);
         for (uint32_t j = 0; j < count; ++j)
-          if (places[j] != Places<T>::none)
-            out = __builtin_fmaf(weight[j], (float)(static_cast<const T*>(args.value_cache) + (uint64_t)places[j] * kPiece)[at],
-                                 out);
+          if (places[j] != Places<T>::none) {
+            const T* v = static_cast<const T*>(args.value_cache) + (uint64_t)places[j] * kPiece;
+            out = __builtin_fmaf(weight[j], (float)v[at], out);
+          }
       }
     }
     if (item.parts == 1u) {
@@ -967,9 +969,9 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
 // The kernel of many rows, f16: a workgroup of 4 wavefronts with 32 rows each,
 // which share tiles of 64 tokens in LDS, two of them: while one is used, the next one
 // is loaded straight to the other, 16 tokens by each wavefront; where some of these 16 are hidden or
-// have no page they go through registers, zeros in their places. Keys are read as operands of v_mfma_f32_32x32x16_f16, 16 bytes of
-// a token, values transposed, four tokens of a channel, in the order in which
-// the scores lie: scores 8u .. 8u + 7 of a lane are tokens 16u + 4 half + 0..3 and 8 more.
+// have no page they go through registers, zeros in their places. Keys are read as operands of
+// v_mfma_f32_32x32x16_f16, 16 bytes of a token, values transposed, four tokens of a channel, in the order
+// in which the scores lie: scores 8u .. 8u + 7 of a lane are tokens 16u + 4 half + 0..3 and 8 more.
 // Both are laid out so that the lanes that read together read different banks: pieces
 // of 16 bytes of a key, and of 32 bytes of a value, are exchanged by a number of the row.
 //
@@ -1039,7 +1041,8 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
   }
   Seen any = {0, 0}, all = {0, 0};
   if (32u * wave < item.rows) {
-    const uint32_t first = args.group.under(item.first + 32u * wave), last = args.group.under(item.first + min(item.rows, 32u * wave + 32u) - 1u);
+    const uint32_t first = args.group.under(item.first + 32u * wave),
+                   last = args.group.under(item.first + min(item.rows, 32u * wave + 32u) - 1u);
     const Seen a = seen_by(args, item.length, item.position + first), b = seen_by(args, item.length, item.position + last);
     all = {b.low, a.high};
     any = {a.low, b.high};
@@ -1131,7 +1134,8 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         const uint32_t row = staged_row(i), at = 16u * wave + row;
-        const uint32_t place = runs ? places + row * map.row : (uint32_t)__builtin_amdgcn_ds_bpermute((int)(at * 4u), (int)places);
+        const uint32_t place = runs ? places + row * map.row
+                                    : (uint32_t)__builtin_amdgcn_ds_bpermute((int)(at * 4u), (int)places);
         half8 key = half8{}, value = half8{};
         if (live_next >> at & 1u) {
           if (WHOLE || key_piece(row) < pieces)
@@ -1165,7 +1169,8 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void cache_attention_ma
       for (int k = 0; k < KS; ++k)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const half8 x = *reinterpret_cast<const half8*>(k_from + (32u * t + col) * DP + ((2u * k + half) ^ key_turn(col)) * 8u);
+          const uint32_t piece = (2u * k + half) ^ key_turn(col);
+          const half8 x = *reinterpret_cast<const half8*>(k_from + (32u * t + col) * DP + piece * 8u);
           s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, query[k], s[t], 0, 0, 0);
         }
       const bool whole = live == ~0ull && t0 >= all.low && t0 + STEP <= all.high;

@@ -217,8 +217,8 @@ struct Weights {
   __device__ Weights(const VerifyArgs& args, const double* table, const End& end, bool residual)
       : z(static_cast<const T*>(args.target) + end.row * args.target_stride),
         y(args.draft && residual ? static_cast<const T*>(args.draft) + end.row * args.draft_stride : nullptr),
-        refused(end.draft), p(table, end.p.m, args.scale), q(table, y ? end.q.m : 0.0, args.scale), inverse(p.right / end.p.sum),
-        draft_inverse(y ? q.right / end.q.sum : 0.0), residual(residual) {}
+        refused(end.draft), p(table, end.p.m, args.scale), q(table, y ? end.q.m : 0.0, args.scale),
+        inverse(p.right / end.p.sum), draft_inverse(y ? q.right / end.q.sum : 0.0), residual(residual) {}
   // `whole` gets the target's probability.
   __device__ __forceinline__ double of(float target, float draft, uint32_t i, double* whole) const {
 #pragma clang fp contract(off)  // equal probabilities leave 0
@@ -301,8 +301,8 @@ __device__ __forceinline__ uint32_t find_token(const double (&w)[N], uint32_t fi
 
 // The rows [first, first + count) of a sequence in turn, from their sums (`each` apart: of the target, and of the
 // draft behind it): where it ends, if it does. Threads decide a row each first.
-__device__ __forceinline__ bool decide(const VerifyArgs& args, const Rows& rows, const Judged& judged, uint32_t first, uint32_t count,
-                                       const RowSum* sums, uint32_t each, uint32_t* states, End* end) {
+__device__ __forceinline__ bool decide(const VerifyArgs& args, const Rows& rows, const Judged& judged, uint32_t first,
+                                       uint32_t count, const RowSum* sums, uint32_t each, uint32_t* states, End* end) {
   enum { kStands = 0, kDraws = 1, kNone = 2 };
   if (threadIdx.x < count) {
     const uint32_t draft = judged.draft;
@@ -534,7 +534,8 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs args, 
     for (int i = 0; i < kSumsHeld; ++i)
 #pragma unroll
       for (int c = 0; c < VEC; ++c)
-        best = Larger()(best, (unsigned long long)key_of((float)held[i][c], part.first + part.head + (at + i * kThreads) * VEC + c));
+        best = Larger()(best, (unsigned long long)key_of((float)held[i][c],
+                                                         part.first + part.head + (at + i * kThreads) * VEC + c));
     sum.best = reduce_group<kThreads>(best, scratch, Larger());
     sum.sum = sum.best ? 1.0 : 0.0;
   } else {
@@ -575,8 +576,8 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs args, 
 // Where a sequence ends: groups of 16 lanes join the parts of a row each, 8 rows at a time,
 // and the decisions are read from them in turn.
 template <typename T>
-__device__ __forceinline__ End find_end(const VerifyArgs& args, const Workspace& work, uint32_t s, uint32_t parts, RowSum* sums,
-                                        uint32_t* states) {
+__device__ __forceinline__ End find_end(const VerifyArgs& args, const Workspace& work, uint32_t s, uint32_t parts,
+                                        RowSum* sums, uint32_t* states) {
   constexpr uint32_t kTogether = kThreads / 32;
   const Rows rows(args, s);
   const uint32_t group = threadIdx.x / 16, lane = threadIdx.x % 16;
@@ -721,7 +722,8 @@ __global__ __launch_bounds__(kSequence) void verify_token_kernel(VerifyArgs args
 bool together(const VerifyArgs& args) { return args.columns <= kShort && args.rows <= 16ull * args.sequences; }
 
 template <typename Kernel, typename... Args>
-hipError_t launch(Kernel kernel, dim3 grid, dim3 block, hipStream_t stream, hipEvent_t start, hipEvent_t stop, Args... args) {
+hipError_t launch(Kernel kernel, dim3 grid, dim3 block, hipStream_t stream, hipEvent_t start, hipEvent_t stop,
+                  Args... args) {
   if (start || stop)
     hipExtLaunchKernelGGL(kernel, grid, block, 0, stream, start, stop, 0, args...);
   else
@@ -737,8 +739,8 @@ hipError_t launch_typed(const VerifyArgs& args, hipStream_t stream, hipEvent_t s
   const uint32_t parts = parts_of<T>(args.columns), sequences = args.sequences;
   const bool two = args.draft && !args.greedy;
   const uint32_t sums_parts = sums_parts_of<T>(args.columns);
-  if (const hipError_t e = launch(verify_sums_kernel<T>, dim3(args.rows, sums_parts * (two ? 2u : 1u)), dim3(kThreads), stream,
-                                  start, nullptr, args, sums_parts))
+  if (const hipError_t e = launch(verify_sums_kernel<T>, dim3(args.rows, sums_parts * (two ? 2u : 1u)), dim3(kThreads),
+                                  stream, start, nullptr, args, sums_parts))
     return e;
   const hipError_t e = launch(verify_weights_kernel<T>, dim3(sequences, args.greedy ? 1u : parts), dim3(kThreads), stream,
                               nullptr, args.greedy ? stop : nullptr, args, parts, sequences);
@@ -753,7 +755,8 @@ uint64_t workspace_typed(const VerifyArgs& args) {
   one.sequences = 1;
   if (together(one)) return 0;
   const uint64_t parts = parts_of<T>(args.columns);
-  return 2ull * args.rows * sums_parts_of<T>(args.columns) * sizeof(RowSum) + args.sequences * (sizeof(End) + parts * sizeof(double2));
+  return 2ull * args.rows * sums_parts_of<T>(args.columns) * sizeof(RowSum) +
+         args.sequences * (sizeof(End) + parts * sizeof(double2));
 }
 
 }  // namespace

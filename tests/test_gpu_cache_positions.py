@@ -13,8 +13,8 @@ pytestmark = pytest.mark.gpu
 @pytest.mark.parametrize("count,length", [(3, 1), (4, 0), (30, 20), (40, 39), (120, 50), (300, 200)])
 @pytest.mark.parametrize("dim", [64, 128, 200])
 def test_rows_before_position_zero(abi, ctx, scope, dtype, count, length, dim):
-    run = lambda **kw: run_attention(abi, ctx, scope, np.random.default_rng(count), dtype, [count, 2], [count, 30], 4, 2, dim,
-                                     16, **kw)
+    run = lambda **kw: run_attention(abi, ctx, scope, np.random.default_rng(count), dtype, [count, 2], [count, 30], 4, 2,
+                                     dim, 16, **kw)
 
     def spoil(cache, queries):
         cache.lengths[0] = length

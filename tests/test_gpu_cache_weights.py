@@ -9,7 +9,8 @@ from test_gpu_cache import attention_rows, run_attention, scope  # noqa: F401
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("count,heads,kv_heads,dim", [(1, 4, 4, 64), (1, 2, 1, 128), (9, 4, 2, 64), (30, 2, 1, 40), (140, 2, 1, 128)])
+@pytest.mark.parametrize("count,heads,kv_heads,dim", [(1, 4, 4, 64), (1, 2, 1, 128), (9, 4, 2, 64), (30, 2, 1, 40),
+                                                      (140, 2, 1, 128)])
 @pytest.mark.parametrize("gap", [10.0, 14.0, 16.0, 17.0, 17.5])
 @pytest.mark.parametrize("rising", [False, True])
 def test_small_weights(abi, ctx, scope, count, heads, kv_heads, dim, gap, rising):
@@ -28,8 +29,8 @@ def test_small_weights(abi, ctx, scope, count, heads, kv_heads, dim, gap, rising
             at = cache.place(0, 0) + h * 16 * dim
             cache.keys[at] = gap
             cache.values[at:at + dim] = 0
-    cache, got, queries = run_attention(abi, ctx, scope, np.random.default_rng(1), np.float16, [count], [length], heads, kv_heads,
-                                        dim, 16, scale=1.0, spoil=sink, check=False)
+    cache, got, queries = run_attention(abi, ctx, scope, np.random.default_rng(1), np.float16, [count], [length], heads,
+                                        kv_heads, dim, 16, scale=1.0, spoil=sink, check=False)
     want, size, slack, least = attention_rows(cache, queries, heads, scale=1.0)
     half = 2.0 ** -11
     weights = 2 * (dim + 4) * 2.0 ** -24 * slack + (8 + 4 * length ** 0.5) * 2.0 ** -24 + half
@@ -55,8 +56,8 @@ def test_values_of_the_largest_number(abi, ctx, scope, counts, heads, kv_heads, 
             for t in range(int(n)):
                 for h in range(kv_heads):
                     cache.keys[cache.place(s, t) + h * 16 * dim] = 0.00055 if t >= 128 else 0
-    cache, got, queries = run_attention(abi, ctx, scope, np.random.default_rng(dim), np.float16, counts, [length, 500], heads,
-                                        kv_heads, dim, 16, scale=1.0, spoil=spoil, check=False)
+    cache, got, queries = run_attention(abi, ctx, scope, np.random.default_rng(dim), np.float16, counts, [length, 500],
+                                        heads, kv_heads, dim, 16, scale=1.0, spoil=spoil, check=False)
     got = got.astype(np.float64)
     assert np.isfinite(got).all()
     # the weights' rounding, half a step, and the sums'
