@@ -289,7 +289,7 @@ def _op(case, t, outputs):
                 _context, queries=b["queries"], query_stride=t["queries"].stride(0), query_output=b["rotated"],
                 keys=b["keys"], key_stride=t["keys"].stride(0), values=b["values"],
                 value_stride=t["values"].stride(0), rotary_dim=case["rotary_dim"], rotary=case["pairs"],
-                frequencies=b["frequencies"], positions=b["positions"], **cache)
+                frequencies=b["frequencies"], positions=b["positions"] if case["rotary_dim"] else None, **cache)
         else:
             op = abi.CacheAttentionOp(
                 _context, queries=b["queries"], output=b["output"], causal=case["causal"], window=case["window"],
