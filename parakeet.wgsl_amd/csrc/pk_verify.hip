@@ -219,27 +219,21 @@ struct Weights {
         y(args.draft && residual ? static_cast<const T*>(args.draft) + end.row * args.draft_stride : nullptr),
         refused(end.draft), p(table, end.p.m, args.scale), q(table, y ? end.q.m : 0.0, args.scale),
         inverse(p.right / end.p.sum), draft_inverse(y ? q.right / end.q.sum : 0.0), residual(residual) {}
-  // `whole` gets the target's probability.
-  __device__ __forceinline__ double of(float target, float draft, uint32_t i, double* whole) const {
+  __device__ __forceinline__ double of(float target, float draft, uint32_t i) const {
 #pragma clang fp contract(off)  // equal probabilities leave 0
     double w = p.at(target) * inverse;
-    *whole = w > kLeast ? w : 0.0;  // as it counts where p is drawn from: a part that is masked whole has none
     if (y) w -= q.at(draft) * draft_inverse;
     else if (residual && i == refused) w -= 1.0;
     return w > kLeast ? w : 0.0;
   }
   // Of N columns from `first` on, `count` of them there; the others' are 0.
   template <int N>
-  __device__ __forceinline__ void run(uint32_t first, uint32_t count, double (&w)[N], double* whole = nullptr) const {
+  __device__ __forceinline__ void run(uint32_t first, uint32_t count, double (&w)[N]) const {
     float target[N], draft[N];
     load_run<N>(z + first, count, target);
     if (y) load_run<N>(y + first, count, draft);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      double p = 0.0;
-      w[i] = (uint32_t)i < count ? of(target[i], y ? draft[i] : 0.0f, first + i, &p) : 0.0;
-      if (whole) *whole += p;
-    }
+    for (int i = 0; i < N; ++i) w[i] = (uint32_t)i < count ? of(target[i], y ? draft[i] : 0.0f, first + i) : 0.0;
   }
 };
 
@@ -451,7 +445,7 @@ __global__ __launch_bounds__(kSequence) void verify_sequence_kernel(VerifyArgs a
 struct Workspace {
   RowSum* sums;     // [rows][2][sums parts]
   End* ends;        // [sequences]
-  double2* weights;  // [sequences][parts]: of max(p - q, 0), and of p
+  double* weights;  // [sequences][parts]: of max(p - q, 0), or of p
 };
 template <typename T>
 __host__ __device__ uint32_t parts_of(uint32_t columns) {
@@ -466,7 +460,7 @@ __host__ __device__ Workspace bind(const VerifyArgs& args, uint64_t sequences) {
   Workspace w;
   w.sums = static_cast<RowSum*>(args.workspace);
   w.ends = reinterpret_cast<End*>(w.sums + 2ull * args.rows * sums_parts_of<T>(args.columns));
-  w.weights = reinterpret_cast<double2*>(w.ends + sequences);
+  w.weights = reinterpret_cast<double*>(w.ends + sequences);
   return w;
 }
 
@@ -638,18 +632,17 @@ __global__ __launch_bounds__(kThreads) void verify_weights_kernel(VerifyArgs arg
   if (args.greedy || end.token == kNoToken) return;
   const Weights<T> weights(args, table, end, end.draft != kNoToken);
   constexpr int kRun = 16 / sizeof(T);
-  double mine = 0.0, all = 0.0;
+  double mine = 0.0;
 #pragma unroll
   for (int j = 0; j < kHeld; ++j) {
     const uint32_t first = part_index * kSpan<T> + (j * kThreads + at) * kRun;
     double w[kRun];
-    weights.run(first, args.columns > first ? args.columns - first : 0u, w, &all);
+    weights.run(first, args.columns > first ? args.columns - first : 0u, w);
 #pragma unroll
     for (int i = 0; i < kRun; ++i) mine += w[i];
   }
   mine = reduce_group<kThreads>(mine, scratch, Add());
-  all = reduce_group<kThreads>(all, scratch, Add());
-  if (at == 0) work.weights[(uint64_t)s * parts + part_index] = make_double2(mine, all);
+  if (at == 0) work.weights[(uint64_t)s * parts + part_index] = mine;
 }
 
 // Finds the part of the row whose weights the draw ends in, and in it the token.
@@ -665,25 +658,40 @@ __global__ __launch_bounds__(kSequence) void verify_token_kernel(VerifyArgs args
   const End end = work.ends[s];
   if (end.token == kNoToken) return;
   bool residual = end.draft != kNoToken;
-  // The parts' weights: of p - q, or of p where that is nothing.
-  double whole = 0.0;
-  const auto part_weight = [&](uint32_t i) {
-    const double2 w = work.weights[(uint64_t)s * parts + i];
-    return residual ? w.x : w.y;
-  };
-  for (;;) {
+  constexpr int kRun = Weights<T>::kRun;
+  double* part_weights = work.weights + (uint64_t)s * parts;
+  const auto sum_parts = [&] {
     double mine = 0.0;
-    for (uint32_t i = at; i < parts; i += kSequence) mine += part_weight(i);
-    whole = reduce_group<kSequence>(mine, scratch, Add());
-    if (whole > 0.0 || !residual) break;
+    for (uint32_t i = at; i < parts; i += kSequence) mine += part_weights[i];
+    return reduce_group<kSequence>(mine, scratch, Add());
+  };
+  // This thread's weights of a part, and where they start.
+  double w[kRun];
+  uint32_t first = 0;
+  const auto weigh = [&](uint32_t part) {
+    first = part * kSpan<T> + at * kRun;
+    Weights<T>(args, table, end, residual).run(first, args.columns > first ? args.columns - first : 0u, w);
+    double mine = 0.0;
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) mine += w[i];
+    return mine;
+  };
+  double whole = sum_parts();
+  if (!(whole > 0.0) && residual) {  // p is nowhere above q, which is rare: the parts' weights of p
     residual = false;
+    for (uint32_t i = 0; i < parts; ++i) {
+      const double mine = reduce_group<kSequence>(weigh(i), scratch, Add());
+      if (at == 0) part_weights[i] = mine;
+    }
+    __syncthreads();
+    whole = sum_parts();
   }
   const double want = wanted(args.draws[s], whole);
   if (at < 64u) {  // the first wavefront, 64 parts at a time
     double before = 0.0, last_before = 0.0;
     uint32_t part = kNoToken, last = kNoToken;
     for (uint32_t base = 0; base < parts && part == kNoToken; base += 64u) {
-      const double w = base + at < parts ? part_weight(base + at) : 0.0;
+      const double w = base + at < parts ? part_weights[base + at] : 0.0;
       const double running = wave::running_sum(w);
       const uint64_t hit = __ballot(w > 0.0 && before + running > want), live = __ballot(w > 0.0);
       const int lane = hit ? __builtin_ctzll(hit) : live ? 63 - __builtin_clzll(live) : 0;
@@ -705,12 +713,7 @@ __global__ __launch_bounds__(kSequence) void verify_token_kernel(VerifyArgs args
     if (at == 0) args.next_tokens[s] = kNoToken;
     return;
   }
-  constexpr int kRun = Weights<T>::kRun;
-  const uint32_t first = found_part * kSpan<T> + at * kRun;
-  double w[kRun], mine = 0.0;
-  Weights<T>(args, table, end, residual).run(first, args.columns > first ? args.columns - first : 0u, w);
-#pragma unroll
-  for (int i = 0; i < kRun; ++i) mine += w[i];
+  const double mine = weigh(found_part);
   const uint32_t token = find_token(w, first, found_before + running_sum(mine, scratch).before, want, scratch);
   if (at == 0) args.next_tokens[s] = token;
 }
@@ -756,7 +759,7 @@ uint64_t workspace_typed(const VerifyArgs& args) {
   if (together(one)) return 0;
   const uint64_t parts = parts_of<T>(args.columns);
   return 2ull * args.rows * sums_parts_of<T>(args.columns) * sizeof(RowSum) +
-         args.sequences * (sizeof(End) + parts * sizeof(double2));
+         args.sequences * (sizeof(End) + parts * sizeof(double));
 }
 
 }  // namespace
