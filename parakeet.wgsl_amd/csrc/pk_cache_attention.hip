@@ -567,13 +567,14 @@ __device__ __forceinline__ void careful_item(const CacheAttentionArgs& args, con
 // two steps ahead leave one wavefront a SIMD and twice the code: 201 us for 64 sequences below and
 // not 182, 10.2 for one token where one was 9.5. Eight wavefronts a workgroup: 197, and 9.7.
 //
-// f16, 32 heads over 8 of 128 channels: 4 sequences with 131072 tokens 368 us, 5.8 TB/s of keys and
+// f16, 32 heads over 8 of 128 channels: 4 sequences with 131072 tokens 367 us, 5.8 TB/s of keys and
 // values, 64 with 200 to 16384 182, 5.3. One token of 8 heads over 376 9.0 us, by the clock from the
 // first instruction on: 0.7 for the item, 0.5 for the pages, 2.1 for keys, values and queries, 3.1 for
 // three steps, 1.4 for the end; the launch is the rest. 16 drafts of 4 to 8 tokens over up to 6000 (16
-// heads over 2 of 64 channels, a window, capped scores) 20.7 us: 1.8, 0.9, 1.8, 8 for four steps,
-// 2.7, then the join. f32, 16 chunks of up to 188 rows with windows of 376: 40 to 42 us, 23 of them
-// the matrix instructions, of which a SIMD has one wavefront or two.
+// heads over 2 of 64 channels, a window, capped scores) 20.6 us: 1.8, 0.9, 1.8, 8 for four steps,
+// 2.7, then the join. f32, 16 chunks of up to 188 rows with windows of 376: 40 us; a SIMD has one wavefront or
+// two, and over all of them the matrix instructions are busy 30 % of the time. f32 tokens: 64 sequences 351 us,
+// 6.1 TB/s, one over 376 14.7; 16 drafts 38.
 template <typename T>
 struct Step;
 template <>
@@ -975,10 +976,10 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
 // Both are laid out so that the lanes that read together read different banks: pieces
 // of 16 bytes of a key, and of 32 bytes of a value, are exchanged by a number of the row.
 //
-// 4 chunks of 700 to 1024 rows over up to 8192 tokens, 32 heads over 8 of 128 channels: 252 to 260 us, 780
+// 4 chunks of 700 to 1024 rows over up to 8192 tokens, 32 heads over 8 of 128 channels: 252 to 267 us, 780
 // TF where a large product reaches 1032; blocks of 64 rows by the kernel above took 1024. Matrix
-// instructions and exponentials hardly overlap: two wavefronts share a SIMD, and their sum is
-// the time. Pages of 8, 24 or 100 tokens take 270 to 274 us (through registers 378). Of DP channels of a tile
+// instructions are busy 36 % of the time and the VALU, by its instructions, some 48 %: two wavefronts
+// share a SIMD, and these hardly overlap. Pages of 8, 24 or 100 tokens take 270 to 274 us (through registers 378). Of DP channels of a tile
 // USED take part in the products, all or three quarters: heads of 96 and 80 channels 236 and 224 us, of
 // 192 among 256 380; with all 259, 250 and 447.
 template <int DP>
