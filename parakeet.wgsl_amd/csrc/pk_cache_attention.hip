@@ -979,9 +979,9 @@ __global__ __launch_bounds__(kThreads, RB > 1 && DP <= 128 && DP * RB <= 256 ? 2
 // 4 chunks of 700 to 1024 rows over up to 8192 tokens, 32 heads over 8 of 128 channels: 252 to 267 us, 780
 // TF where a large product reaches 1032; blocks of 64 rows by the kernel above took 1024. Matrix
 // instructions are busy 36 % of the time and the VALU, by its instructions, some 48 %: two wavefronts
-// share a SIMD, and these hardly overlap. Pages of 8, 24 or 100 tokens take 270 to 274 us (through registers 378). Of DP channels of a tile
-// USED take part in the products, all or three quarters: heads of 96 and 80 channels 236 and 224 us, of
-// 192 among 256 380; with all 259, 250 and 447.
+// share a SIMD, and these hardly overlap. Pages of 8, 24 or 100 tokens take 270 to 274 us (through
+// registers 378). Of DP channels of a tile USED take part in the products, all or three quarters: heads of 96
+// and 80 channels 236 and 224 us, of 192 among 256 380; with all 259, 250 and 447.
 template <int DP>
 struct ManyShape {
   static constexpr int kTokens = 64, kRows = 128;

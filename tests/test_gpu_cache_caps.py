@@ -38,6 +38,6 @@ def test_large_caps(abi, ctx, scope, dtype, counts, cap, std):
 @pytest.mark.parametrize("dim", [40, 64, 80, 128, 192, 256])
 def test_large_caps_of_every_unit(abi, ctx, scope, dtype, count, dim):
     cap = 65536.0
-    cache, got, queries = run_attention(abi, ctx, scope, np.random.default_rng(dim), dtype, [count, 1], [1200, 150], 4, 2, dim,
-                                        16, cap=cap, check=False)
+    cache, got, queries = run_attention(abi, ctx, scope, np.random.default_rng(dim), dtype, [count, 1], [1200, 150], 4, 2,
+                                        dim, 16, cap=cap, check=False)
     check_capped(cache, got, queries, 4, cap, 1200)
